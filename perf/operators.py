@@ -380,12 +380,14 @@ class _Memory:
 
 
 def _own_cache(x, room):
+    # the same codes as the plain form's, bit for bit, not requantized
     import eakv_amd
     layers, _, n_kv, t, d = x.shape
     c = eakv_amd.Cache(layers, n_kv, d, room)
+    for to, plane in zip(_own_planes(c, 0, t), _quantize(x)):
+        to.copy_(plane)
+    c.advance(t)
     torch.cuda.synchronize()
-    _must(eakv_amd.lib().eakv_cache_load_raw_device(c.h, x.data_ptr(), t, None))
-    c.sync()
     return c
 
 
@@ -396,8 +398,8 @@ def _must(rc):
 
 
 def _own_planes(c, at, n):
-    """Views of tokens [at, at + n) of every block's planes:
-    [2 * layers][n_kv][n][...]."""
+    """Views of tokens [at, at + n) of every block's planes,
+    [layers][2][n_kv][n][...], that keep the cache."""
     at_0, at_1 = c.planes_device(0, 0), c.planes_device(0, 1)
     step, gpd = at_1[0] - at_0[0], c.head_dim // 64
     got = []
@@ -406,6 +408,7 @@ def _own_planes(c, at, n):
         got.append(torch.as_tensor(_Memory(ptr + at * row, (2 * c.n_layers, c.n_heads, n, per),
                                            (step, c.max_seq_len * row, row, size), kind),
                                    device="cuda").unflatten(0, (c.n_layers, 2)))
+        got[-1].cache = c       # the memory lives as long as the view
     return got
 
 
