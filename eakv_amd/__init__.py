@@ -26,6 +26,10 @@ EAKV_ERR_ALLOC = -3
 EAKV_ERR_INVALID = -4
 EAKV_ERR_DEVICE = -5
 
+EAKV_F32 = 0
+EAKV_BF16 = 1
+EAKV_TREE_MAX = 64
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libeakv.so")
 
@@ -72,6 +76,21 @@ SIGNATURES = {
         C.c_int, [_vp, C.c_int, C.c_int, _vp, C.c_int, C.c_int, _vp, _vp]),
     "eakv_attention_fused_batch_device_noalloc": (
         C.c_int, [_vp, C.c_int, C.c_int, _vp, C.c_int, C.c_int, _vp, _vp]),
+    "eakv_attention_window_batch_device": (
+        C.c_int, [_vp, C.c_int, C.c_int, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp,
+                  C.c_size_t, _vp]),
+    "eakv_attention_window_work_bytes": (
+        C.c_size_t, [_vp, C.c_int, _vp, _vp, C.c_int, C.c_int, C.c_int]),
+    "eakv_verify_drafts_device": (
+        C.c_int, [C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, C.c_int64, _vp, C.c_int64, _vp, _vp,
+                  _vp, _vp, C.c_size_t, _vp]),
+    "eakv_verify_drafts_work_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    "eakv_cache_copy_batch_device": (
+        C.c_int, [_vp, C.c_int, _vp, C.c_int, C.c_int, C.c_int, _vp]),
+    "eakv_cache_gather_batch_device": (C.c_int, [_vp, _vp, C.c_int, _vp, _vp, _vp, _vp]),
+    "eakv_cache_fork": (_vp, [_vp, C.c_int, C.c_int]),
+    "eakv_cache_compact": (C.c_int, [_vp, C.c_int, _vp, C.c_int]),
+    "eakv_cache_planes_device": (C.c_int, [_vp, C.c_int, C.c_int, _vp, _vp, _vp]),
     "eakv_attention_fused_plan": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp]),
     "eakv_dequantize_range_device": (
         C.c_int, [_vp, C.c_int, C.c_int, C.c_int64, C.c_int64, _vp, _vp]),
@@ -264,6 +283,29 @@ class Cache:
         _check(lib().eakv_validate(self.h, _ptr(res)))
         return res
 
+    def planes_device(self, layer, kv_idx):
+        """Device addresses of a block's packed codes, scales and biases."""
+        p = [_vp() for _ in range(3)]
+        _check(lib().eakv_cache_planes_device(self.h, layer, kv_idx, *map(C.byref, p)))
+        return tuple(x.value for x in p)
+
+    # -- tokens moved
+    def fork(self, n_tokens=None, max_seq_len=None):
+        """A new cache holding the first n_tokens (all) of this one."""
+        L = lib()
+        L.eakv_clear_error()
+        h = L.eakv_cache_fork(self.h, self.seq_len if n_tokens is None else n_tokens,
+                              self.max_seq_len if max_seq_len is None else max_seq_len)
+        if not h:
+            code, msg = last_error()
+            raise EakvError(code or EAKV_ERR_INVALID, msg or "cache_fork failed")
+        return type(self)(0, 0, 0, 0, _handle=h)
+
+    def compact(self, keep, start=0):
+        """Keep the tokens before start and, of the others, those at `keep`."""
+        k = np.ascontiguousarray(keep, dtype=np.int32)
+        return _check(lib().eakv_cache_compact(self.h, start, _ptr(k), k.size))
+
     def sync(self):
         return _check(lib().eakv_cache_sync(self.h))
 
@@ -284,6 +326,40 @@ def handles(caches):
     for i, c in enumerate(caches):
         arr[i] = c.h
     return arr
+
+
+def ints(values):
+    """ctypes int32 array for the batched entry points."""
+    return (C.c_int32 * len(values))(*values)
+
+
+class WindowPlan:
+    """One shape of eakv_attention_window_batch_device: the caches, the tokens of each
+    window, where the windows begin (None: at each cache's seq_len when run) and the
+    head split.  Buffers are device addresses."""
+
+    def __init__(self, caches, n_tokens, n_q, n_kv, starts=None, dtype="f32"):
+        self.caches = list(caches)
+        self._h, self._n = handles(self.caches), ints(n_tokens)
+        self._starts = None if starts is None else ints(starts)
+        self._args = ({"f32": EAKV_F32, "bf16": EAKV_BF16}[dtype], n_q, n_kv)
+
+    @property
+    def work_bytes(self):
+        """Bytes of scratch that a run with a workspace of its own needs."""
+        L = lib()
+        L.eakv_clear_error()
+        n = L.eakv_attention_window_work_bytes(self._h, len(self.caches), self._starts, self._n,
+                                               *self._args)
+        code, msg = last_error()
+        if code:
+            raise EakvError(code, msg)
+        return n
+
+    def run(self, layer, d_q, d_out, d_tree=None, d_work=None, work_bytes=0, stream=None):
+        return _check(lib().eakv_attention_window_batch_device(
+            self._h, len(self.caches), layer, self._starts, self._n, d_q, *self._args, d_tree,
+            d_out, d_work, work_bytes, stream))
 
 
 FUSED_PLAN_KEYS = ("mfma", "chunks", "merge_levels", "tile_tokens", "waves_per_block",

@@ -10,7 +10,7 @@
 
 #include "internal.h"
 
-static int attn_check(const eakv_cache_t *c, int layer, int n_q, int n_kv)
+int eakvi_attn_check(const eakv_cache_t *c, int layer, int n_q, int n_kv)
 {
     if (!c) return eakvi_set_error(EAKV_ERR_INVALID, "attention: NULL cache");
     if (c->head_dim != 64 && c->head_dim != 128)
@@ -26,6 +26,19 @@ static int attn_check(const eakv_cache_t *c, int layer, int n_q, int n_kv)
     return EAKV_OK;
 }
 
+int eakvi_same_batch(eakv_cache_t *const *caches, int n, const char *what)
+{
+    for (int i = 0; i < n; i++) {
+        if (!caches[i]) return eakvi_set_error(EAKV_ERR_INVALID, "%s: NULL cache", what);
+        const eakv_cache_t *a = caches[0], *b = caches[i];
+        if (a->n_layers != b->n_layers || a->n_kv_heads != b->n_kv_heads ||
+            a->head_dim != b->head_dim || a->max_seq_len != b->max_seq_len ||
+            a->device != b->device)
+            return eakvi_set_error(EAKV_ERR_INVALID, "%s: caches differ in shape", what);
+    }
+    return EAKV_OK;
+}
+
 static size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 
@@ -36,7 +49,7 @@ int eakv_attention_scores_device(const eakv_cache_t *c, const float *d_q,
                                  int layer, int n_q, int n_kv,
                                  float *d_scores, void *stream)
 {
-    int rc = attn_check(c, layer, n_q, n_kv);
+    int rc = eakvi_attn_check(c, layer, n_q, n_kv);
     if (rc) return rc;
     if (!d_q || !d_scores)
         return eakvi_set_error(EAKV_ERR_INVALID, "scores: NULL buffer");
@@ -60,7 +73,7 @@ void eakv_attention_scores(const eakv_cache_t *cc, const float *queries,
                            int layer, int n_q, int n_kv, float *scores_out)
 {
     eakv_cache_t *c = (eakv_cache_t *)cc;
-    if (attn_check(c, layer, n_q, n_kv)) return;
+    if (eakvi_attn_check(c, layer, n_q, n_kv)) return;
     if (!queries || !scores_out) {
         eakvi_set_error(EAKV_ERR_INVALID, "scores: NULL buffer");
         return;
@@ -98,7 +111,7 @@ int eakv_attention_output_device(const eakv_cache_t *cc, const float *d_w,
                                  void *stream)
 {
     eakv_cache_t *c = (eakv_cache_t *)cc;
-    int rc = attn_check(c, layer, n_q, n_kv);
+    int rc = eakvi_attn_check(c, layer, n_q, n_kv);
     if (rc) return rc;
     if (!d_w || !d_out)
         return eakvi_set_error(EAKV_ERR_INVALID, "output: NULL buffer");
@@ -127,7 +140,7 @@ void eakv_attention_output(const eakv_cache_t *cc, const float *weights,
                            int layer, int n_q, int n_kv, float *output_out)
 {
     eakv_cache_t *c = (eakv_cache_t *)cc;
-    if (attn_check(c, layer, n_q, n_kv)) return;
+    if (eakvi_attn_check(c, layer, n_q, n_kv)) return;
     if (!weights || !output_out) {
         eakvi_set_error(EAKV_ERR_INVALID, "output: NULL buffer");
         return;
@@ -188,18 +201,10 @@ int eakv_attention_fused_batch_device(eakv_cache_t *const *caches,
 {
     if (!caches || n_caches <= 0 || n_caches > EAKVD_MAX_BATCH || !d_q || !d_out)
         return eakvi_set_error(EAKV_ERR_INVALID, "fused_batch: invalid argument");
-    for (int i = 0; i < n_caches; i++) {
-        if (!caches[i])
-            return eakvi_set_error(EAKV_ERR_INVALID, "fused_batch: NULL cache");
-        const eakv_cache_t *a = caches[0], *b = caches[i];
-        if (a->n_layers != b->n_layers || a->n_kv_heads != b->n_kv_heads ||
-            a->head_dim != b->head_dim || a->max_seq_len != b->max_seq_len ||
-            a->device != b->device)
-            return eakvi_set_error(EAKV_ERR_INVALID,
-                                  "fused_batch: caches differ in shape");
-    }
+    int rc = eakvi_same_batch(caches, n_caches, "fused_batch");
+    if (rc) return rc;
     eakv_cache_t *c0 = caches[0];
-    int rc = attn_check(c0, layer, n_q, n_kv);
+    rc = eakvi_attn_check(c0, layer, n_q, n_kv);
     if (rc) return rc;
     int prev;
     rc = eakvi_enter(c0, &prev);
@@ -230,7 +235,7 @@ int eakv_attention_fused(const eakv_cache_t *cc, const float *queries,
                          int layer, int n_q, int n_kv, float *output_out)
 {
     eakv_cache_t *c = (eakv_cache_t *)cc;
-    int rc = attn_check(c, layer, n_q, n_kv);
+    int rc = eakvi_attn_check(c, layer, n_q, n_kv);
     if (rc) return rc;
     if (!queries || !output_out)
         return eakvi_set_error(EAKV_ERR_INVALID, "fused: NULL buffer");
@@ -276,18 +281,10 @@ int eakv_attention_fused_batch_device_noalloc(eakv_cache_t *const *caches,
 {
     if (!caches || n_caches <= 0 || n_caches > EAKVD_MAX_BATCH || !d_q || !d_out)
         return eakvi_set_error(EAKV_ERR_INVALID, "fused_noalloc: invalid argument");
-    for (int i = 0; i < n_caches; i++) {
-        if (!caches[i])
-            return eakvi_set_error(EAKV_ERR_INVALID, "fused_noalloc: NULL cache");
-        const eakv_cache_t *a = caches[0], *b = caches[i];
-        if (a->n_layers != b->n_layers || a->n_kv_heads != b->n_kv_heads ||
-            a->head_dim != b->head_dim || a->max_seq_len != b->max_seq_len ||
-            a->device != b->device)
-            return eakvi_set_error(EAKV_ERR_INVALID,
-                                  "fused_noalloc: caches differ in shape");
-    }
+    int rc = eakvi_same_batch(caches, n_caches, "fused_noalloc");
+    if (rc) return rc;
     eakv_cache_t *c0 = caches[0];
-    int rc = attn_check(c0, layer, n_q, n_kv);
+    rc = eakvi_attn_check(c0, layer, n_q, n_kv);
     if (rc) return rc;
     eakvd_batch b;
     memset(&b, 0, sizeof(b));
@@ -332,7 +329,7 @@ int eakv_attention_fused_plan(eakv_cache_t *const *caches, int n_caches, int n_q
         if (!caches[i])
             return eakvi_set_error(EAKV_ERR_INVALID, "fused_plan: NULL cache");
     eakv_cache_t *c0 = caches[0];
-    int rc = attn_check(c0, 0, n_q, n_kv);
+    int rc = eakvi_attn_check(c0, 0, n_q, n_kv);
     if (rc) return rc;
     eakvd_batch b;
     memset(&b, 0, sizeof(b));

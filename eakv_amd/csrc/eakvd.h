@@ -78,6 +78,7 @@ int  eakvd_memcpy_d2h_async(void *dst, const void *src, size_t n, void *s);
 int  eakvd_copy_in(void *dst, const void *src, size_t n, void *s);
 int  eakvd_memcpy_d2d_async(void *dst, const void *src, size_t n, void *s);
 const char *eakvd_error_string(int err);
+int  eakvd_stream_capturing(void *s, int *yes);   /* whether s records a graph */
 
 /* ---- quantize (hip/quantize.hip)
  * Source row r starts at src + r*row_stride and holds n_g groups of 64
@@ -161,6 +162,48 @@ size_t eakvd_fused_launch_bytes(const eakvd_geom *g, const eakvd_batch *b,
  * Returns 0 or a HIP error. */
 #define EAKVD_SCRATCH_BYTES ((size_t)16 << 20)
 int eakvd_scratch(void **p);
+
+/* ---- windows of new tokens (hip/window.hip)
+ * Query i < ntok[c] of sequence c is at position start[c] + i; q and out:
+ * [sum ntok][n_q][head_dim] (f32, or bf16 where bf16 != 0).  tree != NULL: word
+ * i's bit j says that query i sees token start + j (windows of at most 64
+ * tokens); else the window is causal.  work: eakvd_window_work_bytes() of
+ * device scratch; launches that share it must not overlap. */
+typedef struct {
+    int            n_seq;
+    const uint8_t *base[EAKVD_MAX_BATCH];
+    int            start[EAKVD_MAX_BATCH];
+    int            ntok[EAKVD_MAX_BATCH];
+} eakvd_window;
+
+size_t eakvd_window_work_bytes(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv);
+int eakvd_window_attend(const eakvd_geom *g, const eakvd_window *b, int layer, const void *q,
+                        int bf16, int n_q, int n_kv, const uint64_t *tree, void *out, void *work,
+                        void *stream);
+
+/* ---- tokens between and within caches (hip/move.hip); gs, gd: the layouts of
+ * sources and destinations, which differ in max_seq_len at most */
+int eakvd_copy_tokens(const eakvd_geom *gs, const eakvd_geom *gd, const uint8_t *src, int src_pos,
+                      uint8_t *const *dst, int n_dst, int dst_pos, int n_tokens, void *stream);
+/* Sequence c: dst token dst_pos[c] + i = src token index[first[c] + i], i <
+ * n_tokens[c]; src[c] == dst[c] with ascending index[i] >= dst_pos + i only. */
+typedef struct {
+    int            n_seq;
+    const uint8_t *src[EAKVD_MAX_BATCH];
+    uint8_t       *dst[EAKVD_MAX_BATCH];
+    int            dst_pos[EAKVD_MAX_BATCH];
+    int            n_tokens[EAKVD_MAX_BATCH];
+    int64_t        first[EAKVD_MAX_BATCH];
+    const int32_t *index;
+} eakvd_gather;
+int eakvd_gather_tokens(const eakvd_geom *gs, const eakvd_geom *gd, const eakvd_gather *job,
+                        void *stream);
+
+/* ---- drafts against the target (hip/verify.hip); see eakv_verify_drafts_device */
+size_t eakvd_verify_work_bytes(int n_seqs, int vocab);
+int eakvd_verify(int n_seqs, int k, int vocab, const int32_t *count, const int32_t *token,
+                 const float *draft, int64_t ld_draft, const float *target, int64_t ld_target,
+                 const float *uniform, int32_t *kept, int32_t *next, void *work, void *stream);
 
 /* ---- whole-plane kernels (hip/planes.hip)
  * eakvd_dequantize: groups [g0, g0 + n) of block (layer, kv) to out

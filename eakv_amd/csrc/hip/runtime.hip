@@ -113,6 +113,14 @@ int eakvd_memcpy_d2d_async(void *dst, const void *src, size_t n, void *s)
                                (hipStream_t)s);
 }
 
+int eakvd_stream_capturing(void *s, int *yes)
+{
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    const hipError_t e = hipStreamIsCapturing((hipStream_t)s, &st);
+    *yes = e == hipSuccess && st != hipStreamCaptureStatusNone;
+    return (int)e;
+}
+
 const char *eakvd_error_string(int err)
 {
     return hipGetErrorString((hipError_t)err);

@@ -1,0 +1,265 @@
+// verify.hip — which drafted tokens the target model keeps, and the token after
+// them (speculative sampling), for a padded batch of drafts.
+//
+// Draft i with token x is kept while u_i * q_i(x) < p_i(x) (u in [0, 1), so kept
+// with probability min(1, p/q)).  a = the number kept.  The next token is drawn
+// from r = max(p_a - q_a, 0) after a rejection, from r = p_a when all were kept:
+// the least j whose sum r[0..j] exceeds u * sum(r).
+//
+// Every comparison is of exact products and differences of f32 values in f64, and
+// the sums are f64: the result does not depend on the order of a sum unless the
+// drawn number lies within 1e-15 of a step.
+//
+// Work: one row of p and one of q per sequence, bound by HBM for large batches and
+// by latency for small ones.  Two launches: each block sums one segment of its
+// sequence's row; one block per sequence then finds the segment and scans it
+// (out of L2).
+#include "common.h"
+
+namespace {
+
+constexpr int kVerThreads = 256;
+
+typedef float v4f4 __attribute__((ext_vector_type(4), aligned(4)));
+
+struct VerJob {
+    int k, vocab, n_seg, seg;
+    const int32_t *count, *token;
+    const float *draft, *target, *uniform;
+    int64_t ld_draft, ld_target;
+    int32_t *kept, *next;
+    double *part;               // [n_seqs][n_seg][2]: sums of r and of p
+};
+
+__device__ __forceinline__ int count_of(const VerJob &J, int s)
+{
+    const int n = J.count ? J.count[s] : J.k;
+    return n < 0 ? 0 : n > J.k ? J.k : n;
+}
+
+// The drafts of sequence s that are kept (every lane of a wave gets it).
+__device__ __forceinline__ int kept_of(const VerJob &J, int s, int n, int lane)
+{
+    for (int i0 = 0; i0 < n; i0 += 64) {
+        const int i = i0 + lane;
+        bool ok = false;
+        if (i < n) {
+            const int64_t at = (int64_t)s * J.k + i;
+            const int x = J.token[at];
+            if (x >= 0 && x < J.vocab) {
+                const float p = J.target[((int64_t)s * (J.k + 1) + i) * J.ld_target + x];
+                const float q = J.draft ? J.draft[at * J.ld_draft + x] : 1.0f;
+                ok = (double)J.uniform[(int64_t)s * (J.k + 1) + i] * (double)q < (double)p;
+            }
+        }
+        const uint64_t bad = __ballot(i < n && !ok);
+        if (bad) return i0 + __ffsll((unsigned long long)bad) - 1;
+    }
+    return n;
+}
+
+// The row that the next token is drawn from.
+struct Row {
+    const float *p, *q;         // q NULL: no draft row
+    int less;                   // a token whose weight is 0 (one-hot draft), or -1
+    __device__ __forceinline__ double at(double p_, double q_, int j) const
+    {
+        const double r = q ? p_ - q_ : p_;
+        return j != less && r > 0.0 ? r : 0.0;
+    }
+};
+
+__device__ __forceinline__ Row row_of(const VerJob &J, int s, int n, int kept)
+{
+    Row r;
+    r.p = J.target + ((int64_t)s * (J.k + 1) + kept) * J.ld_target;
+    const int64_t at = (int64_t)s * J.k + kept;
+    r.q = kept < n && J.draft ? J.draft + at * J.ld_draft : nullptr;
+    r.less = kept < n && !J.draft ? J.token[at] : -1;
+    return r;
+}
+
+__device__ __forceinline__ double wave_sum_d(double v)
+{
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+__global__ __launch_bounds__(kVerThreads) void verify_sum_kernel(VerJob J)
+{
+    __shared__ double sh[2][kVerThreads / 64];
+    const int s = blockIdx.y, b = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int n = count_of(J, s);
+    const int kept = kept_of(J, s, n, lane);
+    if (b == 0 && tid == 0) J.kept[s] = kept;
+    const Row R = row_of(J, s, n, kept);
+    const int lo = b * J.seg, hi = min(J.vocab, lo + J.seg);
+    double sr = 0.0, sp = 0.0;
+    int j = lo + 4 * tid;
+    for (; j + 4 <= hi; j += 4 * kVerThreads) {
+        const v4f4 p = *(const v4f4 *)(R.p + j);
+        v4f4 q = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (R.q) q = *(const v4f4 *)(R.q + j);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            sr += R.at((double)p[e], (double)q[e], j + e);
+            sp += p[e] > 0.0f ? (double)p[e] : 0.0;
+        }
+    }
+    for (int e = 0; e < 4 && j + e < hi; e++) {
+        const float p = R.p[j + e];
+        sr += R.at((double)p, R.q ? (double)R.q[j + e] : 0.0, j + e);
+        sp += p > 0.0f ? (double)p : 0.0;
+    }
+    sr = wave_sum_d(sr);
+    sp = wave_sum_d(sp);
+    if (lane == 0) {
+        sh[0][w] = sr;
+        sh[1][w] = sp;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        double *o = J.part + ((int64_t)s * J.n_seg + b) * 2;
+        o[0] = (sh[0][0] + sh[0][1]) + (sh[0][2] + sh[0][3]);
+        o[1] = (sh[1][0] + sh[1][1]) + (sh[1][2] + sh[1][3]);
+    }
+}
+
+// Inclusive sum over the block's threads; *total gets the block's.
+__device__ __forceinline__ double block_scan(double v, double *sh, int tid, double *total)
+{
+    const int lane = tid & 63, w = tid >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double u = __shfl_up(v, o, 64);
+        if (lane >= o) v += u;
+    }
+    __syncthreads();
+    if (lane == 63) sh[w] = v;
+    __syncthreads();
+    double before = 0.0, all = 0.0;
+#pragma unroll
+    for (int i = 0; i < kVerThreads / 64; i++) {
+        if (i < w) before += sh[i];
+        all += sh[i];
+    }
+    *total = all;
+    return before + v;
+}
+
+__global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerJob J)
+{
+    __shared__ double sh[kVerThreads / 64];
+    __shared__ double s_before;
+    __shared__ int s_first, s_last;
+    const int s = blockIdx.x, tid = threadIdx.x;
+    const int n = count_of(J, s);
+    const int kept = J.kept[s];
+    Row R = row_of(J, s, n, kept);
+    // n_seg <= kVerThreads
+    const double *o = J.part + ((int64_t)s * J.n_seg + tid) * 2;
+    const double pr = tid < J.n_seg ? o[0] : 0.0, pp = tid < J.n_seg ? o[1] : 0.0;
+    if (tid == 0) {
+        s_first = INT32_MAX;
+        s_last = -1;
+        s_before = 0.0;
+    }
+    double total, cum = block_scan(pr, sh, tid, &total);
+    double mine = pr;
+    if (!(total > 0.0)) {
+        // nothing left of p - q: the target's own row
+        R.q = nullptr;
+        R.less = -1;
+        mine = pp;
+        cum = block_scan(pp, sh, tid, &total);
+    }
+    if (!(total > 0.0)) {
+        if (tid == 0) J.next[s] = -1;
+        return;
+    }
+    const double want = (double)J.uniform[(int64_t)s * (J.k + 1) + J.k] * total;
+    if (tid < J.n_seg && mine > 0.0) {
+        if (cum > want) atomicMin(&s_first, tid);
+        atomicMax(&s_last, tid);
+    }
+    __syncthreads();
+    const int b = s_first == INT32_MAX ? s_last : s_first;
+    if (tid == b) s_before = cum - mine;
+    __syncthreads();
+    double before = s_before;
+    __syncthreads();
+    if (tid == 0) {
+        s_first = INT32_MAX;
+        s_last = -1;
+    }
+    const int lo = b * J.seg, hi = min(J.vocab, lo + J.seg);
+    for (int j0 = lo; j0 < hi; j0 += 4 * kVerThreads) {
+        const int j = j0 + 4 * tid;
+        double r[4], sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            r[e] = j + e < hi ? R.at((double)R.p[j + e], R.q ? (double)R.q[j + e] : 0.0, j + e) : 0.0;
+            sum += r[e];
+        }
+        double all;
+        double upto = before + (block_scan(sum, sh, tid, &all) - sum);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            upto += r[e];
+            if (r[e] > 0.0) {
+                atomicMax(&s_last, j + e);
+                if (upto > want) atomicMin(&s_first, j + e);
+            }
+        }
+        __syncthreads();
+        if (s_first != INT32_MAX) break;
+        before += all;
+    }
+    if (tid == 0) J.next[s] = s_first != INT32_MAX ? s_first : s_last;
+}
+
+// Segments of 1024 values where that leaves the chip unfilled, else of 4096;
+// at most one per thread of the second launch.
+int seg_of(int n_seqs, int vocab)
+{
+    int64_t seg = (int64_t)n_seqs * vocab >= (int64_t)1024 * 4096 ? 4096 : 1024;
+    while ((vocab + seg - 1) / seg > kVerThreads) seg *= 2;
+    return (int)seg;
+}
+
+}  // namespace
+
+extern "C" size_t eakvd_verify_work_bytes(int n_seqs, int vocab)
+{
+    const int seg = seg_of(n_seqs, vocab);
+    return (size_t)n_seqs * ((vocab + (int64_t)seg - 1) / seg) * 2 * sizeof(double);
+}
+
+extern "C" int eakvd_verify(int n_seqs, int k, int vocab, const int32_t *count, const int32_t *token,
+                            const float *draft, int64_t ld_draft, const float *target,
+                            int64_t ld_target, const float *uniform, int32_t *kept, int32_t *next,
+                            void *work, void *stream)
+{
+    VerJob J;
+    J.k = k;
+    J.vocab = vocab;
+    J.seg = seg_of(n_seqs, vocab);
+    J.n_seg = (int)((vocab + (int64_t)J.seg - 1) / J.seg);
+    J.count = count;
+    J.token = token;
+    J.draft = draft;
+    J.target = target;
+    J.uniform = uniform;
+    J.ld_draft = ld_draft;
+    J.ld_target = ld_target;
+    J.kept = kept;
+    J.next = next;
+    J.part = (double *)work;
+    const hipStream_t st = (hipStream_t)stream;
+    hipLaunchKernelGGL(verify_sum_kernel, dim3((unsigned)J.n_seg, (unsigned)n_seqs), dim3(kVerThreads),
+                       0, st, J);
+    hipLaunchKernelGGL(verify_pick_kernel, dim3((unsigned)n_seqs), dim3(kVerThreads), 0, st, J);
+    return (int)hipGetLastError();
+}

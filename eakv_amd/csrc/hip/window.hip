@@ -1,0 +1,969 @@
+// window.hip — attention of several new tokens of each sequence over the packed
+// cache: query i of a window that begins at position `start` sees the cache's
+// tokens before start and, in the window, the tokens up to its own (causal) or
+// the ones its mask word names (a tree of drafts).
+//
+//   out[i][h] = sum_t softmax_t(q[i][h].K[t] / sqrt(d)) V[t],
+//   K[t] = n*s + b per group of 64 dims (n the nibble), V likewise.
+//
+// A kv head's rows (window tokens x the q heads that share it) are the columns
+// of both products, so one pass over the packed planes serves all of them:
+//   S^T = K Q^T    v_mfma_f32_32x32x16_f16, 32 tokens x 32 rows
+//   O^T = V^T P^T  32 dims x 32 rows; a lane's 16 scores belong to one row, and
+//                  the tokens of a K = 16 step are numbered so that the scores'
+//                  registers are P's operand as they stand.
+// K's operands are n - z, exact in f16 (z: the nibble nearest the value 0): score =
+// sum over groups of s*(q.(n - z)) + c*sum(q), c = b + z*s, with s applied to the f32
+// dots and the c terms computed by one bf16 product of three pieces each (24 bits).
+// The nibbles become f16 once per block in LDS, in operand order, and are read
+// by all waves that need them (WR waves of 32 rows each x WT waves that take
+// different tokens).
+//
+// Two arithmetics:
+//   f32 queries   Q and the weights p*s are pairs of f16 (24 bits together),
+//                 V's operands n - z; its c terms are f32 sums of p*c.
+//   bf16 queries  Q (8 bits) is exact in f16.  V is dequantized to f16,
+//                 (n - z)*s + c with s and c rounded to f16, and p is rounded
+//                 to f16: 2^-12 relative each, against the output's 2^-9.
+// f16's range: Q rows are scaled by a power of two to below 2^15, V tiles (bf16) by
+// theirs; the softmax's reference point M includes the exponent of the
+// tile's V, so that every weight operand stays below 2^15 and keeps its
+// precision down to 2^-29 of that.
+//
+// Softmax in the log2 domain, f32: M moves only when a score passes it by
+// kTau; sums, weighted sums and M are f32.  Tokens are split into chunks where
+// rows alone do not fill the chip; partial (O, M, l) are merged by a second
+// launch.  No atomics: results are the same bits on every call.
+#include <string.h>
+
+#include "common.h"
+
+namespace {
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+constexpr int kWinWaves = 8;           // waves of a block: two per SIMD
+constexpr float kWinTau = 4.0f;        // headroom of the lazy M, log2 units
+constexpr float kWinTop = 11.0f;       // weights below 2^(kWinTop + kWinTau) = 2^15
+constexpr float kMInit = -3.4028234664e38f;
+constexpr int kExpLow = -60;           // tile exponents below this count as this
+
+struct WinJob {
+    int n_seq, n_q, n_kv, qpk, layer;
+    const uint8_t *base[EAKVD_MAX_BATCH];
+    int start[EAKVD_MAX_BATCH];
+    int ntok[EAKVD_MAX_BATCH];
+    int tok0[EAKVD_MAX_BATCH];          // the window's first row of q and out
+    int mc[EAKVD_MAX_BATCH];            // chunks
+    int clen[EAKVD_MAX_BATCH];          // tokens per chunk
+    int pre[EAKVD_MAX_BATCH + 1];       // blocks before this sequence's
+    int64_t part[EAKVD_MAX_BATCH];      // first partial row
+    int64_t part_rows;                  // partial rows in all
+};
+
+// LDS of one 32-token sub-tile.
+template <int D, bool F32>
+struct __align__(16) SubTile {
+    static constexpr int GPD = D / 64;
+    uint4 k[GPD * 4][64];               // operand (g, octet, nibble), by lane
+    uint4 v[GPD * 4][64];               // operand (g, nibble, 16-token step), by lane
+    uint4 kb[64];                       // K's biases in bf16 pieces, by lane
+    float ks[GPD][32];                  // K's scales
+    float vs[F32 ? GPD : 1][32];        // f32: scales and biases of V
+    float vc[F32 ? GPD : 1][32];
+    int ev[2];                          // exponent of V, by unit
+    uint32_t bad[2][2];                 // bf16: tokens with non-finite V, by unit and group
+};
+
+// What a lane has in flight of one unit (a 64-lane share of a sub-tile's
+// conversion): 16 packed bytes and their scales and biases.
+struct Raw {
+    uint4 x;
+    float s[4], b[4];
+};
+
+__device__ __forceinline__ uint32_t u_of(h2 v) { return __builtin_bit_cast(uint32_t, v); }
+__device__ __forceinline__ h2 h_of(uint32_t v) { return __builtin_bit_cast(h2, v); }
+// Two roundings to nearest even.  The empty asm statements (no instruction that
+// the compiler's hazard handling would miss behind a transcendental) hold a and b
+// to f32 and the result to one rounding: the compiler otherwise rounds a product
+// straight to f16 in one place and by way of f32 in another, and a pair's low part
+// must be what the high part left.
+__device__ __forceinline__ h2 pk(float a, float b)
+{
+    asm("" : "+v"(a));
+    asm("" : "+v"(b));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    uint32_t r = u_of(__builtin_convertvector((f2{a, b}), h2));
+    asm("" : "+v"(r));
+    return h_of(r);
+}
+// what pk(a, b) left of a and b, exact, in f16
+__device__ __forceinline__ h2 pk_rest(h2 hi, float a, float b)
+{
+    return pk(fmaf((float)hi[0], -1.0f, a), fmaf((float)hi[1], -1.0f, b));
+}
+
+// n - z of the low (HI false) or high nibbles of bytes 0 and 2 of x, exact: the
+// nibble is put into the mantissa of 1024 (its lowest bits) or of 64 (four bits up)
+// and 1024 + z or 64 + z taken off.  off: -z of the two bytes.  9 instructions
+// for 8 nibbles.
+template <bool HI>
+__device__ __forceinline__ h2 nib2(uint32_t x, h2 off)
+{
+    if constexpr (HI)
+        return h_of((x & 0x00f000f0u) | 0x54005400u) + (off - h2{(_Float16)64.0f, (_Float16)64.0f});
+    else
+        return h_of((x & 0x000f000fu) | 0x64006400u) +
+               (off - h2{(_Float16)1024.0f, (_Float16)1024.0f});
+}
+
+// z: the nibble whose value is nearest 0, so that (n - z)*s and c = b + z*s are of
+// the size of the value and cancel nothing (a group with an outlier has b and
+// s far above its other values).
+__device__ __forceinline__ float zero_nibble(float s, float b)
+{
+    const float z = __builtin_rintf(-b * __builtin_amdgcn_rcpf(s));
+    return fminf(fmaxf(z, 0.0f), 15.0f);
+}
+
+__device__ __forceinline__ float wave_top(float v)
+{
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+__device__ __forceinline__ int exp_of(float a)
+{
+    const int e = (int)(__float_as_uint(a) >> 23) - 126;     // a < 2^e
+    return e < kExpLow ? kExpLow : e;
+}
+// x * 2^e, one rounding, for any e
+__device__ __forceinline__ float scale2(float x, int e)
+{
+    return __builtin_amdgcn_ldexpf(x, e);
+}
+
+// p * v, 0 * anything = 0: a hidden token's scale or bias may be non-finite
+__device__ __forceinline__ float mul_hidden(float p, float v)
+{
+    return p == 0.0f ? 0.0f : p * v;
+}
+
+// Three bf16 pieces of x, together 24 bits.
+__device__ __forceinline__ void pieces(float x, __bf16 &a, __bf16 &b, __bf16 &c)
+{
+    a = (__bf16)x;
+    const float r = __fsub_rn(x, (float)a);
+    b = (__bf16)r;
+    c = (__bf16)__fsub_rn(r, (float)b);
+}
+
+// The 8 consecutive dims of one operand (a multiple of 8 dims from the row's
+// start) as f32.  Rows of q are 16-byte aligned or read by elements.
+template <bool F32>
+__device__ __forceinline__ void load_q8(const void *q, int64_t at, bool vec, float *o)
+{
+    if constexpr (F32) {
+        const float *p = (const float *)q + at;
+        if (vec) {
+            const v4f a = *(const v4f *)p, b = *(const v4f *)(p + 4);
+#pragma unroll
+            for (int j = 0; j < 4; j++) { o[j] = a[j]; o[4 + j] = b[j]; }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) o[j] = p[j];
+        }
+    } else {
+        const uint16_t *p = (const uint16_t *)q + at;
+        if (vec) {
+            const uint4 a = *(const uint4 *)p;
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                o[2 * j] = __uint_as_float(w[j] << 16);
+                o[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) o[j] = __uint_as_float((uint32_t)p[j] << 16);
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t bf16_bits(float x)
+{
+    return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)x);
+}
+
+template <bool F32>
+__device__ __forceinline__ void store4(void *out, int64_t at, bool vec, const float *o)
+{
+    if constexpr (F32) {
+        float *p = (float *)out + at;
+        if (vec) *(v4f *)p = v4f{o[0], o[1], o[2], o[3]};
+        else
+            for (int j = 0; j < 4; j++) p[j] = o[j];
+    } else {
+        uint16_t *p = (uint16_t *)out + at;
+        if (vec)
+            *(uint2 *)p = uint2{bf16_bits(o[0]) | bf16_bits(o[1]) << 16,
+                                bf16_bits(o[2]) | bf16_bits(o[3]) << 16};
+        else
+            for (int j = 0; j < 4; j++) p[j] = (uint16_t)bf16_bits(o[j]);
+    }
+}
+
+// Everything a lane keeps of its row.
+template <int D, bool F32>
+struct Acc {
+    v16f o[D / 32];                     // dims 32f + 8(i/4) + 4h + i%4 of register i
+    float vc[D / 64];                   // f32: sum p*c by group (this half's tokens)
+    float l;                            // sum p (this half's tokens)
+    float m;                            // M
+};
+
+template <int D, bool F32, int WR, int SPW>
+__global__ __launch_bounds__(64 * kWinWaves, 2) void window_kernel(
+    eakvd_geom geo, WinJob job, const void *q, const uint64_t *tree, void *out, float *part,
+    float rsd, int vec)
+{
+    constexpr int GPD = D / 64;
+    constexpr int WT = kWinWaves / WR;
+    constexpr int TS = WT * SPW;                     // sub-tiles of a tile
+    constexpr int UPS = 2 * GPD;                     // units of a sub-tile: GPD of K, GPD of V
+    constexpr int UPW = TS * UPS / kWinWaves;        // units of a wave
+    static_assert(UPW * kWinWaves == TS * UPS, "whole units");
+    constexpr int NB = WR == 1 ? 1 : 2;              // buffers; WR == 1: a wave's own sub-tile
+    typedef SubTile<D, F32> Sub;
+    extern __shared__ __align__(16) uint8_t lds[];
+    Sub *sub = (Sub *)lds;
+
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int wr = w % WR, wt = w / WR;
+    const int n32 = lane & 31, h = lane >> 5;
+
+    // this block's sequence, rows, chunk and kv head; long row blocks first
+    int c = 0;
+    while (c + 1 < job.n_seq && (int)blockIdx.x >= job.pre[c + 1]) c++;
+    int rem = (int)blockIdx.x - job.pre[c];
+    const int kvh = rem % job.n_kv;
+    rem /= job.n_kv;
+    const int mc = job.mc[c], chunk = rem % mc;
+    const int m = job.ntok[c], start = job.start[c], qpk = job.qpk;
+    const int rows = m * qpk;
+    const int n_rb = (rows + 32 * WR - 1) / (32 * WR);
+    const int rb = n_rb - 1 - rem / mc;
+    const int last_row = min(rows, (rb + 1) * 32 * WR) - 1;
+    const int t_end = tree ? start + m : start + last_row / qpk + 1;    // tokens of this block
+    const int lo = chunk * job.clen[c];
+    const int hi = min(t_end, lo + job.clen[c]);
+
+    const int r0 = rb * 32 * WR + wr * 32;           // this wave's first row
+    const bool active = r0 < rows;
+    const int row = min(r0 + n32, rows - 1);
+    const int tok = row / qpk, head = kvh * qpk + row - tok * qpk;
+    const int64_t qrow = ((int64_t)(job.tok0[c] + tok) * job.n_q + head) * D;
+    // tokens that this row, the wave's first row and the wave's last row see
+    const int vis = start + tok + 1;
+    const int vis_min = tree ? start : start + min(r0, rows - 1) / qpk + 1;
+    const int vis_max = tree ? start + m : start + min(r0 + 31, rows - 1) / qpk + 1;
+    const uint64_t word = tree ? tree[job.tok0[c] + tok] : 0;
+
+    // ---- Q operands: (g, octet, nibble) like K's; the row scaled to below 2^15
+    h8 qa[GPD * 4], qb[F32 ? GPD * 4 : 1];
+    b8 qbias;
+    float rf;
+    {
+        float x[GPD * 4][8];
+        float top = 0.0f;
+#pragma unroll
+        for (int g = 0; g < GPD; g++)
+#pragma unroll
+            for (int o = 0; o < 2; o++)
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    float *xx = x[g * 4 + o * 2 + n];
+                    load_q8<F32>(q, qrow + g * 64 + 32 * n + 16 * h + 8 * o, vec, xx);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(xx[j]));
+                }
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        // q' = q * 2^(15 - e); a row of zeros or below 2^-110 keeps e = -110
+        int e = (int)(__float_as_uint(top) >> 23) - 126;
+        e = e < -110 ? -110 : e;
+        float qs[GPD];
+#pragma unroll
+        for (int g = 0; g < GPD; g++) {
+            qs[g] = 0.0f;
+#pragma unroll
+            for (int f = 0; f < 4; f++) {
+                float y[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) y[j] = scale2(x[g * 4 + f][j], 15 - e);
+                qs[g] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+                uint32_t a[4], b[4];
+#pragma unroll
+                for (int p = 0; p < 4; p++) {
+                    // nib2's order of a dword's bytes: 0 and 2, 1 and 3
+                    const int j = (p >> 1) * 4 + (p & 1);
+                    const h2 hi2 = pk(y[j], y[j + 2]);
+                    a[p] = u_of(hi2);
+                    if constexpr (F32)
+                        b[p] = u_of(pk_rest(hi2, y[j], y[j + 2]));
+                }
+                qa[g * 4 + f] = __builtin_bit_cast(h8, uint4{a[0], a[1], a[2], a[3]});
+                if constexpr (F32)
+                    qb[g * 4 + f] = __builtin_bit_cast(h8, uint4{b[0], b[1], b[2], b[3]});
+            }
+            qs[g] += __shfl_xor(qs[g], 32, 64);
+        }
+        rf = scale2(rsd * EAKV_LOG2E, e - 15);
+        {
+            // half h of the bias product's 16 terms: group h's sum of q in
+            // pieces, against K's pieces c1 c1 c1 c2 c2 c3 0 0
+            __bf16 p1, p2, p3;
+            const float z = h < GPD ? qs[h < GPD ? (GPD == 1 ? 0 : h) : 0] : 0.0f;
+            pieces(z, p1, p2, p3);
+            const __bf16 zero = (__bf16)0.0f;
+            qbias = b8{p1, p2, p3, p1, p2, p1, zero, zero};
+        }
+    }
+
+    Acc<D, F32> A;
+#pragma unroll
+    for (int f = 0; f < D / 32; f++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) A.o[f][i] = 0.0f;
+#pragma unroll
+    for (int g = 0; g < GPD; g++) A.vc[g] = 0.0f;
+    A.l = 0.0f;
+    A.m = kMInit;
+
+    const Planes K = planes_of(geo, job.base[c], job.layer, 0);
+    const Planes V = planes_of(geo, job.base[c], job.layer, 1);
+    const int64_t g0 = (int64_t)kvh * geo.gph;
+    const int t_last = t_end - 1;                    // loads stay within the sequence
+
+    // ---- a unit's loads.  K unit g: lane = (token n32, bytes 16h of group g)
+    // with the scales of group h.  V unit u: lane = (column quad, h, 16-token
+    // step, x): four consecutive tokens' dwords; x is the group (d = 128) or
+    // the 4-token half of the operand (d = 64), u the other one.
+    const int cq = lane & 7, vh = (lane >> 3) & 1, vstep = (lane >> 4) & 1, vx = lane >> 5;
+    auto load_unit = [&](int uu, int t0, Raw &r) {
+        const int st = uu / UPS, kind = uu % UPS;
+        const int tb = t0 + 32 * st;
+        if (kind < GPD) {
+            const int64_t t = min(tb + n32, t_last);
+            r.x = *(const uint4 *)(K.w + (g0 + t * GPD + kind) * 32 + 16 * h);
+            const int64_t gi = g0 + t * GPD + (GPD == 2 ? h : 0);
+            r.s[0] = K.s[gi];
+            r.b[0] = K.b[gi];
+        } else {
+            const int u = kind - GPD;
+            const int g = GPD == 2 ? vx : 0, jh = GPD == 2 ? u : vx;
+            const int tq = tb + 16 * vstep + 8 * jh + 4 * vh;
+            uint32_t xx[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int64_t t = min(tq + j, t_last);
+                const int64_t gi = g0 + t * GPD + g;
+                xx[j] = *(const uint32_t *)(V.w + gi * 32 + 4 * cq);
+                r.s[j] = V.s[gi];
+                r.b[j] = V.b[gi];
+            }
+            r.x = uint4{xx[0], xx[1], xx[2], xx[3]};
+        }
+    };
+
+    // ---- a unit's conversion into the sub-tile's operands
+    auto put_unit = [&](int uu, Sub *buf, const Raw &r) {
+        const int st = uu / UPS, kind = uu % UPS;
+        Sub &S = buf[st];
+        if (kind < GPD) {
+            const int g = kind;
+            // lanes of half g (d = 64: all) hold group g's scale and bias
+            float z = zero_nibble(r.s[0], r.b[0]);
+            if (GPD == 1 || h == g) {
+                const float s = r.s[0], cc = fmaf(z, s, r.b[0]);
+                if (GPD == 2 || h == 0) S.ks[g][n32] = s;
+                __bf16 p1, p2, p3;
+                const __bf16 zero = (__bf16)0.0f;
+                pieces(cc, p1, p2, p3);
+                b8 v = b8{p1, p1, p1, p2, p2, p3, zero, zero};
+                if (GPD == 1 && h == 1) v = b8{zero, zero, zero, zero, zero, zero, zero, zero};
+                S.kb[lane] = __builtin_bit_cast(uint4, v);
+            }
+            if (GPD == 2) z = __shfl(z, 32 * g + n32, 64);
+            const h2 off = pk(-z, -z);
+            const uint32_t x[4] = {r.x.x, r.x.y, r.x.z, r.x.w};
+#pragma unroll
+            for (int o = 0; o < 2; o++) {
+                uint32_t a[4], bb[4];
+#pragma unroll
+                for (int d = 0; d < 2; d++) {
+                    const uint32_t x0 = x[2 * o + d], x1 = x0 >> 8;
+                    a[2 * d] = u_of(nib2<false>(x0, off));
+                    a[2 * d + 1] = u_of(nib2<false>(x1, off));
+                    bb[2 * d] = u_of(nib2<true>(x0, off));
+                    bb[2 * d + 1] = u_of(nib2<true>(x1, off));
+                }
+                S.k[g * 4 + o * 2][lane] = uint4{a[0], a[1], a[2], a[3]};
+                S.k[g * 4 + o * 2 + 1][lane] = uint4{bb[0], bb[1], bb[2], bb[3]};
+            }
+        } else {
+            const int u = kind - GPD;
+            const int g = GPD == 2 ? vx : 0, jh = GPD == 2 ? u : vx;
+            h2 s16[2], c16[2];
+            float z[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) z[j] = zero_nibble(r.s[j], r.b[j]);
+            const h2 off[2] = {pk(-z[0], -z[2]), pk(-z[1], -z[3])};
+            if constexpr (F32) {
+                float top = 0.0f;
+                float cc[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    cc[j] = fmaf(z[j], r.s[j], r.b[j]);
+                    const float a = fabsf(r.s[j]);
+                    top = fmaxf(top, a < __builtin_inff() ? a : 0.0f);
+                }
+                top = wave_top(top);
+                const int tq = 16 * vstep + 8 * jh + 4 * vh;
+                if (cq == 0) {
+                    *(float4 *)&S.vs[g][tq] = make_float4(r.s[0], r.s[1], r.s[2], r.s[3]);
+                    *(float4 *)&S.vc[g][tq] = make_float4(cc[0], cc[1], cc[2], cc[3]);
+                }
+                if (lane == 0) {
+                    S.ev[u] = exp_of(top);
+                    if (GPD == 1) S.ev[1] = exp_of(top);
+                }
+            } else {
+                float top = 0.0f;
+                bool fin[4], all = true;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float a = fmaxf(fabsf(r.b[j]), fabsf(fmaf(15.0f, r.s[j], r.b[j])));
+                    fin[j] = a < __builtin_inff() && r.b[j] == r.b[j] && r.s[j] == r.s[j];
+                    all = all && fin[j];
+                    top = fmaxf(top, fin[j] ? a : 0.0f);
+                }
+                const int e = exp_of(wave_top(top));
+                float ss[4], cc[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    ss[j] = scale2(r.s[j], 15 - e);
+                    cc[j] = scale2(fmaf(z[j], r.s[j], r.b[j]), 15 - e);
+                }
+                if (lane == 0) {
+                    S.ev[u] = e;
+                    S.bad[u][0] = S.bad[u][1] = 0;
+                    if (GPD == 1) {
+                        S.ev[1] = e;
+                        S.bad[1][0] = S.bad[1][1] = 0;
+                    }
+                }
+                if (__ballot(!all) != 0) {
+                    // non-finite groups: 0 in the operand, named in `bad`
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        if (!fin[j]) {
+                            ss[j] = 0.0f;
+                            cc[j] = 0.0f;
+                            if (cq == 0)
+                                atomicOr(&S.bad[u][g], 1u << (16 * vstep + 8 * jh + 4 * vh + j));
+                        }
+                    }
+                }
+                s16[0] = pk(ss[0], ss[2]);
+                s16[1] = pk(ss[1], ss[3]);
+                c16[0] = pk(cc[0], cc[2]);
+                c16[1] = pk(cc[1], cc[3]);
+            }
+            // 4x4 byte transpose: y[i] = column 4cq + i of the four tokens
+            const uint32_t x[4] = {r.x.x, r.x.y, r.x.z, r.x.w};
+            const uint32_t a0 = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u);   // 0a 1a 0b 1b
+            const uint32_t a1 = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u);
+            const uint32_t a2 = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u);
+            const uint32_t a3 = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
+            const uint32_t y[4] = {__builtin_amdgcn_perm(a1, a0, 0x05040100u),
+                                   __builtin_amdgcn_perm(a1, a0, 0x07060302u),
+                                   __builtin_amdgcn_perm(a3, a2, 0x05040100u),
+                                   __builtin_amdgcn_perm(a3, a2, 0x07060302u)};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t x0 = y[i], x1 = x0 >> 8;
+                h2 v[4] = {nib2<false>(x0, off[0]), nib2<false>(x1, off[1]),
+                           nib2<true>(x0, off[0]), nib2<true>(x1, off[1])};
+                if constexpr (!F32) {
+#pragma unroll
+                    for (int p = 0; p < 4; p++)
+                        v[p] = __builtin_elementwise_fma(v[p], s16[p & 1], c16[p & 1]);
+                }
+                const int slot = 32 * vh + 4 * cq + i;
+                uint2 *lo2 = (uint2 *)&S.v[g * 4 + 0 + vstep][slot] + jh;
+                uint2 *hi2 = (uint2 *)&S.v[g * 4 + 2 + vstep][slot] + jh;
+                *lo2 = uint2{u_of(v[0]), u_of(v[1])};
+                *hi2 = uint2{u_of(v[2]), u_of(v[3])};
+            }
+        }
+    };
+
+    // ---- one sub-tile's scores, softmax and weighted sum for this wave's rows
+    auto step = [&](const Sub &S, int t0, auto masked) {
+        constexpr bool MASK = decltype(masked)::value;
+        v16f s;
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] = 0.0f;
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, S.kb[lane]), qbias, s, 0, 0,
+                                                    0);
+#pragma unroll
+        for (int g = 0; g < GPD; g++) {
+            v16f acc;
+#pragma unroll
+            for (int i = 0; i < 16; i++) acc[i] = 0.0f;
+#pragma unroll
+            for (int f = 0; f < 4; f++) {
+                const h8 a = __builtin_bit_cast(h8, S.k[g * 4 + f][lane]);
+                if constexpr (F32)
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qb[g * 4 + f], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qa[g * 4 + f], acc, 0, 0, 0);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float4 sc = *(const float4 *)&S.ks[g][8 * k + 4 * h];
+                s[4 * k] = fmaf(sc.x, acc[4 * k], s[4 * k]);
+                s[4 * k + 1] = fmaf(sc.y, acc[4 * k + 1], s[4 * k + 1]);
+                s[4 * k + 2] = fmaf(sc.z, acc[4 * k + 2], s[4 * k + 2]);
+                s[4 * k + 3] = fmaf(sc.w, acc[4 * k + 3], s[4 * k + 3]);
+            }
+        }
+        if constexpr (MASK) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int t = t0 + 8 * (i >> 2) + 4 * h + (i & 3);
+                bool see = t < vis;
+                if (tree) {
+                    const int d = t - start;
+                    see = d < 0 || (d < m && ((word >> (d & 63)) & 1));
+                }
+                s[i] = see ? s[i] : -__builtin_inff();
+            }
+        }
+        const int ev0 = S.ev[0], ev1 = S.ev[1];
+        const int evm = max(ev0, ev1);
+        float top = fmaxf(fmaxf(s[0], s[1]), s[2]);
+#pragma unroll
+        for (int i = 3; i < 16; i++) top = fmaxf(top, s[i]);
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float need = fmaf(top, rf, (float)evm - kWinTop);
+        if (__ballot(need > A.m + kWinTau) != 0) {
+            const float mn = fmaxf(A.m, need);
+            const float al = __builtin_amdgcn_exp2f(A.m - mn);
+            A.m = mn;
+            A.l *= al;
+#pragma unroll
+            for (int f = 0; f < D / 32; f++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) A.o[f][i] *= al;
+            if constexpr (F32)
+#pragma unroll
+                for (int g = 0; g < GPD; g++) A.vc[g] *= al;
+        }
+        if constexpr (F32) {
+            float p[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], rf, -A.m));
+            A.l += ((((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]))) +
+                    (((p[8] + p[9]) + (p[10] + p[11])) + ((p[12] + p[13]) + (p[14] + p[15]))));
+#pragma unroll
+            for (int g = 0; g < GPD; g++) {
+                uint32_t a[8], b[8];
+                float cs = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const float4 sc = *(const float4 *)&S.vs[g][8 * k + 4 * h];
+                    const float4 cc = *(const float4 *)&S.vc[g][8 * k + 4 * h];
+                    float x[4];
+                    if constexpr (MASK) {
+                        x[0] = mul_hidden(p[4 * k], sc.x);
+                        x[1] = mul_hidden(p[4 * k + 1], sc.y);
+                        x[2] = mul_hidden(p[4 * k + 2], sc.z);
+                        x[3] = mul_hidden(p[4 * k + 3], sc.w);
+                        cs += mul_hidden(p[4 * k], cc.x) + mul_hidden(p[4 * k + 1], cc.y);
+                        cs += mul_hidden(p[4 * k + 2], cc.z) + mul_hidden(p[4 * k + 3], cc.w);
+                    } else {
+                        x[0] = p[4 * k] * sc.x;
+                        x[1] = p[4 * k + 1] * sc.y;
+                        x[2] = p[4 * k + 2] * sc.z;
+                        x[3] = p[4 * k + 3] * sc.w;
+                        cs = fmaf(p[4 * k], cc.x, cs);
+                        cs = fmaf(p[4 * k + 1], cc.y, cs);
+                        cs = fmaf(p[4 * k + 2], cc.z, cs);
+                        cs = fmaf(p[4 * k + 3], cc.w, cs);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const h2 hi2 = pk(x[e], x[e + 2]);
+                        a[2 * k + e] = u_of(hi2);
+                        b[2 * k + e] = u_of(pk_rest(hi2, x[e], x[e + 2]));
+                    }
+                }
+                A.vc[g] += cs;
+#pragma unroll
+                for (int ks = 0; ks < 2; ks++) {
+                    const h8 pa = __builtin_bit_cast(h8, uint4{a[4 * ks], a[4 * ks + 1],
+                                                               a[4 * ks + 2], a[4 * ks + 3]});
+                    const h8 pb = __builtin_bit_cast(h8, uint4{b[4 * ks], b[4 * ks + 1],
+                                                               b[4 * ks + 2], b[4 * ks + 3]});
+#pragma unroll
+                    for (int n = 0; n < 2; n++) {
+                        const h8 v = __builtin_bit_cast(h8, S.v[g * 4 + n * 2 + ks][lane]);
+                        A.o[g * 2 + n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                            v, pb, A.o[g * 2 + n], 0, 0, 0);
+                        A.o[g * 2 + n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                            v, pa, A.o[g * 2 + n], 0, 0, 0);
+                    }
+                }
+            }
+        } else {
+            // V's unit jh has an exponent of its own: tokens with (i >> 2) & 1
+            // = jh (d = 64: one for both)
+            const float d0 = (float)ev0 - A.m, d1 = (float)ev1 - A.m;
+            float p[16], sum[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], rf, (i >> 2) & 1 ? d1 : d0));
+                sum[(i >> 2) & 1] += p[i];
+            }
+            A.l += scale2(sum[0], -ev0) + scale2(sum[1], -ev1);
+            uint32_t a[8];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                a[2 * k] = u_of(pk(p[4 * k], p[4 * k + 2]));
+                a[2 * k + 1] = u_of(pk(p[4 * k + 1], p[4 * k + 3]));
+            }
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) {
+                const h8 pa = __builtin_bit_cast(h8, uint4{a[4 * ks], a[4 * ks + 1], a[4 * ks + 2],
+                                                           a[4 * ks + 3]});
+#pragma unroll
+                for (int f = 0; f < D / 32; f++)
+                    A.o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                        __builtin_bit_cast(h8, S.v[(f >> 1) * 4 + (f & 1) * 2 + ks][lane]), pa,
+                        A.o[f], 0, 0, 0);
+            }
+            uint32_t bad[2] = {S.bad[0][0] | S.bad[1][0], S.bad[0][1] | S.bad[1][1]};
+            if (__builtin_amdgcn_readfirstlane(bad[0] | bad[1])) {
+                // rows that see a token with a non-finite V group: NaN there
+                uint32_t seen = 0;
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    seen |= (s[i] != -__builtin_inff() ? 1u : 0u)
+                            << (8 * (i >> 2) + 4 * h + (i & 3));
+                seen |= __shfl_xor(seen, 32, 64);
+#pragma unroll
+                for (int g = 0; g < GPD; g++)
+                    if (seen & bad[g])
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            A.o[2 * g][i] = A.o[2 * g + 1][i] = __builtin_nanf("");
+            }
+        }
+    };
+
+    // ---- tiles of 32 * TS tokens; the next tile's loads are in flight while
+    // one is computed
+    Raw raw[UPW];
+    const int n_tiles = hi > lo ? (hi - lo + 32 * TS - 1) / (32 * TS) : 0;
+    auto load_tile = [&](int i) {
+#pragma unroll
+        for (int k = 0; k < UPW; k++) load_unit(w * UPW + k, lo + 32 * TS * i, raw[k]);
+    };
+    if (n_tiles) load_tile(0);
+    for (int i = 0; i < n_tiles; i++) {
+        Sub *buf = sub + (NB == 2 ? (i & 1) * TS : 0);
+        // WR == 1: the wave's own sub-tile, ordered by its LDS instructions' order
+        if constexpr (WR == 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int k = 0; k < UPW; k++) put_unit(w * UPW + k, buf, raw[k]);
+        if (i + 1 < n_tiles) load_tile(i + 1);
+        if constexpr (WR > 1) __syncthreads();
+        else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const int tb = lo + 32 * TS * i;
+#pragma unroll
+        for (int k = 0; k < SPW; k++) {
+            const int st = WR == 1 ? w : wt * SPW + k;
+            const int t0 = tb + 32 * st;
+            if (!active || t0 >= min(vis_max, hi)) continue;
+            if (t0 + 32 <= vis_min) step(buf[st], t0, std::false_type{});
+            else step(buf[st], t0, std::true_type{});
+        }
+    }
+
+    // ---- both halves of a row's tokens, then the WT waves of these rows
+    float l = A.l + __shfl_xor(A.l, 32, 64);
+    if constexpr (F32) {
+#pragma unroll
+        for (int g = 0; g < GPD; g++) {
+            const float cs = A.vc[g] + __shfl_xor(A.vc[g], 32, 64);
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) A.o[2 * g + n][i] += cs;
+        }
+    } else {
+        // the operands carried 2^15
+#pragma unroll
+        for (int f = 0; f < D / 32; f++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) A.o[f][i] *= 0x1p-15f;
+    }
+    float mm = A.m;
+    if constexpr (WT > 1) {
+        float *xo = (float *)lds;                            // [WT/2][WR][D/2][64]
+        constexpr int OW = D / 2 * 64;                       // floats of one wave's O
+        float *xm = xo + (size_t)(WT / 2) * WR * OW;         // [WT/2][WR][2][64]
+        for (int half = WT / 2; half >= 1; half >>= 1) {
+            __syncthreads();
+            if (wt >= half && wt < 2 * half) {
+                float *po = xo + (size_t)((wt - half) * WR + wr) * OW;
+                float *pm = xm + (size_t)((wt - half) * WR + wr) * 128;
+#pragma unroll
+                for (int f = 0; f < D / 32; f++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) po[(f * 16 + i) * 64 + lane] = A.o[f][i];
+                pm[lane] = mm;
+                pm[64 + lane] = l;
+            }
+            __syncthreads();
+            if (wt < half) {
+                const float *po = xo + (size_t)(wt * WR + wr) * OW;
+                const float *pm = xm + (size_t)(wt * WR + wr) * 128;
+                const float m2 = pm[lane], l2 = pm[64 + lane];
+                const float mn = fmaxf(mm, m2);
+                const float a1 = __builtin_amdgcn_exp2f(mm - mn), a2 = __builtin_amdgcn_exp2f(m2 - mn);
+                mm = mn;
+                l = l * a1 + l2 * a2;
+#pragma unroll
+                for (int f = 0; f < D / 32; f++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        A.o[f][i] = A.o[f][i] * a1 + po[(f * 16 + i) * 64 + lane] * a2;
+            }
+        }
+        if (wt != 0) return;
+    }
+    if (!active || r0 + n32 >= rows) return;
+    if (mc == 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int f = 0; f < D / 32; f++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float o4[4] = {A.o[f][4 * k] * inv, A.o[f][4 * k + 1] * inv,
+                                     A.o[f][4 * k + 2] * inv, A.o[f][4 * k + 3] * inv};
+                store4<F32>(out, qrow + 32 * f + 8 * k + 4 * h, vec, o4);
+            }
+    } else {
+        const int64_t prow = job.part[c] + (int64_t)chunk * m * job.n_q +
+                             (int64_t)tok * job.n_q + head;
+        float *po = part + prow * D;
+        if (l != 0.0f) {
+#pragma unroll
+            for (int f = 0; f < D / 32; f++)
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    *(v4f *)(po + 32 * f + 8 * k + 4 * h) = v4f{A.o[f][4 * k], A.o[f][4 * k + 1],
+                                                                A.o[f][4 * k + 2],
+                                                                A.o[f][4 * k + 3]};
+        }
+        if (h == 0) {
+            float *pm = part + job.part_rows * D + prow * 2;
+            pm[0] = mm;
+            pm[1] = l;
+        }
+    }
+}
+
+// One wave per (window token, q head) of the sequences with chunks: the
+// chunks' (O, M, l) joined.  A chunk without visible tokens has l = 0 and no O.
+template <int D, bool F32>
+__global__ __launch_bounds__(256) void window_merge_kernel(WinJob job, const float *part,
+                                                           void *out, int n_rows)
+{
+    constexpr int E = D / 64;
+    const int r = (int)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (r >= n_rows) return;
+    const int tok = r / job.n_q;
+    int c = 0;
+    while (c + 1 < job.n_seq && tok >= job.tok0[c + 1]) c++;
+    const int mc = job.mc[c];
+    if (mc == 1) return;
+    const int64_t per = (int64_t)job.ntok[c] * job.n_q;
+    const int64_t first = job.part[c] + r - (int64_t)job.tok0[c] * job.n_q;
+    const float *ml = part + job.part_rows * D;
+    float m = kMInit;
+    for (int k = lane; k < mc; k += 64) {
+        const float2 x = *(const float2 *)(ml + (first + k * per) * 2);
+        if (x.y != 0.0f) m = fmaxf(m, x.x);
+    }
+    m = wave_max(m);
+    float l = 0.0f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) o[e] = 0.0f;
+    for (int k = 0; k < mc; k++) {
+        const float2 x = *(const float2 *)(ml + (first + k * per) * 2);
+        if (x.y == 0.0f) continue;
+        const float a = __builtin_amdgcn_exp2f(x.x - m);
+        l = fmaf(a, x.y, l);
+        const float *po = part + (first + k * per) * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = fmaf(a, po[e], o[e]);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const int64_t at = (int64_t)r * D + lane * E + e;
+        if constexpr (F32) ((float *)out)[at] = o[e] * inv;
+        else ((uint16_t *)out)[at] = (uint16_t)bf16_bits(o[e] * inv);
+    }
+}
+
+struct WinPlan {
+    WinJob job;
+    int wr;                 // waves by rows
+    int n_rows;             // window tokens x q heads
+    size_t bytes;           // of partials
+    bool merge;
+};
+
+int tile_of(int wr, int d)
+{
+    const int spw = wr == 8 ? (d == 128 ? 2 : 4) : wr == 4 ? (d == 128 ? 1 : 2) : 1;
+    return 32 * (kWinWaves / wr) * spw;
+}
+
+void win_plan(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv, WinPlan *p)
+{
+    memset(p, 0, sizeof(*p));
+    WinJob &j = p->job;
+    const int qpk = n_q / n_kv;
+    j.n_seq = b->n_seq;
+    j.n_q = n_q;
+    j.n_kv = n_kv;
+    j.qpk = qpk;
+    int64_t most = 0;
+    for (int i = 0; i < b->n_seq; i++)
+        most = (int64_t)b->ntok[i] * qpk > most ? (int64_t)b->ntok[i] * qpk : most;
+    p->wr = most <= 32 ? 1 : most <= 64 ? 2 : most <= 128 ? 4 : 8;
+    const int rbr = 32 * p->wr, tile = tile_of(p->wr, g->head_dim);
+    // tiles of all blocks, were no sequence split
+    int64_t tiles = 0;
+    for (int i = 0; i < b->n_seq; i++) {
+        const int64_t rows = (int64_t)b->ntok[i] * qpk, nrb = (rows + rbr - 1) / rbr;
+        for (int64_t r = 0; r < nrb; r++) {
+            const int64_t last = (rows < (r + 1) * rbr ? rows : (r + 1) * rbr) - 1;
+            // (a tree's rows may all see the whole window; it is short)
+            const int64_t end = (int64_t)b->start[i] +
+                                (b->ntok[i] <= 64 ? b->ntok[i] : last / qpk + 1);
+            tiles += (end + tile - 1) / tile * n_kv;
+        }
+    }
+    const int cus = cu_count();
+    // an even share of the chip, and at least four tiles
+    int64_t share = (tiles + cus - 1) / cus;
+    if (share < 4) share = 4;
+    int64_t part = 0;
+    int tok0 = 0;
+    for (int i = 0; i < b->n_seq; i++) {
+        const int64_t rows = (int64_t)b->ntok[i] * qpk, nrb = (rows + rbr - 1) / rbr;
+        const int64_t n_t = ((int64_t)b->start[i] + b->ntok[i] + tile - 1) / tile;
+        int64_t mc = b->ntok[i] ? (n_t + share - 1) / share : 1;
+        const int64_t per = n_t ? (n_t + mc - 1) / mc : 1;
+        mc = n_t ? (n_t + per - 1) / per : 1;
+        j.base[i] = b->base[i];
+        j.start[i] = b->start[i];
+        j.ntok[i] = b->ntok[i];
+        j.tok0[i] = tok0;
+        j.mc[i] = (int)mc;
+        j.clen[i] = (int)(per * tile);
+        j.pre[i + 1] = j.pre[i] + (int)(nrb * mc * n_kv);
+        j.part[i] = part;
+        if (mc > 1) {
+            part += rows * n_kv * mc;
+            p->merge = true;
+        }
+        tok0 += b->ntok[i];
+    }
+    j.part_rows = part;
+    p->n_rows = tok0 * n_q;
+    p->bytes = (size_t)part * (g->head_dim + 2) * sizeof(float);
+}
+
+template <int D, bool F32, int WR, int SPW>
+int launch(const eakvd_geom *g, const WinPlan &p, const void *q, const uint64_t *tree, void *out,
+           float *part, int vec, hipStream_t st)
+{
+    constexpr int WT = kWinWaves / WR;
+    constexpr size_t tiles = (size_t)WT * SPW * (WR == 1 ? 1 : 2) * sizeof(SubTile<D, F32>);
+    constexpr size_t join = WT > 1 ? (size_t)(WT / 2) * WR * (D / 2 * 64 + 128) * 4 : 0;
+    constexpr size_t bytes = tiles > join ? tiles : join;
+    static_assert(bytes <= 160 * 1024, "LDS");
+    auto *kern = window_kernel<D, F32, WR, SPW>;
+    hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)bytes);
+    if (e != hipSuccess) return (int)e;
+    const float rsd = 1.0f / sqrtf((float)D);
+    hipLaunchKernelGGL(kern, dim3((unsigned)p.job.pre[p.job.n_seq]), dim3(64 * kWinWaves), bytes, st,
+                       *g, p.job, q, tree, out, part, rsd, vec);
+    if (p.merge)
+        hipLaunchKernelGGL((window_merge_kernel<D, F32>), dim3((unsigned)((p.n_rows + 3) / 4)),
+                           dim3(256), 0, st, p.job, part, out, p.n_rows);
+    return (int)hipGetLastError();
+}
+
+template <int D, bool F32>
+int launch_wr(const eakvd_geom *g, const WinPlan &p, const void *q, const uint64_t *tree, void *out,
+              float *part, int vec, hipStream_t st)
+{
+    switch (p.wr) {
+    case 1: return launch<D, F32, 1, 1>(g, p, q, tree, out, part, vec, st);
+    case 2: return launch<D, F32, 2, 1>(g, p, q, tree, out, part, vec, st);
+    case 4: return launch<D, F32, 4, D == 128 ? 1 : 2>(g, p, q, tree, out, part, vec, st);
+    default: return launch<D, F32, 8, D == 128 ? 2 : 4>(g, p, q, tree, out, part, vec, st);
+    }
+}
+
+}  // namespace
+
+extern "C" size_t eakvd_window_work_bytes(const eakvd_geom *g, const eakvd_window *b, int n_q,
+                                          int n_kv)
+{
+    WinPlan p;
+    win_plan(g, b, n_q, n_kv, &p);
+    return p.bytes;
+}
+
+extern "C" int eakvd_window_attend(const eakvd_geom *g, const eakvd_window *b, int layer,
+                                   const void *q, int bf16, int n_q, int n_kv,
+                                   const uint64_t *tree, void *out, void *work, void *stream)
+{
+    WinPlan p;
+    win_plan(g, b, n_q, n_kv, &p);
+    p.job.layer = layer;
+    if (p.job.pre[p.job.n_seq] == 0) return 0;
+    const hipStream_t st = (hipStream_t)stream;
+    // 16-byte loads of q and 16- or 8-byte stores of out
+    const int vec = (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0;
+    float *part = (float *)work;
+    if (g->head_dim == 64)
+        return bf16 ? launch_wr<64, false>(g, p, q, tree, out, part, vec, st)
+                    : launch_wr<64, true>(g, p, q, tree, out, part, vec, st);
+    return bf16 ? launch_wr<128, false>(g, p, q, tree, out, part, vec, st)
+                : launch_wr<128, true>(g, p, q, tree, out, part, vec, st);
+}

@@ -45,6 +45,11 @@ struct eakv_cache {
 int  eakvi_set_error(int code, const char *fmt, ...);
 int  eakvi_hip_fail(int hip_err, const char *what);
 
+/* Argument checks of the attention calls (attention.c): a cache, layer and head
+ * split; caches of one shape and device. */
+int  eakvi_attn_check(const eakv_cache_t *c, int layer, int n_q, int n_kv);
+int  eakvi_same_batch(eakv_cache_t *const *caches, int n, const char *what);
+
 /* Make the cache's device current; returns the previous device via *prev. */
 int  eakvi_enter(const eakv_cache_t *c, int *prev);
 void eakvi_leave(int prev);

@@ -14,7 +14,9 @@
  *     (kernels/fused_attention.ea:190-373) but never wires into its C API;
  *   - plane read-back and an error side channel for the void attention calls;
  *   - dequantization and the integrity check of GPU-resident planes, which the
- *     reference runs on its host planes from its benchmark and CLI.
+ *     reference runs on its host planes from its benchmark and CLI;
+ *   - serving with drafts: attention of several new tokens, the drafts' verification,
+ *     and tokens copied and gathered between caches.
  * Device-pointer calls return when the work is enqueued; results are ready
  * after eakv_cache_sync() or a wait on the stream.  The host-pointer calls
  * of include/eakv.h (and eakv_attention_fused, eakv_cache_read_planes,
@@ -145,6 +147,109 @@ int eakv_attention_fused_batch_device_noalloc(eakv_cache_t *const *caches,
  * [7] virtual kv heads per kv head (groups above 8 q heads). */
 int eakv_attention_fused_plan(eakv_cache_t *const *caches, int n_caches, int n_q_heads,
                               int n_kv_heads, int noalloc, int32_t *plan);
+
+/* Attention of several new tokens of each sequence over its packed cache (drafted
+ * tokens, a piece of a prompt), softmax(q.k/sqrt(d)).v in one launch for n_caches
+ * same-shape caches.  No counterpart in the reference.
+ *   starts     host int32[n_caches], or NULL: each cache's seq_len.  Query i of
+ *              cache c is the token at position starts[c] + i; the window's K and V
+ *              are in the cache (appended, advanced or not).  starts[c] <= seq_len.
+ *   n_tokens   host int32[n_caches]: queries of each cache, 0 or more
+ *   d_q, d_out [sum of n_tokens][n_q_heads][head_dim] on the device, the caches'
+ *              windows one after the other, of type dtype: EAKV_F32 or EAKV_BF16
+ *   d_tree     NULL: query i sees the tokens up to its own.  Else one word for
+ *              each query (device, 8-byte aligned, windows of at most
+ *              EAKV_TREE_MAX tokens): bit j says that it sees token starts[c] + j
+ *              of its window; bits beyond the window are ignored.  Every query sees
+ *              the tokens before starts[c].
+ * A query that sees no token gives zeros.  What a query does not see has no part in
+ * its result, NaN and infinities included.  f32 queries: all sums in f32, results
+ * about 1e-6 off the exact ones; one token per sequence without a tree takes the
+ * launch of eakv_attention_fused_batch_device.  bf16 queries: the matrix products'
+ * operands are rounded to f16 (2^-12 relative), sums in f32, the result to bf16.
+ * A non-finite scale or bias gives NaN in the scores of its token or in its 64 dims.
+ *   d_work     device scratch of the call's own, 16-byte aligned and of at least
+ *              eakv_attention_window_work_bytes() for the same arguments, or NULL:
+ *              caches[0]'s workspace (grown when needed).  Calls that share one and
+ *              overlap in time race.  A call on a stream that records a graph needs
+ *              its own (unless 0 bytes are needed), allocates nothing and waits for
+ *              nothing outside the graph: starts and n_tokens are recorded as they
+ *              are, and the work pending for the caches must be done before a replay.
+ * Streams: as eakv_attention_fused_batch_device. */
+#define EAKV_F32  0
+#define EAKV_BF16 1
+#define EAKV_TREE_MAX 64
+int eakv_attention_window_batch_device(eakv_cache_t *const *caches, int n_caches, int layer,
+                                       const int32_t *starts, const int32_t *n_tokens,
+                                       const void *d_q, int dtype, int n_q_heads,
+                                       int n_kv_heads, const uint64_t *d_tree, void *d_out,
+                                       void *d_work, size_t work_bytes, void *stream);
+/* 0 also for invalid arguments (recorded). */
+size_t eakv_attention_window_work_bytes(eakv_cache_t *const *caches, int n_caches,
+                                        const int32_t *starts, const int32_t *n_tokens,
+                                        int dtype, int n_q_heads, int n_kv_heads);
+
+/* Drafted tokens against the target model's probabilities (speculative sampling),
+ * on the current HIP device and the given stream (NULL: the default stream).  No
+ * counterpart in the reference.  For each of n_seqs sequences, up to n_drafts drafts:
+ *   d_counts   int32[n_seqs], drafts of each (clamped to 0..n_drafts), or NULL: all
+ *   d_tokens   int32[n_seqs][n_drafts]
+ *   d_draft    f32[n_seqs][n_drafts][ld_draft], the distributions that the drafts
+ *              were drawn from, or NULL: drafts without one (weight 1 on the token)
+ *   d_target   f32[n_seqs][n_drafts + 1][ld_target], the target's, the last row of a
+ *              sequence's drafts that of the token after them (row count)
+ *   d_uniform  f32[n_seqs][n_drafts + 1] in [0, 1)
+ * Draft i with token x is kept while d_uniform[s][i] * q_i(x) < p_i(x); a token
+ * outside the vocabulary is not.  d_accepted[s] = a, the number kept before the
+ * first that is not.  d_next[s] is drawn from r = max(p_a - q_a, 0) after a rejection,
+ * from r = p_a when all were kept: the least j with r[0] + .. + r[j] >
+ * d_uniform[s][n_drafts] * sum(r), or the last j with r[j] > 0 where rounding leaves
+ * none.  Where nothing is left of p - q it is drawn from p_a, and -1 where that
+ * holds nothing either; NaN and negative values count as 0.  Products, differences
+ * and sums in f64.  d_work: eakv_verify_drafts_work_bytes() of device scratch,
+ * 8-byte aligned, the call's own.  Asynchronous; may be recorded in a graph. */
+int eakv_verify_drafts_device(int n_seqs, int n_drafts, int vocab, const int32_t *d_counts,
+                              const int32_t *d_tokens, const float *d_draft, int64_t ld_draft,
+                              const float *d_target, int64_t ld_target,
+                              const float *d_uniform, int32_t *d_accepted, int32_t *d_next,
+                              void *d_work, size_t work_bytes, void *stream);
+size_t eakv_verify_drafts_work_bytes(int n_seqs, int n_drafts, int vocab);
+
+/* Tokens moved between caches, every layer, K and V, as they are packed (no
+ * counterpart in the reference).  Caches of one n_layers, n_kv_heads, head_dim (64 or
+ * 128) and device; the destinations share max_seq_len.  Like an append, these calls
+ * do not change seq_len (eakv_cache_advance or eakv_restore does) and write at
+ * most at seq_len.  Sources may lie beyond seq_len (appended, not advanced).  Streams:
+ * as eakv_append_batch_device for every named cache, sources included; not on a
+ * stream that records a graph.
+ * _copy_batch: [src_pos, src_pos + n_tokens) of src to [dst_pos, ...) of each of the
+ * n_dsts destinations (forking a sequence); src itself may be one if the ranges do
+ * not overlap, and none is named twice. */
+int eakv_cache_copy_batch_device(const eakv_cache_t *src, int src_pos,
+                                 eakv_cache_t *const *dsts, int n_dsts, int dst_pos,
+                                 int n_tokens, void *stream);
+/* _gather_batch: token dst_pos[c] + i of dsts[c] becomes token d_index[first + i] of
+ * srcs[c], i < n_tokens[c] (host arrays), the caches' lists one after the other in
+ * d_index (device).  dsts[c] may be srcs[c]; its list must then ascend strictly,
+ * with d_index[first + i] >= dst_pos[c] + i (compaction in place), else the moved
+ * tokens are unspecified.  Positions outside the source's room are clamped to it.  A
+ * destination is no other pair's source or destination; the sources share
+ * max_seq_len too. */
+int eakv_cache_gather_batch_device(eakv_cache_t *const *srcs, eakv_cache_t *const *dsts,
+                                   int n_caches, const int32_t *dst_pos,
+                                   const int32_t *d_index, const int32_t *n_tokens,
+                                   void *stream);
+/* Synchronous forms.  _fork: a new cache with room for max_seq_len tokens that holds
+ * src's first n_tokens; NULL on failure (recorded).  _compact: of the tokens from
+ * start on, only those at keep[0..n_keep) (host, ascending, below seq_len) stay;
+ * seq_len becomes start + n_keep. */
+eakv_cache_t *eakv_cache_fork(const eakv_cache_t *src, int n_tokens, int max_seq_len);
+int eakv_cache_compact(eakv_cache_t *cache, int start, const int32_t *keep, int n_keep);
+
+/* Device addresses of the planes of block (layer, kv_idx): packed codes, scales and
+ * biases in the group order of eakv_dequantize_range_device.  Any may be NULL. */
+int eakv_cache_planes_device(const eakv_cache_t *cache, int layer, int kv_idx,
+                             uint8_t **weights, float **scales, float **biases);
 
 /* Dequantize groups [group_start, group_start + group_count) of the (layer,
  * kv_idx) planes to f32, 64 values per group in group order: value =
