@@ -176,7 +176,9 @@ typedef struct {
     int            ntok[EAKVD_MAX_BATCH];
 } eakvd_window;
 
-size_t eakvd_window_work_bytes(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv);
+#define EAKVD_TREE_MAX 64
+size_t eakvd_window_work_bytes(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv,
+                               int bf16);
 int eakvd_window_attend(const eakvd_geom *g, const eakvd_window *b, int layer, const void *q,
                         int bf16, int n_q, int n_kv, const uint64_t *tree, void *out, void *work,
                         void *stream);

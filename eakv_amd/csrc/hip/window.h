@@ -1,0 +1,294 @@
+// window.h — what the window attention's kernels share (window.hip,
+// window_prompt.hip; the mathematics stands in window.hip).
+#pragma once
+
+#include <type_traits>
+
+#include "common.h"
+
+struct WinJob {
+    int n_seq, n_q, n_kv, qpk, layer;
+    const uint8_t *base[EAKVD_MAX_BATCH];
+    int start[EAKVD_MAX_BATCH];
+    int ntok[EAKVD_MAX_BATCH];
+    int tok0[EAKVD_MAX_BATCH];          // the window's first row of q and out
+    int mc[EAKVD_MAX_BATCH];            // chunks
+    int clen[EAKVD_MAX_BATCH];          // tokens per chunk
+    int pre[EAKVD_MAX_BATCH + 1];       // blocks before this sequence's
+    int lead[EAKVD_MAX_BATCH];          // window tokens of this launch's sequences before it
+    int64_t part[EAKVD_MAX_BATCH];      // first partial row
+    int64_t part_rows;                  // partial rows in all
+    int64_t img[EAKVD_MAX_BATCH];       // expanded sub-tiles before this sequence's
+    int nsub[EAKVD_MAX_BATCH];          // expanded sub-tiles of one kv head
+};
+
+namespace {
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+constexpr float kWinTau = 4.0f;        // headroom of the lazy M, log2 units
+constexpr float kWinTop = 11.0f;       // weights below 2^(kWinTop + kWinTau) = 2^15
+constexpr float kMInit = -3.4028234664e38f;
+constexpr int kExpLow = -60;           // tile exponents below this count as this
+
+
+__device__ __forceinline__ uint32_t u_of(h2 v) { return __builtin_bit_cast(uint32_t, v); }
+__device__ __forceinline__ h2 h_of(uint32_t v) { return __builtin_bit_cast(h2, v); }
+// Two roundings to nearest even.  The empty asm statements (no instruction that
+// the compiler's hazard handling would miss behind a transcendental) hold a and b
+// to f32 and the result to one rounding: the compiler otherwise rounds a product
+// straight to f16 in one place and by way of f32 in another, and a pair's low part
+// must be what the high part left.
+__device__ __forceinline__ h2 pk(float a, float b)
+{
+    asm("" : "+v"(a));
+    asm("" : "+v"(b));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    uint32_t r = u_of(__builtin_convertvector((f2{a, b}), h2));
+    asm("" : "+v"(r));
+    return h_of(r);
+}
+// pk of two transcendentals' results (nothing to fuse with)
+__device__ __forceinline__ h2 pk_exp(float a, float b)
+{
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    return __builtin_convertvector((f2{a, b}), h2);
+}
+// what pk(a, b) left of a and b, exact, in f16
+__device__ __forceinline__ h2 pk_rest(h2 hi, float a, float b)
+{
+    return pk(fmaf((float)hi[0], -1.0f, a), fmaf((float)hi[1], -1.0f, b));
+}
+
+// n - z of the low (HI false) or high nibbles of bytes 0 and 2 of x, exact: the
+// nibble is put into the mantissa of 1024 (its lowest bits) or of 64 (four bits up)
+// and 1024 + z or 64 + z taken off.  off: -z of the two bytes.  9 instructions
+// for 8 nibbles.
+template <bool HI>
+__device__ __forceinline__ h2 nib2(uint32_t x, h2 off)
+{
+    if constexpr (HI)
+        return h_of((x & 0x00f000f0u) | 0x54005400u) + (off - h2{(_Float16)64.0f, (_Float16)64.0f});
+    else
+        return h_of((x & 0x000f000fu) | 0x64006400u) +
+               (off - h2{(_Float16)1024.0f, (_Float16)1024.0f});
+}
+
+// z: the nibble whose value is nearest 0, so that (n - z)*s and c = b + z*s are of
+// the size of the value and cancel nothing (a group with an outlier has b and
+// s far above its other values).
+__device__ __forceinline__ float zero_nibble(float s, float b)
+{
+    const float z = __builtin_rintf(-b * __builtin_amdgcn_rcpf(s));
+    return fminf(fmaxf(z, 0.0f), 15.0f);
+}
+
+__device__ __forceinline__ float wave_top(float v)
+{
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+__device__ __forceinline__ int exp_of(float a)
+{
+    const int e = (int)(__float_as_uint(a) >> 23) - 126;     // a < 2^e
+    return e < kExpLow ? kExpLow : e;
+}
+// x * 2^e, one rounding, for any e
+__device__ __forceinline__ float scale2(float x, int e)
+{
+    return __builtin_amdgcn_ldexpf(x, e);
+}
+
+// p * v, 0 * anything = 0: a hidden token's scale or bias may be non-finite
+__device__ __forceinline__ float mul_hidden(float p, float v)
+{
+    return p == 0.0f ? 0.0f : p * v;
+}
+
+// Three bf16 pieces of x, together 24 bits.
+__device__ __forceinline__ void pieces(float x, __bf16 &a, __bf16 &b, __bf16 &c)
+{
+    a = (__bf16)x;
+    const float r = __fsub_rn(x, (float)a);
+    b = (__bf16)r;
+    c = (__bf16)__fsub_rn(r, (float)b);
+}
+
+// The 8 consecutive dims of one operand (a multiple of 8 dims from the row's
+// start) as f32.  Rows of q are 16-byte aligned or read by elements.
+template <bool F32>
+__device__ __forceinline__ void load_q8(const void *q, int64_t at, bool vec, float *o)
+{
+    if constexpr (F32) {
+        const float *p = (const float *)q + at;
+        if (vec) {
+            const v4f a = *(const v4f *)p, b = *(const v4f *)(p + 4);
+#pragma unroll
+            for (int j = 0; j < 4; j++) { o[j] = a[j]; o[4 + j] = b[j]; }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) o[j] = p[j];
+        }
+    } else {
+        const uint16_t *p = (const uint16_t *)q + at;
+        if (vec) {
+            const uint4 a = *(const uint4 *)p;
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                o[2 * j] = __uint_as_float(w[j] << 16);
+                o[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) o[j] = __uint_as_float((uint32_t)p[j] << 16);
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t bf16_bits(float x)
+{
+    return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)x);
+}
+
+template <bool F32>
+__device__ __forceinline__ void store4(void *out, int64_t at, bool vec, const float *o)
+{
+    if constexpr (F32) {
+        float *p = (float *)out + at;
+        if (vec) *(v4f *)p = v4f{o[0], o[1], o[2], o[3]};
+        else
+            for (int j = 0; j < 4; j++) p[j] = o[j];
+    } else {
+        uint16_t *p = (uint16_t *)out + at;
+        if (vec)
+            *(uint2 *)p = uint2{bf16_bits(o[0]) | bf16_bits(o[1]) << 16,
+                                bf16_bits(o[2]) | bf16_bits(o[3]) << 16};
+        else
+            for (int j = 0; j < 4; j++) p[j] = (uint16_t)bf16_bits(o[j]);
+    }
+}
+
+// A row's query as the columns' operand of S^T = K Q^T, one lane's share: operand
+// (g, octet o, nibble n) of half h holds dims 64g + 32n + 16h + 8o + 0..7 in nib2's
+// order (0 2 1 3 4 6 5 7).  The row is scaled by a power of two to below 2^15.
+template <int D, bool F32>
+struct QOp {
+    h8 a[D / 16];                       // f16, high parts
+    h8 b[F32 ? D / 16 : 1];             // f32 queries: low parts
+    b8 bias;                            // half h: pieces of group h's sum of q
+    float rf;                           // score = dot * rf, log2 units
+};
+
+template <int D, bool F32>
+__device__ __forceinline__ void build_q(QOp<D, F32> &Q, const void *q, int64_t qrow, bool vec,
+                                        float rsd, int h)
+{
+    constexpr int GPD = D / 64;
+    float x[GPD * 4][8];
+    float top = 0.0f;
+#pragma unroll
+    for (int g = 0; g < GPD; g++)
+#pragma unroll
+        for (int o = 0; o < 2; o++)
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                float *xx = x[g * 4 + o * 2 + n];
+                load_q8<F32>(q, qrow + g * 64 + 32 * n + 16 * h + 8 * o, vec, xx);
+#pragma unroll
+                for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(xx[j]));
+            }
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    // q' = q * 2^(15 - e); a row of zeros or below 2^-110 keeps e = -110
+    int e = (int)(__float_as_uint(top) >> 23) - 126;
+    e = e < -110 ? -110 : e;
+    float qs[GPD];
+#pragma unroll
+    for (int g = 0; g < GPD; g++) {
+        qs[g] = 0.0f;
+#pragma unroll
+        for (int f = 0; f < 4; f++) {
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = scale2(x[g * 4 + f][j], 15 - e);
+            qs[g] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+            uint32_t a[4], b[4];
+#pragma unroll
+            for (int p = 0; p < 4; p++) {
+                const int j = (p >> 1) * 4 + (p & 1);
+                const h2 hi2 = pk(y[j], y[j + 2]);
+                a[p] = u_of(hi2);
+                if constexpr (F32) b[p] = u_of(pk_rest(hi2, y[j], y[j + 2]));
+            }
+            Q.a[g * 4 + f] = __builtin_bit_cast(h8, uint4{a[0], a[1], a[2], a[3]});
+            if constexpr (F32)
+                Q.b[g * 4 + f] = __builtin_bit_cast(h8, uint4{b[0], b[1], b[2], b[3]});
+        }
+        qs[g] += __shfl_xor(qs[g], 32, 64);
+    }
+    Q.rf = scale2(rsd * EAKV_LOG2E, e - 15);
+    // half h of the bias product's 16 terms: group h's sum of q in pieces,
+    // against K's pieces c1 c1 c1 c2 c2 c3 0 0
+    __bf16 p1, p2, p3;
+    const float z = GPD == 2 ? (h ? qs[GPD - 1] : qs[0]) : (h ? 0.0f : qs[0]);
+    pieces(z, p1, p2, p3);
+    const __bf16 zero = (__bf16)0.0f;
+    Q.bias = b8{p1, p2, p3, p1, p2, p1, zero, zero};
+}
+
+// The maximum of a lane's value and the other half's (lane ^ 32), in both.
+__device__ __forceinline__ float half_max(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// What a lane writes of its row: final outputs (mc == 1) or the chunk's partial.
+// o[f][i]: dim 32f + 8(i/4) + 4h + i%4.
+template <int D, bool F32>
+__device__ __forceinline__ void put_row(const v16f *o, float l, float m, const WinJob &job, int c,
+                                        int chunk, int tok, int head, int h, int64_t qrow,
+                                        bool vec, void *out, float *part)
+{
+    if (job.mc[c] == 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int f = 0; f < D / 32; f++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float o4[4] = {o[f][4 * k] * inv, o[f][4 * k + 1] * inv, o[f][4 * k + 2] * inv,
+                                     o[f][4 * k + 3] * inv};
+                store4<F32>(out, qrow + 32 * f + 8 * k + 4 * h, vec, o4);
+            }
+        return;
+    }
+    const int64_t prow = job.part[c] + (int64_t)chunk * job.ntok[c] * job.n_q +
+                         (int64_t)tok * job.n_q + head;
+    float *po = part + prow * D;
+    if (l != 0.0f) {
+#pragma unroll
+        for (int f = 0; f < D / 32; f++)
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                *(v4f *)(po + 32 * f + 8 * k + 4 * h) =
+                    v4f{o[f][4 * k], o[f][4 * k + 1], o[f][4 * k + 2], o[f][4 * k + 3]};
+    }
+    if (h == 0) {
+        float *pm = part + job.part_rows * D + prow * 2;
+        pm[0] = m;
+        pm[1] = l;
+    }
+}
+
+}  // namespace
+
+// Expands K and V of the sequences' kv heads into `img` and attends
+// (window_prompt.hip).  img: win_prompt_bytes() of device scratch; job.img: each
+// sequence's first sub-tile there.
+size_t win_prompt_bytes(int head_dim, bool bf16, int64_t subtiles);
+int win_prompt(const eakvd_geom &g, const WinJob &job, int64_t subtiles, bool bf16, const void *q,
+               void *out, float *part, uint8_t *img, bool vec, hipStream_t st);

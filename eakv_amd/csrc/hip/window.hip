@@ -36,33 +36,11 @@
 // launch.  No atomics: results are the same bits on every call.
 #include <string.h>
 
-#include "common.h"
+#include "window.h"
 
 namespace {
 
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-typedef float v16f __attribute__((ext_vector_type(16)));
-
 constexpr int kWinWaves = 8;           // waves of a block: two per SIMD
-constexpr float kWinTau = 4.0f;        // headroom of the lazy M, log2 units
-constexpr float kWinTop = 11.0f;       // weights below 2^(kWinTop + kWinTau) = 2^15
-constexpr float kMInit = -3.4028234664e38f;
-constexpr int kExpLow = -60;           // tile exponents below this count as this
-
-struct WinJob {
-    int n_seq, n_q, n_kv, qpk, layer;
-    const uint8_t *base[EAKVD_MAX_BATCH];
-    int start[EAKVD_MAX_BATCH];
-    int ntok[EAKVD_MAX_BATCH];
-    int tok0[EAKVD_MAX_BATCH];          // the window's first row of q and out
-    int mc[EAKVD_MAX_BATCH];            // chunks
-    int clen[EAKVD_MAX_BATCH];          // tokens per chunk
-    int pre[EAKVD_MAX_BATCH + 1];       // blocks before this sequence's
-    int64_t part[EAKVD_MAX_BATCH];      // first partial row
-    int64_t part_rows;                  // partial rows in all
-};
 
 // LDS of one 32-token sub-tile.
 template <int D, bool F32>
@@ -84,138 +62,6 @@ struct Raw {
     uint4 x;
     float s[4], b[4];
 };
-
-__device__ __forceinline__ uint32_t u_of(h2 v) { return __builtin_bit_cast(uint32_t, v); }
-__device__ __forceinline__ h2 h_of(uint32_t v) { return __builtin_bit_cast(h2, v); }
-// Two roundings to nearest even.  The empty asm statements (no instruction that
-// the compiler's hazard handling would miss behind a transcendental) hold a and b
-// to f32 and the result to one rounding: the compiler otherwise rounds a product
-// straight to f16 in one place and by way of f32 in another, and a pair's low part
-// must be what the high part left.
-__device__ __forceinline__ h2 pk(float a, float b)
-{
-    asm("" : "+v"(a));
-    asm("" : "+v"(b));
-    typedef float f2 __attribute__((ext_vector_type(2)));
-    uint32_t r = u_of(__builtin_convertvector((f2{a, b}), h2));
-    asm("" : "+v"(r));
-    return h_of(r);
-}
-// what pk(a, b) left of a and b, exact, in f16
-__device__ __forceinline__ h2 pk_rest(h2 hi, float a, float b)
-{
-    return pk(fmaf((float)hi[0], -1.0f, a), fmaf((float)hi[1], -1.0f, b));
-}
-
-// n - z of the low (HI false) or high nibbles of bytes 0 and 2 of x, exact: the
-// nibble is put into the mantissa of 1024 (its lowest bits) or of 64 (four bits up)
-// and 1024 + z or 64 + z taken off.  off: -z of the two bytes.  9 instructions
-// for 8 nibbles.
-template <bool HI>
-__device__ __forceinline__ h2 nib2(uint32_t x, h2 off)
-{
-    if constexpr (HI)
-        return h_of((x & 0x00f000f0u) | 0x54005400u) + (off - h2{(_Float16)64.0f, (_Float16)64.0f});
-    else
-        return h_of((x & 0x000f000fu) | 0x64006400u) +
-               (off - h2{(_Float16)1024.0f, (_Float16)1024.0f});
-}
-
-// z: the nibble whose value is nearest 0, so that (n - z)*s and c = b + z*s are of
-// the size of the value and cancel nothing (a group with an outlier has b and
-// s far above its other values).
-__device__ __forceinline__ float zero_nibble(float s, float b)
-{
-    const float z = __builtin_rintf(-b * __builtin_amdgcn_rcpf(s));
-    return fminf(fmaxf(z, 0.0f), 15.0f);
-}
-
-__device__ __forceinline__ float wave_top(float v)
-{
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
-}
-__device__ __forceinline__ int exp_of(float a)
-{
-    const int e = (int)(__float_as_uint(a) >> 23) - 126;     // a < 2^e
-    return e < kExpLow ? kExpLow : e;
-}
-// x * 2^e, one rounding, for any e
-__device__ __forceinline__ float scale2(float x, int e)
-{
-    return __builtin_amdgcn_ldexpf(x, e);
-}
-
-// p * v, 0 * anything = 0: a hidden token's scale or bias may be non-finite
-__device__ __forceinline__ float mul_hidden(float p, float v)
-{
-    return p == 0.0f ? 0.0f : p * v;
-}
-
-// Three bf16 pieces of x, together 24 bits.
-__device__ __forceinline__ void pieces(float x, __bf16 &a, __bf16 &b, __bf16 &c)
-{
-    a = (__bf16)x;
-    const float r = __fsub_rn(x, (float)a);
-    b = (__bf16)r;
-    c = (__bf16)__fsub_rn(r, (float)b);
-}
-
-// The 8 consecutive dims of one operand (a multiple of 8 dims from the row's
-// start) as f32.  Rows of q are 16-byte aligned or read by elements.
-template <bool F32>
-__device__ __forceinline__ void load_q8(const void *q, int64_t at, bool vec, float *o)
-{
-    if constexpr (F32) {
-        const float *p = (const float *)q + at;
-        if (vec) {
-            const v4f a = *(const v4f *)p, b = *(const v4f *)(p + 4);
-#pragma unroll
-            for (int j = 0; j < 4; j++) { o[j] = a[j]; o[4 + j] = b[j]; }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) o[j] = p[j];
-        }
-    } else {
-        const uint16_t *p = (const uint16_t *)q + at;
-        if (vec) {
-            const uint4 a = *(const uint4 *)p;
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                o[2 * j] = __uint_as_float(w[j] << 16);
-                o[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) o[j] = __uint_as_float((uint32_t)p[j] << 16);
-        }
-    }
-}
-
-__device__ __forceinline__ uint32_t bf16_bits(float x)
-{
-    return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)x);
-}
-
-template <bool F32>
-__device__ __forceinline__ void store4(void *out, int64_t at, bool vec, const float *o)
-{
-    if constexpr (F32) {
-        float *p = (float *)out + at;
-        if (vec) *(v4f *)p = v4f{o[0], o[1], o[2], o[3]};
-        else
-            for (int j = 0; j < 4; j++) p[j] = o[j];
-    } else {
-        uint16_t *p = (uint16_t *)out + at;
-        if (vec)
-            *(uint2 *)p = uint2{bf16_bits(o[0]) | bf16_bits(o[1]) << 16,
-                                bf16_bits(o[2]) | bf16_bits(o[3]) << 16};
-        else
-            for (int j = 0; j < 4; j++) p[j] = (uint16_t)bf16_bits(o[j]);
-    }
-}
 
 // Everything a lane keeps of its row.
 template <int D, bool F32>
@@ -273,65 +119,9 @@ __global__ __launch_bounds__(64 * kWinWaves, 2) void window_kernel(
     const int vis_max = tree ? start + m : start + min(r0 + 31, rows - 1) / qpk + 1;
     const uint64_t word = tree ? tree[job.tok0[c] + tok] : 0;
 
-    // ---- Q operands: (g, octet, nibble) like K's; the row scaled to below 2^15
-    h8 qa[GPD * 4], qb[F32 ? GPD * 4 : 1];
-    b8 qbias;
-    float rf;
-    {
-        float x[GPD * 4][8];
-        float top = 0.0f;
-#pragma unroll
-        for (int g = 0; g < GPD; g++)
-#pragma unroll
-            for (int o = 0; o < 2; o++)
-#pragma unroll
-                for (int n = 0; n < 2; n++) {
-                    float *xx = x[g * 4 + o * 2 + n];
-                    load_q8<F32>(q, qrow + g * 64 + 32 * n + 16 * h + 8 * o, vec, xx);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(xx[j]));
-                }
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        // q' = q * 2^(15 - e); a row of zeros or below 2^-110 keeps e = -110
-        int e = (int)(__float_as_uint(top) >> 23) - 126;
-        e = e < -110 ? -110 : e;
-        float qs[GPD];
-#pragma unroll
-        for (int g = 0; g < GPD; g++) {
-            qs[g] = 0.0f;
-#pragma unroll
-            for (int f = 0; f < 4; f++) {
-                float y[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) y[j] = scale2(x[g * 4 + f][j], 15 - e);
-                qs[g] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
-                uint32_t a[4], b[4];
-#pragma unroll
-                for (int p = 0; p < 4; p++) {
-                    // nib2's order of a dword's bytes: 0 and 2, 1 and 3
-                    const int j = (p >> 1) * 4 + (p & 1);
-                    const h2 hi2 = pk(y[j], y[j + 2]);
-                    a[p] = u_of(hi2);
-                    if constexpr (F32)
-                        b[p] = u_of(pk_rest(hi2, y[j], y[j + 2]));
-                }
-                qa[g * 4 + f] = __builtin_bit_cast(h8, uint4{a[0], a[1], a[2], a[3]});
-                if constexpr (F32)
-                    qb[g * 4 + f] = __builtin_bit_cast(h8, uint4{b[0], b[1], b[2], b[3]});
-            }
-            qs[g] += __shfl_xor(qs[g], 32, 64);
-        }
-        rf = scale2(rsd * EAKV_LOG2E, e - 15);
-        {
-            // half h of the bias product's 16 terms: group h's sum of q in
-            // pieces, against K's pieces c1 c1 c1 c2 c2 c3 0 0
-            __bf16 p1, p2, p3;
-            const float z = h < GPD ? qs[h < GPD ? (GPD == 1 ? 0 : h) : 0] : 0.0f;
-            pieces(z, p1, p2, p3);
-            const __bf16 zero = (__bf16)0.0f;
-            qbias = b8{p1, p2, p3, p1, p2, p1, zero, zero};
-        }
-    }
+    QOp<D, F32> Q;
+    build_q<D, F32>(Q, q, qrow, vec, rsd, h);
+    const float rf = Q.rf;
 
     Acc<D, F32> A;
 #pragma unroll
@@ -518,7 +308,7 @@ __global__ __launch_bounds__(64 * kWinWaves, 2) void window_kernel(
         v16f s;
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = 0.0f;
-        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, S.kb[lane]), qbias, s, 0, 0,
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, S.kb[lane]), Q.bias, s, 0, 0,
                                                     0);
 #pragma unroll
         for (int g = 0; g < GPD; g++) {
@@ -529,8 +319,8 @@ __global__ __launch_bounds__(64 * kWinWaves, 2) void window_kernel(
             for (int f = 0; f < 4; f++) {
                 const h8 a = __builtin_bit_cast(h8, S.k[g * 4 + f][lane]);
                 if constexpr (F32)
-                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qb[g * 4 + f], acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qa[g * 4 + f], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, Q.b[g * 4 + f], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, Q.a[g * 4 + f], acc, 0, 0, 0);
             }
 #pragma unroll
             for (int k = 0; k < 4; k++) {
@@ -558,7 +348,7 @@ __global__ __launch_bounds__(64 * kWinWaves, 2) void window_kernel(
         float top = fmaxf(fmaxf(s[0], s[1]), s[2]);
 #pragma unroll
         for (int i = 3; i < 16; i++) top = fmaxf(top, s[i]);
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        top = half_max(top);
         const float need = fmaf(top, rf, (float)evm - kWinTop);
         if (__ballot(need > A.m + kWinTau) != 0) {
             const float mn = fmaxf(A.m, need);
@@ -643,8 +433,8 @@ __global__ __launch_bounds__(64 * kWinWaves, 2) void window_kernel(
             uint32_t a[8];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                a[2 * k] = u_of(pk(p[4 * k], p[4 * k + 2]));
-                a[2 * k + 1] = u_of(pk(p[4 * k + 1], p[4 * k + 3]));
+                a[2 * k] = u_of(pk_exp(p[4 * k], p[4 * k + 2]));
+                a[2 * k + 1] = u_of(pk_exp(p[4 * k + 1], p[4 * k + 3]));
             }
 #pragma unroll
             for (int ks = 0; ks < 2; ks++) {
@@ -758,35 +548,7 @@ __global__ __launch_bounds__(64 * kWinWaves, 2) void window_kernel(
         if (wt != 0) return;
     }
     if (!active || r0 + n32 >= rows) return;
-    if (mc == 1) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-        for (int f = 0; f < D / 32; f++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const float o4[4] = {A.o[f][4 * k] * inv, A.o[f][4 * k + 1] * inv,
-                                     A.o[f][4 * k + 2] * inv, A.o[f][4 * k + 3] * inv};
-                store4<F32>(out, qrow + 32 * f + 8 * k + 4 * h, vec, o4);
-            }
-    } else {
-        const int64_t prow = job.part[c] + (int64_t)chunk * m * job.n_q +
-                             (int64_t)tok * job.n_q + head;
-        float *po = part + prow * D;
-        if (l != 0.0f) {
-#pragma unroll
-            for (int f = 0; f < D / 32; f++)
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-                    *(v4f *)(po + 32 * f + 8 * k + 4 * h) = v4f{A.o[f][4 * k], A.o[f][4 * k + 1],
-                                                                A.o[f][4 * k + 2],
-                                                                A.o[f][4 * k + 3]};
-        }
-        if (h == 0) {
-            float *pm = part + job.part_rows * D + prow * 2;
-            pm[0] = mm;
-            pm[1] = l;
-        }
-    }
+    put_row<D, F32>(A.o, l, mm, job, c, chunk, tok, head, h, qrow, vec, out, part);
 }
 
 // One wave per (window token, q head) of the sequences with chunks: the
@@ -801,11 +563,12 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WinJob job, const flo
     if (r >= n_rows) return;
     const int tok = r / job.n_q;
     int c = 0;
-    while (c + 1 < job.n_seq && tok >= job.tok0[c + 1]) c++;
+    while (c + 1 < job.n_seq && tok >= job.lead[c + 1]) c++;
     const int mc = job.mc[c];
     if (mc == 1) return;
     const int64_t per = (int64_t)job.ntok[c] * job.n_q;
-    const int64_t first = job.part[c] + r - (int64_t)job.tok0[c] * job.n_q;
+    const int64_t local = r - (int64_t)job.lead[c] * job.n_q;
+    const int64_t first = job.part[c] + local;
     const float *ml = part + job.part_rows * D;
     float m = kMInit;
     for (int k = lane; k < mc; k += 64) {
@@ -828,19 +591,28 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WinJob job, const flo
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int e = 0; e < E; e++) {
-        const int64_t at = (int64_t)r * D + lane * E + e;
+        const int64_t at = ((int64_t)job.tok0[c] * job.n_q + local) * D + lane * E + e;
         if constexpr (F32) ((float *)out)[at] = o[e] * inv;
         else ((uint16_t *)out)[at] = (uint16_t)bf16_bits(o[e] * inv);
     }
 }
 
-struct WinPlan {
+// The sequences of one launch: those of few rows (window_kernel) or of many
+// (win_prompt).
+struct WinPart {
     WinJob job;
-    int wr;                 // waves by rows
-    int n_rows;             // window tokens x q heads
-    size_t bytes;           // of partials
+    int wr;                 // window_kernel: waves by rows
+    int n_tok;              // window tokens of its sequences
+    int64_t subtiles;       // win_prompt: expanded
+    size_t part_bytes, bytes;
     bool merge;
 };
+
+struct WinPlan {
+    WinPart few, many;
+};
+
+size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 int tile_of(int wr, int d)
 {
@@ -848,48 +620,105 @@ int tile_of(int wr, int d)
     return 32 * (kWinWaves / wr) * spw;
 }
 
-void win_plan(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv, WinPlan *p)
+// Whether a window's K and V are expanded first (never a tree's): where several
+// blocks of 256 rows share them.  Expanded against not, 32Q/8KV d128: bf16 256 tokens
+// at 30000 192 against 226 us, at 2000 39 against 41, 100 tokens (400 rows) at 30000
+// 123 against 130, at 2000 34.6 against 33.1; f32 1000 tokens 71 against 79, but 256
+// at 30000 440 against 363 (the products there are twice as many, so conversions
+// weigh less).
+bool is_many(int ntok, int qpk, bool bf16)
+{
+    return ntok > EAKVD_TREE_MAX && (int64_t)ntok * qpk > (bf16 ? 256 : 2048);
+}
+
+// Tiles of a chunk, window_kernel: an even share of the chip, and at least four.
+int64_t few_share(int64_t tiles, int cus)
+{
+    const int64_t s = (tiles + cus - 1) / cus;
+    return s < 4 ? 4 : s;
+}
+
+// Tiles of a chunk, win_prompt: the split of the longest context in k that ends first,
+// by a model of a launch in tile times (256 rows x 32 tokens: about 1.05 us at d = 128
+// in bf16, 1.6 in f32).  Blocks beyond the chip's slots run as slots come free, the
+// longest first; partials are written and read at about 5 TB/s, the merge is
+// a launch of its own.
+int64_t many_share(const WinJob &j, int64_t tiles, int cus, int head_dim, bool bf16)
+{
+    int64_t longest = 1, blocks = 0, rows = 0;
+    for (int i = 0; i < j.n_seq; i++) {
+        const int64_t n_t = ((int64_t)j.start[i] + j.ntok[i] + 31) / 32;
+        const int64_t r = (int64_t)j.ntok[i] * j.qpk;
+        longest = n_t > longest ? n_t : longest;
+        blocks += (r + 255) / 256 * j.n_kv;
+        rows += r * j.n_kv;
+    }
+    const double tile_us = (bf16 ? 1.05 : 1.6) * head_dim / 128;
+    const double merge_k = 2.0 * rows * (head_dim + 2) * 4 / 5e6 / tile_us, merge_0 = 6 / tile_us;
+    double best = 0;
+    int64_t share = longest;
+    for (int k = 1; k <= 64 && (k == 1 || longest / k >= 8); k = k < 4 ? k + 1 : k + k / 2) {
+        const int64_t part = (longest + k - 1) / k;
+        double t = part;
+        if (blocks * k > cus) {
+            const double even = (double)tiles / cus + 0.5 * part;
+            t = even > t ? even : t;
+        }
+        if (k > 1) t += merge_0 + merge_k * k;
+        if (k == 1 || t < best) {
+            best = t;
+            share = part;
+        }
+    }
+    return share;
+}
+
+void plan_part(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv, bool bf16, bool many,
+               WinPart *p)
 {
     memset(p, 0, sizeof(*p));
     WinJob &j = p->job;
     const int qpk = n_q / n_kv;
-    j.n_seq = b->n_seq;
     j.n_q = n_q;
     j.n_kv = n_kv;
     j.qpk = qpk;
     int64_t most = 0;
-    for (int i = 0; i < b->n_seq; i++)
-        most = (int64_t)b->ntok[i] * qpk > most ? (int64_t)b->ntok[i] * qpk : most;
+    int tok0 = 0;
+    for (int i = 0; i < b->n_seq; i++) {
+        if (b->ntok[i] && is_many(b->ntok[i], qpk, bf16) == many) {
+            const int k = j.n_seq++;
+            const int64_t rows = (int64_t)b->ntok[i] * qpk;
+            most = rows > most ? rows : most;
+            j.base[k] = b->base[i];
+            j.start[k] = b->start[i];
+            j.ntok[k] = b->ntok[i];
+            j.tok0[k] = tok0;
+        }
+        tok0 += b->ntok[i];
+    }
     p->wr = most <= 32 ? 1 : most <= 64 ? 2 : most <= 128 ? 4 : 8;
-    const int rbr = 32 * p->wr, tile = tile_of(p->wr, g->head_dim);
+    const int rbr = many ? 256 : 32 * p->wr, tile = many ? 32 : tile_of(p->wr, g->head_dim);
     // tiles of all blocks, were no sequence split
     int64_t tiles = 0;
-    for (int i = 0; i < b->n_seq; i++) {
-        const int64_t rows = (int64_t)b->ntok[i] * qpk, nrb = (rows + rbr - 1) / rbr;
+    for (int i = 0; i < j.n_seq; i++) {
+        const int64_t rows = (int64_t)j.ntok[i] * qpk, nrb = (rows + rbr - 1) / rbr;
         for (int64_t r = 0; r < nrb; r++) {
             const int64_t last = (rows < (r + 1) * rbr ? rows : (r + 1) * rbr) - 1;
             // (a tree's rows may all see the whole window; it is short)
-            const int64_t end = (int64_t)b->start[i] +
-                                (b->ntok[i] <= 64 ? b->ntok[i] : last / qpk + 1);
+            const int64_t end = (int64_t)j.start[i] + (many ? last / qpk + 1 : j.ntok[i]);
             tiles += (end + tile - 1) / tile * n_kv;
         }
     }
     const int cus = cu_count();
-    // an even share of the chip, and at least four tiles
-    int64_t share = (tiles + cus - 1) / cus;
-    if (share < 4) share = 4;
+    const int64_t share = many ? many_share(j, tiles, cus, g->head_dim, bf16)
+                               : few_share(tiles, cus);
     int64_t part = 0;
-    int tok0 = 0;
-    for (int i = 0; i < b->n_seq; i++) {
-        const int64_t rows = (int64_t)b->ntok[i] * qpk, nrb = (rows + rbr - 1) / rbr;
-        const int64_t n_t = ((int64_t)b->start[i] + b->ntok[i] + tile - 1) / tile;
-        int64_t mc = b->ntok[i] ? (n_t + share - 1) / share : 1;
-        const int64_t per = n_t ? (n_t + mc - 1) / mc : 1;
-        mc = n_t ? (n_t + per - 1) / per : 1;
-        j.base[i] = b->base[i];
-        j.start[i] = b->start[i];
-        j.ntok[i] = b->ntok[i];
-        j.tok0[i] = tok0;
+    for (int i = 0; i < j.n_seq; i++) {
+        const int64_t rows = (int64_t)j.ntok[i] * qpk, nrb = (rows + rbr - 1) / rbr;
+        const int64_t n_t = ((int64_t)j.start[i] + j.ntok[i] + tile - 1) / tile;
+        int64_t mc = (n_t + share - 1) / share;
+        const int64_t per = (n_t + mc - 1) / mc;
+        mc = (n_t + per - 1) / per;
         j.mc[i] = (int)mc;
         j.clen[i] = (int)(per * tile);
         j.pre[i + 1] = j.pre[i] + (int)(nrb * mc * n_kv);
@@ -898,15 +727,39 @@ void win_plan(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv, Win
             part += rows * n_kv * mc;
             p->merge = true;
         }
-        tok0 += b->ntok[i];
+        j.lead[i] = p->n_tok;
+        p->n_tok += j.ntok[i];
+        j.nsub[i] = (j.start[i] + j.ntok[i] + 31) / 32;
+        j.img[i] = p->subtiles;
+        p->subtiles += (int64_t)j.nsub[i] * n_kv;
     }
     j.part_rows = part;
-    p->n_rows = tok0 * n_q;
-    p->bytes = (size_t)part * (g->head_dim + 2) * sizeof(float);
+    p->part_bytes = align256((size_t)part * (g->head_dim + 2) * sizeof(float));
+    p->bytes = p->part_bytes;
+    if (many && j.n_seq) p->bytes += align256(win_prompt_bytes(g->head_dim, bf16, p->subtiles));
+}
+
+void win_plan(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv, bool bf16, WinPlan *p)
+{
+    plan_part(g, b, n_q, n_kv, bf16, false, &p->few);
+    plan_part(g, b, n_q, n_kv, bf16, true, &p->many);
+}
+
+int merge(const eakvd_geom *g, const WinPart &p, bool bf16, const float *part, void *out,
+          hipStream_t st)
+{
+    if (!p.merge) return 0;
+    const int n_rows = p.n_tok * p.job.n_q;
+    auto *kern = g->head_dim == 64
+                     ? (bf16 ? window_merge_kernel<64, false> : window_merge_kernel<64, true>)
+                     : (bf16 ? window_merge_kernel<128, false> : window_merge_kernel<128, true>);
+    hipLaunchKernelGGL(kern, dim3((unsigned)((n_rows + 3) / 4)), dim3(256), 0, st, p.job, part, out,
+                       n_rows);
+    return (int)hipGetLastError();
 }
 
 template <int D, bool F32, int WR, int SPW>
-int launch(const eakvd_geom *g, const WinPlan &p, const void *q, const uint64_t *tree, void *out,
+int launch(const eakvd_geom *g, const WinPart &p, const void *q, const uint64_t *tree, void *out,
            float *part, int vec, hipStream_t st)
 {
     constexpr int WT = kWinWaves / WR;
@@ -921,14 +774,11 @@ int launch(const eakvd_geom *g, const WinPlan &p, const void *q, const uint64_t 
     const float rsd = 1.0f / sqrtf((float)D);
     hipLaunchKernelGGL(kern, dim3((unsigned)p.job.pre[p.job.n_seq]), dim3(64 * kWinWaves), bytes, st,
                        *g, p.job, q, tree, out, part, rsd, vec);
-    if (p.merge)
-        hipLaunchKernelGGL((window_merge_kernel<D, F32>), dim3((unsigned)((p.n_rows + 3) / 4)),
-                           dim3(256), 0, st, p.job, part, out, p.n_rows);
     return (int)hipGetLastError();
 }
 
 template <int D, bool F32>
-int launch_wr(const eakvd_geom *g, const WinPlan &p, const void *q, const uint64_t *tree, void *out,
+int launch_wr(const eakvd_geom *g, const WinPart &p, const void *q, const uint64_t *tree, void *out,
               float *part, int vec, hipStream_t st)
 {
     switch (p.wr) {
@@ -942,11 +792,11 @@ int launch_wr(const eakvd_geom *g, const WinPlan &p, const void *q, const uint64
 }  // namespace
 
 extern "C" size_t eakvd_window_work_bytes(const eakvd_geom *g, const eakvd_window *b, int n_q,
-                                          int n_kv)
+                                          int n_kv, int bf16)
 {
     WinPlan p;
-    win_plan(g, b, n_q, n_kv, &p);
-    return p.bytes;
+    win_plan(g, b, n_q, n_kv, bf16, &p);
+    return p.few.bytes + p.many.bytes;
 }
 
 extern "C" int eakvd_window_attend(const eakvd_geom *g, const eakvd_window *b, int layer,
@@ -954,16 +804,28 @@ extern "C" int eakvd_window_attend(const eakvd_geom *g, const eakvd_window *b, i
                                    const uint64_t *tree, void *out, void *work, void *stream)
 {
     WinPlan p;
-    win_plan(g, b, n_q, n_kv, &p);
-    p.job.layer = layer;
-    if (p.job.pre[p.job.n_seq] == 0) return 0;
+    win_plan(g, b, n_q, n_kv, bf16, &p);
+    p.few.job.layer = p.many.job.layer = layer;
     const hipStream_t st = (hipStream_t)stream;
     // 16-byte loads of q and 16- or 8-byte stores of out
     const int vec = (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0;
-    float *part = (float *)work;
-    if (g->head_dim == 64)
-        return bf16 ? launch_wr<64, false>(g, p, q, tree, out, part, vec, st)
-                    : launch_wr<64, true>(g, p, q, tree, out, part, vec, st);
-    return bf16 ? launch_wr<128, false>(g, p, q, tree, out, part, vec, st)
-                : launch_wr<128, true>(g, p, q, tree, out, part, vec, st);
+    uint8_t *w = (uint8_t *)work;
+    int e = 0;
+    if (p.many.job.n_seq) {
+        e = win_prompt(*g, p.many.job, p.many.subtiles, bf16, q, out, (float *)w,
+                       w + p.many.part_bytes, vec, st);
+        if (!e) e = merge(g, p.many, bf16, (const float *)w, out, st);
+        w += p.many.bytes;
+    }
+    if (!e && p.few.job.n_seq) {
+        float *part = (float *)w;
+        if (g->head_dim == 64)
+            e = bf16 ? launch_wr<64, false>(g, p.few, q, tree, out, part, vec, st)
+                     : launch_wr<64, true>(g, p.few, q, tree, out, part, vec, st);
+        else
+            e = bf16 ? launch_wr<128, false>(g, p.few, q, tree, out, part, vec, st)
+                     : launch_wr<128, true>(g, p.few, q, tree, out, part, vec, st);
+        if (!e) e = merge(g, p.few, bf16, part, out, st);
+    }
+    return e;
 }

@@ -68,7 +68,8 @@ size_t eakv_attention_window_work_bytes(eakv_cache_t *const *caches, int n_cache
         return 0;
     int prev;
     if (eakvi_enter(caches[0], &prev)) return 0;
-    size_t need = eakvd_window_work_bytes(&caches[0]->geom, &b, n_q, n_kv);
+    size_t need = eakvd_window_work_bytes(&caches[0]->geom, &b, n_q, n_kv,
+                                          dtype == EAKV_BF16);
     /* with a tree one token of each sequence is a window like others */
     if (is_decode(&b, dtype, 0, &d)) {
         const size_t dec = eakvd_fused_launch_bytes(&caches[0]->geom, &d, n_q, n_kv);
@@ -101,7 +102,8 @@ int eakv_attention_window_batch_device(eakv_cache_t *const *caches, int n_caches
     if (rc) return rc;
     const int decode = is_decode(&b, dtype, d_tree != NULL, &d);
     const size_t need = decode ? eakvd_fused_launch_bytes(&c0->geom, &d, n_q, n_kv)
-                               : eakvd_window_work_bytes(&c0->geom, &b, n_q, n_kv);
+                               : eakvd_window_work_bytes(&c0->geom, &b, n_q, n_kv,
+                                                         dtype == EAKV_BF16);
     const int own = !d_work;
     int capturing = 0;
     if (d_work && work_bytes < need) {

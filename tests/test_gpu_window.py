@@ -86,6 +86,12 @@ SHAPES = [
     (128, 1, 3, [(40, 171)]),
     (128, 2, 2, [(0, 300), (700, 1), (33, 0), (90, 200)]),
     (64, 2, 40, [(511, 5)]),
+    # K and V expanded first: bf16 beyond 256 rows, f32 beyond 2048
+    (128, 2, 8, [(33, 65)]),
+    (128, 1, 16, [(100, 140)]),
+    (64, 1, 32, [(0, 70), (500, 3), (95, 97)]),
+    (128, 1, 32, [(1, 65)]),
+    (64, 1, 16, [(1500, 130)]),
 ]
 
 
@@ -112,6 +118,7 @@ def test_chunks_and_ragged_batch(E, rng, bf16):
     compare(E, rng, 128, 1, 4, [(9000, 6), (0, 1), (100, 8), (4001, 3)], bf16)
     compare(E, rng, 64, 2, 4, [(int(97 * 1.13 ** i), 1 + i % 5) for i in range(32)], bf16)
     compare(E, rng, 128, 1, 2, [(2500, 150)], bf16)
+    compare(E, rng, 64, 1, 24, [(6000, 100), (6100, 0), (3, 88)], bf16)
 
 
 def test_long_context(E, rng):
@@ -134,6 +141,7 @@ def test_magnitudes(E, rng, scale):
     s[0, 1] = scale
     for bf16 in (False, True):
         compare(E, rng, 128, 2, 4, [(100, 9)], bf16, scale=s)
+        compare(E, rng, 128, 1, 32, [(40, 66)], bf16, scale=s)
 
 
 def test_outlier_channels(E, rng):
@@ -142,6 +150,7 @@ def test_outlier_channels(E, rng):
     s[..., [5, 70, 71]] = 30.0
     for bf16 in (False, True):
         compare(E, rng, 128, 2, 8, [(333, 8)], bf16, scale=s)
+        compare(E, rng, 128, 1, 32, [(90, 66)], bf16, scale=s)
 
 
 def test_beyond_32_bit_offsets(E, rng):
@@ -161,6 +170,35 @@ def test_beyond_32_bit_offsets(E, rng):
         outs.append(call.get())
     assert np.array_equal(outs[0].view(np.uint32), outs[1].view(np.uint32))
     c.free()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+def test_hidden_nonfinite_many_rows(E, rng, d, bf16):
+    """As below for windows whose K and V are expanded first."""
+    n_kv, n_q, start, m = 1, 8 if bf16 else 32, 30, 80
+    c = E.Cache(1, n_kv, d, 128)
+    x = rng.standard_normal((1, 2, n_kv, 128, d), dtype=np.float32)
+    q = rng.standard_normal((m, n_q, d), dtype=np.float32)
+    got = []
+    for bad in (False, True):
+        if bad:
+            x[0, 0, 0, start + 70, 0] = np.nan
+            x[0, 1, 0, start + 40, d - 64] = np.nan
+            x[0, :, :, start + m:] = np.nan
+        c.clear()
+        c.load_raw(x, 128)
+        c.restore(start + m)
+        call = W.Call(E, [c], [m], n_q, n_kv, bf16, [start])
+        call.put(q)
+        call.run()
+        got.append(call.get())
+    nan = np.isnan(got[1])
+    want = np.zeros_like(nan)
+    want[70:] = True
+    want[40:, :, d - 64:] = True
+    assert np.array_equal(nan, want)
+    assert np.array_equal(got[0][~want].view(np.uint32), got[1][~want].view(np.uint32))
 
 
 @pytest.mark.parametrize("bf16", [False, True])

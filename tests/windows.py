@@ -16,7 +16,8 @@ Bounds, with e = 2^-24 (f32), h = 2^-11 (f16), o = 2^-8 (bf16), each half a step
   and by 40 e max(|v| + |c|) in the weighted sum (chain of tiles, joined in a tree).
   bf16.  V's operand rounds s, c and the value to f16, p is rounded once:
   h (|n - z| s + |c| + |v| + |v|) <= h (3 max|v| + 2 max s), and the result to bf16:
-  o |out|.
+  o |out|.  Windows of many rows (k16) have K rounded to f16 too: |dS| grows by
+  h sum_i |q_i| |k_i| / sqrt(d), the output by 2 |dS| * 2 max|v|.
 
 The 2-norm over a case is held to a third of that scale, as roundings of random
 sign: 4e-6 of the norm for f32 (A is about 15 for the normal data used: 40 roundings
@@ -47,6 +48,11 @@ def visible(start, m, words=None):
     return see
 
 
+def k16(m, n_q, n_kv):
+    """Whether a bf16 window of m tokens has K rounded to f16."""
+    return m > 64 and m * (n_q // n_kv) > 256
+
+
 def attend(cache, layer, q, start, n_q, n_kv, words=None):
     """Exact outputs f64 [m][n_q][d] and the bound of each output's f32 part."""
     m, _, d = q.shape
@@ -74,6 +80,8 @@ def attend(cache, layer, q, start, n_q, n_kv, words=None):
             sm = sh[t].max(0)
             tol[i, h] = (80 * E32 * a + 4 * E32) * 2 * vm + 40 * E32 * (vm + sm)
             half[i, h] = H16 * (3 * vm + 2 * sm)
+            if k16(m, n_q, n_kv):
+                half[i, h] += 4 * H16 * (np.abs(kh[t]) @ np.abs(qi)).max() / np.sqrt(d) * vm
     return out, tol, half
 
 
