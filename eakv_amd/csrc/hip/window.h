@@ -2,6 +2,7 @@
 // window_prompt.hip; the mathematics stands in window.hip).
 #pragma once
 
+#include <atomic>
 #include <type_traits>
 
 #include "common.h"
@@ -247,45 +248,152 @@ __device__ __forceinline__ float half_max(float v)
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// What a lane writes of its row: final outputs (mc == 1) or the chunk's partial.
-// o[f][i]: dim 32f + 8(i/4) + 4h + i%4.
-template <int D, bool F32>
-__device__ __forceinline__ void put_row(const v16f *o, float l, float m, const WinJob &job, int c,
-                                        int chunk, int tok, int head, int h, int64_t qrow,
-                                        bool vec, void *out, float *part)
+// The row that a lane writes: final outputs (mc == 1) or its chunk's partial.
+struct RowOut {
+    int64_t at;                         // first value, in out or in part
+    float *ml;                          // the partial's M and l, or NULL
+    bool final, vec;
+};
+
+__device__ __forceinline__ RowOut row_out(const WinJob &job, int c, int chunk, int tok, int head,
+                                          int D, int64_t qrow, bool vec, float *part)
 {
-    if (job.mc[c] == 1) {
+    RowOut r;
+    r.final = job.mc[c] == 1;
+    r.vec = vec;
+    r.at = qrow;
+    r.ml = nullptr;
+    if (!r.final) {
+        const int64_t prow = job.part[c] + (int64_t)chunk * job.ntok[c] * job.n_q +
+                             (int64_t)tok * job.n_q + head;
+        r.at = prow * D;
+        r.ml = part + job.part_rows * D + prow * 2;
+    }
+    return r;
+}
+
+// Four values of a row: dims d..d+3, unscaled.  (A partial with l = 0 has no O.)
+template <bool F32>
+__device__ __forceinline__ void put4(const RowOut &r, int d, const float *o, float l, void *out,
+                                     float *part)
+{
+    if (r.final) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float o4[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+        store4<F32>(out, r.at + d, r.vec, o4);
+    } else if (l != 0.0f) {
+        *(v4f *)(part + r.at + d) = v4f{o[0], o[1], o[2], o[3]};
+    }
+}
+
+// A wave's whole rows: o[f][i] holds dim 32f + 8(i/4) + 4h + i%4.
+template <int D, bool F32>
+__device__ __forceinline__ void put_rows(const RowOut &r, const v16f *o, float l, float m, int h,
+                                         void *out, float *part)
+{
+#pragma unroll
+    for (int f = 0; f < D / 32; f++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float o4[4] = {o[f][4 * k], o[f][4 * k + 1], o[f][4 * k + 2], o[f][4 * k + 3]};
+            put4<F32>(r, 32 * f + 8 * k + 4 * h, o4, l, out, part);
+        }
+    if (r.ml && h == 0) {
+        r.ml[0] = m;
+        r.ml[1] = l;
+    }
+}
+
+// Joins the WT waves of a block that hold the same rows (O, l, M of other tokens)
+// through LDS and writes the rows: every wave its WT-th part of the dims.  All waves of
+// the block call it, with kJoinBytes of LDS.  (In a tree of log2(WT) steps instead, a
+// draft of 4 tokens at 500 of 32Q/8KV took 14.0 us.)
+template <int D>
+constexpr size_t kJoinBytes = (size_t)8 * (D / 2 + 2) * 64 * 4;
+
+template <int D, bool F32, int WT>
+__device__ __forceinline__ void join_put(float *lds, int wt, int group, int groups, int lane,
+                                         const v16f *o, float l, float m, bool live, const RowOut &r,
+                                         void *out, float *part)
+{
+    constexpr int OW = D / 2 * 64, N = D / 2 / WT;       // floats of a wave's O; of a lane's part
+    float *ml = lds + 8 * OW;
+    const int h = lane >> 5;
+    __syncthreads();
+    {
+        float *po = lds + (size_t)(wt * groups + group) * OW + lane;
 #pragma unroll
         for (int f = 0; f < D / 32; f++)
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const float o4[4] = {o[f][4 * k] * inv, o[f][4 * k + 1] * inv, o[f][4 * k + 2] * inv,
-                                     o[f][4 * k + 3] * inv};
-                store4<F32>(out, qrow + 32 * f + 8 * k + 4 * h, vec, o4);
-            }
-        return;
+            for (int i = 0; i < 16; i++) po[(f * 16 + i) * 64] = o[f][i];
+        ml[(wt * groups + group) * 128 + lane] = m;
+        ml[(wt * groups + group) * 128 + 64 + lane] = l;
     }
-    const int64_t prow = job.part[c] + (int64_t)chunk * job.ntok[c] * job.n_q +
-                         (int64_t)tok * job.n_q + head;
-    float *po = part + prow * D;
-    if (l != 0.0f) {
+    __syncthreads();
+    float a[WT], mm = kMInit, ll = 0.0f;
 #pragma unroll
-        for (int f = 0; f < D / 32; f++)
+    for (int t = 0; t < WT; t++) {
+        a[t] = ml[(t * groups + group) * 128 + lane];
+        mm = fmaxf(mm, a[t]);
+    }
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-                *(v4f *)(po + 32 * f + 8 * k + 4 * h) =
-                    v4f{o[f][4 * k], o[f][4 * k + 1], o[f][4 * k + 2], o[f][4 * k + 3]};
+    for (int t = 0; t < WT; t++) {
+        a[t] = __builtin_amdgcn_exp2f(a[t] - mm);
+        ll = fmaf(a[t], ml[(t * groups + group) * 128 + 64 + lane], ll);
     }
-    if (h == 0) {
-        float *pm = part + job.part_rows * D + prow * 2;
-        pm[0] = m;
-        pm[1] = l;
+#pragma unroll
+    for (int k = 0; k < N / 4; k++) {
+        const int e = wt * N + 4 * k;                    // register f * 16 + i
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int t = 0; t < WT; t++) {
+            const float *po = lds + (size_t)(t * groups + group) * OW + lane + e * 64;
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = fmaf(a[t], po[j * 64], x[j]);
+        }
+        if (live) put4<F32>(r, 32 * (e >> 4) + 8 * ((e & 15) >> 2) + 4 * h, x, ll, out, part);
     }
+    if (live && r.ml && h == 0 && wt == 0) {
+        r.ml[0] = mm;
+        r.ml[1] = ll;
+    }
+}
+
+// The sequence of block b: the last one whose first block is not behind it.
+__device__ __forceinline__ int seq_of(const int *pre, int n_seq, int b, int lane)
+{
+    // (pre has EAKVD_MAX_BATCH entries at least)
+    const bool past = lane > 0 && lane < n_seq && b >= pre[lane < EAKVD_MAX_BATCH ? lane : 0];
+    return (int)__popcll(__ballot(past));
+}
+
+// Lets a kernel use `bytes` of dynamic LDS on the current device, once per device
+// (`done`: the devices it was done on, of one kernel).
+inline int allow_lds(const void *kern, size_t bytes, std::atomic<uint64_t> &done)
+{
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return (int)e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (bit & done.load(std::memory_order_relaxed)) return 0;
+    e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return (int)e;
+}
+
+// s_waitcnt vmcnt(N) alone (gfx9 encoding)
+template <int N>
+__device__ __forceinline__ void wait_loads()
+{
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
 }
 
 }  // namespace
 
+// Windows of at most 32 rows per kv head (window_draft.hip).
+int win_draft(const eakvd_geom &g, const WinJob &job, bool bf16, const void *q, const uint64_t *tree,
+              void *out, float *part, bool vec, hipStream_t st);
 // Expands K and V of the sequences' kv heads into `img` and attends
 // (window_prompt.hip).  img: win_prompt_bytes() of device scratch; job.img: each
 // sequence's first sub-tile there.

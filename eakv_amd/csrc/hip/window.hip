@@ -93,8 +93,7 @@ __global__ __launch_bounds__(64 * kWinWaves, 2) void window_kernel(
     const int n32 = lane & 31, h = lane >> 5;
 
     // this block's sequence, rows, chunk and kv head; long row blocks first
-    int c = 0;
-    while (c + 1 < job.n_seq && (int)blockIdx.x >= job.pre[c + 1]) c++;
+    const int c = seq_of(job.pre, job.n_seq, (int)blockIdx.x, lane);
     int rem = (int)blockIdx.x - job.pre[c];
     const int kvh = rem % job.n_kv;
     rem /= job.n_kv;
@@ -495,7 +494,7 @@ __global__ __launch_bounds__(64 * kWinWaves, 2) void window_kernel(
     }
 
     // ---- both halves of a row's tokens, then the WT waves of these rows
-    float l = A.l + __shfl_xor(A.l, 32, 64);
+    const float l = A.l + __shfl_xor(A.l, 32, 64);
     if constexpr (F32) {
 #pragma unroll
         for (int g = 0; g < GPD; g++) {
@@ -512,43 +511,13 @@ __global__ __launch_bounds__(64 * kWinWaves, 2) void window_kernel(
 #pragma unroll
             for (int i = 0; i < 16; i++) A.o[f][i] *= 0x1p-15f;
     }
-    float mm = A.m;
+    const RowOut ro = row_out(job, c, chunk, tok, head, D, qrow, vec, part);
     if constexpr (WT > 1) {
-        float *xo = (float *)lds;                            // [WT/2][WR][D/2][64]
-        constexpr int OW = D / 2 * 64;                       // floats of one wave's O
-        float *xm = xo + (size_t)(WT / 2) * WR * OW;         // [WT/2][WR][2][64]
-        for (int half = WT / 2; half >= 1; half >>= 1) {
-            __syncthreads();
-            if (wt >= half && wt < 2 * half) {
-                float *po = xo + (size_t)((wt - half) * WR + wr) * OW;
-                float *pm = xm + (size_t)((wt - half) * WR + wr) * 128;
-#pragma unroll
-                for (int f = 0; f < D / 32; f++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) po[(f * 16 + i) * 64 + lane] = A.o[f][i];
-                pm[lane] = mm;
-                pm[64 + lane] = l;
-            }
-            __syncthreads();
-            if (wt < half) {
-                const float *po = xo + (size_t)(wt * WR + wr) * OW;
-                const float *pm = xm + (size_t)(wt * WR + wr) * 128;
-                const float m2 = pm[lane], l2 = pm[64 + lane];
-                const float mn = fmaxf(mm, m2);
-                const float a1 = __builtin_amdgcn_exp2f(mm - mn), a2 = __builtin_amdgcn_exp2f(m2 - mn);
-                mm = mn;
-                l = l * a1 + l2 * a2;
-#pragma unroll
-                for (int f = 0; f < D / 32; f++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        A.o[f][i] = A.o[f][i] * a1 + po[(f * 16 + i) * 64 + lane] * a2;
-            }
-        }
-        if (wt != 0) return;
+        join_put<D, F32, WT>((float *)lds, wt, wr, WR, lane, A.o, l, A.m, active && r0 + n32 < rows, ro, out,
+                             part);
+    } else if (active && r0 + n32 < rows) {
+        put_rows<D, F32>(ro, A.o, l, A.m, h, out, part);
     }
-    if (!active || r0 + n32 >= rows) return;
-    put_row<D, F32>(A.o, l, mm, job, c, chunk, tok, head, h, qrow, vec, out, part);
 }
 
 // One wave per (window token, q head) of the sequences with chunks: the
@@ -562,8 +531,7 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WinJob job, const flo
     const int lane = threadIdx.x & 63;
     if (r >= n_rows) return;
     const int tok = r / job.n_q;
-    int c = 0;
-    while (c + 1 < job.n_seq && tok >= job.lead[c + 1]) c++;
+    const int c = seq_of(job.lead, job.n_seq, tok, lane);
     const int mc = job.mc[c];
     if (mc == 1) return;
     const int64_t per = (int64_t)job.ntok[c] * job.n_q;
@@ -626,16 +594,24 @@ int tile_of(int wr, int d)
 // 123 against 130, at 2000 34.6 against 33.1; f32 1000 tokens 71 against 79, but 256
 // at 30000 440 against 363 (the products there are twice as many, so conversions
 // weigh less).
+#ifndef LD_
+#define LD_ 1
+#endif
+constexpr int kLeastDraft = LD_;
 bool is_many(int ntok, int qpk, bool bf16)
 {
     return ntok > EAKVD_TREE_MAX && (int64_t)ntok * qpk > (bf16 ? 256 : 2048);
 }
 
-// Tiles of a chunk, window_kernel: an even share of the chip, and at least four.
-int64_t few_share(int64_t tiles, int cus)
+// Tiles of a chunk, window_kernel and win_draft: an even share of the chip, and at
+// least `least`; at most 2^25 tokens (win_draft's offsets from a chunk's first token
+// are 32 bits).
+int64_t few_share(int64_t tiles, int cus, int tile, int least)
 {
-    const int64_t s = (tiles + cus - 1) / cus;
-    return s < 4 ? 4 : s;
+    int64_t s = (tiles + cus - 1) / cus;
+    s = s < least ? least : s;
+    const int64_t most = (1 << 25) / tile;
+    return s < most ? s : most;
 }
 
 // Tiles of a chunk, win_prompt: the split of the longest context in k that ends first,
@@ -711,7 +687,7 @@ void plan_part(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv, bo
     }
     const int cus = cu_count();
     const int64_t share = many ? many_share(j, tiles, cus, g->head_dim, bf16)
-                               : few_share(tiles, cus);
+                               : few_share(tiles, cus, tile, p->wr == 1 ? kLeastDraft : 4);
     int64_t part = 0;
     for (int i = 0; i < j.n_seq; i++) {
         const int64_t rows = (int64_t)j.ntok[i] * qpk, nrb = (rows + rbr - 1) / rbr;
@@ -764,13 +740,13 @@ int launch(const eakvd_geom *g, const WinPart &p, const void *q, const uint64_t 
 {
     constexpr int WT = kWinWaves / WR;
     constexpr size_t tiles = (size_t)WT * SPW * (WR == 1 ? 1 : 2) * sizeof(SubTile<D, F32>);
-    constexpr size_t join = WT > 1 ? (size_t)(WT / 2) * WR * (D / 2 * 64 + 128) * 4 : 0;
+    constexpr size_t join = WT > 1 ? kJoinBytes<D> : 0;
     constexpr size_t bytes = tiles > join ? tiles : join;
     static_assert(bytes <= 160 * 1024, "LDS");
     auto *kern = window_kernel<D, F32, WR, SPW>;
-    hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)bytes);
-    if (e != hipSuccess) return (int)e;
+    static std::atomic<uint64_t> done;
+    const int e = allow_lds((const void *)kern, bytes, done);
+    if (e) return e;
     const float rsd = 1.0f / sqrtf((float)D);
     hipLaunchKernelGGL(kern, dim3((unsigned)p.job.pre[p.job.n_seq]), dim3(64 * kWinWaves), bytes, st,
                        *g, p.job, q, tree, out, part, rsd, vec);
@@ -782,7 +758,7 @@ int launch_wr(const eakvd_geom *g, const WinPart &p, const void *q, const uint64
               float *part, int vec, hipStream_t st)
 {
     switch (p.wr) {
-    case 1: return launch<D, F32, 1, 1>(g, p, q, tree, out, part, vec, st);
+    case 1: return win_draft(*g, p.job, !F32, q, tree, out, part, vec, st);
     case 2: return launch<D, F32, 2, 1>(g, p, q, tree, out, part, vec, st);
     case 4: return launch<D, F32, 4, D == 128 ? 1 : 2>(g, p, q, tree, out, part, vec, st);
     default: return launch<D, F32, 8, D == 128 ? 2 : 4>(g, p, q, tree, out, part, vec, st);

@@ -1,0 +1,461 @@
+// window_draft.hip — the window attention of at most 32 rows per kv head (a few drafted
+// tokens), where reading the packed planes once is the work: the mathematics of
+// window.hip with nothing shared between waves.
+//
+// A block's 8 waves take 32-token sub-tiles in turn, all of them for the same 32 rows,
+// and join at the end.  Each wave
+//   - keeps kAhead sub-tiles in flight, by buffer loads whose tile offset is scalar:
+//     K's bytes and the scales to registers, V's bytes to LDS;
+//   - makes K's operands in registers (a lane's bytes are its operand's);
+//   - reads V's bytes back transposed (ds_read_b64_tr_b8: 8 tokens of a byte column
+//     per lane) and makes its operands in registers, the tokens' scales from LDS, in
+//     operand order;
+// so no operand passes through LDS as f16, and no wave waits for another.
+#include "window.h"
+
+namespace {
+
+constexpr int kDWaves = 8;
+constexpr int kAhead = 3;               // slots of V's bytes; kAhead - 1 sub-tiles in flight
+
+typedef int v2i __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) v2i *lds_v2i;
+typedef __attribute__((address_space(3))) void *lds_v;
+
+template <int D, bool F32>
+struct __align__(16) DraftLds {
+    static constexpr int GPD = D / 64;
+    uint8_t v[kAhead][32 * 32 * GPD];   // V's bytes: rows of 32 GPD, their 16-byte units swizzled
+    float ks[GPD][32];                  // K's scales
+    float vs[F32 ? GPD : 1][32];        // f32: V's scales and biases
+    float vc[F32 ? GPD : 1][32];
+    // of V's operand (g, 16-token step, h), 8 tokens in operand order: -(1024 + z),
+    // -(64 + z); bf16: scales and biases in f16
+    _Float16 zl[GPD][2][2][8], zh[GPD][2][2][8];
+    _Float16 s16[F32 ? 1 : GPD][2][2][8], c16[F32 ? 1 : GPD][2][2][8];
+};
+
+struct Stage {
+    uint4 k[2];
+    float ks, kb, vs, vb;
+};
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void *p, int64_t bytes)
+{
+    // dword3 0x00020000: raw 32-bit buffer; reads beyond `bytes` return 0
+    const int64_t most = 0xfffffff0ll;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0,
+                                             (int)(uint32_t)(bytes < most ? bytes : most), 0x00020000);
+}
+
+// the unit permutation of token row t
+template <int GPD>
+__device__ __forceinline__ int swz(int t)
+{
+    return GPD == 2 ? (t >> 2) & 3 : (t >> 3) & 1;
+}
+
+// maximum over lanes that differ in bits 3, 4 and 5 .. all of a wave
+__device__ __forceinline__ float wave_max_fast(float v)
+{
+    auto ror = [](float x, auto c) {
+        constexpr int ctrl = decltype(c)::value;
+        return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), ctrl, 0xf, 0xf, true));
+    };
+    v = fmaxf(v, ror(v, std::integral_constant<int, 0x128>{}));     // row_ror:8
+    v = fmaxf(v, ror(v, std::integral_constant<int, 0x124>{}));
+    v = fmaxf(v, ror(v, std::integral_constant<int, 0x122>{}));
+    v = fmaxf(v, ror(v, std::integral_constant<int, 0x121>{}));
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    return half_max(v);
+}
+
+template <int D, bool F32>
+__global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, WinJob job,
+                                                                const void *q, const uint64_t *tree,
+                                                                void *out, float *part, float rsd,
+                                                                int vec)
+{
+    constexpr int GPD = D / 64, RB = 32 * GPD;
+    typedef DraftLds<D, F32> Lds;
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    Lds &S = ((Lds *)lds)[w];
+    const int n32 = lane & 31, h = lane >> 5;
+
+    const int c = seq_of(job.pre, job.n_seq, (int)blockIdx.x, lane);
+    int rem = (int)blockIdx.x - job.pre[c];
+    const int kvh = rem % job.n_kv, chunk = rem / job.n_kv;
+    const int m = job.ntok[c], start = job.start[c], qpk = job.qpk;
+    const int rows = m * qpk;                        // at most 32
+    const int t_end = start + m;
+    const int lo = chunk * job.clen[c], hi = min(t_end, lo + job.clen[c]);
+
+    const int row = min(n32, rows - 1);
+    const int tok = row / qpk, head = kvh * qpk + row - tok * qpk;
+    const int64_t qrow = ((int64_t)(job.tok0[c] + tok) * job.n_q + head) * D;
+    const int vis = start + tok + 1;
+    const int vis_min = tree ? start : start + 1;
+    const uint64_t word = tree ? tree[job.tok0[c] + tok] : 0;
+
+    // ---- the planes of this kv head from token lo on
+    const Planes K = planes_of(geo, job.base[c], job.layer, 0);
+    const Planes V = planes_of(geo, job.base[c], job.layer, 1);
+    const int64_t g0 = (int64_t)kvh * geo.gph + (int64_t)lo * GPD;
+    const int64_t room = (int64_t)(geo.max_seq_len - lo) * GPD;          // groups
+    const auto rkw = rsrc(K.w + g0 * 32, room * 32), rvw = rsrc(V.w + g0 * 32, room * 32);
+    const auto rks = rsrc(K.s + g0, room * 4), rkb = rsrc(K.b + g0, room * 4);
+    const auto rvs = rsrc(V.s + g0, room * 4), rvb = rsrc(V.b + g0, room * 4);
+    // K: token n32, bytes 16h of each group; scales: token n32, group h
+    const int ok = n32 * RB + 16 * h;
+    const int os = (n32 * GPD + (GPD == 2 ? h : 0)) * 4;
+    // V: 16-byte unit `lane` of a slot's first KB is unit (lane % UPT) of row lane / UPT
+    constexpr int UPT = RB / 16;
+    const int vt = lane / UPT, ov = vt * RB + 16 * ((lane % UPT) ^ swz<GPD>(vt));
+    constexpr int NV = RB * 32 / 1024;
+    constexpr int kLoads = NV + GPD + 4;
+    auto load = [&](int i, Stage &s) __attribute__((always_inline)) {
+        const int t = __builtin_amdgcn_readfirstlane(32 * (w + kDWaves * i));
+        uint8_t *slot = S.v[i % kAhead];
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rvw, (lds_v)(slot + 1024 * j), 16, ov, t * RB + 1024 * j,
+                                                     0, 2);
+#pragma unroll
+        for (int g = 0; g < GPD; g++) {
+            const auto x = __builtin_amdgcn_raw_buffer_load_b128(rkw, ok + 32 * g, t * RB, 2);
+            s.k[g] = uint4{x[0], x[1], x[2], x[3]};
+        }
+        const int ts = t * GPD * 4;
+        s.ks = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rks, os, ts, 2));
+        s.kb = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rkb, os, ts, 2));
+        s.vs = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rvs, os, ts, 2));
+        s.vb = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rvb, os, ts, 2));
+    };
+    // transposed reads of V: lane supplies 8 bytes of row j = lane%16 / 2 of its 16-lane
+    // group's 8 tokens and gets 8 tokens of byte column n32
+    const int jr = (lane & 15) >> 1, trow = 8 * (jr >> 2) + 4 * h + (jr & 3);
+    int vrd[GPD];
+#pragma unroll
+    for (int g = 0; g < GPD; g++)
+        vrd[g] = trow * RB + 16 * ((2 * g + ((lane >> 4) & 1)) ^ swz<GPD>(trow)) + 8 * (lane & 1);
+    // where this lane's token (n32, group h) stands among V's operands
+    const int pj = 4 * ((n32 >> 3) & 1) + (n32 & 3);
+    const int pos = (pj & 4) | ((pj & 1) << 1) | ((pj >> 1) & 1);
+    const int p_step = n32 >> 4, p_half = (n32 >> 2) & 1;
+    const bool owner = GPD == 2 || h == 0;
+
+    // this wave's sub-tiles; the first loads are on their way while Q is made (loads
+    // behind the last sub-tile stay within the planes or return 0)
+    const int n_sub = hi > lo ? (hi - lo + 31) / 32 : 0;
+    const int n_i = n_sub > w ? (n_sub - w + kDWaves - 1) / kDWaves : 0;
+    Stage st[kAhead];
+    if (n_i > 0)
+#pragma unroll
+        for (int k = 0; k < kAhead - 1; k++) load(k, st[k]);
+
+    QOp<D, F32> Q;
+    build_q<D, F32>(Q, q, qrow, vec, rsd, h);
+    v16f O[D / 32];
+    float M = kMInit, L = 0.0f, C[GPD];
+#pragma unroll
+    for (int f = 0; f < D / 32; f++)
+#pragma unroll
+        for (int k = 0; k < 16; k++) O[f][k] = 0.0f;
+#pragma unroll
+    for (int g = 0; g < GPD; g++) C[g] = 0.0f;
+    uint32_t poison = 0;
+
+    auto consume = [&](int i, const Stage &st) __attribute__((always_inline)) {
+        const int t0 = lo + 32 * (w + kDWaves * i);
+        // tokens behind the last have no part in this (their bytes may be anything)
+        const bool live = t0 + n32 < t_end;
+        const float zk = zero_nibble(st.ks, st.kb), ck = fmaf(zk, st.ks, st.kb);
+        const float vs = live ? st.vs : 0.0f, vb = live ? st.vb : 0.0f;
+        const float zv = zero_nibble(vs, vb), cv = fmaf(zv, vs, vb);
+        // ---- scales to LDS
+        uint64_t bad = 0;
+        int ev;
+        if (owner) S.ks[GPD == 2 ? h : 0][n32] = st.ks;
+        if (owner) {
+            S.zl[GPD == 2 ? h : 0][p_step][p_half][pos] = (_Float16)(-1024.0f - zv);
+            S.zh[GPD == 2 ? h : 0][p_step][p_half][pos] = (_Float16)(-64.0f - zv);
+        }
+        if constexpr (F32) {
+            const float a = fabsf(vs);
+            ev = exp_of(wave_max_fast(a < __builtin_inff() ? a : 0.0f));
+            if (owner) {
+                S.vs[GPD == 2 ? h : 0][n32] = vs;
+                S.vc[GPD == 2 ? h : 0][n32] = cv;
+            }
+        } else {
+            const float a = fmaxf(fabsf(vb), fabsf(fmaf(15.0f, vs, vb)));
+            const bool fin = a < __builtin_inff() && vb == vb && vs == vs;
+            bad = __ballot(!fin);
+            ev = exp_of(wave_max_fast(fin ? a : 0.0f));
+            if (owner) {
+                S.s16[GPD == 2 ? h : 0][p_step][p_half][pos] = (_Float16)(fin ? scale2(vs, 15 - ev) : 0.0f);
+                S.c16[GPD == 2 ? h : 0][p_step][p_half][pos] = (_Float16)(fin ? scale2(cv, 15 - ev) : 0.0f);
+            }
+        }
+        ev = __builtin_amdgcn_readfirstlane(ev);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        // ---- scores
+        v16f s;
+#pragma unroll
+        for (int k = 0; k < 16; k++) s[k] = 0.0f;
+        {
+            __bf16 p1, p2, p3;
+            const __bf16 zero = (__bf16)0.0f;
+            pieces(owner ? ck : 0.0f, p1, p2, p3);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b8{p1, p1, p1, p2, p2, p3, zero, zero}, Q.bias, s, 0,
+                                                        0, 0);
+        }
+        float zg[2] = {zk, zk};
+        if constexpr (GPD == 2) {
+            const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(zk), __float_as_uint(zk), false,
+                                                            false);
+            zg[0] = __uint_as_float(r[0]);
+            zg[1] = __uint_as_float(r[1]);
+        }
+#pragma unroll
+        for (int g = 0; g < GPD; g++) {
+            const h2 off = pk(-zg[g], -zg[g]);
+            const uint32_t x[4] = {st.k[g].x, st.k[g].y, st.k[g].z, st.k[g].w};
+            v16f acc;
+#pragma unroll
+            for (int k = 0; k < 16; k++) acc[k] = 0.0f;
+#pragma unroll
+            for (int o = 0; o < 2; o++) {
+                uint32_t a[4], b[4];
+#pragma unroll
+                for (int d = 0; d < 2; d++) {
+                    const uint32_t x0 = x[2 * o + d], x1 = x0 >> 8;
+                    a[2 * d] = u_of(nib2<false>(x0, off));
+                    a[2 * d + 1] = u_of(nib2<false>(x1, off));
+                    b[2 * d] = u_of(nib2<true>(x0, off));
+                    b[2 * d + 1] = u_of(nib2<true>(x1, off));
+                }
+                const h8 ka = __builtin_bit_cast(h8, uint4{a[0], a[1], a[2], a[3]});
+                const h8 kb = __builtin_bit_cast(h8, uint4{b[0], b[1], b[2], b[3]});
+                const int f = g * 4 + 2 * o;
+                if constexpr (F32) {
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, Q.b[f], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kb, Q.b[f + 1], acc, 0, 0, 0);
+                }
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, Q.a[f], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kb, Q.a[f + 1], acc, 0, 0, 0);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const v4f sc = *(const v4f *)&S.ks[g][8 * k + 4 * h];
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[4 * k + e] = fmaf(sc[e], acc[4 * k + e], s[4 * k + e]);
+            }
+        }
+        // ---- V's bytes, transposed (their loads are done: K's of the same sub-tile,
+        // issued behind them, are)
+        v2i vx[GPD][2];
+        const uint8_t *slot = S.v[i % kAhead];
+#pragma unroll
+        for (int g = 0; g < GPD; g++)
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++)
+                vx[g][ks] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i)(slot + vrd[g] + 16 * ks * RB));
+        // ---- softmax
+        const bool masked = t0 + 32 > vis_min;
+        if (masked) {
+            const int d0 = t0 + 4 * h - start;           // this lane's first token, of the window
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                const int d = d0 + 8 * (k >> 2) + (k & 3);
+                const bool see = tree ? d < 0 || (d < m && ((word >> (d & 63)) & 1)) : d + start < vis;
+                s[k] = see ? s[k] : -__builtin_inff();
+            }
+        }
+        float top = fmaxf(fmaxf(s[0], s[1]), s[2]);
+#pragma unroll
+        for (int k = 3; k < 16; k++) top = fmaxf(top, s[k]);
+        const float need = fmaf(half_max(top), Q.rf, (float)ev - kWinTop);
+        if (__ballot(need > M + kWinTau) != 0) {
+            const float mn = fmaxf(M, need);
+            const float al = __builtin_amdgcn_exp2f(M - mn);
+            M = mn;
+            L *= al;
+#pragma unroll
+            for (int f = 0; f < D / 32; f++)
+#pragma unroll
+                for (int k = 0; k < 16; k++) O[f][k] *= al;
+            if constexpr (F32)
+#pragma unroll
+                for (int g = 0; g < GPD; g++) C[g] *= al;
+        }
+        if constexpr (!F32) {
+            if (bad) {
+                // rows that see a token with a non-finite V group
+                uint32_t seen = 0;
+#pragma unroll
+                for (int k = 0; k < 16; k++)
+                    seen |= s[k] != -__builtin_inff() ? 1u << (8 * (k >> 2) + (k & 3)) : 0u;
+                seen <<= 4 * h;
+                poison |= (seen & (uint32_t)bad ? 1u : 0u) |
+                          (GPD == 2 && (seen & (uint32_t)(bad >> 32)) ? 2u : 0u);
+            }
+        }
+        const float mr = F32 ? -M : (float)ev - M;
+        float p[16];
+#pragma unroll
+        for (int k = 0; k < 16; k++) p[k] = __builtin_amdgcn_exp2f(fmaf(s[k], Q.rf, mr));
+        const float sum = (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]))) +
+                          (((p[8] + p[9]) + (p[10] + p[11])) + ((p[12] + p[13]) + (p[14] + p[15])));
+        L += F32 ? sum : scale2(sum, -ev);
+        // ---- weighted sum
+#pragma unroll
+        for (int g = 0; g < GPD; g++) {
+            h8 P[F32 ? 2 : 1][2];
+            if constexpr (F32) {
+                uint32_t a[8], b[8];
+                float cs = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const v4f sc = *(const v4f *)&S.vs[g][8 * k + 4 * h];
+                    const v4f cc = *(const v4f *)&S.vc[g][8 * k + 4 * h];
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        if (masked) {
+                            x[e] = mul_hidden(p[4 * k + e], sc[e]);
+                            cs += mul_hidden(p[4 * k + e], cc[e]);
+                        } else {
+                            x[e] = p[4 * k + e] * sc[e];
+                            cs = fmaf(p[4 * k + e], cc[e], cs);
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const h2 hi2 = pk(x[e], x[e + 2]);
+                        a[2 * k + e] = u_of(hi2);
+                        b[2 * k + e] = u_of(pk_rest(hi2, x[e], x[e + 2]));
+                    }
+                }
+                C[g] += cs;
+#pragma unroll
+                for (int ks = 0; ks < 2; ks++) {
+                    P[0][ks] = __builtin_bit_cast(h8, uint4{a[4 * ks], a[4 * ks + 1], a[4 * ks + 2],
+                                                            a[4 * ks + 3]});
+                    P[F32 ? 1 : 0][ks] = __builtin_bit_cast(h8, uint4{b[4 * ks], b[4 * ks + 1],
+                                                                      b[4 * ks + 2], b[4 * ks + 3]});
+                }
+            } else {
+#pragma unroll
+                for (int ks = 0; ks < 2; ks++) {
+                    const float *pp = p + 8 * ks;
+                    P[0][ks] = __builtin_bit_cast(
+                        h8, uint4{u_of(pk_exp(pp[0], pp[2])), u_of(pk_exp(pp[1], pp[3])),
+                                  u_of(pk_exp(pp[4], pp[6])), u_of(pk_exp(pp[5], pp[7]))});
+                }
+            }
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) {
+                const uint4 zl = *(const uint4 *)S.zl[g][ks][h], zh = *(const uint4 *)S.zh[g][ks][h];
+                const uint32_t zls[4] = {zl.x, zl.y, zl.z, zl.w}, zhs[4] = {zh.x, zh.y, zh.z, zh.w};
+                uint32_t a[4], b[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t y = (uint32_t)vx[g][ks][k >> 1] >> (8 * (k & 1));
+                    h2 lo2 = h_of((y & 0x000f000fu) | 0x64006400u) + h_of(zls[k]);
+                    h2 hi2 = h_of((y & 0x00f000f0u) | 0x54005400u) + h_of(zhs[k]);
+                    if constexpr (!F32) {
+                        const h2 ss = h_of(((const uint32_t *)S.s16[g][ks][h])[k]);
+                        const h2 cc = h_of(((const uint32_t *)S.c16[g][ks][h])[k]);
+                        lo2 = __builtin_elementwise_fma(lo2, ss, cc);
+                        hi2 = __builtin_elementwise_fma(hi2, ss, cc);
+                    }
+                    a[k] = u_of(lo2);
+                    b[k] = u_of(hi2);
+                }
+                const h8 va = __builtin_bit_cast(h8, uint4{a[0], a[1], a[2], a[3]});
+                const h8 vb8 = __builtin_bit_cast(h8, uint4{b[0], b[1], b[2], b[3]});
+                if constexpr (F32) {
+                    O[2 * g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, P[F32 ? 1 : 0][ks], O[2 * g], 0, 0, 0);
+                    O[2 * g + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vb8, P[F32 ? 1 : 0][ks],
+                                                                          O[2 * g + 1], 0, 0, 0);
+                }
+                O[2 * g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, P[0][ks], O[2 * g], 0, 0, 0);
+                O[2 * g + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vb8, P[0][ks], O[2 * g + 1], 0, 0, 0);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    };
+
+    if (n_i > 0) {
+        for (int i = 0; i < n_i; i += kAhead) {
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                if (i + k >= n_i) break;
+                load(i + k + kAhead - 1, st[(k + kAhead - 1) % kAhead]);
+                // all loads but those of the kAhead - 1 sub-tiles behind this one
+                __builtin_amdgcn_sched_barrier(0);
+                wait_loads<(kAhead - 1) * kLoads>();
+                __builtin_amdgcn_sched_barrier(0);
+                consume(i + k, st[k]);
+            }
+        }
+        wait_loads<0>();
+    }
+
+    const float l = L + __shfl_xor(L, 32, 64);
+    if constexpr (F32) {
+#pragma unroll
+        for (int g = 0; g < GPD; g++) {
+            const float cs = C[g] + __shfl_xor(C[g], 32, 64);
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int k = 0; k < 16; k++) O[2 * g + n][k] += cs;
+        }
+    } else {
+#pragma unroll
+        for (int f = 0; f < D / 32; f++)
+#pragma unroll
+            for (int k = 0; k < 16; k++) O[f][k] *= 0x1p-15f;          // V's operands carried 2^15
+        poison |= __shfl_xor(poison, 32, 64);
+        if (poison)
+#pragma unroll
+            for (int f = 0; f < D / 32; f++)
+                if (poison >> (f >> 1) & 1)
+#pragma unroll
+                    for (int k = 0; k < 16; k++) O[f][k] = __builtin_nanf("");
+    }
+    join_put<D, F32, kDWaves>((float *)lds, w, 0, 1, lane, O, l, M, n32 < rows,
+                              row_out(job, c, chunk, tok, head, D, qrow, vec, part), out, part);
+}
+
+template <int D, bool F32>
+int launch(const eakvd_geom &g, const WinJob &job, const void *q, const uint64_t *tree, void *out,
+           float *part, bool vec, hipStream_t st)
+{
+    constexpr size_t tiles = kDWaves * sizeof(DraftLds<D, F32>), join = kJoinBytes<D>;
+    constexpr size_t bytes = tiles > join ? tiles : join;
+    auto *kern = draft_kernel<D, F32>;
+    static std::atomic<uint64_t> done;
+    const int e = allow_lds((const void *)kern, bytes, done);
+    if (e) return e;
+    hipLaunchKernelGGL(kern, dim3((unsigned)job.pre[job.n_seq]), dim3(64 * kDWaves), bytes, st, g, job, q,
+                       tree, out, part, 1.0f / sqrtf((float)D), (int)vec);
+    return (int)hipGetLastError();
+}
+
+}  // namespace
+
+int win_draft(const eakvd_geom &g, const WinJob &job, bool bf16, const void *q, const uint64_t *tree,
+              void *out, float *part, bool vec, hipStream_t st)
+{
+    if (g.head_dim == 64)
+        return bf16 ? launch<64, false>(g, job, q, tree, out, part, vec, st)
+                    : launch<64, true>(g, job, q, tree, out, part, vec, st);
+    return bf16 ? launch<128, false>(g, job, q, tree, out, part, vec, st)
+                : launch<128, true>(g, job, q, tree, out, part, vec, st);
+}

@@ -166,14 +166,6 @@ __global__ __launch_bounds__(64 * 4 * (D / 64)) void expand_kernel(eakvd_geom ge
     }
 }
 
-// s_waitcnt vmcnt(N) alone (gfx9 encoding)
-template <int N>
-__device__ __forceinline__ void wait_loads()
-{
-    static_assert(N >= 0 && N < 64, "vmcnt range");
-    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
-}
-
 template <int D, bool F32>
 __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
     WinJob job, const uint8_t *img, const Meta *meta, const void *q, void *out, float *part, float rsd,
@@ -186,8 +178,7 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
     const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int n32 = lane & 31, h = lane >> 5;
 
-    int c = 0;
-    while (c + 1 < job.n_seq && (int)blockIdx.x >= job.pre[c + 1]) c++;
+    const int c = seq_of(job.pre, job.n_seq, (int)blockIdx.x, lane);
     int rem = (int)blockIdx.x - job.pre[c];
     const int kvh = rem % job.n_kv;
     rem /= job.n_kv;
@@ -481,7 +472,7 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
                     for (int k = 0; k < 16; k++) O[f][k] = __builtin_nanf("");
     }
     if (r0 + n32 < rows)
-        put_row<D, F32>(O, l, M, job, c, chunk, tok, head, h, qrow, vec, out, part);
+        put_rows<D, F32>(row_out(job, c, chunk, tok, head, D, qrow, vec, part), O, l, M, h, out, part);
 }
 
 template <int D, bool F32>
@@ -495,9 +486,9 @@ int launch(const eakvd_geom &g, const WinJob &job, int64_t subtiles, const void 
     auto *kern = prompt_kernel<D, F32>;
     constexpr int bytes = kRing * I::BYTES;
     static_assert(bytes <= 160 * 1024, "LDS");
-    const hipError_t e = hipFuncSetAttribute((const void *)kern,
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != hipSuccess) return (int)e;
+    static std::atomic<uint64_t> done;
+    const int e = allow_lds((const void *)kern, bytes, done);
+    if (e) return e;
     hipLaunchKernelGGL(kern, dim3((unsigned)job.pre[job.n_seq]), dim3(64 * kPWaves), bytes, st, job, img,
                        meta, q, out, part, 1.0f / sqrtf((float)D), (int)vec);
     return (int)hipGetLastError();
