@@ -66,16 +66,31 @@ __device__ __forceinline__ h2 pk_rest(h2 hi, float a, float b)
 
 // n - z of the low (HI false) or high nibbles of bytes 0 and 2 of x, exact: the
 // nibble is put into the mantissa of 1024 (its lowest bits) or of 64 (four bits up)
-// and 1024 + z or 64 + z taken off.  off: -z of the two bytes.  9 instructions
-// for 8 nibbles.
+// and 1024 + z or 64 + z taken off.  off: minus that, of the two bytes; c: the
+// exponents, in registers, so that mask and exponent are one instruction.
+struct NibConst {
+    uint32_t lo = 0x64006400u, hi = 0x54005400u;
+    __device__ __forceinline__ void hold() { asm("" : "+v"(lo), "+v"(hi)); }
+};
 template <bool HI>
-__device__ __forceinline__ h2 nib2(uint32_t x, h2 off)
+__device__ __forceinline__ h2 nib2(uint32_t x, h2 off, const NibConst &c)
 {
-    if constexpr (HI)
-        return h_of((x & 0x00f000f0u) | 0x54005400u) + (off - h2{(_Float16)64.0f, (_Float16)64.0f});
-    else
-        return h_of((x & 0x000f000fu) | 0x64006400u) +
-               (off - h2{(_Float16)1024.0f, (_Float16)1024.0f});
+    return h_of(HI ? (x & 0x00f000f0u) | c.hi : (x & 0x000f000fu) | c.lo) + off;
+}
+// the offsets of z
+template <bool HI>
+__device__ __forceinline__ h2 nib_off(float z0, float z1)
+{
+    constexpr float k = HI ? -64.0f : -1024.0f;
+    return pk(k - z0, k - z1);
+}
+
+// The nibbles as they stand, as subnormal f16: n * 2^-24 (low) or n * 2^-20 (high).
+// The matrix cores take subnormal operands exactly.
+template <bool HI>
+__device__ __forceinline__ uint32_t nib_sub(uint32_t x)
+{
+    return x & (HI ? 0x00f000f0u : 0x000f000fu);
 }
 
 // z: the nibble whose value is nearest 0, so that (n - z)*s and c = b + z*s are of
@@ -87,12 +102,6 @@ __device__ __forceinline__ float zero_nibble(float s, float b)
     return fminf(fmaxf(z, 0.0f), 15.0f);
 }
 
-__device__ __forceinline__ float wave_top(float v)
-{
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
-}
 __device__ __forceinline__ int exp_of(float a)
 {
     const int e = (int)(__float_as_uint(a) >> 23) - 126;     // a < 2^e
@@ -177,6 +186,8 @@ __device__ __forceinline__ void store4(void *out, int64_t at, bool vec, const fl
 // A row's query as the columns' operand of S^T = K Q^T, one lane's share: operand
 // (g, octet o, nibble n) of half h holds dims 64g + 32n + 16h + 8o + 0..7 in nib2's
 // order (0 2 1 3 4 6 5 7).  The row is scaled by a power of two to below 2^15.
+// SUB: against nib_sub's operands: the high nibbles' dims 2^-4 of that, and the
+// dots (with K's biases scaled alike) come out 2^-24 of theirs.
 template <int D, bool F32>
 struct QOp {
     h8 a[D / 16];                       // f16, high parts
@@ -185,7 +196,7 @@ struct QOp {
     float rf;                           // score = dot * rf, log2 units
 };
 
-template <int D, bool F32>
+template <int D, bool F32, bool SUB>
 __device__ __forceinline__ void build_q(QOp<D, F32> &Q, const void *q, int64_t qrow, bool vec,
                                         float rsd, int h)
 {
@@ -217,6 +228,9 @@ __device__ __forceinline__ void build_q(QOp<D, F32> &Q, const void *q, int64_t q
 #pragma unroll
             for (int j = 0; j < 8; j++) y[j] = scale2(x[g * 4 + f][j], 15 - e);
             qs[g] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+            if (SUB && (f & 1))
+#pragma unroll
+                for (int j = 0; j < 8; j++) y[j] *= 0x1p-4f;
             uint32_t a[4], b[4];
 #pragma unroll
             for (int p = 0; p < 4; p++) {
@@ -231,7 +245,7 @@ __device__ __forceinline__ void build_q(QOp<D, F32> &Q, const void *q, int64_t q
         }
         qs[g] += __shfl_xor(qs[g], 32, 64);
     }
-    Q.rf = scale2(rsd * EAKV_LOG2E, e - 15);
+    Q.rf = scale2(rsd * EAKV_LOG2E, e - 15 + (SUB ? 24 : 0));
     // half h of the bias product's 16 terms: group h's sum of q in pieces,
     // against K's pieces c1 c1 c1 c2 c2 c3 0 0
     __bf16 p1, p2, p3;
@@ -246,6 +260,22 @@ __device__ __forceinline__ float half_max(float v)
 {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// The maximum of a wave's values, in all lanes
+__device__ __forceinline__ float wave_top(float v)
+{
+    auto ror = [](float x, auto c) {
+        constexpr int ctrl = decltype(c)::value;
+        return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), ctrl, 0xf, 0xf, true));
+    };
+    v = fmaxf(v, ror(v, std::integral_constant<int, 0x128>{}));     // row_ror:8
+    v = fmaxf(v, ror(v, std::integral_constant<int, 0x124>{}));
+    v = fmaxf(v, ror(v, std::integral_constant<int, 0x122>{}));
+    v = fmaxf(v, ror(v, std::integral_constant<int, 0x121>{}));
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    return half_max(v);
 }
 
 // The row that a lane writes: final outputs (mc == 1) or its chunk's partial.
@@ -312,7 +342,7 @@ template <int D>
 constexpr size_t kJoinBytes = (size_t)8 * (D / 2 + 2) * 64 * 4;
 
 template <int D, bool F32, int WT>
-__device__ __forceinline__ void join_put(float *lds, int wt, int group, int groups, int lane,
+__device__ __forceinline__ void join_put(float *lds, int wt, int lane,
                                          const v16f *o, float l, float m, bool live, const RowOut &r,
                                          void *out, float *part)
 {
@@ -321,25 +351,25 @@ __device__ __forceinline__ void join_put(float *lds, int wt, int group, int grou
     const int h = lane >> 5;
     __syncthreads();
     {
-        float *po = lds + (size_t)(wt * groups + group) * OW + lane;
+        float *po = lds + (size_t)wt * OW + lane;
 #pragma unroll
         for (int f = 0; f < D / 32; f++)
 #pragma unroll
             for (int i = 0; i < 16; i++) po[(f * 16 + i) * 64] = o[f][i];
-        ml[(wt * groups + group) * 128 + lane] = m;
-        ml[(wt * groups + group) * 128 + 64 + lane] = l;
+        ml[wt * 128 + lane] = m;
+        ml[wt * 128 + 64 + lane] = l;
     }
     __syncthreads();
     float a[WT], mm = kMInit, ll = 0.0f;
 #pragma unroll
     for (int t = 0; t < WT; t++) {
-        a[t] = ml[(t * groups + group) * 128 + lane];
+        a[t] = ml[t * 128 + lane];
         mm = fmaxf(mm, a[t]);
     }
 #pragma unroll
     for (int t = 0; t < WT; t++) {
         a[t] = __builtin_amdgcn_exp2f(a[t] - mm);
-        ll = fmaf(a[t], ml[(t * groups + group) * 128 + 64 + lane], ll);
+        ll = fmaf(a[t], ml[t * 128 + 64 + lane], ll);
     }
 #pragma unroll
     for (int k = 0; k < N / 4; k++) {
@@ -347,7 +377,7 @@ __device__ __forceinline__ void join_put(float *lds, int wt, int group, int grou
         float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int t = 0; t < WT; t++) {
-            const float *po = lds + (size_t)(t * groups + group) * OW + lane + e * 64;
+            const float *po = lds + (size_t)t * OW + lane + e * 64;
 #pragma unroll
             for (int j = 0; j < 4; j++) x[j] = fmaf(a[t], po[j * 64], x[j]);
         }
@@ -391,7 +421,9 @@ __device__ __forceinline__ void wait_loads()
 
 }  // namespace
 
-// Windows of at most 32 rows per kv head (window_draft.hip).
+// Attends without scratch but for the chunks' partials (window_draft.hip); a chunk is a
+// whole number of tiles of kDraftTile tokens.
+constexpr int kDraftTile = 256;
 int win_draft(const eakvd_geom &g, const WinJob &job, bool bf16, const void *q, const uint64_t *tree,
               void *out, float *part, bool vec, hipStream_t st);
 // Expands K and V of the sequences' kv heads into `img` and attends

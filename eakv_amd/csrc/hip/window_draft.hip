@@ -1,9 +1,9 @@
-// window_draft.hip — the window attention of at most 32 rows per kv head (a few drafted
-// tokens), where reading the packed planes once is the work: the mathematics of
-// window.hip with nothing shared between waves.
+// window_draft.hip — the window attention of few rows per kv head (some drafted tokens),
+// where reading the packed planes once is the work: the mathematics of window.hip with
+// nothing shared between waves.
 //
-// A block's 8 waves take 32-token sub-tiles in turn, all of them for the same 32 rows,
-// and join at the end.  Each wave
+// A block has 32 rows; its 8 waves take 32-token sub-tiles in turn and join at the end.
+// Each wave
 //   - keeps kAhead sub-tiles in flight, by buffer loads whose tile offset is scalar:
 //     K's bytes and the scales to registers, V's bytes to LDS;
 //   - makes K's operands in registers (a lane's bytes are its operand's);
@@ -16,7 +16,11 @@
 namespace {
 
 constexpr int kDWaves = 8;
-constexpr int kAhead = 3;               // slots of V's bytes; kAhead - 1 sub-tiles in flight
+static_assert(kDraftTile == 32 * kDWaves, "a sub-tile for each wave");
+// Slots of V's bytes.  bf16: two sub-tiles are in flight while one is worked on.  f32: the
+// next one is asked for as soon as K's registers are free, in the middle of one.
+template <bool F32>
+constexpr int kAheadOf = F32 ? 2 : 3;
 
 typedef int v2i __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) v2i *lds_v2i;
@@ -24,7 +28,7 @@ typedef __attribute__((address_space(3))) void *lds_v;
 
 template <int D, bool F32>
 struct __align__(16) DraftLds {
-    static constexpr int GPD = D / 64;
+    static constexpr int GPD = D / 64, kAhead = kAheadOf<F32>;
     uint8_t v[kAhead][32 * 32 * GPD];   // V's bytes: rows of 32 GPD, their 16-byte units swizzled
     float ks[GPD][32];                  // K's scales
     float vs[F32 ? GPD : 1][32];        // f32: V's scales and biases
@@ -55,29 +59,14 @@ __device__ __forceinline__ int swz(int t)
     return GPD == 2 ? (t >> 2) & 3 : (t >> 3) & 1;
 }
 
-// maximum over lanes that differ in bits 3, 4 and 5 .. all of a wave
-__device__ __forceinline__ float wave_max_fast(float v)
-{
-    auto ror = [](float x, auto c) {
-        constexpr int ctrl = decltype(c)::value;
-        return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), ctrl, 0xf, 0xf, true));
-    };
-    v = fmaxf(v, ror(v, std::integral_constant<int, 0x128>{}));     // row_ror:8
-    v = fmaxf(v, ror(v, std::integral_constant<int, 0x124>{}));
-    v = fmaxf(v, ror(v, std::integral_constant<int, 0x122>{}));
-    v = fmaxf(v, ror(v, std::integral_constant<int, 0x121>{}));
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    return half_max(v);
-}
-
 template <int D, bool F32>
 __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, WinJob job,
                                                                 const void *q, const uint64_t *tree,
                                                                 void *out, float *part, float rsd,
                                                                 int vec)
 {
-    constexpr int GPD = D / 64, RB = 32 * GPD;
+    constexpr int GPD = D / 64, RB = 32 * GPD, kAhead = kAheadOf<F32>;
+    constexpr int kStages = F32 ? 1 : kAhead;
     typedef DraftLds<D, F32> Lds;
     extern __shared__ __align__(16) uint8_t lds[];
     const int lane = threadIdx.x & 63;
@@ -87,17 +76,20 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
 
     const int c = seq_of(job.pre, job.n_seq, (int)blockIdx.x, lane);
     int rem = (int)blockIdx.x - job.pre[c];
-    const int kvh = rem % job.n_kv, chunk = rem / job.n_kv;
+    const int kvh = rem % job.n_kv;
+    rem /= job.n_kv;
     const int m = job.ntok[c], start = job.start[c], qpk = job.qpk;
-    const int rows = m * qpk;                        // at most 32
-    const int t_end = start + m;
+    // row blocks of one kv head and chunk run side by side and share its planes in the caches
+    const int rows = m * qpk, n_rb = (rows + 31) / 32;
+    const int chunk = rem / n_rb, r0 = 32 * (rem - chunk * n_rb);
+    const int t_end = start + (tree ? m : (min(r0 + 32, rows) - 1) / qpk + 1);
     const int lo = chunk * job.clen[c], hi = min(t_end, lo + job.clen[c]);
 
-    const int row = min(n32, rows - 1);
+    const int row = min(r0 + n32, rows - 1);
     const int tok = row / qpk, head = kvh * qpk + row - tok * qpk;
     const int64_t qrow = ((int64_t)(job.tok0[c] + tok) * job.n_q + head) * D;
     const int vis = start + tok + 1;
-    const int vis_min = tree ? start : start + 1;
+    const int vis_min = tree ? start : start + r0 / qpk + 1;
     const uint64_t word = tree ? tree[job.tok0[c] + tok] : 0;
 
     // ---- the planes of this kv head from token lo on
@@ -151,13 +143,13 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
     // behind the last sub-tile stay within the planes or return 0)
     const int n_sub = hi > lo ? (hi - lo + 31) / 32 : 0;
     const int n_i = n_sub > w ? (n_sub - w + kDWaves - 1) / kDWaves : 0;
-    Stage st[kAhead];
+    Stage st[kStages];
     if (n_i > 0)
 #pragma unroll
         for (int k = 0; k < kAhead - 1; k++) load(k, st[k]);
 
     QOp<D, F32> Q;
-    build_q<D, F32>(Q, q, qrow, vec, rsd, h);
+    build_q<D, F32, !F32>(Q, q, qrow, vec, rsd, h);
     v16f O[D / 32];
     float M = kMInit, L = 0.0f, C[GPD];
 #pragma unroll
@@ -167,12 +159,16 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
 #pragma unroll
     for (int g = 0; g < GPD; g++) C[g] = 0.0f;
     uint32_t poison = 0;
+    NibConst nc;
+    nc.hold();
 
-    auto consume = [&](int i, const Stage &st) __attribute__((always_inline)) {
+    auto consume = [&](int i, Stage &st) __attribute__((always_inline)) {
         const int t0 = lo + 32 * (w + kDWaves * i);
         // tokens behind the last have no part in this (their bytes may be anything)
         const bool live = t0 + n32 < t_end;
-        const float zk = zero_nibble(st.ks, st.kb), ck = fmaf(zk, st.ks, st.kb);
+        // (bf16: K's nibbles as they stand, z = 0, everything scaled by 2^-24)
+        const float zk = F32 ? zero_nibble(st.ks, st.kb) : 0.0f;
+        const float ck = F32 ? fmaf(zk, st.ks, st.kb) : scale2(st.kb, -24);
         const float vs = live ? st.vs : 0.0f, vb = live ? st.vb : 0.0f;
         const float zv = zero_nibble(vs, vb), cv = fmaf(zv, vs, vb);
         // ---- scales to LDS
@@ -185,7 +181,7 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
         }
         if constexpr (F32) {
             const float a = fabsf(vs);
-            ev = exp_of(wave_max_fast(a < __builtin_inff() ? a : 0.0f));
+            ev = exp_of(wave_top(a < __builtin_inff() ? a : 0.0f));
             if (owner) {
                 S.vs[GPD == 2 ? h : 0][n32] = vs;
                 S.vc[GPD == 2 ? h : 0][n32] = cv;
@@ -194,7 +190,7 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
             const float a = fmaxf(fabsf(vb), fabsf(fmaf(15.0f, vs, vb)));
             const bool fin = a < __builtin_inff() && vb == vb && vs == vs;
             bad = __ballot(!fin);
-            ev = exp_of(wave_max_fast(fin ? a : 0.0f));
+            ev = exp_of(wave_top(fin ? a : 0.0f));
             if (owner) {
                 S.s16[GPD == 2 ? h : 0][p_step][p_half][pos] = (_Float16)(fin ? scale2(vs, 15 - ev) : 0.0f);
                 S.c16[GPD == 2 ? h : 0][p_step][p_half][pos] = (_Float16)(fin ? scale2(cv, 15 - ev) : 0.0f);
@@ -214,7 +210,7 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
                                                         0, 0);
         }
         float zg[2] = {zk, zk};
-        if constexpr (GPD == 2) {
+        if constexpr (F32 && GPD == 2) {
             const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(zk), __float_as_uint(zk), false,
                                                             false);
             zg[0] = __uint_as_float(r[0]);
@@ -222,7 +218,7 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
         }
 #pragma unroll
         for (int g = 0; g < GPD; g++) {
-            const h2 off = pk(-zg[g], -zg[g]);
+            const h2 off_l = nib_off<false>(zg[g], zg[g]), off_h = nib_off<true>(zg[g], zg[g]);
             const uint32_t x[4] = {st.k[g].x, st.k[g].y, st.k[g].z, st.k[g].w};
             v16f acc;
 #pragma unroll
@@ -233,10 +229,10 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
 #pragma unroll
                 for (int d = 0; d < 2; d++) {
                     const uint32_t x0 = x[2 * o + d], x1 = x0 >> 8;
-                    a[2 * d] = u_of(nib2<false>(x0, off));
-                    a[2 * d + 1] = u_of(nib2<false>(x1, off));
-                    b[2 * d] = u_of(nib2<true>(x0, off));
-                    b[2 * d + 1] = u_of(nib2<true>(x1, off));
+                    a[2 * d] = F32 ? u_of(nib2<false>(x0, off_l, nc)) : nib_sub<false>(x0);
+                    a[2 * d + 1] = F32 ? u_of(nib2<false>(x1, off_l, nc)) : nib_sub<false>(x1);
+                    b[2 * d] = F32 ? u_of(nib2<true>(x0, off_h, nc)) : nib_sub<true>(x0);
+                    b[2 * d + 1] = F32 ? u_of(nib2<true>(x1, off_h, nc)) : nib_sub<true>(x1);
                 }
                 const h8 ka = __builtin_bit_cast(h8, uint4{a[0], a[1], a[2], a[3]});
                 const h8 kb = __builtin_bit_cast(h8, uint4{b[0], b[1], b[2], b[3]});
@@ -264,6 +260,11 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
 #pragma unroll
             for (int ks = 0; ks < 2; ks++)
                 vx[g][ks] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i)(slot + vrd[g] + 16 * ks * RB));
+        if constexpr (F32) {
+            __builtin_amdgcn_sched_barrier(0);
+            load(i + 1, st);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         // ---- softmax
         const bool masked = t0 + 32 > vis_min;
         if (masked) {
@@ -365,8 +366,8 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const uint32_t y = (uint32_t)vx[g][ks][k >> 1] >> (8 * (k & 1));
-                    h2 lo2 = h_of((y & 0x000f000fu) | 0x64006400u) + h_of(zls[k]);
-                    h2 hi2 = h_of((y & 0x00f000f0u) | 0x54005400u) + h_of(zhs[k]);
+                    h2 lo2 = nib2<false>(y, h_of(zls[k]), nc);
+                    h2 hi2 = nib2<true>(y, h_of(zhs[k]), nc);
                     if constexpr (!F32) {
                         const h2 ss = h_of(((const uint32_t *)S.s16[g][ks][h])[k]);
                         const h2 cc = h_of(((const uint32_t *)S.c16[g][ks][h])[k]);
@@ -395,12 +396,12 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
 #pragma unroll
             for (int k = 0; k < kAhead; k++) {
                 if (i + k >= n_i) break;
-                load(i + k + kAhead - 1, st[(k + kAhead - 1) % kAhead]);
-                // all loads but those of the kAhead - 1 sub-tiles behind this one
+                // all loads but those of the sub-tiles behind this one
+                if constexpr (!F32) load(i + k + kAhead - 1, st[(k + kAhead - 1) % kAhead]);
                 __builtin_amdgcn_sched_barrier(0);
-                wait_loads<(kAhead - 1) * kLoads>();
+                wait_loads<F32 ? 0 : (kAhead - 1) * kLoads>();
                 __builtin_amdgcn_sched_barrier(0);
-                consume(i + k, st[k]);
+                consume(i + k, st[F32 ? 0 : k]);
             }
         }
         wait_loads<0>();
@@ -429,7 +430,7 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
 #pragma unroll
                     for (int k = 0; k < 16; k++) O[f][k] = __builtin_nanf("");
     }
-    join_put<D, F32, kDWaves>((float *)lds, w, 0, 1, lane, O, l, M, n32 < rows,
+    join_put<D, F32, kDWaves>((float *)lds, w, lane, O, l, M, r0 + n32 < rows,
                               row_out(job, c, chunk, tok, head, D, qrow, vec, part), out, part);
 }
 

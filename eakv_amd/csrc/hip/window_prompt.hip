@@ -92,15 +92,17 @@ __global__ __launch_bounds__(64 * 4 * (D / 64)) void expand_kernel(eakvd_geom ge
         const float bg = GPD == 2 ? __shfl(b, 32 * g + n32, 64) : b;
         uint32_t lo[4], hi[4];
         const float z = zero_nibble(sg, bg);
-        const h2 off = pk(-z, -z);
+        const h2 off_l = nib_off<false>(z, z), off_h = nib_off<true>(z, z);
+        NibConst nc;
+        nc.hold();
 #pragma unroll
         for (int d = 0; d < 2; d++)
 #pragma unroll
             for (int p = 0; p < 2; p++) {
                 const uint32_t y = xs[d] >> (8 * p);     // bytes p and p + 2
                 if constexpr (F32) {
-                    lo[2 * d + p] = u_of(nib2<false>(y, off));
-                    hi[2 * d + p] = u_of(nib2<true>(y, off));
+                    lo[2 * d + p] = u_of(nib2<false>(y, off_l, nc));
+                    hi[2 * d + p] = u_of(nib2<true>(y, off_h, nc));
                 } else {
                     auto val = [&](uint32_t n) {
                         return scale2(fmaf((float)(n & 15), sg, bg), 15 - e);
@@ -201,7 +203,7 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
     const int64_t qrow = ((int64_t)(job.tok0[c] + tok) * job.n_q + head) * D;
     const int vis = start + tok + 1;
     QOp<D, F32> Q;
-    build_q<D, F32>(Q, q, qrow, vec, rsd, h);
+    build_q<D, F32, false>(Q, q, qrow, vec, rsd, h);
     v16f O[D / 32];
     float M = kMInit, L = 0.0f, C[GPD];
 #pragma unroll
