@@ -11,19 +11,20 @@
 // drawn number lies within 1e-15 of a step.
 //
 // Work: one row of p and one of q per sequence, bound by HBM for large batches and
-// by latency for small ones.  Two launches: each block sums one segment of its
-// sequence's row; one block per sequence then finds the segment and scans it
-// (out of L2).
+// by latency for small ones.  Two launches: each wave sums one segment of its
+// sequence's row; one block per sequence then finds the segment and scans it, in one
+// step up to 2^18 tokens.
 #include "common.h"
 
 namespace {
 
 constexpr int kVerThreads = 256;
+constexpr int kVerStep = 1024;          // values of a wave's step, a multiple of 256
 
 typedef float v4f4 __attribute__((ext_vector_type(4), aligned(4)));
 
 struct VerJob {
-    int k, vocab, n_seg, seg;
+    int k, vocab, n_seg, seg;   // seg: values of a wave's segment
     const int32_t *count, *token;
     const float *draft, *target, *uniform;
     int64_t ld_draft, ld_target;
@@ -88,42 +89,41 @@ __device__ __forceinline__ double wave_sum_d(double v)
 
 __global__ __launch_bounds__(kVerThreads) void verify_sum_kernel(VerJob J)
 {
-    __shared__ double sh[2][kVerThreads / 64];
-    const int s = blockIdx.y, b = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int s = blockIdx.y, lane = threadIdx.x & 63;
+    const int b = (int)blockIdx.x * (kVerThreads / 64) + (threadIdx.x >> 6);
+    if (b >= J.n_seg) return;
     const int n = count_of(J, s);
     const int kept = kept_of(J, s, n, lane);
-    if (b == 0 && tid == 0) J.kept[s] = kept;
+    if (b == 0 && lane == 0) J.kept[s] = kept;
     const Row R = row_of(J, s, n, kept);
     const int lo = b * J.seg, hi = min(J.vocab, lo + J.seg);
     double sr = 0.0, sp = 0.0;
-    int j = lo + 4 * tid;
-    for (; j + 4 <= hi; j += 4 * kVerThreads) {
-        const v4f4 p = *(const v4f4 *)(R.p + j);
-        v4f4 q = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (R.q) q = *(const v4f4 *)(R.q + j);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            sr += R.at((double)p[e], (double)q[e], j + e);
-            sp += p[e] > 0.0f ? (double)p[e] : 0.0;
-        }
-    }
-    for (int e = 0; e < 4 && j + e < hi; e++) {
-        const float p = R.p[j + e];
-        sr += R.at((double)p, R.q ? (double)R.q[j + e] : 0.0, j + e);
+    auto add = [&](float p, float q, int j) {
+        sr += R.at((double)p, (double)q, j);
         sp += p > 0.0f ? (double)p : 0.0;
+    };
+    int j = lo + 4 * lane;
+    // a whole step: all loads in flight before the first sum
+    for (; j - 4 * lane + kVerStep <= hi; j += kVerStep) {
+        v4f4 p[kVerStep / 256], q[kVerStep / 256];
+#pragma unroll
+        for (int i = 0; i < kVerStep / 256; i++) p[i] = *(const v4f4 *)(R.p + j + 256 * i);
+#pragma unroll
+        for (int i = 0; i < kVerStep / 256; i++)
+            q[i] = R.q ? *(const v4f4 *)(R.q + j + 256 * i) : v4f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < kVerStep / 256; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) add(p[i][e], q[i][e], j + 256 * i + e);
     }
+    for (; j < hi; j += 256)
+        for (int e = 0; e < 4 && j + e < hi; e++) add(R.p[j + e], R.q ? R.q[j + e] : 0.0f, j + e);
     sr = wave_sum_d(sr);
     sp = wave_sum_d(sp);
     if (lane == 0) {
-        sh[0][w] = sr;
-        sh[1][w] = sp;
-    }
-    __syncthreads();
-    if (tid == 0) {
         double *o = J.part + ((int64_t)s * J.n_seg + b) * 2;
-        o[0] = (sh[0][0] + sh[0][1]) + (sh[0][2] + sh[0][3]);
-        o[1] = (sh[1][0] + sh[1][1]) + (sh[1][2] + sh[1][3]);
+        o[0] = sr;
+        o[1] = sp;
     }
 }
 
@@ -147,6 +147,16 @@ __device__ __forceinline__ double block_scan(double v, double *sh, int tid, doub
     }
     *total = all;
     return before + v;
+}
+
+// The least `first` and the greatest `last` of a block's threads, both rising with the
+// thread where they are not INT32_MAX or -1: one atomic of a wave.
+__device__ __forceinline__ void least_and_most(int *least, int *most, int first, int last)
+{
+    const uint64_t a = __ballot(first != INT32_MAX), b = __ballot(last >= 0);
+    const int lane = threadIdx.x & 63;
+    if (a && lane == __ffsll((unsigned long long)a) - 1) atomicMin(least, first);
+    if (b && lane == 63 - __clzll((long long)b)) atomicMax(most, last);
 }
 
 __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerJob J)
@@ -180,10 +190,8 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerJob J)
         return;
     }
     const double want = (double)J.uniform[(int64_t)s * (J.k + 1) + J.k] * total;
-    if (tid < J.n_seg && mine > 0.0) {
-        if (cum > want) atomicMin(&s_first, tid);
-        atomicMax(&s_last, tid);
-    }
+    const bool some = tid < J.n_seg && mine > 0.0;
+    least_and_most(&s_first, &s_last, some && cum > want ? tid : INT32_MAX, some ? tid : -1);
     __syncthreads();
     const int b = s_first == INT32_MAX ? s_last : s_first;
     if (tid == b) s_before = cum - mine;
@@ -205,14 +213,16 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerJob J)
         }
         double all;
         double upto = before + (block_scan(sum, sh, tid, &all) - sum);
+        int first = INT32_MAX, last = -1;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             upto += r[e];
             if (r[e] > 0.0) {
-                atomicMax(&s_last, j + e);
-                if (upto > want) atomicMin(&s_first, j + e);
+                last = j + e;
+                if (upto > want && first == INT32_MAX) first = j + e;
             }
         }
+        least_and_most(&s_first, &s_last, first, last);
         __syncthreads();
         if (s_first != INT32_MAX) break;
         before += all;
@@ -220,11 +230,11 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerJob J)
     if (tid == 0) J.next[s] = s_first != INT32_MAX ? s_first : s_last;
 }
 
-// Segments of 1024 values where that leaves the chip unfilled, else of 4096;
-// at most one per thread of the second launch.
-int seg_of(int n_seqs, int vocab)
+// One step of a wave, so that the second launch scans a segment in one step; at most
+// one segment per thread of that launch.
+int seg_of(int vocab)
 {
-    int64_t seg = (int64_t)n_seqs * vocab >= (int64_t)1024 * 4096 ? 4096 : 1024;
+    int64_t seg = kVerStep;
     while ((vocab + seg - 1) / seg > kVerThreads) seg *= 2;
     return (int)seg;
 }
@@ -233,7 +243,7 @@ int seg_of(int n_seqs, int vocab)
 
 extern "C" size_t eakvd_verify_work_bytes(int n_seqs, int vocab)
 {
-    const int seg = seg_of(n_seqs, vocab);
+    const int seg = seg_of(vocab);
     return (size_t)n_seqs * ((vocab + (int64_t)seg - 1) / seg) * 2 * sizeof(double);
 }
 
@@ -245,7 +255,7 @@ extern "C" int eakvd_verify(int n_seqs, int k, int vocab, const int32_t *count, 
     VerJob J;
     J.k = k;
     J.vocab = vocab;
-    J.seg = seg_of(n_seqs, vocab);
+    J.seg = seg_of(vocab);
     J.n_seg = (int)((vocab + (int64_t)J.seg - 1) / J.seg);
     J.count = count;
     J.token = token;
@@ -258,8 +268,9 @@ extern "C" int eakvd_verify(int n_seqs, int k, int vocab, const int32_t *count, 
     J.next = next;
     J.part = (double *)work;
     const hipStream_t st = (hipStream_t)stream;
-    hipLaunchKernelGGL(verify_sum_kernel, dim3((unsigned)J.n_seg, (unsigned)n_seqs), dim3(kVerThreads),
-                       0, st, J);
+    hipLaunchKernelGGL(verify_sum_kernel,
+                       dim3((unsigned)((J.n_seg + kVerThreads / 64 - 1) / (kVerThreads / 64)), (unsigned)n_seqs),
+                       dim3(kVerThreads), 0, st, J);
     hipLaunchKernelGGL(verify_pick_kernel, dim3((unsigned)n_seqs), dim3(kVerThreads), 0, st, J);
     return (int)hipGetLastError();
 }

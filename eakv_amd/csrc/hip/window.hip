@@ -74,13 +74,17 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WinJob job, const flo
         const float al = lane < n && x.y != 0.0f ? __builtin_amdgcn_exp2f(x.x - m) : 0.0f;
         l = fmaf(al, x.y, l);
         const float *po = part + (first + k0 * per) * D + lane * E;
-#pragma unroll 8
-        for (int k = 0; k < n; k++) {
-            const float a = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(al), k));
+        for (int k8 = 0; k8 < n; k8 += 8) {
+            float v[8][E];
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                const float v = po[k * per * D + e];
-                o[e] = a != 0.0f ? fmaf(a, v, o[e]) : o[e];
+            for (int k = 0; k < 8; k++)
+#pragma unroll
+                for (int e = 0; e < E; e++) v[k][e] = po[min(k8 + k, n - 1) * per * D + e];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float a = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(al), k8 + k));
+#pragma unroll
+                for (int e = 0; e < E; e++) o[e] = a != 0.0f ? fmaf(a, v[k][e], o[e]) : o[e];
             }
         }
     }
@@ -113,8 +117,8 @@ size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 // share a kv head: where so many blocks convert the same bytes that the converted
 // values' way through memory costs less.  Expanded / not, in us: 264 rows of 8 at 10000
 // bf16 291 / 231, f32 476 / 386; 512 of 8 at 10000 330 / 313, 531 / 519; 768 at 30000
-// 154 / 208, 293 / 375; 1024 at 30000 185 / 211, 440 / 373; 1024 of 4 at 30000 693 / 825, 1344 / 1488; 2100 of 4 at 4000, d = 64
-// 57 / 70, 86 / 100.
+// 154 / 208, 293 / 375; 1024 at 30000 185 / 211, 440 / 373; 1024 of 4 at 30000 693 / 825,
+// 1344 / 1488; 2100 of 4 at 4000, d = 64 57 / 70, 86 / 100.
 bool is_many(int ntok, int qpk)
 {
     return ntok > EAKVD_TREE_MAX && (int64_t)ntok * qpk > 512;
