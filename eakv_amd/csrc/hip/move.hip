@@ -4,8 +4,9 @@
 // byte of a token is read once and written once (copy: once per destination).
 //
 // A row is one kv head of one (layer, kv) block: its tokens' packed bytes, scales
-// and biases, each contiguous.  A block moves 1024 groups of a row (40 KB), all
-// its loads in flight before the first store.
+// and biases, each contiguous.  A block of the copy moves 1024 groups of a row (40 KB),
+// all its loads in flight before the first store: 32768 tokens of 4 layers x 8 heads,
+// d = 128, into 4 caches take 159 us (839 MB, 5.3 TB/s, what a large copy reaches).
 #include "common.h"
 
 namespace {
@@ -83,12 +84,23 @@ __global__ __launch_bounds__(kMoveThreads) void copy_kernel(eakvd_geom gs, eakvd
 // all loads are done (the barrier) before the first store.  Positions are
 // clamped to the cache's room (in place: from dst_pos + i on), so that any list
 // stays within the planes.
+//
+// 13001 of 30011 tokens, 8 layers of 8 heads, d = 128: 80 us a call in a row of them
+// (3.35 TB/s of 266 MB; contiguous tokens 66 us): tokens of 64 packed bytes fill half of
+// a 128-byte line, and a list that skips tokens fetches lines for one of the two.
+// Passes of 256 groups against 1024: 80 against 86 us; with loads past the caches,
+// 83 and 93; with stores through them, 93 and more.  In place the passes wait for one
+// another, and the longer ones are kept.
+template <bool SERIAL>
+constexpr int kGatherGroups = SERIAL ? kMoveGroups : 256;
+
 template <int GPD, bool SERIAL>
 __global__ __launch_bounds__(kMoveThreads) void gather_kernel(eakvd_geom gs, eakvd_geom gd,
                                                               eakvd_gather job, int rows_per,
                                                               int n_rows)
 {
-    constexpr int T = kMoveGroups / GPD;                         // tokens of a pass
+    constexpr int G = kGatherGroups<SERIAL>, T = G / GPD;        // groups, tokens of a pass
+    constexpr int W = G * 2 / kMoveThreads, S = G / kMoveThreads;
     const int tid = threadIdx.x;
     for (int row = blockIdx.y; row < n_rows; row += gridDim.y) {
         const int c = row / rows_per, r = row - c * rows_per;
@@ -108,16 +120,16 @@ __global__ __launch_bounds__(kMoveThreads) void gather_kernel(eakvd_geom gs, eak
                 t = t < low ? low : t > top ? top : t;
                 return s0 + (int64_t)t * GPD + g % GPD;
             };
-            v4u x[kMoveW];
-            float a[kMoveS], b[kMoveS];
+            v4u x[W];
+            float a[S], b[S];
 #pragma unroll
-            for (int k = 0; k < kMoveW; k++) {
+            for (int k = 0; k < W; k++) {
                 const int i = tid + k * kMoveThreads;
                 if (i < 2 * cnt)
-                    x[k] = __builtin_nontemporal_load((const v4u *)(sb + from(i >> 1) * 32) + (i & 1));
+                    x[k] = ((const v4u *)(sb + from(i >> 1) * 32))[i & 1];
             }
 #pragma unroll
-            for (int k = 0; k < kMoveS; k++) {
+            for (int k = 0; k < S; k++) {
                 const int i = tid + k * kMoveThreads;
                 if (i < cnt) {
                     const int64_t g = from(i);
@@ -135,12 +147,12 @@ __global__ __launch_bounds__(kMoveThreads) void gather_kernel(eakvd_geom gs, eak
             float *ds = (float *)(db + gd.s_off) + d;
             float *dc = (float *)(db + gd.b_off) + d;
 #pragma unroll
-            for (int k = 0; k < kMoveW; k++) {
+            for (int k = 0; k < W; k++) {
                 const int i = tid + k * kMoveThreads;
                 if (i < 2 * cnt) __builtin_nontemporal_store(x[k], dw + i);
             }
 #pragma unroll
-            for (int k = 0; k < kMoveS; k++) {
+            for (int k = 0; k < S; k++) {
                 const int i = tid + k * kMoveThreads;
                 if (i < cnt) {
                     __builtin_nontemporal_store(a[k], ds + i);
@@ -188,7 +200,7 @@ extern "C" int eakvd_gather_tokens(const eakvd_geom *gs, const eakvd_geom *gd,
     const int per = 2 * gs->n_layers * gs->n_kv_heads;
     const int64_t rows = (int64_t)per * job->n_seq;
     if (rows > INT32_MAX) return (int)hipErrorInvalidValue;
-    const int t = kMoveGroups / (int)gs->gpd;
+    const int t = kGatherGroups<false> / (int)gs->gpd;
     const dim3 grid(serial ? 1u : (unsigned)((most + t - 1) / t), grid_y(rows));
     auto *kern = gs->gpd == 2 ? (serial ? gather_kernel<2, true> : gather_kernel<2, false>)
                               : (serial ? gather_kernel<1, true> : gather_kernel<1, false>);
