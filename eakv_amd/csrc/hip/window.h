@@ -38,15 +38,12 @@ constexpr int kExpLow = -60;           // tile exponents below this count as thi
 
 __device__ __forceinline__ uint32_t u_of(h2 v) { return __builtin_bit_cast(uint32_t, v); }
 __device__ __forceinline__ h2 h_of(uint32_t v) { return __builtin_bit_cast(h2, v); }
-// Two roundings to nearest even.  The empty asm statements (no instruction that
-// the compiler's hazard handling would miss behind a transcendental) hold a and b
-// to f32 and the result to one rounding: the compiler otherwise rounds a product
-// straight to f16 in one place and by way of f32 in another, and a pair's low part
-// must be what the high part left.
+// Two roundings to nearest even.  The empty asm (no instruction that the compiler's
+// hazard handling would miss behind a transcendental) holds the result to one rounding:
+// the compiler otherwise rounds a product straight to f16 in one place and by way of
+// f32 in another, and a pair's low part must be what the high part left.
 __device__ __forceinline__ h2 pk(float a, float b)
 {
-    asm("" : "+v"(a));
-    asm("" : "+v"(b));
     typedef float f2 __attribute__((ext_vector_type(2)));
     uint32_t r = u_of(__builtin_convertvector((f2{a, b}), h2));
     asm("" : "+v"(r));
@@ -58,10 +55,14 @@ __device__ __forceinline__ h2 pk_exp(float a, float b)
     typedef float f2 __attribute__((ext_vector_type(2)));
     return __builtin_convertvector((f2{a, b}), h2);
 }
-// what pk(a, b) left of a and b, exact, in f16
+// What pk(a, b) left of a and b, in f16 (the differences are exact in f32).  minus: -1
+// in a register, or else the compiler makes a conversion, a difference and another
+// conversion of what is one v_fma_mix of each value.
 __device__ __forceinline__ h2 pk_rest(h2 hi, float a, float b)
 {
-    return pk(fmaf((float)hi[0], -1.0f, a), fmaf((float)hi[1], -1.0f, b));
+    float minus = -1.0f;
+    asm("" : "+s"(minus));
+    return h2{(_Float16)fmaf((float)hi[0], minus, a), (_Float16)fmaf((float)hi[1], minus, b)};
 }
 
 // n - z of the low (HI false) or high nibbles of bytes 0 and 2 of x, exact: the
@@ -111,12 +112,6 @@ __device__ __forceinline__ int exp_of(float a)
 __device__ __forceinline__ float scale2(float x, int e)
 {
     return __builtin_amdgcn_ldexpf(x, e);
-}
-
-// p * v, 0 * anything = 0: a hidden token's scale or bias may be non-finite
-__device__ __forceinline__ float mul_hidden(float p, float v)
-{
-    return p == 0.0f ? 0.0f : p * v;
 }
 
 // Three bf16 pieces of x, together 24 bits.

@@ -135,7 +135,7 @@ int64_t few_share(int64_t tiles, int cus)
 
 // Tiles of a chunk, win_prompt: the split of the longest context in k that ends first,
 // by a model of a launch in tile times (256 rows x 32 tokens: about 1.05 us at d = 128
-// in bf16, 1.6 in f32).  Blocks beyond the chip's slots run as slots come free, the
+// in bf16, 2.2 in f32).  Blocks beyond the chip's slots run as slots come free, the
 // longest first; partials are written and read at about 5 TB/s, the merge is
 // a launch of its own.
 int64_t many_share(const WinJob &j, int64_t tiles, int cus, int head_dim, bool bf16)
@@ -148,7 +148,7 @@ int64_t many_share(const WinJob &j, int64_t tiles, int cus, int head_dim, bool b
         blocks += (r + 255) / 256 * j.n_kv;
         rows += r * j.n_kv;
     }
-    const double tile_us = (bf16 ? 1.05 : 1.6) * head_dim / 128;
+    const double tile_us = (bf16 ? 1.05 : 2.2) * head_dim / 128;
     const double merge_k = 2.0 * rows * (head_dim + 2) * 4 / 5e6 / tile_us, merge_0 = 6 / tile_us;
     double best = 0;
     int64_t share = longest;

@@ -169,34 +169,31 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
         // (bf16: K's nibbles as they stand, z = 0, everything scaled by 2^-24)
         const float zk = F32 ? zero_nibble(st.ks, st.kb) : 0.0f;
         const float ck = F32 ? fmaf(zk, st.ks, st.kb) : scale2(st.kb, -24);
-        const float vs = live ? st.vs : 0.0f, vb = live ? st.vb : 0.0f;
+        // (a non-finite group counts as zeros and makes the rows that see it NaN)
+        const float va = fmaxf(fabsf(st.vb), fabsf(fmaf(15.0f, st.vs, st.vb)));
+        const bool fin = va < __builtin_inff() && st.vs == st.vs;
+        const uint64_t bad = __ballot(live && !fin);
+        const float vs = live && fin ? st.vs : 0.0f, vb = live && fin ? st.vb : 0.0f;
         const float zv = zero_nibble(vs, vb), cv = fmaf(zv, vs, vb);
         // ---- scales to LDS
-        uint64_t bad = 0;
-        int ev;
         if (owner) S.ks[GPD == 2 ? h : 0][n32] = st.ks;
         if (owner) {
             S.zl[GPD == 2 ? h : 0][p_step][p_half][pos] = (_Float16)(-1024.0f - zv);
             S.zh[GPD == 2 ? h : 0][p_step][p_half][pos] = (_Float16)(-64.0f - zv);
         }
+        const int ev = __builtin_amdgcn_readfirstlane(
+            exp_of(wave_top(F32 ? fabsf(vs) : live && fin ? va : 0.0f)));
         if constexpr (F32) {
-            const float a = fabsf(vs);
-            ev = exp_of(wave_top(a < __builtin_inff() ? a : 0.0f));
             if (owner) {
                 S.vs[GPD == 2 ? h : 0][n32] = vs;
                 S.vc[GPD == 2 ? h : 0][n32] = cv;
             }
         } else {
-            const float a = fmaxf(fabsf(vb), fabsf(fmaf(15.0f, vs, vb)));
-            const bool fin = a < __builtin_inff() && vb == vb && vs == vs;
-            bad = __ballot(!fin);
-            ev = exp_of(wave_top(fin ? a : 0.0f));
             if (owner) {
-                S.s16[GPD == 2 ? h : 0][p_step][p_half][pos] = (_Float16)(fin ? scale2(vs, 15 - ev) : 0.0f);
-                S.c16[GPD == 2 ? h : 0][p_step][p_half][pos] = (_Float16)(fin ? scale2(cv, 15 - ev) : 0.0f);
+                S.s16[GPD == 2 ? h : 0][p_step][p_half][pos] = (_Float16)scale2(vs, 15 - ev);
+                S.c16[GPD == 2 ? h : 0][p_step][p_half][pos] = (_Float16)scale2(cv, 15 - ev);
             }
         }
-        ev = __builtin_amdgcn_readfirstlane(ev);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         // ---- scores
         v16f s;
@@ -293,17 +290,15 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
 #pragma unroll
                 for (int g = 0; g < GPD; g++) C[g] *= al;
         }
-        if constexpr (!F32) {
-            if (bad) {
-                // rows that see a token with a non-finite V group
-                uint32_t seen = 0;
+        if (bad) {
+            // rows that see a token with a non-finite V group
+            uint32_t seen = 0;
 #pragma unroll
-                for (int k = 0; k < 16; k++)
-                    seen |= s[k] != -__builtin_inff() ? 1u << (8 * (k >> 2) + (k & 3)) : 0u;
-                seen <<= 4 * h;
-                poison |= (seen & (uint32_t)bad ? 1u : 0u) |
-                          (GPD == 2 && (seen & (uint32_t)(bad >> 32)) ? 2u : 0u);
-            }
+            for (int k = 0; k < 16; k++)
+                seen |= s[k] != -__builtin_inff() ? 1u << (8 * (k >> 2) + (k & 3)) : 0u;
+            seen <<= 4 * h;
+            poison |= (seen & (uint32_t)bad ? 1u : 0u) |
+                      (GPD == 2 && (seen & (uint32_t)(bad >> 32)) ? 2u : 0u);
         }
         const float mr = F32 ? -M : (float)ev - M;
         float p[16];
@@ -326,13 +321,8 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
                     float x[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        if (masked) {
-                            x[e] = mul_hidden(p[4 * k + e], sc[e]);
-                            cs += mul_hidden(p[4 * k + e], cc[e]);
-                        } else {
-                            x[e] = p[4 * k + e] * sc[e];
-                            cs = fmaf(p[4 * k + e], cc[e], cs);
-                        }
+                        x[e] = p[4 * k + e] * sc[e];
+                        cs = fmaf(p[4 * k + e], cc[e], cs);
                     }
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
@@ -422,14 +412,14 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
         for (int f = 0; f < D / 32; f++)
 #pragma unroll
             for (int k = 0; k < 16; k++) O[f][k] *= 0x1p-15f;          // V's operands carried 2^15
-        poison |= __shfl_xor(poison, 32, 64);
-        if (poison)
-#pragma unroll
-            for (int f = 0; f < D / 32; f++)
-                if (poison >> (f >> 1) & 1)
-#pragma unroll
-                    for (int k = 0; k < 16; k++) O[f][k] = __builtin_nanf("");
     }
+    poison |= __shfl_xor(poison, 32, 64);
+    if (poison)
+#pragma unroll
+        for (int f = 0; f < D / 32; f++)
+            if (poison >> (f >> 1) & 1)
+#pragma unroll
+                for (int k = 0; k < 16; k++) O[f][k] = __builtin_nanf("");
     join_put<D, F32, kDWaves>((float *)lds, w, lane, O, l, M, r0 + n32 < rows,
                               row_out(job, c, chunk, tok, head, D, qrow, vec, part), out, part);
 }

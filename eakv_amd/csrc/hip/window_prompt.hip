@@ -11,12 +11,10 @@
 // to f16, 2^-12 relative.  f32 queries: n - z, exact, with the scales and biases
 // beside them, as in window.hip.
 //
-// Attention: 4 waves per block, one per SIMD, 64 rows each: every operand read from
-// LDS serves two products (at 32 rows a wave the reads would take as long as the
-// products).  Software pipeline over 32-token sub-tiles: the scores of the next one
-// are computed beside the softmax and the weighted sum of this one, as the matrix
-// cores and the vector ALUs of a SIMD run beside one another.  A ring of 8 sub-tiles
-// in LDS, loads 6 ahead, one barrier per sub-tile.
+// Attention: 8 waves per block, two per SIMD, 32 rows each, through a ring of 8 sub-tiles
+// in LDS with a barrier every kStep.  A step of a wave is the products (the next
+// sub-tile's scores and this one's weighted sum), then the softmax; a SIMD's two
+// waves are in different halves of it.  bf16 operands are read ahead of their step.
 #include <string.h>
 
 #include "window.h"
@@ -51,7 +49,7 @@ struct Img {
 struct Meta {
     float ek;                           // bf16: the K operands are values * 1/ek
     int ev;                             // exponent of V; kSomeBad added where bad is not 0
-    uint32_t bad[2];                    // bf16: tokens with non-finite V, by group
+    uint32_t bad[2];                    // tokens with non-finite V, by group
 };
 constexpr int kSomeBad = 1 << 16;
 
@@ -81,9 +79,9 @@ __global__ __launch_bounds__(64 * 4 * (D / 64)) void expand_kernel(eakvd_geom ge
     const int64_t tn = min(t0 + n32, t_last);
     const int64_t gi = g0 + tn * GPD + (GPD == 2 ? h : 0);
     const float s = P.s[gi], b = P.b[gi];
-    const float a = F32 && is_v ? fabsf(s) : fmaxf(fabsf(b), fabsf(fmaf(15.0f, s, b)));
-    const bool fin = a < __builtin_inff() && s == s && b == b;
-    const int e = exp_of(wave_top(fin ? a : 0.0f));
+    const float a = fmaxf(fabsf(b), fabsf(fmaf(15.0f, s, b)));
+    const bool fin = a < __builtin_inff() && s == s;
+    const int e = exp_of(wave_top(!fin ? 0.0f : F32 && is_v ? fabsf(s) : a));
     if (!is_v) {
         if (g == 0 && x == 0 && lane == 0) meta[blockIdx.x].ek = scale2(1.0f, e - 15);
         const uint2 by = *(const uint2 *)(P.w + (g0 + tn * GPD + g) * 32 + 16 * h + 8 * x);
@@ -128,7 +126,7 @@ __global__ __launch_bounds__(64 * 4 * (D / 64)) void expand_kernel(eakvd_geom ge
     } else {
         const uint64_t bad = __ballot(!fin);
         if (g == 0 && x == 0 && lane == 0) {
-            meta[blockIdx.x].ev = e + (!F32 && bad ? kSomeBad : 0);
+            meta[blockIdx.x].ev = e + (bad ? kSomeBad : 0);
             meta[blockIdx.x].bad[0] = (uint32_t)bad;
             meta[blockIdx.x].bad[1] = GPD == 2 ? (uint32_t)(bad >> 32) : 0;
         }
@@ -160,9 +158,10 @@ __global__ __launch_bounds__(64 * 4 * (D / 64)) void expand_kernel(eakvd_geom ge
                         u_of(pk(v1[5], v1[7]))};
         if constexpr (F32) {
             if (g == 0 && x == 0 && (GPD == 2 || h == 0)) {
+                // (a non-finite group counts as zeros and makes the rows that see it NaN)
                 const float z = zero_nibble(s, b);
-                ((float *)(o + I::VS))[lane] = s;
-                ((float *)(o + I::VC))[lane] = fmaf(z, s, b);
+                ((float *)(o + I::VS))[lane] = fin ? s : 0.0f;
+                ((float *)(o + I::VC))[lane] = fin ? fmaf(z, s, b) : 0.0f;
             }
         }
     }
@@ -314,11 +313,11 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
     };
 
     // vector phase: scores, M, weights
-    uint32_t poison = 0;                // bf16: groups of this row that are NaN
+    uint32_t poison = 0;                // groups of this row that are NaN
     auto softmax = [&](int i) __attribute__((always_inline)) {
         const uint8_t *t = lds + (i & (kRing - 1)) * I::BYTES;
         const int ev_b = F32 ? __builtin_amdgcn_readlane(m_ev, i & 63) : m_ev;
-        const int ev = F32 || ev_b < kSomeBad / 2 ? ev_b : ev_b - kSomeBad;
+        const int ev = ev_b < kSomeBad / 2 ? ev_b : ev_b - kSomeBad;
         v16f &s = S[0];
         if constexpr (F32) {
 #pragma unroll
@@ -356,16 +355,14 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
 #pragma unroll
                 for (int g = 0; g < GPD; g++) C[g] *= al;
         }
-        if constexpr (!F32) {
-            if (ev_b >= kSomeBad / 2) {
-                // rows that see a token with a non-finite V group
-                uint32_t seen = 0;
+        if (ev_b >= kSomeBad / 2) {
+            // rows that see a token with a non-finite V group
+            uint32_t seen = 0;
 #pragma unroll
-                for (int k = 0; k < 16; k++)
-                    seen |= s[k] != -__builtin_inff() ? 1u << (8 * (k >> 2) + (k & 3)) : 0u;
-                seen <<= 4 * h;
-                poison |= (seen & mt[i].bad[0] ? 1u : 0u) | (seen & mt[i].bad[1] ? 2u : 0u);
-            }
+            for (int k = 0; k < 16; k++)
+                seen |= s[k] != -__builtin_inff() ? 1u << (8 * (k >> 2) + (k & 3)) : 0u;
+            seen <<= 4 * h;
+            poison |= (seen & mt[i].bad[0] ? 1u : 0u) | (seen & mt[i].bad[1] ? 2u : 0u);
         }
         const float mr = F32 ? -M : (float)ev - M;
         float p[16];
@@ -384,18 +381,10 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
                     const v4f sc = *(const v4f *)((const float *)(t + I::VS) + 32 * g + 8 * k + 4 * h);
                     const v4f cc = *(const v4f *)((const float *)(t + I::VC) + 32 * g + 8 * k + 4 * h);
                     float x[4];
-                    if (masked) {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            x[e] = mul_hidden(p[4 * k + e], sc[e]);
-                            cs += mul_hidden(p[4 * k + e], cc[e]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            x[e] = p[4 * k + e] * sc[e];
-                            cs = fmaf(p[4 * k + e], cc[e], cs);
-                        }
+                    for (int e = 0; e < 4; e++) {
+                        x[e] = p[4 * k + e] * sc[e];
+                        cs = fmaf(p[4 * k + e], cc[e], cs);
                     }
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
@@ -465,14 +454,14 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
         for (int f = 0; f < D / 32; f++)
 #pragma unroll
             for (int k = 0; k < 16; k++) O[f][k] *= 0x1p-15f;          // V's operands carried 2^15
-        poison |= __shfl_xor(poison, 32, 64);
-        if (poison)
-#pragma unroll
-            for (int f = 0; f < D / 32; f++)
-                if (poison >> (f >> 1) & 1)
-#pragma unroll
-                    for (int k = 0; k < 16; k++) O[f][k] = __builtin_nanf("");
     }
+    poison |= __shfl_xor(poison, 32, 64);
+    if (poison)
+#pragma unroll
+        for (int f = 0; f < D / 32; f++)
+            if (poison >> (f >> 1) & 1)
+#pragma unroll
+                for (int k = 0; k < 16; k++) O[f][k] = __builtin_nanf("");
     if (r0 + n32 < rows)
         put_rows<D, F32>(row_out(job, c, chunk, tok, head, D, qrow, vec, part), O, l, M, h, out, part);
 }
