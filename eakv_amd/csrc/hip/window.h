@@ -123,34 +123,32 @@ __device__ __forceinline__ void pieces(float x, __bf16 &a, __bf16 &b, __bf16 &c)
     c = (__bf16)__fsub_rn(r, (float)b);
 }
 
-// The 8 consecutive dims of one operand (a multiple of 8 dims from the row's
-// start) as f32.  Rows of q are 16-byte aligned or read by elements.
-template <bool F32>
-__device__ __forceinline__ void load_q8(const void *q, int64_t at, bool vec, float *o)
+// A lane's share of a row of q as it stands in memory: the 8 consecutive dims of each
+// operand (QOp).  Rows are 16-byte aligned (vec) or read by elements.
+template <int D, bool F32>
+struct QRaw {
+    uint4 x[F32 ? D / 8 : D / 16];
+};
+
+template <int D, bool F32>
+__device__ __forceinline__ void load_q(QRaw<D, F32> &r, const void *q, int64_t qrow, bool vec, int h)
 {
-    if constexpr (F32) {
-        const float *p = (const float *)q + at;
-        if (vec) {
-            const v4f a = *(const v4f *)p, b = *(const v4f *)(p + 4);
+    constexpr int W = F32 ? 2 : 1;                   // 16-byte pieces of an operand
 #pragma unroll
-            for (int j = 0; j < 4; j++) { o[j] = a[j]; o[4 + j] = b[j]; }
-        } else {
+    for (int f = 0; f < D / 16; f++) {
+        const int64_t at = qrow + (f >> 2) * 64 + 32 * (f & 1) + 16 * h + 8 * ((f >> 1) & 1);
 #pragma unroll
-            for (int j = 0; j < 8; j++) o[j] = p[j];
-        }
-    } else {
-        const uint16_t *p = (const uint16_t *)q + at;
-        if (vec) {
-            const uint4 a = *(const uint4 *)p;
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                o[2 * j] = __uint_as_float(w[j] << 16);
-                o[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        for (int j = 0; j < W; j++) {
+            if (vec) {
+                r.x[W * f + j] = *(const uint4 *)((const uint8_t *)q + at * (F32 ? 4 : 2) + 16 * j);
+            } else if constexpr (F32) {
+                const uint32_t *p = (const uint32_t *)q + at + 4 * j;
+                r.x[W * f + j] = uint4{p[0], p[1], p[2], p[3]};
+            } else {
+                const uint16_t *p = (const uint16_t *)q + at;
+                r.x[f] = uint4{p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16,
+                               p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16};
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) o[j] = __uint_as_float((uint32_t)p[j] << 16);
         }
     }
 }
@@ -178,6 +176,13 @@ __device__ __forceinline__ void store4(void *out, int64_t at, bool vec, const fl
     }
 }
 
+// The maximum of a lane's value and the other half's (lane ^ 32), in both.
+__device__ __forceinline__ float half_max(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // A row's query as the columns' operand of S^T = K Q^T, one lane's share: operand
 // (g, octet o, nibble n) of half h holds dims 64g + 32n + 16h + 8o + 0..7 in nib2's
 // order (0 2 1 3 4 6 5 7).  The row is scaled by a power of two to below 2^15.
@@ -192,53 +197,57 @@ struct QOp {
 };
 
 template <int D, bool F32, bool SUB>
-__device__ __forceinline__ void build_q(QOp<D, F32> &Q, const void *q, int64_t qrow, bool vec,
-                                        float rsd, int h)
+__device__ __forceinline__ void build_q(QOp<D, F32> &Q, const QRaw<D, F32> &raw, float rsd, int h)
 {
     constexpr int GPD = D / 64;
-    float x[GPD * 4][8];
+    auto dim = [&](int f, int j) {                   // dim j of operand f
+        if constexpr (F32) {
+            const uint4 &x = raw.x[2 * f + (j >> 2)];
+            return __uint_as_float((j & 3) == 0 ? x.x : (j & 3) == 1 ? x.y : (j & 3) == 2 ? x.z : x.w);
+        } else {
+            const uint4 &x = raw.x[f];
+            const uint32_t y = (j >> 1) == 0 ? x.x : (j >> 1) == 1 ? x.y : (j >> 1) == 2 ? x.z : x.w;
+            return __uint_as_float(j & 1 ? y & 0xffff0000u : y << 16);
+        }
+    };
     float top = 0.0f;
 #pragma unroll
-    for (int g = 0; g < GPD; g++)
+    for (int f = 0; f < D / 16; f++)
 #pragma unroll
-        for (int o = 0; o < 2; o++)
-#pragma unroll
-            for (int n = 0; n < 2; n++) {
-                float *xx = x[g * 4 + o * 2 + n];
-                load_q8<F32>(q, qrow + g * 64 + 32 * n + 16 * h + 8 * o, vec, xx);
-#pragma unroll
-                for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(xx[j]));
-            }
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
+        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(dim(f, j)));
+    top = half_max(top);
     // q' = q * 2^(15 - e); a row of zeros or below 2^-110 keeps e = -110
     int e = (int)(__float_as_uint(top) >> 23) - 126;
     e = e < -110 ? -110 : e;
+    const float scale = scale2(1.0f, 15 - e), less = SUB ? scale * 0x1p-4f : scale;
     float qs[GPD];
 #pragma unroll
     for (int g = 0; g < GPD; g++) {
-        qs[g] = 0.0f;
+        v16f sum;                                    // of the group's 64 dims, in every register
 #pragma unroll
-        for (int f = 0; f < 4; f++) {
-            float y[8];
+        for (int k = 0; k < 16; k++) sum[k] = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = scale2(x[g * 4 + f][j], 15 - e);
-            qs[g] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
-            if (SUB && (f & 1))
-#pragma unroll
-                for (int j = 0; j < 8; j++) y[j] *= 0x1p-4f;
+        for (int f = 4 * g; f < 4 * g + 4; f++) {
+            const float by = f & 1 ? less : scale;
+            const _Float16 one = (_Float16)(SUB && (f & 1) ? 16.0f : 1.0f);
+            const h8 ones = h8{one, one, one, one, one, one, one, one};
             uint32_t a[4], b[4];
 #pragma unroll
             for (int p = 0; p < 4; p++) {
                 const int j = (p >> 1) * 4 + (p & 1);
-                const h2 hi2 = pk(y[j], y[j + 2]);
+                const float y0 = dim(f, j) * by, y1 = dim(f, j + 2) * by;
+                const h2 hi2 = pk(y0, y1);
                 a[p] = u_of(hi2);
-                if constexpr (F32) b[p] = u_of(pk_rest(hi2, y[j], y[j + 2]));
+                if constexpr (F32) b[p] = u_of(pk_rest(hi2, y0, y1));
             }
-            Q.a[g * 4 + f] = __builtin_bit_cast(h8, uint4{a[0], a[1], a[2], a[3]});
-            if constexpr (F32)
-                Q.b[g * 4 + f] = __builtin_bit_cast(h8, uint4{b[0], b[1], b[2], b[3]});
+            Q.a[f] = __builtin_bit_cast(h8, uint4{a[0], a[1], a[2], a[3]});
+            sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(ones, Q.a[f], sum, 0, 0, 0);
+            if constexpr (F32) {
+                Q.b[f] = __builtin_bit_cast(h8, uint4{b[0], b[1], b[2], b[3]});
+                sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(ones, Q.b[f], sum, 0, 0, 0);
+            }
         }
-        qs[g] += __shfl_xor(qs[g], 32, 64);
+        qs[g] = sum[0];
     }
     Q.rf = scale2(rsd * EAKV_LOG2E, e - 15 + (SUB ? 24 : 0));
     // half h of the bias product's 16 terms: group h's sum of q in pieces,
@@ -248,13 +257,6 @@ __device__ __forceinline__ void build_q(QOp<D, F32> &Q, const void *q, int64_t q
     pieces(z, p1, p2, p3);
     const __bf16 zero = (__bf16)0.0f;
     Q.bias = b8{p1, p2, p3, p1, p2, p1, zero, zero};
-}
-
-// The maximum of a lane's value and the other half's (lane ^ 32), in both.
-__device__ __forceinline__ float half_max(float v)
-{
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 // The maximum of a wave's values, in all lanes
@@ -346,11 +348,12 @@ __device__ __forceinline__ void join_put(float *lds, int wt, int lane,
     const int h = lane >> 5;
     __syncthreads();
     {
-        float *po = lds + (size_t)wt * OW + lane;
+        v4f *po = (v4f *)(lds + (size_t)wt * OW) + lane;
 #pragma unroll
         for (int f = 0; f < D / 32; f++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) po[(f * 16 + i) * 64] = o[f][i];
+            for (int i = 0; i < 4; i++)
+                po[(f * 4 + i) * 64] = v4f{o[f][4 * i], o[f][4 * i + 1], o[f][4 * i + 2], o[f][4 * i + 3]};
         ml[wt * 128 + lane] = m;
         ml[wt * 128 + 64 + lane] = l;
     }
@@ -372,9 +375,9 @@ __device__ __forceinline__ void join_put(float *lds, int wt, int lane,
         float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int t = 0; t < WT; t++) {
-            const float *po = lds + (size_t)t * OW + lane + e * 64;
+            const v4f po = ((const v4f *)(lds + (size_t)t * OW))[(e >> 2) * 64 + lane];
 #pragma unroll
-            for (int j = 0; j < 4; j++) x[j] = fmaf(a[t], po[j * 64], x[j]);
+            for (int j = 0; j < 4; j++) x[j] = fmaf(a[t], po[j], x[j]);
         }
         if (live) put4<F32>(r, 32 * (e >> 4) + 8 * ((e & 15) >> 2) + 4 * h, x, ll, out, part);
     }
@@ -387,6 +390,7 @@ __device__ __forceinline__ void join_put(float *lds, int wt, int lane,
 // The sequence of block b: the last one whose first block is not behind it.
 __device__ __forceinline__ int seq_of(const int *pre, int n_seq, int b, int lane)
 {
+    if (n_seq == 1) return 0;
     // (pre has EAKVD_MAX_BATCH entries at least)
     const bool past = lane > 0 && lane < n_seq && b >= pre[lane < EAKVD_MAX_BATCH ? lane : 0];
     return (int)__popcll(__ballot(past));

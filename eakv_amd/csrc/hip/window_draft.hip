@@ -139,8 +139,10 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
     const int p_step = n32 >> 4, p_half = (n32 >> 2) & 1;
     const bool owner = GPD == 2 || h == 0;
 
-    // this wave's sub-tiles; the first loads are on their way while Q is made (loads
-    // behind the last sub-tile stay within the planes or return 0)
+    // this wave's sub-tiles; the first loads are on their way while Q is made, behind Q's
+    // own (loads behind the last sub-tile stay within the planes or return 0)
+    QRaw<D, F32> raw;
+    load_q<D, F32>(raw, q, qrow, vec, h);
     const int n_sub = hi > lo ? (hi - lo + 31) / 32 : 0;
     const int n_i = n_sub > w ? (n_sub - w + kDWaves - 1) / kDWaves : 0;
     Stage st[kStages];
@@ -149,7 +151,7 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
         for (int k = 0; k < kAhead - 1; k++) load(k, st[k]);
 
     QOp<D, F32> Q;
-    build_q<D, F32, !F32>(Q, q, qrow, vec, rsd, h);
+    build_q<D, F32, !F32>(Q, raw, rsd, h);
     v16f O[D / 32];
     float M = kMInit, L = 0.0f, C[GPD];
 #pragma unroll

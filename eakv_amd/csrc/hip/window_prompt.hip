@@ -202,7 +202,11 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
     const int64_t qrow = ((int64_t)(job.tok0[c] + tok) * job.n_q + head) * D;
     const int vis = start + tok + 1;
     QOp<D, F32> Q;
-    build_q<D, F32, false>(Q, q, qrow, vec, rsd, h);
+    {
+        QRaw<D, F32> raw;
+        load_q<D, F32>(raw, q, qrow, vec, h);
+        build_q<D, F32, false>(Q, raw, rsd, h);
+    }
     v16f O[D / 32];
     float M = kMInit, L = 0.0f, C[GPD];
 #pragma unroll
