@@ -104,6 +104,7 @@ struct WinPart {
     int n_tok;              // window tokens of its sequences
     int64_t subtiles;       // win_prompt: expanded
     size_t part_bytes, bytes;
+    double us;              // estimated
     bool merge;
 };
 
@@ -112,17 +113,6 @@ struct WinPlan {
 };
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
-
-// Whether a window's K and V are expanded first (never a tree's), by the rows that
-// share a kv head: where so many blocks convert the same bytes that the converted
-// values' way through memory costs less.  Expanded / not, in us: 264 rows of 8 at 10000
-// bf16 291 / 231, f32 476 / 386; 512 of 8 at 10000 330 / 313, 531 / 519; 768 at 30000
-// 154 / 208, 293 / 375; 1024 at 30000 185 / 211, 440 / 373; 1024 of 4 at 30000 693 / 825,
-// 1344 / 1488; 2100 of 4 at 4000, d = 64 57 / 70, 86 / 100.
-bool is_many(int ntok, int qpk)
-{
-    return ntok > EAKVD_TREE_MAX && (int64_t)ntok * qpk > 512;
-}
 
 // Tiles of a chunk, win_draft: an even share of the chip (4 tokens at 2048 of 32Q/8KV,
 // 8 tiles: one each 16.6 us, two each 17.3, four each 19.9).  At most 2^25 tokens:
@@ -134,11 +124,10 @@ int64_t few_share(int64_t tiles, int cus)
 }
 
 // Tiles of a chunk, win_prompt: the split of the longest context in k that ends first,
-// by a model of a launch in tile times (256 rows x 32 tokens: about 1.05 us at d = 128
-// in bf16, 2.2 in f32).  Blocks beyond the chip's slots run as slots come free, the
-// longest first; partials are written and read at about 5 TB/s, the merge is
-// a launch of its own.
-int64_t many_share(const WinJob &j, int64_t tiles, int cus, int head_dim, bool bf16)
+// by a model of a launch in tile times (256 rows x 32 tokens).  Blocks beyond the
+// chip's slots run as slots come free, the longest first; partials are written and
+// read at about 5 TB/s, the merge is a launch of its own.  us: of that split.
+int64_t many_share(const WinJob &j, int64_t tiles, int cus, int head_dim, bool bf16, double *us)
 {
     int64_t longest = 1, blocks = 0, rows = 0;
     for (int i = 0; i < j.n_seq; i++) {
@@ -148,7 +137,7 @@ int64_t many_share(const WinJob &j, int64_t tiles, int cus, int head_dim, bool b
         blocks += (r + 255) / 256 * j.n_kv;
         rows += r * j.n_kv;
     }
-    const double tile_us = (bf16 ? 1.05 : 2.2) * head_dim / 128;
+    const double tile_us = head_dim == 128 ? (bf16 ? 1.05 : 2.2) : (bf16 ? 0.68 : 1.3);
     const double merge_k = 2.0 * rows * (head_dim + 2) * 4 / 5e6 / tile_us, merge_0 = 6 / tile_us;
     double best = 0;
     int64_t share = longest;
@@ -165,11 +154,14 @@ int64_t many_share(const WinJob &j, int64_t tiles, int cus, int head_dim, bool b
             share = part;
         }
     }
+    *us = best * tile_us;
     return share;
 }
 
+// The sequences with in[i] as one launch, by way of the expanded operands or without.
+// p->us: about what it takes.
 void plan_part(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv, bool bf16, bool many,
-               WinPart *p)
+               const bool *in, WinPart *p)
 {
     memset(p, 0, sizeof(*p));
     WinJob &j = p->job;
@@ -179,7 +171,7 @@ void plan_part(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv, bo
     j.qpk = qpk;
     int tok0 = 0;
     for (int i = 0; i < b->n_seq; i++) {
-        if (b->ntok[i] && is_many(b->ntok[i], qpk) == many) {
+        if (b->ntok[i] && in[i]) {
             const int k = j.n_seq++;
             j.base[k] = b->base[i];
             j.start[k] = b->start[i];
@@ -188,22 +180,21 @@ void plan_part(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv, bo
         }
         tok0 += b->ntok[i];
     }
+    if (j.n_seq == 0) return;
     const int rbr = many ? 256 : 32, tile = many ? 32 : kDraftTile;
-    // tiles of all blocks, were no sequence split
+    // tiles of all blocks, were no sequence split (the mean of a sequence's first and last
+    // row block; a tree's rows may all see the whole window, which is short)
     int64_t tiles = 0;
     for (int i = 0; i < j.n_seq; i++) {
         const int64_t rows = (int64_t)j.ntok[i] * qpk, nrb = (rows + rbr - 1) / rbr;
-        for (int64_t r = 0; r < nrb; r++) {
-            const int64_t last = (rows < (r + 1) * rbr ? rows : (r + 1) * rbr) - 1;
-            // (a tree's rows may all see the whole window; it is short)
-            const int64_t end = (int64_t)j.start[i] + (many ? last / qpk + 1 : j.ntok[i]);
-            tiles += (end + tile - 1) / tile * n_kv;
-        }
+        const int64_t first = (j.start[i] + (int64_t)(rows < rbr ? rows : rbr) / qpk + tile) / tile;
+        const int64_t last = ((int64_t)j.start[i] + j.ntok[i] + tile - 1) / tile;
+        tiles += (nrb * (first + last) + 1) / 2 * n_kv;
     }
     const int cus = cu_count();
-    const int64_t share = many ? many_share(j, tiles, cus, g->head_dim, bf16)
+    const int64_t share = many ? many_share(j, tiles, cus, g->head_dim, bf16, &p->us)
                                : few_share(tiles, cus);
-    int64_t part = 0;
+    int64_t part = 0, longest = 0;
     for (int i = 0; i < j.n_seq; i++) {
         const int64_t rows = (int64_t)j.ntok[i] * qpk, nrb = (rows + rbr - 1) / rbr;
         const int64_t n_t = ((int64_t)j.start[i] + j.ntok[i] + tile - 1) / tile;
@@ -211,6 +202,7 @@ void plan_part(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv, bo
         int64_t mc = !many && n_t <= 2 ? 1 : (n_t + share - 1) / share;
         const int64_t per = (n_t + mc - 1) / mc;
         mc = (n_t + per - 1) / per;
+        longest = per > longest ? per : longest;
         j.mc[i] = (int)mc;
         j.clen[i] = (int)(per * tile);
         j.pre[i + 1] = j.pre[i] + (int)(nrb * mc * n_kv);
@@ -228,13 +220,47 @@ void plan_part(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv, bo
     j.part_rows = part;
     p->part_bytes = align256((size_t)part * (g->head_dim + 2) * sizeof(float));
     p->bytes = p->part_bytes;
-    if (many && j.n_seq) p->bytes += align256(win_prompt_bytes(g->head_dim, bf16, p->subtiles));
+    if (many) {
+        // the expansion: a launch, and both forms of K and V at about 4 TB/s
+        const size_t img = win_prompt_bytes(g->head_dim, bf16, p->subtiles);
+        p->bytes += align256(img);
+        p->us += 8 + 1.3 * img / 4e6;
+    } else {
+        const bool wide = g->head_dim == 128;
+        const double tile_us = wide ? (bf16 ? 1.75 : 2.7) : (bf16 ? 1.05 : 1.35), block_us = wide ? 9 : 6;
+        const int64_t blocks = j.pre[j.n_seq];
+        const double even = (tiles * tile_us + blocks * block_us) / cus + 0.25 * longest * tile_us;
+        const double one = longest * tile_us + block_us;
+        p->us = (blocks > cus && even > one ? even : one) +
+                (p->merge ? 6 + 2.0 * part * (g->head_dim + 2) * 4 / 5e6 : 0);
+    }
 }
 
+// Whether windows' K and V are expanded first: causal ones that no tree is allowed for,
+// of more than 512 rows per kv head, if both estimates say so.  Rates of the estimates
+// and what they choose between, in us, expanded / not: 8 of 264 rows at 10000 of
+// 32Q/8KV bf16 295 / 230, f32 436 / 320 (never asked); 768 rows at 30000 149 / 208,
+// 273 / 308; 2000 tokens at 2000 of 32Q/32KV 84 / 133, 161 / 167, of 8Q/8KV 46 / 35, 65 / 47;
+// 3000 at 3000 of 40Q/8KV 122 / 258, 231 / 351; 4000 at 4000 of 12Q/12KV, d = 64, 90 / 89,
+// 140 / 116; 8 of 600 at 600 of 32Q/8KV 67 / 181, 114 / 223.
 void win_plan(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv, bool bf16, WinPlan *p)
 {
-    plan_part(g, b, n_q, n_kv, bf16, false, &p->few);
-    plan_part(g, b, n_q, n_kv, bf16, true, &p->many);
+    bool few[EAKVD_MAX_BATCH], many[EAKVD_MAX_BATCH], any = false;
+    for (int i = 0; i < b->n_seq; i++) {
+        many[i] = b->ntok[i] > EAKVD_TREE_MAX && (int64_t)b->ntok[i] * (n_q / n_kv) > 512;
+        few[i] = !many[i];
+        any = any || many[i];
+    }
+    memset(&p->many, 0, sizeof(p->many));
+    if (any) {
+        plan_part(g, b, n_q, n_kv, bf16, false, many, &p->few);
+        plan_part(g, b, n_q, n_kv, bf16, true, many, &p->many);
+        if (p->few.us < p->many.us) {
+            memset(&p->many, 0, sizeof(p->many));
+            for (int i = 0; i < b->n_seq; i++) few[i] = true;
+        }
+    }
+    plan_part(g, b, n_q, n_kv, bf16, false, few, &p->few);
 }
 
 int merge(const eakvd_geom *g, const WinPart &p, bool bf16, const float *part, void *out,
