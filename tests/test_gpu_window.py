@@ -86,7 +86,7 @@ SHAPES = [
     (128, 1, 3, [(40, 171)]),
     (128, 2, 2, [(0, 300), (700, 1), (33, 0), (90, 200)]),
     (64, 2, 40, [(511, 5)]),
-    # K and V expanded first: bf16 beyond 256 rows, f32 beyond 2048
+    # many blocks of rows
     (128, 2, 8, [(33, 65)]),
     (128, 1, 16, [(100, 140)]),
     (64, 1, 32, [(0, 70), (500, 3), (95, 97)]),
@@ -175,7 +175,7 @@ def test_beyond_32_bit_offsets(E, rng):
 @pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("d", [64, 128])
 def test_hidden_nonfinite_many_rows(E, rng, d, bf16):
-    """As below for windows whose K and V are expanded first."""
+    """As below for windows of many rows."""
     n_kv, n_q, start, m = 1, 8 if bf16 else 32, 30, 80
     c = E.Cache(1, n_kv, d, 128)
     x = rng.standard_normal((1, 2, n_kv, 128, d), dtype=np.float32)

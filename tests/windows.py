@@ -49,13 +49,15 @@ def visible(start, m, words=None):
 
 
 def k16(m, n_q, n_kv):
-    """Whether a bf16 window of m tokens has K rounded to f16."""
+    """Whether a bf16 window of m tokens may have K rounded to f16."""
     return m > 64 and m * (n_q // n_kv) > 256
 
 
-def attend(cache, layer, q, start, n_q, n_kv, words=None):
-    """Exact outputs f64 [m][n_q][d] and the bound of each output's f32 part."""
+def attend(cache, layer, q, start, n_q, n_kv, words=None, wide=None):
+    """Exact outputs f64 [m][n_q][d] and the bound of each output's f32 part.
+    wide: whether K is rounded to f16 (of more rows than q has)."""
     m, _, d = q.shape
+    wide = k16(m, n_q, n_kv) if wide is None else wide
     k, ks = values(cache, layer, 0)
     v, vs = values(cache, layer, 1)
     see = visible(start, m, words)
@@ -80,7 +82,7 @@ def attend(cache, layer, q, start, n_q, n_kv, words=None):
             sm = sh[t].max(0)
             tol[i, h] = (80 * E32 * a + 4 * E32) * 2 * vm + 40 * E32 * (vm + sm)
             half[i, h] = H16 * (3 * vm + 2 * sm)
-            if k16(m, n_q, n_kv):
+            if wide:
                 half[i, h] += 4 * H16 * (np.abs(kh[t]) @ np.abs(qi)).max() / np.sqrt(d) * vm
     return out, tol, half
 
