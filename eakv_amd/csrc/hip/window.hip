@@ -204,7 +204,7 @@ void plan_part(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv, bo
         mc = (n_t + per - 1) / per;
         longest = per > longest ? per : longest;
         j.mc[i] = (int)mc;
-        j.clen[i] = (int)(per * tile);
+        j.clen[i] = (int)(per * tile < INT32_MAX ? per * tile : INT32_MAX);
         j.pre[i + 1] = j.pre[i] + (int)(nrb * mc * n_kv);
         j.part[i] = part;
         if (mc > 1) {

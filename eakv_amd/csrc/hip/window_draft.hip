@@ -83,7 +83,8 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
     const int rows = m * qpk, n_rb = (rows + 31) / 32;
     const int chunk = rem / n_rb, r0 = 32 * (rem - chunk * n_rb);
     const int t_end = start + (tree ? m : (min(r0 + 32, rows) - 1) / qpk + 1);
-    const int lo = chunk * job.clen[c], hi = min(t_end, lo + job.clen[c]);
+    const int lo = chunk * job.clen[c];
+    const int hi = t_end - lo > job.clen[c] ? lo + job.clen[c] : t_end;
 
     const int row = min(r0 + n32, rows - 1);
     const int tok = row / qpk, head = kvh * qpk + row - tok * qpk;

@@ -191,7 +191,7 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
     const int first_row = rb * kPRows, last_row = min(rows, first_row + kPRows) - 1;
     const int t_end = start + last_row / qpk + 1;
     const int lo = chunk * job.clen[c];
-    const int hi = min(t_end, lo + job.clen[c]);
+    const int hi = t_end - lo > job.clen[c] ? lo + job.clen[c] : t_end;
     const int n_i = hi > lo ? (hi - lo + 31) / 32 : 0;   // sub-tiles of this block
     // the first that some row of the block does not see whole
     const int vis_min = start + first_row / qpk + 1;

@@ -17,9 +17,8 @@ static int dim_ok(const eakv_cache_t *c) { return c->head_dim == 64 || c->head_d
  * ways; that cannot be recorded in a graph. */
 static int not_captured(const eakv_cache_t *c, void *stream, const char *what)
 {
-    if (!stream || stream == c->stream) return EAKV_OK;
     int yes = 0;
-    int e = eakvd_stream_capturing(stream, &yes);
+    int e = eakvd_stream_capturing(stream ? stream : c->stream, &yes);
     if (e) return eakvi_hip_fail(e, what);
     return yes ? eakvi_set_error(EAKV_ERR_INVALID, "%s: the stream records a graph", what)
                : EAKV_OK;

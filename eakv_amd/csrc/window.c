@@ -109,8 +109,8 @@ int eakv_attention_window_batch_device(eakv_cache_t *const *caches, int n_caches
     if (d_work && work_bytes < need) {
         rc = eakvi_set_error(EAKV_ERR_INVALID, "window: %zu bytes of workspace, %zu needed",
                              work_bytes, need);
-    } else if (stream && stream != c0->stream) {
-        int e = eakvd_stream_capturing(stream, &capturing);
+    } else {
+        int e = eakvd_stream_capturing(stream ? stream : c0->stream, &capturing);
         if (e) rc = eakvi_hip_fail(e, "window");
         /* a graph would keep the address of a workspace that later calls
          * replace and share */

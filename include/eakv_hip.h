@@ -149,7 +149,7 @@ int eakv_attention_fused_plan(eakv_cache_t *const *caches, int n_caches, int n_q
                               int n_kv_heads, int noalloc, int32_t *plan);
 
 /* Attention of several new tokens of each sequence over its packed cache (drafted
- * tokens, a piece of a prompt), softmax(q.k/sqrt(d)).v in one launch for n_caches
+ * tokens, a piece of a prompt), softmax(q.k/sqrt(d)).v in one call for n_caches
  * same-shape caches.  No counterpart in the reference.
  *   starts     host int32[n_caches], or NULL: each cache's seq_len.  Query i of
  *              cache c is the token at position starts[c] + i; the window's K and V
@@ -205,9 +205,10 @@ size_t eakv_attention_window_work_bytes(eakv_cache_t *const *caches, int n_cache
  * from r = p_a when all were kept: the least j with r[0] + .. + r[j] >
  * d_uniform[s][n_drafts] * sum(r), or the last j with r[j] > 0 where rounding leaves
  * none.  Where nothing is left of p - q it is drawn from p_a, and -1 where that
- * holds nothing either; NaN and negative values count as 0.  Products, differences
- * and sums in f64.  d_work: eakv_verify_drafts_work_bytes() of device scratch,
- * 8-byte aligned, the call's own.  Asynchronous; may be recorded in a graph. */
+ * holds nothing either; NaN and negative values count as 0 (infinite ones make d_next
+ * some token of positive weight).  Products, differences and sums in f64.  d_work:
+ * eakv_verify_drafts_work_bytes() of device scratch, 8-byte aligned, the call's own.
+ * Asynchronous; may be recorded in a graph. */
 int eakv_verify_drafts_device(int n_seqs, int n_drafts, int vocab, const int32_t *d_counts,
                               const int32_t *d_tokens, const float *d_draft, int64_t ld_draft,
                               const float *d_target, int64_t ld_target,

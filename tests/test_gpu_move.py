@@ -181,6 +181,39 @@ def test_refusals(E, rng):
         assert e.value.code == E.EAKV_ERR_INVALID
 
 
+def test_shared_stream_that_records_a_graph(E, rng):
+    """Copies, gathers and windows without scratch of their own are refused on the
+    caches' shared stream too while it records."""
+    import ctypes as C
+    from eakv_amd import hipmem
+    from eakv_amd.hipmem import DeviceArray
+    a, b = W.build(E, rng, [3000, 100], 2, 128, 3010)
+    buf = DeviceArray((1 << 16,))
+    index = DeviceArray.from_host(np.arange(4, dtype=np.int32))
+    L, h = E.lib(), hipmem.hip()
+    shared = L.eakv_cache_stream(a.h)
+    a.sync()
+    hipmem.check(h.hipStreamBeginCapture(C.c_void_p(shared), 2), "begin")
+    try:
+        copy = L.eakv_cache_copy_batch_device(a.h, 0, E.handles([b]), 1, 0, 4, None)
+        gather = L.eakv_cache_gather_batch_device(E.handles([a]), E.handles([b]), 1, E.ints([0]),
+                                                  index.ptr, E.ints([4]), None)
+        window = L.eakv_attention_window_batch_device(E.handles([a]), 1, 0, None, E.ints([4]), buf.ptr,
+                                                      0, 8, 2, None, buf.ptr, None, 0, None)
+    finally:
+        graph = C.c_void_p()
+        rc = h.hipStreamEndCapture(C.c_void_p(shared), C.byref(graph))
+    hipmem.check(rc, "end")
+    h.hipGraphDestroy(graph)
+    assert (copy, gather, window) == (E.EAKV_ERR_INVALID,) * 3
+    # and work again afterwards
+    assert L.eakv_cache_copy_batch_device(a.h, 0, E.handles([b]), 1, 0, 4, None) == 0
+    a.sync()
+    for x, y in zip(a.read_planes(0, 0), b.read_planes(0, 0)):
+        n, m = 3010 * 2, 3010 * 2
+        assert np.array_equal(x[:8], y[:8]) and np.array_equal(x[n:n + 8], y[m:m + 8])
+
+
 def test_orders_with_other_streams(E, rng):
     """A copy on a caller's stream right behind an append on the shared stream, then an
     append to the source on the shared stream and a host call on the copy."""
