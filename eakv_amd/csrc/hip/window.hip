@@ -40,62 +40,63 @@
 
 namespace {
 
-// One wave per (window token, q head) of the sequences with chunks: the chunks'
-// (O, M, l) joined.  A chunk without visible tokens has l = 0 and no O.  A lane reads
-// one chunk's M and l, so that the loads of O wait for nothing but these.
+// The chunks' (O, M, l) of a row (window token, q head) joined, d/4 lanes to a row of
+// the sequences with chunks.  A chunk without visible tokens has l = 0 and no O.  A lane
+// reads one chunk's M and l, so that the loads of O, 16 bytes each, wait for nothing but
+// these.  Bound by HBM for many rows (37 MB of partials 12.8 us; a row to a wave, 4 bytes
+// to a lane 23.6), else a dependent launch of 3 to 5 us.
 template <int D, bool F32>
 __global__ __launch_bounds__(256) void window_merge_kernel(WinJob job, const float *part,
-                                                           void *out, int n_rows)
+                                                           void *out, int n_rows, int vec)
 {
-    constexpr int E = D / 64;
-    const int r = (int)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (r >= n_rows) return;
-    const int tok = r / job.n_q;
-    const int c = seq_of(job.lead, job.n_seq, tok, lane);
+    constexpr int W = D / 4, RPW = 64 / W;           // lanes of a row, rows of a wave
+    const int lane = threadIdx.x & 63, sub = lane % W;
+    const int r0 = ((int)blockIdx.x * 4 + (threadIdx.x >> 6)) * RPW + lane / W;
+    const int r = min(r0, n_rows - 1), tok = r / job.n_q;
+    int c = 0;
+    for (int i = 1; i < job.n_seq; i++) c += tok >= job.lead[i] ? 1 : 0;
     const int mc = job.mc[c];
-    if (mc == 1) return;
+    int most = mc;                                   // of the wave's rows
+#pragma unroll
+    for (int o = W; o < 64; o *= 2) most = max(most, __shfl_xor(most, o, 64));
+    if (most == 1) return;
     const int64_t per = (int64_t)job.ntok[c] * job.n_q;
     const int64_t local = r - (int64_t)job.lead[c] * job.n_q;
-    const int64_t first = job.part[c] + local;
+    // (a row of one chunk has no partial: it reads another's and writes nothing)
+    const int64_t first = mc > 1 ? job.part[c] + local : 0;
     const float2 *ml = (const float2 *)(part + job.part_rows * D) + first;
     float m = kMInit;
-    for (int k = lane; k < mc; k += 64) {
-        const float2 x = ml[k * per];
+    for (int k = sub; k < most; k += W) {
+        const float2 x = ml[min(k, mc - 1) * per];
         if (x.y != 0.0f) m = fmaxf(m, x.x);
     }
-    m = wave_max(m);
-    float l = 0.0f, o[E];
 #pragma unroll
-    for (int e = 0; e < E; e++) o[e] = 0.0f;
-    for (int k0 = 0; k0 < mc; k0 += 64) {
-        const int n = min(64, mc - k0);
-        const float2 x = ml[(k0 + min(lane, n - 1)) * per];
-        const float al = lane < n && x.y != 0.0f ? __builtin_amdgcn_exp2f(x.x - m) : 0.0f;
+    for (int o = 1; o < W; o *= 2) m = fmaxf(m, __shfl_xor(m, o, 64));
+    float l = 0.0f;
+    v4f o4 = {0.0f, 0.0f, 0.0f, 0.0f};
+    const float *po = part + first * D + sub * 4;
+    for (int k0 = 0; k0 < most; k0 += W) {
+        const float2 x = ml[min(k0 + sub, mc - 1) * per];
+        const float al = k0 + sub < mc && x.y != 0.0f ? __builtin_amdgcn_exp2f(x.x - m) : 0.0f;
         l = fmaf(al, x.y, l);
-        const float *po = part + (first + k0 * per) * D + lane * E;
-        for (int k8 = 0; k8 < n; k8 += 8) {
-            float v[8][E];
+        for (int k8 = k0; k8 < min(k0 + W, most); k8 += 8) {
+            v4f v[8];
 #pragma unroll
-            for (int k = 0; k < 8; k++)
-#pragma unroll
-                for (int e = 0; e < E; e++) v[k][e] = po[min(k8 + k, n - 1) * per * D + e];
+            for (int k = 0; k < 8; k++) v[k] = *(const v4f *)(po + min(k8 + k, mc - 1) * per * D);
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const float a = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(al), k8 + k));
+                const float a = __shfl(al, lane - sub + k8 - k0 + k, 64);
 #pragma unroll
-                for (int e = 0; e < E; e++) o[e] = a != 0.0f ? fmaf(a, v[k][e], o[e]) : o[e];
+                for (int e = 0; e < 4; e++) o4[e] = a != 0.0f ? fmaf(a, v[k][e], o4[e]) : o4[e];
             }
         }
     }
-    l = wave_sum(l);
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        const int64_t at = ((int64_t)job.tok0[c] * job.n_q + local) * D + lane * E + e;
-        if constexpr (F32) ((float *)out)[at] = o[e] * inv;
-        else ((uint16_t *)out)[at] = (uint16_t)bf16_bits(o[e] * inv);
-    }
+    for (int o = 1; o < W; o *= 2) l += __shfl_xor(l, o, 64);
+    if (r0 >= n_rows || mc == 1) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float y[4] = {o4[0] * inv, o4[1] * inv, o4[2] * inv, o4[3] * inv};
+    store4<F32>(out, ((int64_t)job.tok0[c] * job.n_q + local) * D + sub * 4, vec, y);
 }
 
 // The sequences of one launch: those of few rows (win_draft) or of many (win_prompt).
@@ -263,16 +264,16 @@ void win_plan(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv, boo
     plan_part(g, b, n_q, n_kv, bf16, false, few, &p->few);
 }
 
-int merge(const eakvd_geom *g, const WinPart &p, bool bf16, const float *part, void *out,
+int merge(const eakvd_geom *g, const WinPart &p, bool bf16, const float *part, void *out, bool vec,
           hipStream_t st)
 {
     if (!p.merge) return 0;
-    const int n_rows = p.n_tok * p.job.n_q;
+    const int n_rows = p.n_tok * p.job.n_q, per = 4 * 256 / g->head_dim;
     auto *kern = g->head_dim == 64
                      ? (bf16 ? window_merge_kernel<64, false> : window_merge_kernel<64, true>)
                      : (bf16 ? window_merge_kernel<128, false> : window_merge_kernel<128, true>);
-    hipLaunchKernelGGL(kern, dim3((unsigned)((n_rows + 3) / 4)), dim3(256), 0, st, p.job, part, out,
-                       n_rows);
+    hipLaunchKernelGGL(kern, dim3((unsigned)((n_rows + per - 1) / per)), dim3(256), 0, st, p.job,
+                       part, out, n_rows, (int)vec);
     return (int)hipGetLastError();
 }
 
@@ -301,13 +302,13 @@ extern "C" int eakvd_window_attend(const eakvd_geom *g, const eakvd_window *b, i
     if (p.many.job.n_seq) {
         e = win_prompt(*g, p.many.job, p.many.subtiles, bf16, q, out, (float *)w,
                        w + p.many.part_bytes, vec, st);
-        if (!e) e = merge(g, p.many, bf16, (const float *)w, out, st);
+        if (!e) e = merge(g, p.many, bf16, (const float *)w, out, vec, st);
         w += p.many.bytes;
     }
     if (!e && p.few.job.n_seq) {
         float *part = (float *)w;
         e = win_draft(*g, p.few.job, bf16, q, tree, out, part, vec, st);
-        if (!e) e = merge(g, p.few, bf16, part, out, st);
+        if (!e) e = merge(g, p.few, bf16, part, out, vec, st);
     }
     return e;
 }
