@@ -15,6 +15,12 @@
 // in LDS with a barrier every kStep.  A step of a wave is the products (the next
 // sub-tile's scores and this one's weighted sum), then the softmax; a SIMD's two
 // waves are in different halves of it.  bf16 operands are read ahead of their step.
+//
+// Bound by the matrix cores and the vector ALUs together: 2048 tokens at 30720 of
+// 32Q/8KV, bf16 (1.07 Tflop): 1040-1080 us, 990-1020 Tflop/s, with the matrix cores busy 54
+// and the vector ALUs 51 of 100 cycles at about 1.9 GHz; the products alone took 671 us,
+// the softmax alone about 500.  f32, twice the products and 320 vector instructions
+// for 32 x 32: 2.2 us per 32 tokens of a block against 1.05.
 #include <string.h>
 
 #include "window.h"
