@@ -259,20 +259,23 @@ __device__ __forceinline__ void build_q(QOp<D, F32> &Q, const QRaw<D, F32> &raw,
     Q.bias = b8{p1, p2, p3, p1, p2, p1, zero, zero};
 }
 
-// The maximum of a wave's values, in all lanes
+// The maximum of a wave's values, none negative or NaN, in all lanes.  (By their bits: a
+// float maximum first makes quiet NaN of its operands, an instruction each.)
 __device__ __forceinline__ float wave_top(float v)
 {
-    auto ror = [](float x, auto c) {
+    uint32_t u = __float_as_uint(v);
+    auto ror = [](uint32_t x, auto c) {
         constexpr int ctrl = decltype(c)::value;
-        return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), ctrl, 0xf, 0xf, true));
+        return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, ctrl, 0xf, 0xf, true);
     };
-    v = fmaxf(v, ror(v, std::integral_constant<int, 0x128>{}));     // row_ror:8
-    v = fmaxf(v, ror(v, std::integral_constant<int, 0x124>{}));
-    v = fmaxf(v, ror(v, std::integral_constant<int, 0x122>{}));
-    v = fmaxf(v, ror(v, std::integral_constant<int, 0x121>{}));
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    return half_max(v);
+    u = max(u, ror(u, std::integral_constant<int, 0x128>{}));       // row_ror:8
+    u = max(u, ror(u, std::integral_constant<int, 0x124>{}));
+    u = max(u, ror(u, std::integral_constant<int, 0x122>{}));
+    u = max(u, ror(u, std::integral_constant<int, 0x121>{}));
+    auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    u = max((uint32_t)r[0], (uint32_t)r[1]);
+    r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(max((uint32_t)r[0], (uint32_t)r[1]));
 }
 
 // The row that a lane writes: final outputs (mc == 1) or its chunk's partial.

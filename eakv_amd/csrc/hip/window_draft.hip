@@ -14,9 +14,9 @@
 //
 // Bound by vector instructions: per 32 tokens x 32 rows at d = 128 a wave issues about 380
 // (f32 530) beside 17 (33) matrix products and 5 KB of loads.  8 sequences of 8 tokens
-// at 32768 of 32Q/8KV (32 rows, 336 MB): bf16 73 us in the kernel, 4.6 TB/s; f32 115.
+// at 32768 of 32Q/8KV (32 rows, 336 MB): bf16 73 us in the kernel, 4.6 TB/s; f32 112.
 // Rows beyond 32 read the planes again, out of the caches: a block of 64 rows with
-// shared operands in LDS was slower from 33 to 512 rows (64 rows of 8 at 20000 of
+// shared operands in LDS was slower at most sizes up to 512 rows (64 rows of 8 at 20000 of
 // 64Q/8KV bf16 158 against 164 us, but 192 rows of 6: 350 against 274; 64 of 4 at 4000,
 // d = 64: 31 against 24).  For small contexts a block's way bounds it: 1.4 us of
 // arguments and addresses, 2.4 for q, 2.7 for a sub-tile, 2 for the join.

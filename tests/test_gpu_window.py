@@ -259,6 +259,30 @@ def test_hidden_nonfinite(E, rng, d, bf16):
 
 
 @pytest.mark.parametrize("bf16", [False, True])
+def test_one_cache_in_several_windows(E, rng, bf16):
+    """The same cache named three times, its windows overlapping."""
+    c = W.build(E, rng, [400], 2, 128, 410)[0]
+    starts, ms = [390, 100, 385], [10, 40, 12]
+    call = W.Call(E, [c, c, c], ms, 8, 2, bf16, starts)
+    q = call.put(rng.standard_normal((sum(ms), 8, 128), dtype=np.float32))
+    call.run()
+    got = call.get()
+    row = 0
+    for s, m in zip(starts, ms):
+        want, tol, half = W.attend(c, 0, q[row:row + m], s, 8, 2)
+        W.check(got[row:row + m], want, tol, half, bf16)
+        row += m
+
+
+@pytest.mark.parametrize("tree", [None, "tree", "masks"])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_large_groups(E, rng, bf16, tree):
+    """Hundreds of q heads to one kv head: many blocks of rows for a few tokens."""
+    compare(E, rng, 64, 1, 300, [(33, 2), (0, 1)], bf16, tree)
+    compare(E, rng, 128, 1, 40, [(290, 64)], bf16, tree)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
 def test_rows_without_tokens(E, rng, bf16):
     c = W.build(E, rng, [40], 2, 64, 48)[0]
     call = W.Call(E, [c], [3], 4, 2, bf16, [0], [0, 2, 0])
