@@ -173,7 +173,8 @@ __global__ __launch_bounds__(64 * 4 * (D / 64)) void expand_kernel(eakvd_geom ge
     }
 }
 
-template <int D, bool F32>
+// PF: operands are read from LDS ahead of their step (bf16).
+template <int D, bool F32, bool PF>
 __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
     WinJob job, const uint8_t *img, const Meta *meta, const void *q, void *out, float *part, float rsd,
     int vec)
@@ -270,8 +271,7 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
     for (int n = 0; n < NP; n++)
         P[n][0] = P[n][1] = __builtin_bit_cast(h8, uint4{0, 0, 0, 0});
 
-    // operands read ahead of their phase (bf16): V of sub-tile i - 1, K of i
-    constexpr bool PF = !F32;
+    // operands read ahead of their phase: V of sub-tile i - 1, K of i
     h8 KF[PF ? GPD * 4 : 1], VF[PF ? GPD * 4 : 1];
     auto k_op = [&](int i, int f) {
         return __builtin_bit_cast(h8, ((const uint4 *)(lds + (i & (kRing - 1)) * I::BYTES))[f * 64 + lane]);
@@ -484,15 +484,23 @@ int launch(const eakvd_geom &g, const WinJob &job, int64_t subtiles, const void 
     Meta *meta = (Meta *)(img + subtiles * I::BYTES);
     hipLaunchKernelGGL((expand_kernel<D, F32>), dim3((unsigned)subtiles), dim3(64 * 4 * (D / 64)), 0, st,
                        g, job, img, meta);
-    auto *kern = prompt_kernel<D, F32>;
     constexpr int bytes = kRing * I::BYTES;
     static_assert(bytes <= 160 * 1024, "LDS");
-    static std::atomic<uint64_t> done;
-    const int e = allow_lds((const void *)kern, bytes, done);
-    if (e) return e;
-    hipLaunchKernelGGL(kern, dim3((unsigned)job.pre[job.n_seq]), dim3(64 * kPWaves), bytes, st, job, img,
-                       meta, q, out, part, 1.0f / sqrtf((float)D), (int)vec);
-    return (int)hipGetLastError();
+    const unsigned blocks = (unsigned)job.pre[job.n_seq];
+    auto run = [&](auto *kern, std::atomic<uint64_t> &done) {
+        const int e = allow_lds((const void *)kern, bytes, done);
+        if (e) return e;
+        hipLaunchKernelGGL(kern, dim3(blocks), dim3(64 * kPWaves), bytes, st, job, img, meta, q, out, part,
+                           1.0f / sqrtf((float)D), (int)vec);
+        return (int)hipGetLastError();
+    };
+    // d = 64 in bf16: without reading ahead two blocks fit a CU (116 registers against 149),
+    // which is worth more where there are two (4 x 1100 tokens at 5003 of 32Q/4KV 260 against
+    // 289 us, 4000 of 12Q/12KV 83 against 91; but 2000 at 30000, 252 blocks, 646 against 605)
+    static std::atomic<uint64_t> done[2];
+    if constexpr (D == 64 && !F32)
+        if (blocks > (unsigned)cu_count()) return run(prompt_kernel<D, F32, false>, done[0]);
+    return run(prompt_kernel<D, F32, !F32>, done[1]);
 }
 
 }  // namespace
