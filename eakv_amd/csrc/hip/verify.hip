@@ -11,7 +11,8 @@
 // drawn number lies within 1e-15 of a step.
 //
 // Work: one row of p and one of q per sequence, bound by HBM for large batches and
-// by latency for small ones.  Two launches: each wave sums one segment of its
+// by latency for small ones.  Small vocabularies: one launch, a block of 16 waves per
+// sequence.  Else two: each wave sums one segment of its
 // sequence's row; one block per sequence then finds the segment and scans it, in one
 // step up to 2^18 tokens.  7 drafts of 64 sequences, 151665 tokens (77.7 MB): 14.0 us of
 // sums (5.5 TB/s) and 4.6 of scan; with a segment of 4096 values to a block, scanned in
@@ -21,6 +22,10 @@
 namespace {
 
 constexpr int kVerThreads = 256;
+// Vocabularies up to this take one launch (the block's f64 sums take the time of the second
+// launch there): one / two for 32 sequences, us: 2000 5.6 / 9.4, 8000 7.0 / 9.2, 12000 8.0 / 8.9,
+// 16000 8.9 / 8.8, 32000 12.8 / 8.1.
+constexpr int kVerOne = 12288;
 constexpr int kVerStep = 1024;          // values of a wave's step, a multiple of 256
 
 typedef float v4f4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -232,6 +237,110 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerJob J)
     if (tid == 0) J.next[s] = s_first != INT32_MAX ? s_first : s_last;
 }
 
+// Small vocabularies in one launch: a block of 16 waves per sequence, each with a part of
+// the row; the wave whose part the number falls in scans it, out of the caches.
+__global__ __launch_bounds__(1024) void verify_one_kernel(VerJob J)
+{
+    __shared__ double sh[2][16];
+    const int s = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int n = count_of(J, s);
+    const int kept = kept_of(J, s, n, lane);
+    Row R = row_of(J, s, n, kept);
+    const int steps = (J.vocab + 16 * 256 - 1) / (16 * 256);     // of a wave, 256 values each
+    const int j0 = w * steps * 256 + 4 * lane;
+    auto four = [&](const float *x, int j) {
+        if (j + 4 <= J.vocab) return *(const v4f4 *)(x + j);
+        v4f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int e = 0; e < 4; e++)
+            if (j + e < J.vocab) v[e] = x[j + e];
+        return v;
+    };
+    const v4f4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+    double sr = 0.0, sp = 0.0;
+#pragma unroll 4
+    for (int i = 0; i < steps; i++) {
+        const int j = j0 + 256 * i;
+        const v4f4 p = four(R.p, j), q = R.q ? four(R.q, j) : none;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            sr += R.at((double)p[e], (double)q[e], j + e);
+            sp += p[e] > 0.0f ? (double)p[e] : 0.0;
+        }
+    }
+    sr = wave_sum_d(sr);
+    sp = wave_sum_d(sp);
+    if (lane == 0) {
+        sh[0][w] = sr;
+        sh[1][w] = sp;
+    }
+    __syncthreads();
+    // every wave: the sums before each wave's part, and the part that the number falls in
+    auto whole = [&](int k) {
+        double t = 0.0;
+        for (int i = 0; i < 16; i++) t += sh[k][i];
+        return t;
+    };
+    int k = 0;
+    double total = whole(0);
+    if (!(total > 0.0)) {
+        // nothing left of p - q: the target's own row
+        R.q = nullptr;
+        R.less = -1;
+        k = 1;
+        total = whole(1);
+    }
+    if (threadIdx.x == 0) J.kept[s] = kept;
+    if (!(total > 0.0)) {
+        if (threadIdx.x == 0) J.next[s] = -1;
+        return;
+    }
+    const double want = (double)J.uniform[(int64_t)s * (J.k + 1) + J.k] * total;
+    int b = -1;
+    double before = 0.0, cum = 0.0;
+    for (int i = 0; i < 16; i++) {
+        const double mine = sh[k][i];
+        if (mine > 0.0) {
+            b = i;
+            before = cum;
+            if (cum + mine > want) break;
+        }
+        cum += mine;
+    }
+    if (w != b) return;
+    int first = -1, last = -1;
+    for (int i = 0; i < steps && first < 0; i++) {
+        const int j = j0 + 256 * i;
+        const v4f4 p = four(R.p, j), q = R.q ? four(R.q, j) : none;
+        double r[4], sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            r[e] = R.at((double)p[e], (double)q[e], j + e);
+            sum += r[e];
+        }
+        double v = sum;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const double u = __shfl_up(v, o, 64);
+            if (lane >= o) v += u;
+        }
+        double upto = before + (v - sum);
+        int f = -1, l = -1;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            upto += r[e];
+            if (r[e] > 0.0) {
+                l = j + e;
+                if (upto > want && f < 0) f = l;
+            }
+        }
+        const uint64_t hit = __ballot(f >= 0), some = __ballot(l >= 0);
+        if (some) last = __shfl(l, 63 - __clzll((long long)some), 64);
+        if (hit) first = __shfl(f, __ffsll((unsigned long long)hit) - 1, 64);
+        before += __shfl(v, 63, 64);
+    }
+    if (lane == 0) J.next[s] = first >= 0 ? first : last;
+}
+
 // One step of a wave, so that the second launch scans a segment in one step; at most
 // one segment per thread of that launch.
 int seg_of(int vocab)
@@ -270,6 +379,10 @@ extern "C" int eakvd_verify(int n_seqs, int k, int vocab, const int32_t *count, 
     J.next = next;
     J.part = (double *)work;
     const hipStream_t st = (hipStream_t)stream;
+    if (vocab <= kVerOne) {
+        hipLaunchKernelGGL(verify_one_kernel, dim3((unsigned)n_seqs), dim3(1024), 0, st, J);
+        return (int)hipGetLastError();
+    }
     hipLaunchKernelGGL(verify_sum_kernel,
                        dim3((unsigned)((J.n_seg + kVerThreads / 64 - 1) / (kVerThreads / 64)), (unsigned)n_seqs),
                        dim3(kVerThreads), 0, st, J);

@@ -31,7 +31,7 @@
 // precision down to 2^-29 of that.
 //
 // Softmax in the log2 domain, f32: M moves only when a score passes it by
-// kTau; sums, weighted sums and M are f32.  Tokens are split into chunks where
+// kWinTau; sums, weighted sums and M are f32.  Tokens are split into chunks where
 // rows alone do not fill the chip; partial (O, M, l) are merged by a second
 // launch.  No atomics: results are the same bits on every call.
 #include <string.h>

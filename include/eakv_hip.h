@@ -164,7 +164,7 @@ int eakv_attention_fused_plan(eakv_cache_t *const *caches, int n_caches, int n_q
  *              the tokens before starts[c].
  * A query that sees no token gives zeros.  What a query does not see has no part in
  * its result, NaN and infinities included.  f32 queries: all sums in f32, results
- * about 1e-6 off the exact ones; one token per sequence without a tree takes the
+ * 0.5e-6 to 2e-6 off the exact ones (norms); one token per sequence without a tree takes the
  * launch of eakv_attention_fused_batch_device.  bf16 queries: the matrix products'
  * operands are rounded to f16 (2^-12 relative), sums in f32, the result to bf16.
  * A non-finite scale or bias gives NaN in the scores of its token or in its 64 dims.

@@ -111,7 +111,8 @@ def inputs(rng, n, k, vocab, onehot=False, pad=0, sharp=2.0):
 @pytest.mark.parametrize("n,k,vocab,pad", [
     (1, 1, 1, 0), (3, 2, 3, 1), (5, 4, 1023, 0), (2, 7, 1025, 3), (9, 3, 4097, 0), (4, 5, 32000, 0),
     (64, 4, 5000, 1), (300, 2, 777, 0), (2, 1, 270001, 0), (3, 70, 500, 0), (6, 0, 900, 0),
-    (40, 3, 110001, 0)])
+    (40, 3, 110001, 0), (3, 4, 16384, 0), (2, 3, 16385, 2), (7, 2, 32768, 1), (5, 2, 32769, 0),
+    (130, 2, 12288, 0), (9, 2, 12289, 1), (4, 3, 4095, 1), (1, 2, 256, 0)])
 def test_against_definition(E, rng, n, k, vocab, pad, onehot):
     print("verify", n, k, vocab, pad, onehot, flush=True)
     tokens, draft, target, u = inputs(rng, n, k, vocab, onehot, pad)
