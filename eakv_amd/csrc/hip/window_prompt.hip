@@ -3,13 +3,16 @@
 // 256 rows read them from there.
 //
 // One launch writes, for every (kv head, 32 tokens), the operands as LDS holds them:
-// 16 KB (d = 128) against 5 KB packed, once per call.  In the attention launch they
+// 18 KB (d = 128) against 5 KB packed, once per call.  In the attention launch they
 // go from the L2 to LDS without passing a register (buffer loads to LDS), so its
 // vector instructions are the softmax's alone.
 //
-// bf16 queries: values n*s + b (f32) scaled by the sub-tile's power of two and rounded
-// to f16, 2^-12 relative.  f32 queries: n - z, exact, with the scales and biases
-// beside them, as in window.hip.
+// K: n - z, exact, with the scales and biases beside them, as in window.hip.  (Values in
+// f16 instead save the scales' 32 instructions per 32 x 32 and a product, 1071 us against
+// 1311 for the prompt below; but their 2^-12 enters the scores times the scores' size:
+// K on an offset of 100 made outputs 2e-2 off.)  V, f32 queries: likewise; bf16 queries:
+// values n*s + b (f32) scaled by the sub-tile's power of two and rounded to f16, 2^-12
+// relative.
 //
 // Attention: 8 waves per block, two per SIMD, 32 rows each, through a ring of 8 sub-tiles
 // in LDS with a barrier every kStep.  A step of a wave is the products (the next
@@ -17,10 +20,8 @@
 // waves are in different halves of it.  bf16 operands are read ahead of their step.
 //
 // Bound by the matrix cores and the vector ALUs together: 2048 tokens at 30720 of
-// 32Q/8KV, bf16 (1.07 Tflop): 1040-1080 us, 990-1020 Tflop/s, with the matrix cores busy 54
-// and the vector ALUs 51 of 100 cycles at about 1.9 GHz; the products alone took 671 us,
-// the softmax alone about 500.  f32, twice the products and 320 vector instructions
-// for 32 x 32: 2.2 us per 32 tokens of a block against 1.05.
+// 32Q/8KV, bf16 (1.07 Tflop): 1311 us, 813 Tflop/s.  f32, twice the products and 320 vector
+// instructions for 32 x 32: 2.2 us per 32 tokens of a block against 1.3.
 #include <string.h>
 
 #include "window.h"
@@ -37,7 +38,7 @@ constexpr int kStep = 3;
 typedef __attribute__((address_space(3))) void *lds_p;
 
 // Bytes of an expanded sub-tile: K operands (g, octet, nibble), V operands (g, nibble,
-// 16-token step), 1 KB each; f32: K's bias pieces (1 KB), then scales of K, scales and
+// 16-token step), 1 KB each; K's bias pieces (1 KB), then scales of K and (f32) scales and
 // biases of V, [group][token].
 template <int D, bool F32>
 struct Img {
@@ -47,20 +48,20 @@ struct Img {
     static constexpr int KS = KB + 1024;
     static constexpr int VS = KS + GPD * 128;
     static constexpr int VC = VS + GPD * 128;
-    static constexpr int BYTES = F32 ? KB + 2048 : KB;
+    static constexpr int BYTES = KB + 2048;
     static constexpr int LOADS = (BYTES / 1024 + kPWaves - 1) / kPWaves;   // of a wave
 };
 
 // Per sub-tile.
 struct Meta {
-    float ek;                           // bf16: the K operands are values * 1/ek
     int ev;                             // exponent of V; kSomeBad added where bad is not 0
     uint32_t bad[2];                    // tokens with non-finite V, by group
+    uint32_t none;
 };
 constexpr int kSomeBad = 1 << 16;
 
-// One wave per 512 operand bytes... one block per (sub-tile, kv head): wave j < 2 GPD
-// makes K operands (g, o = j), the others V operands (g, step).
+// One block per (sub-tile, kv head), two operands of 1 KB to a wave: wave j < 2 GPD makes
+// K's of (g, octet), the others V's of (g, 16-token step).
 template <int D, bool F32>
 __global__ __launch_bounds__(64 * 4 * (D / 64)) void expand_kernel(eakvd_geom geo, WinJob job,
                                                                    uint8_t *img, Meta *meta)
@@ -85,11 +86,7 @@ __global__ __launch_bounds__(64 * 4 * (D / 64)) void expand_kernel(eakvd_geom ge
     const int64_t tn = min(t0 + n32, t_last);
     const int64_t gi = g0 + tn * GPD + (GPD == 2 ? h : 0);
     const float s = P.s[gi], b = P.b[gi];
-    const float a = fmaxf(fabsf(b), fabsf(fmaf(15.0f, s, b)));
-    const bool fin = a < __builtin_inff() && s == s;
-    const int e = exp_of(wave_top(!fin ? 0.0f : F32 && is_v ? fabsf(s) : a));
     if (!is_v) {
-        if (g == 0 && x == 0 && lane == 0) meta[blockIdx.x].ek = scale2(1.0f, e - 15);
         const uint2 by = *(const uint2 *)(P.w + (g0 + tn * GPD + g) * 32 + 16 * h + 8 * x);
         const uint32_t xs[2] = {by.x, by.y};
         const float sg = GPD == 2 ? __shfl(s, 32 * g + n32, 64) : s;
@@ -104,32 +101,25 @@ __global__ __launch_bounds__(64 * 4 * (D / 64)) void expand_kernel(eakvd_geom ge
 #pragma unroll
             for (int p = 0; p < 2; p++) {
                 const uint32_t y = xs[d] >> (8 * p);     // bytes p and p + 2
-                if constexpr (F32) {
-                    lo[2 * d + p] = u_of(nib2<false>(y, off_l, nc));
-                    hi[2 * d + p] = u_of(nib2<true>(y, off_h, nc));
-                } else {
-                    auto val = [&](uint32_t n) {
-                        return scale2(fmaf((float)(n & 15), sg, bg), 15 - e);
-                    };
-                    lo[2 * d + p] = u_of(pk(val(y), val(y >> 16)));
-                    hi[2 * d + p] = u_of(pk(val(y >> 4), val(y >> 20)));
-                }
+                lo[2 * d + p] = u_of(nib2<false>(y, off_l, nc));
+                hi[2 * d + p] = u_of(nib2<true>(y, off_h, nc));
             }
         uint4 *ok = (uint4 *)o + (g * 4 + 2 * x) * 64 + lane;
         ok[0] = uint4{lo[0], lo[1], lo[2], lo[3]};
         ok[64] = uint4{hi[0], hi[1], hi[2], hi[3]};
-        if constexpr (F32) {
-            if (x == 0 && (GPD == 1 || h == g)) {
-                __bf16 p1, p2, p3;
-                const __bf16 zero = (__bf16)0.0f;
-                pieces(fmaf(z, s, b), p1, p2, p3);
-                b8 v = b8{p1, p1, p1, p2, p2, p3, zero, zero};
-                if (GPD == 1 && h == 1) v = b8{zero, zero, zero, zero, zero, zero, zero, zero};
-                *((uint4 *)(o + I::KB) + lane) = __builtin_bit_cast(uint4, v);
-                if (GPD == 2 || h == 0) ((float *)(o + I::KS))[32 * g + n32] = s;
-            }
+        if (x == 0 && (GPD == 1 || h == g)) {
+            __bf16 p1, p2, p3;
+            const __bf16 zero = (__bf16)0.0f;
+            pieces(fmaf(z, s, b), p1, p2, p3);
+            b8 v = b8{p1, p1, p1, p2, p2, p3, zero, zero};
+            if (GPD == 1 && h == 1) v = b8{zero, zero, zero, zero, zero, zero, zero, zero};
+            *((uint4 *)(o + I::KB) + lane) = __builtin_bit_cast(uint4, v);
+            if (GPD == 2 || h == 0) ((float *)(o + I::KS))[32 * g + n32] = s;
         }
     } else {
+        const float a = fmaxf(fabsf(b), fabsf(fmaf(15.0f, s, b)));
+        const bool fin = a < __builtin_inff() && s == s;
+        const int e = exp_of(wave_top(!fin ? 0.0f : F32 ? fabsf(s) : a));
         const uint64_t bad = __ballot(!fin);
         if (g == 0 && x == 0 && lane == 0) {
             meta[blockIdx.x].ev = e + (bad ? kSomeBad : 0);
@@ -233,16 +223,13 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
     // for with the phase's LDS reads: 183 against 175 us for 2000 tokens of 32Q/32KV);
     // bf16: scalars of this sub-tile (readlane instead: 1113 against 1096 us for 2048
     // tokens at 30720 of 32Q/8KV)
-    float m_ek = 1.0f;
     int m_ev = 0;
     auto load_meta = [&](int i) __attribute__((always_inline)) {
         if constexpr (F32) {
             if (i % 64 == 0) m_ev = mt[min(i + lane, n_i - 1)].ev;
         } else {
             typedef const __attribute__((address_space(4))) Meta *Const;
-            const Const p = (Const)(uintptr_t)mt + min(i, n_i - 1);
-            m_ek = p->ek;
-            m_ev = p->ev;
+            m_ev = ((Const)(uintptr_t)mt + min(i, n_i - 1))->ev;
         }
     };
 
@@ -261,10 +248,9 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
         }
     };
 
-    // What passes from one phase to the next: the dots of a sub-tile (f32: K's bias
-    // terms, then each group's), then its weights as operands (f32: by group, high and
-    // low parts).
-    constexpr int NS = F32 ? GPD + 1 : 1, NP = F32 ? 2 * GPD : 1;
+    // What passes from one phase to the next: the dots of a sub-tile (K's bias terms,
+    // then each group's), then its weights as operands (f32: by group, high and low parts).
+    constexpr int NS = GPD + 1, NP = F32 ? 2 * GPD : 1;
     v16f S[NS];
     h8 P[NP][2];
 #pragma unroll
@@ -273,6 +259,10 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
 
     // operands read ahead of their phase: V of sub-tile i - 1, K of i
     h8 KF[PF ? GPD * 4 : 1], VF[PF ? GPD * 4 : 1];
+    b8 KB;
+    auto kb_op = [&](int i) {
+        return __builtin_bit_cast(b8, ((const uint4 *)(lds + (i & (kRing - 1)) * I::BYTES + I::KB))[lane]);
+    };
     auto k_op = [&](int i, int f) {
         return __builtin_bit_cast(h8, ((const uint4 *)(lds + (i & (kRing - 1)) * I::BYTES))[f * 64 + lane]);
     };
@@ -283,6 +273,7 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
     };
     auto read_ahead = [&](int i) {
         if constexpr (PF) {
+            KB = kb_op(i);
 #pragma unroll
             for (int f = 0; f < GPD * 4; f++) KF[f] = k_op(i, f);
 #pragma unroll
@@ -297,16 +288,11 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
         for (int n = 0; n < NS; n++)
 #pragma unroll
             for (int k = 0; k < 16; k++) S[n][k] = 0.0f;
-        if constexpr (F32) {
-            const uint4 kb = ((const uint4 *)(lds + (i & (kRing - 1)) * I::BYTES + I::KB))[lane];
-            S[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, kb), Q.bias, S[0], 0, 0,
-                                                           0);
-        }
+        S[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(PF ? KB : kb_op(i), Q.bias, S[0], 0, 0, 0);
 #pragma unroll
         for (int f = 0; f < GPD * 4; f++) {
             const h8 a = PF ? KF[PF ? f : 0] : k_op(i, f);
-            constexpr int one = F32 ? 1 : 0;
-            const int n = one * (1 + f / 4);
+            const int n = 1 + f / 4;
             if constexpr (F32) S[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, Q.b[f], S[n], 0, 0, 0);
             S[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, Q.a[f], S[n], 0, 0, 0);
         }
@@ -329,17 +315,14 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
         const int ev_b = F32 ? __builtin_amdgcn_readlane(m_ev, i & 63) : m_ev;
         const int ev = ev_b < kSomeBad / 2 ? ev_b : ev_b - kSomeBad;
         v16f &s = S[0];
-        if constexpr (F32) {
 #pragma unroll
-            for (int g = 0; g < GPD; g++)
+        for (int g = 0; g < GPD; g++)
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const v4f sc = *(const v4f *)((const float *)(t + I::KS) + 32 * g + 8 * k + 4 * h);
+            for (int k = 0; k < 4; k++) {
+                const v4f sc = *(const v4f *)((const float *)(t + I::KS) + 32 * g + 8 * k + 4 * h);
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        s[4 * k + e] = fmaf(sc[e], S[1 + g][4 * k + e], s[4 * k + e]);
-                }
-        }
+                for (int e = 0; e < 4; e++) s[4 * k + e] = fmaf(sc[e], S[1 + g][4 * k + e], s[4 * k + e]);
+            }
         const bool masked = lo + 32 * (i + 1) > vis_min;
         if (masked) {
             const int n = vis - (lo + 32 * i + 4 * h);   // tokens seen from this lane's first on
@@ -347,11 +330,10 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
             for (int k = 0; k < 16; k++)
                 s[k] = 8 * (k >> 2) + (k & 3) < n ? s[k] : -__builtin_inff();
         }
-        const float rft = F32 ? Q.rf : Q.rf * m_ek;
         float top = fmaxf(fmaxf(s[0], s[1]), s[2]);
 #pragma unroll
         for (int k = 3; k < 16; k++) top = fmaxf(top, s[k]);
-        const float need = fmaf(half_max(top), rft, (float)ev - kWinTop);
+        const float need = fmaf(half_max(top), Q.rf, (float)ev - kWinTop);
         if (__ballot(need > M + kWinTau) != 0) {
             const float mn = fmaxf(M, need);
             const float al = __builtin_amdgcn_exp2f(M - mn);
@@ -377,7 +359,7 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
         const float mr = F32 ? -M : (float)ev - M;
         float p[16];
 #pragma unroll
-        for (int k = 0; k < 16; k++) p[k] = __builtin_amdgcn_exp2f(fmaf(s[k], rft, mr));
+        for (int k = 0; k < 16; k++) p[k] = __builtin_amdgcn_exp2f(fmaf(s[k], Q.rf, mr));
         const float sum = (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]))) +
                           (((p[8] + p[9]) + (p[10] + p[11])) + ((p[12] + p[13]) + (p[14] + p[15])));
         L += F32 ? sum : scale2(sum, -ev);

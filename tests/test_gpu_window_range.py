@@ -1,0 +1,121 @@
+"""Windows (eakv_attention_window_batch_device) at values where an operand of 16 bits would
+show: K on an offset, tokens of very different magnitudes side by side, queries of zeros and
+near the end of f32's range; against the exact attention of the cache's own planes in 64
+bits, by both ways that a window takes (kernels of few rows, expanded operands).  Bounds in
+windows.py, and K exact (wide=False) in all of them."""
+import numpy as np
+import pytest
+
+import windows as W
+from test_gpu_window import E  # noqa: F401  (the fixture)
+from test_gpu_window_prompt import Head, expanded
+
+pytestmark = pytest.mark.gpu
+
+# (kv heads, q heads, [(start, tokens)]): few rows per kv head; many, expanded
+FEW = (2, 4, [(40, 12)])
+MANY = (8, 128, [(40, 72)] * 3)
+WAYS = [FEW, MANY]
+
+
+def data(rng, way, d):
+    """Caches' K and V [1][2][n_kv][t][d] and queries, of normal values."""
+    n_kv, n_q, wins = way
+    xs = [rng.standard_normal((1, 2, n_kv, s + m, d), dtype=np.float32) for s, m in wins]
+    return xs, rng.standard_normal((sum(m for _, m in wins), n_q, d), dtype=np.float32)
+
+
+def attend(E, way, d, xs, q, bf16, words=None):
+    """Outputs [rows][n_q][d] and the queries as the kernel reads them, with the caches."""
+    n_kv, n_q, wins = way
+    caches = []
+    for x in xs:
+        c = E.Cache(1, n_kv, d, x.shape[3] + 5)
+        c.load_raw(x, x.shape[3])
+        caches.append(c)
+    call = W.Call(E, caches, [m for _, m in wins], n_q, n_kv, bf16, [s for s, _ in wins], words)
+    assert way is FEW or expanded(call, wins, n_kv)
+    q = call.put(q)
+    call.run()
+    return call.get(), q, caches
+
+
+def sample(n_kv, n_q):
+    """(kv head, q head) pairs to look at."""
+    g = n_q // n_kv
+    return sorted({(k, k * g + i) for k in (0, n_kv - 1) for i in (0, g - 1)})
+
+
+def exact(cache, q, start, k, words=None):
+    return W.attend(Head(cache, k), 0, np.ascontiguousarray(q[:, None]), start, 1, 1, words, wide=False)
+
+
+def verify(way, got, q, caches, bf16, words=None, rows=None):
+    """The sampled heads of every window, or of its `rows` (bool by token)."""
+    n_kv, n_q, wins = way
+    at = 0
+    for c, (s, m) in zip(caches, wins):
+        pick = np.ones(m, bool) if rows is None else rows
+        for k, h in sample(n_kv, n_q):
+            want, tol, half = exact(c, q[at:at + m, h], s, k, words)
+            rel = W.check(got[at:at + m, h][pick], want[pick, 0], tol[pick, 0], half[pick, 0], bf16)
+        print("  rel", rel, flush=True)
+        at += m
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("way", WAYS)
+def test_keys_on_an_offset(E, rng, way, d, bf16):
+    """K = 100 + normal values: rounded to f16 (steps of 1/16) the scores are off by
+    1/16/sqrt(12) = 0.018 each, and the output by as much of its norm.  Exact K: c * sum(q)
+    in three pieces each is off by some 2^-23 * 100 * |sum(q)| / sqrt(d) = 1e-5, in f32 four
+    times the norm's bound at scores of normal data: 4e-5 is asked for."""
+    xs, q = data(rng, way, d)
+    for x in xs:
+        x[:, 0] += 100.0
+    got, q, caches = attend(E, way, d, xs, q, bf16)
+    at = 0
+    n_kv, n_q, wins = way
+    for c, (s, m) in zip(caches, wins):
+        for k, h in sample(n_kv, n_q):
+            want, tol, half = exact(c, q[at:at + m, h], s, k)
+            err = np.abs(got[at:at + m, h] - want[:, 0])
+            lim = tol[:, 0] + (half[:, 0] + W.O16 * np.abs(want[:, 0]) if bf16 else 0.0)
+            assert (err <= lim).all()
+            rel = np.linalg.norm(err) / np.linalg.norm(want)
+            print("  rel", rel, flush=True)
+            assert rel <= (2 * W.O16 / 3 if bf16 else 4e-5)
+        at += m
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("size", [0.0, 1e-30, 1e-3, 1.0])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("way", WAYS)
+def test_queries_of_zeros(E, rng, way, d, size, bf16):
+    """Rows of zeros (and of values far below the normal f16) give the mean of the V that
+    they see, whatever K's size; planes of zeros as a new cache has them among those."""
+    xs, q = data(rng, way, d)
+    for x in xs:
+        x[:, 0] *= size
+    q[::2] = 0.0
+    q[1::4] *= 1e-36
+    got, q, caches = attend(E, way, d, xs, q, bf16)
+    verify(way, got, q, caches, bf16)
+
+
+@pytest.mark.parametrize("way", WAYS)
+def test_room_of_a_new_cache(E, rng, way):
+    """K and V never written, all zeros: zeros come out, for zero queries too."""
+    n_kv, n_q, wins = way
+    for bf16 in (False, True):
+        caches = [E.Cache(1, n_kv, 128, s + m) for s, m in wins]
+        for c, (s, m) in zip(caches, wins):
+            c.advance(s + m)
+        call = W.Call(E, caches, [m for _, m in wins], n_q, n_kv, bf16, [s for s, _ in wins])
+        q = rng.standard_normal((call.total, n_q, 128), dtype=np.float32)
+        q[::3] = 0.0
+        call.put(q)
+        call.run()
+        assert (call.get() == 0.0).all()
