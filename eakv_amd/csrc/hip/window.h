@@ -186,8 +186,9 @@ __device__ __forceinline__ float half_max(float v)
 // A row's query as the columns' operand of S^T = K Q^T, one lane's share: operand
 // (g, octet o, nibble n) of half h holds dims 64g + 32n + 16h + 8o + 0..7 in nib2's
 // order (0 2 1 3 4 6 5 7).  The row is scaled by a power of two to below 2^15.
-// SUB: against nib_sub's operands: the high nibbles' dims 2^-4 of that, and the
-// dots (with K's biases scaled alike) come out 2^-24 of theirs.
+// SUB: against nib_sub's operands: the high nibbles' dims 2^-4 of that; the dots come
+// out 2^-24 of theirs, which K's scales make up for (in rf those 2^24 would pass f32's
+// range for queries from 2^121 on).
 template <int D, bool F32>
 struct QOp {
     h8 a[D / 16];                       // f16, high parts
@@ -249,7 +250,7 @@ __device__ __forceinline__ void build_q(QOp<D, F32> &Q, const QRaw<D, F32> &raw,
         }
         qs[g] = sum[0];
     }
-    Q.rf = scale2(rsd * EAKV_LOG2E, e - 15 + (SUB ? 24 : 0));
+    Q.rf = scale2(rsd * EAKV_LOG2E, e - 15);
     // half h of the bias product's 16 terms: group h's sum of q in pieces,
     // against K's pieces c1 c1 c1 c2 c2 c3 0 0
     __bf16 p1, p2, p3;

@@ -178,9 +178,9 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
         const int t0 = lo + 32 * (w + kDWaves * i);
         // tokens behind the last have no part in this (their bytes may be anything)
         const bool live = t0 + n32 < t_end;
-        // (bf16: K's nibbles as they stand, z = 0, everything scaled by 2^-24)
+        // (bf16: K's nibbles as they stand, z = 0 and 2^-24 of their values)
         const float zk = F32 ? zero_nibble(st.ks, st.kb) : 0.0f;
-        const float ck = F32 ? fmaf(zk, st.ks, st.kb) : scale2(st.kb, -24);
+        const float ck = F32 ? fmaf(zk, st.ks, st.kb) : st.kb;
         // (a non-finite group counts as zeros and makes the rows that see it NaN)
         const float va = fmaxf(fabsf(st.vb), fabsf(fmaf(15.0f, st.vs, st.vb)));
         const bool fin = va < __builtin_inff() && st.vs == st.vs;
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
         const float vs = live && fin ? st.vs : 0.0f, vb = live && fin ? st.vb : 0.0f;
         const float zv = zero_nibble(vs, vb), cv = fmaf(zv, vs, vb);
         // ---- scales to LDS
-        if (owner) S.ks[GPD == 2 ? h : 0][n32] = st.ks;
+        if (owner) S.ks[GPD == 2 ? h : 0][n32] = F32 ? st.ks : scale2(st.ks, 24);
         if (owner) {
             S.zl[GPD == 2 ? h : 0][p_step][p_half][pos] = (_Float16)(-1024.0f - zv);
             S.zh[GPD == 2 ? h : 0][p_step][p_half][pos] = (_Float16)(-64.0f - zv);

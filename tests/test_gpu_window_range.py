@@ -119,3 +119,17 @@ def test_room_of_a_new_cache(E, rng, way):
         call.put(q)
         call.run()
         assert (call.get() == 0.0).all()
+
+
+@pytest.mark.parametrize("way", WAYS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_queries_near_the_end_of_the_range(E, rng, way, d):
+    """bf16 queries beyond 2^121 against K of 2^-116: scores of standard deviation 16.  (The
+    third piece of K's biases lies below bf16's range: 2^-16 of them is lost, 2e-4 of a
+    score, far below the bound.)"""
+    xs, q = data(rng, way, d)
+    for x in xs:
+        x[:, 0] *= 2.0 ** -116
+    q *= np.float32(2.0 ** 120)
+    got, q, caches = attend(E, way, d, xs, q, True)
+    verify(way, got, q, caches, True)
