@@ -31,10 +31,11 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 
 constexpr float kWinTau = 4.0f;        // headroom of the lazy M, log2 units
-constexpr float kWinTop = 11.0f;       // weights below 2^(kWinTop + kWinTau) = 2^15
+constexpr float kWinTop = 11.0f;       // M's distance when set: weights below 2^(11 + 4)
 constexpr float kMInit = -3.4028234664e38f;
-constexpr int kExpLow = -60;           // tile exponents below this count as this
-
+constexpr int kExpLow = -60;           // exponents of q and V below this count as this
+// bf16 queries of usual sizes are read as 2^kQUp of their values
+constexpr int kQUp = 8;
 
 __device__ __forceinline__ uint32_t u_of(h2 v) { return __builtin_bit_cast(uint32_t, v); }
 __device__ __forceinline__ h2 h_of(uint32_t v) { return __builtin_bit_cast(h2, v); }
@@ -185,7 +186,8 @@ __device__ __forceinline__ float half_max(float v)
 
 // A row's query as the columns' operand of S^T = K Q^T, one lane's share: operand
 // (g, octet o, nibble n) of half h holds dims 64g + 32n + 16h + 8o + 0..7 in nib2's
-// order (0 2 1 3 4 6 5 7).  The row is scaled by a power of two to below 2^15.
+// order (0 2 1 3 4 6 5 7).  The row is scaled by a power of two to below 2^15; bf16 rows
+// of usual sizes all by the same one, so that their dots need no factor of their own.
 // SUB: against nib_sub's operands: the high nibbles' dims 2^-4 of that; the dots come
 // out 2^-24 of theirs, which K's scales make up for (in rf those 2^24 would pass f32's
 // range for queries from 2^121 on).
@@ -193,12 +195,28 @@ template <int D, bool F32>
 struct QOp {
     h8 a[D / 16];                       // f16, high parts
     h8 b[F32 ? D / 16 : 1];             // f32 queries: low parts
-    b8 bias;                            // half h: pieces of group h's sum of q
-    float rf;                           // score = dot * rf, log2 units
+    b8 bias;                            // half h: pieces of group h's sum of q; two more
+    float rf;                           // score = dot * rf, a power of two
 };
 
+// What K's scales and (bf16: against sums of q at 2^-24) biases carry beside 1/sqrt(d).
+template <bool F32>
+constexpr float kKScale = F32 ? EAKV_LOG2E : EAKV_LOG2E * (1.0f / (1 << kQUp));
+template <bool F32>
+constexpr float kKBias = F32 ? 1.0f : 0x1p24f;
+
+// K's operand of the bias product, token's half h: c's pieces against the query's, then
+// 1 1 (h = 0) or 1 and the exponent of the token's V.
+__device__ __forceinline__ b8 k_bias(float c, int e, int h)
+{
+    __bf16 p1, p2, p3;
+    const __bf16 one = (__bf16)1.0f;
+    pieces(c, p1, p2, p3);
+    return b8{p1, p1, p1, p2, p2, p3, one, h ? (__bf16)(float)e : one};
+}
+
 template <int D, bool F32, bool SUB>
-__device__ __forceinline__ void build_q(QOp<D, F32> &Q, const QRaw<D, F32> &raw, float rsd, int h)
+__device__ __forceinline__ void build_q(QOp<D, F32> &Q, const QRaw<D, F32> &raw, int h)
 {
     constexpr int GPD = D / 64;
     auto dim = [&](int f, int j) {                   // dim j of operand f
@@ -217,10 +235,10 @@ __device__ __forceinline__ void build_q(QOp<D, F32> &Q, const QRaw<D, F32> &raw,
 #pragma unroll
         for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(dim(f, j)));
     top = half_max(top);
-    // q' = q * 2^(15 - e); a row of zeros or below 2^-110 keeps e = -110
-    int e = (int)(__float_as_uint(top) >> 23) - 126;
-    e = e < -110 ? -110 : e;
-    const float scale = scale2(1.0f, 15 - e), less = SUB ? scale * 0x1p-4f : scale;
+    // q' = q * 2^up
+    int up = 15 - exp_of(top);
+    if (!F32 && (top == 0.0f || (top >= 0x1p-7f && top < 0x1p7f))) up = kQUp;
+    const float scale = scale2(1.0f, up), less = SUB ? scale * 0x1p-4f : scale;
     float qs[GPD];
 #pragma unroll
     for (int g = 0; g < GPD; g++) {
@@ -250,34 +268,145 @@ __device__ __forceinline__ void build_q(QOp<D, F32> &Q, const QRaw<D, F32> &raw,
         }
         qs[g] = sum[0];
     }
-    Q.rf = scale2(rsd * EAKV_LOG2E, e - 15);
-    // half h of the bias product's 16 terms: group h's sum of q in pieces,
-    // against K's pieces c1 c1 c1 c2 c2 c3 0 0
+    const int down = (F32 ? 0 : kQUp) - up;
+    Q.rf = scale2(1.0f, down);
+    // half h of the bias product's 16 terms: group h's sum of q in pieces, against K's
+    // c1 c1 c1 c2 c2 c3; then pieces of minus the reference point (hold_ref) against 1, and,
+    // last, 1/rf against the exponent of the token's V
     __bf16 p1, p2, p3;
     const float z = GPD == 2 ? (h ? qs[GPD - 1] : qs[0]) : (h ? 0.0f : qs[0]);
-    pieces(z, p1, p2, p3);
+    pieces(z * (1.0f / kKBias<F32>), p1, p2, p3);
     const __bf16 zero = (__bf16)0.0f;
-    Q.bias = b8{p1, p2, p3, p1, p2, p1, zero, zero};
+    Q.bias = b8{p1, p2, p3, p1, p2, p1, zero, h ? (__bf16)scale2(1.0f, -down) : zero};
 }
 
-// The maximum of a wave's values, none negative or NaN, in all lanes.  (By their bits: a
-// float maximum first makes quiet NaN of its operands, an instruction each.)
-__device__ __forceinline__ float wave_top(float v)
+// bf16: the bias product takes m off the scores from here on; what it does take off is
+// returned (pieces below bf16's normal range are dropped).
+template <int D>
+__device__ __forceinline__ float hold_ref(QOp<D, false> &Q, float m, int h)
 {
-    uint32_t u = __float_as_uint(v);
-    auto ror = [](uint32_t x, auto c) {
-        constexpr int ctrl = decltype(c)::value;
-        return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, ctrl, 0xf, 0xf, true);
-    };
-    u = max(u, ror(u, std::integral_constant<int, 0x128>{}));       // row_ror:8
-    u = max(u, ror(u, std::integral_constant<int, 0x124>{}));
-    u = max(u, ror(u, std::integral_constant<int, 0x122>{}));
-    u = max(u, ror(u, std::integral_constant<int, 0x121>{}));
-    auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    u = max((uint32_t)r[0], (uint32_t)r[1]);
-    r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    return __uint_as_float(max((uint32_t)r[0], (uint32_t)r[1]));
+    const float inv = __uint_as_float((254u << 23) - __float_as_uint(Q.rf));
+    __bf16 p[3];
+    pieces(-m * inv, p[0], p[1], p[2]);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+        p[i] = fabsf((float)p[i]) < 0x1p-126f ? (__bf16)0.0f : p[i];
+        sum += (float)p[i];
+    }
+    Q.bias[6] = h ? p[2] : p[0];
+    Q.bias[7] = h ? Q.bias[7] : p[1];
+    return -sum * Q.rf;
 }
+
+// The running softmax of a lane's row.
+template <int D, bool F32>
+struct Soft {
+    v16f O[D / 32];
+    float M = kMInit, L = 0.0f, C[D / 64];
+    float high = -__builtin_inff();     // bf16: M moves when a score passes this
+
+    __device__ __forceinline__ void clear()
+    {
+#pragma unroll
+        for (int f = 0; f < D / 32; f++)
+#pragma unroll
+            for (int k = 0; k < 16; k++) O[f][k] = 0.0f;
+#pragma unroll
+        for (int g = 0; g < D / 64; g++) C[g] = 0.0f;
+    }
+    __device__ __forceinline__ void rescale(float al)
+    {
+        L *= al;
+#pragma unroll
+        for (int f = 0; f < D / 32; f++)
+#pragma unroll
+            for (int k = 0; k < 16; k++) O[f][k] *= al;
+        if constexpr (F32)
+#pragma unroll
+            for (int g = 0; g < D / 64; g++) C[g] *= al;
+    }
+    // s: the masked scores (log2) of 16 tokens with their V's exponents added, in units
+    // of rf and, bf16, less M.  On return the weights, 2^e of the softmax's; w: 2^-e.
+    // M follows the largest weight that the row sees: rows move it one by one, so that
+    // no row's result depends on another's tokens.
+    __device__ __forceinline__ void weights(v16f &s, QOp<D, F32> &Q, const float *w, int h, float *p)
+    {
+        float top = fmaxf(fmaxf(s[0], s[1]), s[2]);
+#pragma unroll
+        for (int k = 3; k < 16; k++) top = fmaxf(top, s[k]);
+        top = half_max(top);
+        if constexpr (F32) {
+            const float need = fmaf(top, Q.rf, -kWinTop);
+            if (__ballot(need > M + kWinTau) != 0) {
+                const float mn = need > M + kWinTau ? need : M;
+                rescale(__builtin_amdgcn_exp2f(M - mn));
+                M = mn;
+            }
+#pragma unroll
+            for (int k = 0; k < 16; k++) p[k] = __builtin_amdgcn_exp2f(fmaf(s[k], Q.rf, -M));
+        } else {
+            if (__ballot(top > high) != 0) {
+                // (before a row's first tokens nothing is taken off and M is not set)
+                const bool first = high < 0.0f, move = top > high;
+                const float old = first ? 0.0f : M;
+                const float mn = hold_ref(Q, move ? old + (top - kWinTop) : old, h);
+                const float by = mn - old;
+                rescale(first ? 0.0f : __builtin_amdgcn_exp2f(-by));
+#pragma unroll
+                for (int k = 0; k < 16; k++) s[k] -= by;
+                M = move ? mn : M;
+                high = move ? kWinTop + kWinTau : high;
+            }
+#pragma unroll
+            for (int k = 0; k < 16; k++) p[k] = __builtin_amdgcn_exp2f(s[k]);
+        }
+        float sum[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const v4f w4 = *(const v4f *)(w + 8 * k + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum[e] = k ? fmaf(p[4 * k + e], w4[e], sum[e]) : p[e] * w4[e];
+        }
+        L += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    }
+    // After the last token: O whole (NaN in the groups that are named) and the row's L.
+    __device__ __forceinline__ float finish(uint32_t nan_groups)
+    {
+        if constexpr (F32) {
+#pragma unroll
+            for (int g = 0; g < D / 64; g++) {
+                const float cs = C[g] + __shfl_xor(C[g], 32, 64);
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int k = 0; k < 16; k++) O[2 * g + n][k] += cs;
+            }
+        } else {
+#pragma unroll
+            for (int f = 0; f < D / 32; f++)
+#pragma unroll
+                for (int k = 0; k < 16; k++) O[f][k] *= 0x1p-15f;          // V's operands carried 2^15
+        }
+        if (nan_groups)
+#pragma unroll
+            for (int f = 0; f < D / 32; f++)
+                if (nan_groups >> (f >> 1) & 1)
+#pragma unroll
+                    for (int k = 0; k < 16; k++) O[f][k] = __builtin_nanf("");
+        return L + __shfl_xor(L, 32, 64);
+    }
+    // The 16 weights in operand order for bf16 queries.
+    __device__ __forceinline__ static void operand(const float *p, h8 (&P)[2])
+    {
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+            const float *pp = p + 8 * ks;
+            P[ks] = __builtin_bit_cast(h8, uint4{u_of(pk_exp(pp[0], pp[2])), u_of(pk_exp(pp[1], pp[3])),
+                                                 u_of(pk_exp(pp[4], pp[6])), u_of(pk_exp(pp[5], pp[7]))});
+        }
+    }
+};
 
 // The row that a lane writes: final outputs (mc == 1) or its chunk's partial.
 struct RowOut {

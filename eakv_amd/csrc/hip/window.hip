@@ -24,14 +24,19 @@
 //                 V's operands n - z; its c terms are f32 sums of p*c.
 //   bf16 queries  Q (8 bits) is exact in f16.  V is dequantized to f16,
 //                 (n - z)*s + c with s and c rounded to f16, and p is rounded
-//                 to f16: 2^-12 relative each, against the output's 2^-9.
-// f16's range: Q rows are scaled by a power of two to below 2^15, V tiles (bf16) by
-// theirs; the softmax's reference point M includes the exponent of the
-// tile's V, so that every weight operand stays below 2^15 and keeps its
-// precision down to 2^-29 of that.
+//                 to f16: 2^-12 relative each, against the output's 2^-9 (2e-4 of the
+//                 outputs' norm before that rounding, 1.7e-3 after).
+// f16's range: Q rows are scaled by a power of two to below 2^15, and each token of V by
+// 2^-e of its own, e the exponent of its largest scale (f32) or value (bf16).  Its weight
+// carries the 2^e: e is added to its scores by two spare terms of the c terms' product, so
+// the softmax's reference point M bounds p*2^e of the tokens that a row sees, and nothing
+// else has a part in it; weight operands stay below 2^15 and keep their precision down
+// to 2^-29 of the largest.  (With one exponent for the 32 tokens of a sub-tile, one of
+// them 10^8 times the others made rows 4e-3 off that did not even see it.)  bf16: the
+// same product takes M off, so scores come out as exponents.
 //
-// Softmax in the log2 domain, f32: M moves only when a score passes it by
-// kWinTau; sums, weighted sums and M are f32.  Tokens are split into chunks where
+// Softmax in the log2 domain, f32: M moves only when a row's exponents pass it by
+// kWinTop + kWinTau; sums, weighted sums and M are f32.  Tokens are split into chunks where
 // rows alone do not fill the chip; partial (O, M, l) are merged by a second
 // launch.  No atomics: results are the same bits on every call.
 #include <string.h>

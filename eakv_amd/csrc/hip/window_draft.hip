@@ -14,7 +14,7 @@
 //
 // Bound by vector instructions: per 32 tokens x 32 rows at d = 128 a wave issues about 380
 // (f32 530) beside 17 (33) matrix products and 5 KB of loads.  8 sequences of 8 tokens
-// at 32768 of 32Q/8KV (32 rows, 336 MB): bf16 73 us in the kernel, 4.6 TB/s; f32 112.
+// at 32768 of 32Q/8KV (32 rows, 336 MB): bf16 76 us in the kernel, 4.4 TB/s; f32 116.
 // Rows beyond 32 read the planes again, out of the caches: a block of 64 rows with
 // shared operands in LDS was slower at most sizes up to 512 rows (64 rows of 8 at 20000 of
 // 64Q/8KV bf16 158 against 164 us, but 192 rows of 6: 350 against 274; 64 of 4 at 4000,
@@ -40,10 +40,11 @@ struct __align__(16) DraftLds {
     static constexpr int GPD = D / 64, kAhead = kAheadOf<F32>;
     uint8_t v[kAhead][32 * 32 * GPD];   // V's bytes: rows of 32 GPD, their 16-byte units swizzled
     float ks[GPD][32];                  // K's scales
-    float vs[F32 ? GPD : 1][32];        // f32: V's scales and biases
+    float w[32];                        // 2^-e, e the exponent of a token's V
+    float vs[F32 ? GPD : 1][32];        // f32: V's scales and biases, 2^-e of them
     float vc[F32 ? GPD : 1][32];
     // of V's operand (g, 16-token step, h), 8 tokens in operand order: -(1024 + z),
-    // -(64 + z); bf16: scales and biases in f16
+    // -(64 + z); bf16: scales and biases in f16, 2^(15 - e) of them
     _Float16 zl[GPD][2][2][8], zh[GPD][2][2][8];
     _Float16 s16[F32 ? 1 : GPD][2][2][8], c16[F32 ? 1 : GPD][2][2][8];
 };
@@ -71,7 +72,7 @@ __device__ __forceinline__ int swz(int t)
 template <int D, bool F32>
 __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, WinJob job,
                                                                 const void *q, const uint64_t *tree,
-                                                                void *out, float *part, float rsd,
+                                                                void *out, float *part, float ksc,
                                                                 int vec)
 {
     constexpr int GPD = D / 64, RB = 32 * GPD, kAhead = kAheadOf<F32>;
@@ -161,15 +162,10 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
         for (int k = 0; k < kAhead - 1; k++) load(k, st[k]);
 
     QOp<D, F32> Q;
-    build_q<D, F32, !F32>(Q, raw, rsd, h);
-    v16f O[D / 32];
-    float M = kMInit, L = 0.0f, C[GPD];
-#pragma unroll
-    for (int f = 0; f < D / 32; f++)
-#pragma unroll
-        for (int k = 0; k < 16; k++) O[f][k] = 0.0f;
-#pragma unroll
-    for (int g = 0; g < GPD; g++) C[g] = 0.0f;
+    build_q<D, F32, !F32>(Q, raw, h);
+    const bool own_rf = F32 || __ballot(Q.rf != 1.0f) != 0;
+    Soft<D, F32> R;
+    R.clear();
     uint32_t poison = 0;
     NibConst nc;
     nc.hold();
@@ -180,25 +176,27 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
         const bool live = t0 + n32 < t_end;
         // (bf16: K's nibbles as they stand, z = 0 and 2^-24 of their values)
         const float zk = F32 ? zero_nibble(st.ks, st.kb) : 0.0f;
-        const float ck = F32 ? fmaf(zk, st.ks, st.kb) : st.kb;
+        const float ck = (F32 ? fmaf(zk, st.ks, st.kb) : st.kb) * (ksc * kKBias<F32>);
         // (a non-finite group counts as zeros and makes the rows that see it NaN)
         const float va = fmaxf(fabsf(st.vb), fabsf(fmaf(15.0f, st.vs, st.vb)));
         const bool fin = va < __builtin_inff() && st.vs == st.vs;
         const uint64_t bad = __ballot(live && !fin);
         const float vs = live && fin ? st.vs : 0.0f, vb = live && fin ? st.vb : 0.0f;
         const float zv = zero_nibble(vs, vb), cv = fmaf(zv, vs, vb);
+        // the token's exponent, of both groups
+        const float x = F32 ? fabsf(vs) : live && fin ? va : 0.0f;
+        const int ev = exp_of(GPD == 2 ? half_max(x) : x);
         // ---- scales to LDS
-        if (owner) S.ks[GPD == 2 ? h : 0][n32] = F32 ? st.ks : scale2(st.ks, 24);
+        S.w[n32] = scale2(1.0f, -ev);
+        if (owner) S.ks[GPD == 2 ? h : 0][n32] = st.ks * (F32 ? ksc : ksc * 0x1p24f);
         if (owner) {
             S.zl[GPD == 2 ? h : 0][p_step][p_half][pos] = (_Float16)(-1024.0f - zv);
             S.zh[GPD == 2 ? h : 0][p_step][p_half][pos] = (_Float16)(-64.0f - zv);
         }
-        const int ev = __builtin_amdgcn_readfirstlane(
-            exp_of(wave_top(F32 ? fabsf(vs) : live && fin ? va : 0.0f)));
         if constexpr (F32) {
             if (owner) {
-                S.vs[GPD == 2 ? h : 0][n32] = vs;
-                S.vc[GPD == 2 ? h : 0][n32] = cv;
+                S.vs[GPD == 2 ? h : 0][n32] = scale2(vs, -ev);
+                S.vc[GPD == 2 ? h : 0][n32] = scale2(cv, -ev);
             }
         } else {
             if (owner) {
@@ -211,13 +209,7 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
         v16f s;
 #pragma unroll
         for (int k = 0; k < 16; k++) s[k] = 0.0f;
-        {
-            __bf16 p1, p2, p3;
-            const __bf16 zero = (__bf16)0.0f;
-            pieces(owner ? ck : 0.0f, p1, p2, p3);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b8{p1, p1, p1, p2, p2, p3, zero, zero}, Q.bias, s, 0,
-                                                        0, 0);
-        }
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_bias(owner ? ck : 0.0f, ev, h), Q.bias, s, 0, 0, 0);
         float zg[2] = {zk, zk};
         if constexpr (F32 && GPD == 2) {
             const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(zk), __float_as_uint(zk), false,
@@ -275,6 +267,10 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
             __builtin_amdgcn_sched_barrier(0);
         }
         // ---- softmax
+        if constexpr (!F32)
+            if (own_rf)
+#pragma unroll
+                for (int k = 0; k < 16; k++) s[k] *= Q.rf;
         const bool masked = t0 + 32 > vis_min;
         if (masked) {
             const int d0 = t0 + 4 * h - start;           // this lane's first token, of the window
@@ -284,23 +280,6 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
                 const bool see = tree ? d < 0 || (d < m && ((word >> (d & 63)) & 1)) : d + start < vis;
                 s[k] = see ? s[k] : -__builtin_inff();
             }
-        }
-        float top = fmaxf(fmaxf(s[0], s[1]), s[2]);
-#pragma unroll
-        for (int k = 3; k < 16; k++) top = fmaxf(top, s[k]);
-        const float need = fmaf(half_max(top), Q.rf, (float)ev - kWinTop);
-        if (__ballot(need > M + kWinTau) != 0) {
-            const float mn = fmaxf(M, need);
-            const float al = __builtin_amdgcn_exp2f(M - mn);
-            M = mn;
-            L *= al;
-#pragma unroll
-            for (int f = 0; f < D / 32; f++)
-#pragma unroll
-                for (int k = 0; k < 16; k++) O[f][k] *= al;
-            if constexpr (F32)
-#pragma unroll
-                for (int g = 0; g < GPD; g++) C[g] *= al;
         }
         if (bad) {
             // rows that see a token with a non-finite V group
@@ -312,13 +291,8 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
             poison |= (seen & (uint32_t)bad ? 1u : 0u) |
                       (GPD == 2 && (seen & (uint32_t)(bad >> 32)) ? 2u : 0u);
         }
-        const float mr = F32 ? -M : (float)ev - M;
         float p[16];
-#pragma unroll
-        for (int k = 0; k < 16; k++) p[k] = __builtin_amdgcn_exp2f(fmaf(s[k], Q.rf, mr));
-        const float sum = (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]))) +
-                          (((p[8] + p[9]) + (p[10] + p[11])) + ((p[12] + p[13]) + (p[14] + p[15])));
-        L += F32 ? sum : scale2(sum, -ev);
+        R.weights(s, Q, S.w, h, p);
         // ---- weighted sum
 #pragma unroll
         for (int g = 0; g < GPD; g++) {
@@ -343,7 +317,7 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
                         b[2 * k + e] = u_of(pk_rest(hi2, x[e], x[e + 2]));
                     }
                 }
-                C[g] += cs;
+                R.C[g] += cs;
 #pragma unroll
                 for (int ks = 0; ks < 2; ks++) {
                     P[0][ks] = __builtin_bit_cast(h8, uint4{a[4 * ks], a[4 * ks + 1], a[4 * ks + 2],
@@ -352,13 +326,7 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
                                                                       b[4 * ks + 2], b[4 * ks + 3]});
                 }
             } else {
-#pragma unroll
-                for (int ks = 0; ks < 2; ks++) {
-                    const float *pp = p + 8 * ks;
-                    P[0][ks] = __builtin_bit_cast(
-                        h8, uint4{u_of(pk_exp(pp[0], pp[2])), u_of(pk_exp(pp[1], pp[3])),
-                                  u_of(pk_exp(pp[4], pp[6])), u_of(pk_exp(pp[5], pp[7]))});
-                }
+                Soft<D, F32>::operand(p, P[0]);
             }
 #pragma unroll
             for (int ks = 0; ks < 2; ks++) {
@@ -382,12 +350,12 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
                 const h8 va = __builtin_bit_cast(h8, uint4{a[0], a[1], a[2], a[3]});
                 const h8 vb8 = __builtin_bit_cast(h8, uint4{b[0], b[1], b[2], b[3]});
                 if constexpr (F32) {
-                    O[2 * g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, P[F32 ? 1 : 0][ks], O[2 * g], 0, 0, 0);
-                    O[2 * g + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vb8, P[F32 ? 1 : 0][ks],
-                                                                          O[2 * g + 1], 0, 0, 0);
+                    R.O[2 * g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, P[F32 ? 1 : 0][ks], R.O[2 * g], 0, 0, 0);
+                    R.O[2 * g + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vb8, P[F32 ? 1 : 0][ks],
+                                                                          R.O[2 * g + 1], 0, 0, 0);
                 }
-                O[2 * g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, P[0][ks], O[2 * g], 0, 0, 0);
-                O[2 * g + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vb8, P[0][ks], O[2 * g + 1], 0, 0, 0);
+                R.O[2 * g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, P[0][ks], R.O[2 * g], 0, 0, 0);
+                R.O[2 * g + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vb8, P[0][ks], R.O[2 * g + 1], 0, 0, 0);
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -409,30 +377,9 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
         wait_loads<0>();
     }
 
-    const float l = L + __shfl_xor(L, 32, 64);
-    if constexpr (F32) {
-#pragma unroll
-        for (int g = 0; g < GPD; g++) {
-            const float cs = C[g] + __shfl_xor(C[g], 32, 64);
-#pragma unroll
-            for (int n = 0; n < 2; n++)
-#pragma unroll
-                for (int k = 0; k < 16; k++) O[2 * g + n][k] += cs;
-        }
-    } else {
-#pragma unroll
-        for (int f = 0; f < D / 32; f++)
-#pragma unroll
-            for (int k = 0; k < 16; k++) O[f][k] *= 0x1p-15f;          // V's operands carried 2^15
-    }
-    poison |= __shfl_xor(poison, 32, 64);
-    if (poison)
-#pragma unroll
-        for (int f = 0; f < D / 32; f++)
-            if (poison >> (f >> 1) & 1)
-#pragma unroll
-                for (int k = 0; k < 16; k++) O[f][k] = __builtin_nanf("");
-    join_put<D, F32, kDWaves>((float *)lds, w, lane, O, l, M, r0 + n32 < rows,
+    uint32_t nan_groups = poison | __shfl_xor(poison, 32, 64);
+    const float l = R.finish(nan_groups);
+    join_put<D, F32, kDWaves>((float *)lds, w, lane, R.O, l, R.M, r0 + n32 < rows,
                               row_out(job, c, chunk, tok, head, D, qrow, vec, part), out, part);
 }
 
@@ -447,7 +394,7 @@ int launch(const eakvd_geom &g, const WinJob &job, const void *q, const uint64_t
     const int e = allow_lds((const void *)kern, bytes, done);
     if (e) return e;
     hipLaunchKernelGGL(kern, dim3((unsigned)job.pre[job.n_seq]), dim3(64 * kDWaves), bytes, st, g, job, q,
-                       tree, out, part, 1.0f / sqrtf((float)D), (int)vec);
+                       tree, out, part, kKScale<F32> / sqrtf((float)D), (int)vec);
     return (int)hipGetLastError();
 }
 

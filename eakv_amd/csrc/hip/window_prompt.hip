@@ -8,20 +8,21 @@
 // vector instructions are the softmax's alone.
 //
 // K: n - z, exact, with the scales and biases beside them, as in window.hip.  (Values in
-// f16 instead save the scales' 32 instructions per 32 x 32 and a product, 1071 us against
-// 1311 for the prompt below; but their 2^-12 enters the scores times the scores' size:
+// f16 instead save the scales' 32 instructions per 32 x 32 and a product, 1030 us against
+// 1206 for the prompt below; but their 2^-12 enters the scores times the scores' size:
 // K on an offset of 100 made outputs 2e-2 off.)  V, f32 queries: likewise; bf16 queries:
-// values n*s + b (f32) scaled by the sub-tile's power of two and rounded to f16, 2^-12
+// values n*s + b (f32) scaled by the token's power of two and rounded to f16, 2^-12
 // relative.
 //
 // Attention: 8 waves per block, two per SIMD, 32 rows each, through a ring of 8 sub-tiles
 // in LDS with a barrier every kStep.  A step of a wave is the products (the next
 // sub-tile's scores and this one's weighted sum), then the softmax; a SIMD's two
-// waves are in different halves of it.  bf16 operands are read ahead of their step.
+// waves are in different halves of it.
 //
 // Bound by the matrix cores and the vector ALUs together: 2048 tokens at 30720 of
-// 32Q/8KV, bf16 (1.07 Tflop): 1311 us, 813 Tflop/s.  f32, twice the products and 320 vector
-// instructions for 32 x 32: 2.2 us per 32 tokens of a block against 1.3.
+// 32Q/8KV, bf16 (1.07 Tflop): 1206 us, 884 Tflop/s, no more than one of the two busy at
+// most times.  f32, twice the products and 320 vector instructions for 32 x 32: 2.2 us
+// per 32 tokens of a block against 1.2.
 #include <string.h>
 
 #include "window.h"
@@ -38,33 +39,35 @@ constexpr int kStep = 3;
 typedef __attribute__((address_space(3))) void *lds_p;
 
 // Bytes of an expanded sub-tile: K operands (g, octet, nibble), V operands (g, nibble,
-// 16-token step), 1 KB each; K's bias pieces (1 KB), then scales of K and (f32) scales and
-// biases of V, [group][token].
+// 16-token step), 1 KB each; K's operand of the bias product (1 KB), then scales of K
+// [group][token], 2^-e of the tokens' exponents e of V, and (f32) 2^-e of the scales and
+// biases of V [group][token].
 template <int D, bool F32>
 struct Img {
     static constexpr int GPD = D / 64;
     static constexpr int V = GPD * 4 * 1024;
     static constexpr int KB = 2 * V;
     static constexpr int KS = KB + 1024;
-    static constexpr int VS = KS + GPD * 128;
+    static constexpr int W = KS + GPD * 128;
+    static constexpr int VS = W + 128;
     static constexpr int VC = VS + GPD * 128;
-    static constexpr int BYTES = KB + 2048;
-    static constexpr int LOADS = (BYTES / 1024 + kPWaves - 1) / kPWaves;   // of a wave
+    static constexpr int BYTES = F32 ? VC + GPD * 128 : VS;
+    static constexpr int N = (BYTES + 1023) / 1024;         // pieces of 1 KB, the last one
+                                                            // over the end of the one before
+    static constexpr int LOADS = N / kPWaves;            // of each wave; the first
+    static constexpr int MORE = N % kPWaves;             // MORE waves one more
 };
 
-// Per sub-tile.
+// Per sub-tile: tokens with non-finite V, by group.
 struct Meta {
-    int ev;                             // exponent of V; kSomeBad added where bad is not 0
-    uint32_t bad[2];                    // tokens with non-finite V, by group
-    uint32_t none;
+    uint32_t bad[2];
 };
-constexpr int kSomeBad = 1 << 16;
 
 // One block per (sub-tile, kv head), two operands of 1 KB to a wave: wave j < 2 GPD makes
 // K's of (g, octet), the others V's of (g, 16-token step).
 template <int D, bool F32>
 __global__ __launch_bounds__(64 * 4 * (D / 64)) void expand_kernel(eakvd_geom geo, WinJob job,
-                                                                   uint8_t *img, Meta *meta)
+                                                                   uint8_t *img, Meta *meta, float ksc)
 {
     constexpr int GPD = D / 64;
     typedef Img<D, F32> I;
@@ -86,6 +89,13 @@ __global__ __launch_bounds__(64 * 4 * (D / 64)) void expand_kernel(eakvd_geom ge
     const int64_t tn = min(t0 + n32, t_last);
     const int64_t gi = g0 + tn * GPD + (GPD == 2 ? h : 0);
     const float s = P.s[gi], b = P.b[gi];
+    // V's scales, finite or not, and its token's exponent
+    const Planes Pv = planes_of(geo, job.base[c], job.layer, 1);
+    const float vs = is_v ? s : Pv.s[gi], vb = is_v ? b : Pv.b[gi];
+    const float a = fmaxf(fabsf(vb), fabsf(fmaf(15.0f, vs, vb)));
+    const bool fin = a < __builtin_inff() && vs == vs;
+    const float top = !fin ? 0.0f : F32 ? fabsf(vs) : a;
+    const int e = exp_of(GPD == 2 ? half_max(top) : top);
     if (!is_v) {
         const uint2 by = *(const uint2 *)(P.w + (g0 + tn * GPD + g) * 32 + 16 * h + 8 * x);
         const uint32_t xs[2] = {by.x, by.y};
@@ -108,24 +118,18 @@ __global__ __launch_bounds__(64 * 4 * (D / 64)) void expand_kernel(eakvd_geom ge
         ok[0] = uint4{lo[0], lo[1], lo[2], lo[3]};
         ok[64] = uint4{hi[0], hi[1], hi[2], hi[3]};
         if (x == 0 && (GPD == 1 || h == g)) {
-            __bf16 p1, p2, p3;
-            const __bf16 zero = (__bf16)0.0f;
-            pieces(fmaf(z, s, b), p1, p2, p3);
-            b8 v = b8{p1, p1, p1, p2, p2, p3, zero, zero};
-            if (GPD == 1 && h == 1) v = b8{zero, zero, zero, zero, zero, zero, zero, zero};
-            *((uint4 *)(o + I::KB) + lane) = __builtin_bit_cast(uint4, v);
-            if (GPD == 2 || h == 0) ((float *)(o + I::KS))[32 * g + n32] = s;
+            const float k = fmaf(z, s, b) * (ksc * kKBias<F32>);
+            *((uint4 *)(o + I::KB) + lane) =
+                __builtin_bit_cast(uint4, k_bias(GPD == 1 && h == 1 ? 0.0f : k, e, h));
+            if (GPD == 2 || h == 0) ((float *)(o + I::KS))[32 * g + n32] = s * ksc;
         }
     } else {
-        const float a = fmaxf(fabsf(b), fabsf(fmaf(15.0f, s, b)));
-        const bool fin = a < __builtin_inff() && s == s;
-        const int e = exp_of(wave_top(!fin ? 0.0f : F32 ? fabsf(s) : a));
         const uint64_t bad = __ballot(!fin);
         if (g == 0 && x == 0 && lane == 0) {
-            meta[blockIdx.x].ev = e + (bad ? kSomeBad : 0);
             meta[blockIdx.x].bad[0] = (uint32_t)bad;
             meta[blockIdx.x].bad[1] = GPD == 2 ? (uint32_t)(bad >> 32) : 0;
         }
+        if (g == 0 && x == 0 && h == 0) ((float *)(o + I::W))[n32] = scale2(1.0f, -e);
         // column n32 of group g; tokens 16x + 8(j/4) + 4h + j%4
         float v0[8], v1[8];
         uint32_t n0[8];
@@ -143,8 +147,9 @@ __global__ __launch_bounds__(64 * 4 * (D / 64)) void expand_kernel(eakvd_geom ge
                 v0[j] = (float)(n0[j] & 15) - zz[j];
                 v1[j] = (float)(n0[j] >> 4) - zz[j];
             } else {
-                v0[j] = fj ? 0.0f : scale2(fmaf((float)(n0[j] & 15), sj, bj), 15 - e);
-                v1[j] = fj ? 0.0f : scale2(fmaf((float)(n0[j] >> 4), sj, bj), 15 - e);
+                const int ej = __shfl(e, tl, 64);
+                v0[j] = fj ? 0.0f : scale2(fmaf((float)(n0[j] & 15), sj, bj), 15 - ej);
+                v1[j] = fj ? 0.0f : scale2(fmaf((float)(n0[j] >> 4), sj, bj), 15 - ej);
             }
         }
         uint4 *ov = (uint4 *)(o + I::V) + (g * 4 + x) * 64 + lane;
@@ -156,18 +161,18 @@ __global__ __launch_bounds__(64 * 4 * (D / 64)) void expand_kernel(eakvd_geom ge
             if (g == 0 && x == 0 && (GPD == 2 || h == 0)) {
                 // (a non-finite group counts as zeros and makes the rows that see it NaN)
                 const float z = zero_nibble(s, b);
-                ((float *)(o + I::VS))[lane] = fin ? s : 0.0f;
-                ((float *)(o + I::VC))[lane] = fin ? fmaf(z, s, b) : 0.0f;
+                ((float *)(o + I::VS))[lane] = fin ? scale2(s, -e) : 0.0f;
+                ((float *)(o + I::VC))[lane] = fin ? scale2(fmaf(z, s, b), -e) : 0.0f;
             }
         }
     }
 }
 
-// PF: operands are read from LDS ahead of their step (bf16).
+// PF: operands are read from LDS ahead of their step.  d = 64 in bf16 without: two blocks
+// to a CU.
 template <int D, bool F32, bool PF>
-__global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
-    WinJob job, const uint8_t *img, const Meta *meta, const void *q, void *out, float *part, float rsd,
-    int vec)
+__global__ __launch_bounds__(64 * kPWaves, D == 64 && !F32 && !PF ? 4 : 2) void prompt_kernel(
+    WinJob job, const uint8_t *img, const Meta *meta, const void *q, void *out, float *part, int vec)
 {
     constexpr int GPD = D / 64;
     typedef Img<D, F32> I;
@@ -202,16 +207,11 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
     {
         QRaw<D, F32> raw;
         load_q<D, F32>(raw, q, qrow, vec, h);
-        build_q<D, F32, false>(Q, raw, rsd, h);
+        build_q<D, F32, false>(Q, raw, h);
     }
-    v16f O[D / 32];
-    float M = kMInit, L = 0.0f, C[GPD];
-#pragma unroll
-    for (int f = 0; f < D / 32; f++)
-#pragma unroll
-        for (int k = 0; k < 16; k++) O[f][k] = 0.0f;
-#pragma unroll
-    for (int g = 0; g < GPD; g++) C[g] = 0.0f;
+    const bool own_rf = F32 || __ballot(Q.rf != 1.0f) != 0;
+    Soft<D, F32> R;
+    R.clear();
     // sub-tiles that a row of this wave sees
     const int vis_max = r0 < rows ? start + min(r0 + 31, rows - 1) / qpk + 1 : 0;
     const int n_w = min(n_i, vis_max > lo ? (vis_max - lo + 31) / 32 : 0);
@@ -219,32 +219,37 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
     const int64_t tile0 = job.img[c] + (int64_t)kvh * job.nsub[c] + lo / 32;
     const uint8_t *src = img + tile0 * I::BYTES;
     const Meta *mt = meta + tile0;
-    // f32: lane j holds the meta data of sub-tile 64k + j (scalar loads would be waited
-    // for with the phase's LDS reads: 183 against 175 us for 2000 tokens of 32Q/32KV);
-    // bf16: scalars of this sub-tile (readlane instead: 1113 against 1096 us for 2048
-    // tokens at 30720 of 32Q/8KV)
-    int m_ev = 0;
+    // f32: lane j holds whether sub-tile 64k + j has non-finite V (scalar loads would be
+    // waited for with the phase's LDS reads: 183 against 175 us for 2000 tokens of
+    // 32Q/32KV); bf16: scalars of this sub-tile (readlane instead: 1113 against 1096 us for
+    // 2048 tokens at 30720 of 32Q/8KV)
+    uint32_t m_bad = 0;
     auto load_meta = [&](int i) __attribute__((always_inline)) {
         if constexpr (F32) {
-            if (i % 64 == 0) m_ev = mt[min(i + lane, n_i - 1)].ev;
+            if (i % 64 == 0) {
+                const Meta &x = mt[min(i + lane, n_i - 1)];
+                m_bad = x.bad[0] | x.bad[1];
+            }
         } else {
             typedef const __attribute__((address_space(4))) Meta *Const;
-            m_ev = ((Const)(uintptr_t)mt + min(i, n_i - 1))->ev;
+            const Const x = (Const)(uintptr_t)mt + min(i, n_i - 1);
+            m_bad = x->bad[0] | x->bad[1];
         }
     };
 
-    // sub-tile i into its ring slot: this wave's pieces of 1 KB (the last wave may
-    // repeat one)
+    // sub-tile i into its ring slot: this wave's pieces of 1 KB.  (Lanes all load, or else
+    // the compiler may split and join loads, and sync counts them.)
     auto fetch = [&](int i) {
         const int j = min(i, n_i - 1);
         const uint8_t *p = src + (int64_t)j * I::BYTES;
         uint8_t *slot = lds + (i & (kRing - 1)) * I::BYTES;
 #pragma unroll
-        for (int k = 0; k < I::LOADS; k++) {
-            const int piece = min(w + kPWaves * k, I::BYTES / 1024 - 1);
+        for (int k = 0; k < I::LOADS + 1; k++) {
+            if (k == I::LOADS && w >= I::MORE) break;
+            const int at = min((w + kPWaves * k) * 1024, I::BYTES - 1024);
             __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) void *)(p + piece * 1024 + lane * 16),
-                (lds_p)(slot + piece * 1024), 16, 0, 0);
+                (const __attribute__((address_space(1))) void *)(p + at + lane * 16), (lds_p)(slot + at), 16,
+                0, 0);
         }
     };
 
@@ -257,9 +262,6 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
     for (int n = 0; n < NP; n++)
         P[n][0] = P[n][1] = __builtin_bit_cast(h8, uint4{0, 0, 0, 0});
 
-    // operands read ahead of their phase: V of sub-tile i - 1, K of i
-    h8 KF[PF ? GPD * 4 : 1], VF[PF ? GPD * 4 : 1];
-    b8 KB;
     auto kb_op = [&](int i) {
         return __builtin_bit_cast(b8, ((const uint4 *)(lds + (i & (kRing - 1)) * I::BYTES + I::KB))[lane]);
     };
@@ -271,6 +273,9 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
         return __builtin_bit_cast(h8, ((const uint4 *)(lds + (i & (kRing - 1)) * I::BYTES + I::V))
                                           [((f >> 1) * 4 + (f & 1) * 2 + ks) * 64 + lane]);
     };
+    // operands read ahead of their phase: K of sub-tile i, V of i - 1
+    b8 KB;
+    h8 KF[PF ? GPD * 4 : 1], VF[PF ? GPD * 4 : 1];
     auto read_ahead = [&](int i) {
         if constexpr (PF) {
             KB = kb_op(i);
@@ -288,6 +293,7 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
         for (int n = 0; n < NS; n++)
 #pragma unroll
             for (int k = 0; k < 16; k++) S[n][k] = 0.0f;
+        const uint8_t *t = lds + (i & (kRing - 1)) * I::BYTES;
         S[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(PF ? KB : kb_op(i), Q.bias, S[0], 0, 0, 0);
 #pragma unroll
         for (int f = 0; f < GPD * 4; f++) {
@@ -296,33 +302,37 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
             if constexpr (F32) S[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, Q.b[f], S[n], 0, 0, 0);
             S[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, Q.a[f], S[n], 0, 0, 0);
         }
+        auto weigh = [&](int ks, int f) __attribute__((always_inline)) {
+            const h8 v = PF ? VF[PF ? 2 * f + ks : 0] : v_op(max(i - 1, 0), f, ks);
+            if constexpr (F32)
+                R.O[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, P[2 * (f >> 1) + 1][ks], R.O[f], 0, 0, 0);
+            R.O[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, P[F32 ? 2 * (f >> 1) : 0][ks], R.O[f], 0, 0, 0);
+        };
+        if constexpr (F32)
 #pragma unroll
-        for (int ks = 0; ks < 2; ks++)
+            for (int n = 0; n < D / 16; n++) weigh(n / (D / 32), n % (D / 32));
+        // K's scales (bf16: beside V's products, 1251 us for the prompt above against 1290)
 #pragma unroll
-            for (int f = 0; f < D / 32; f++) {
-                const h8 v = PF ? VF[PF ? 2 * f + ks : 0] : v_op(max(i - 1, 0), f, ks);
-                if constexpr (F32)
-                    O[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, P[2 * (f >> 1) + 1][ks], O[f], 0, 0, 0);
-                O[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, P[F32 ? 2 * (f >> 1) : 0][ks], O[f], 0, 0,
-                                                              0);
-            }
+        for (int n = 0; n < 4 * GPD; n++) {
+            const int g = n >> 2, k = n & 3;
+            const v4f sc = *(const v4f *)((const float *)(t + I::KS) + 32 * g + 8 * k + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                S[0][4 * k + e] = fmaf(sc[e], S[1 + g][4 * k + e], S[0][4 * k + e]);
+            if constexpr (!F32) weigh(n / (D / 32), n % (D / 32));
+        }
     };
 
     // vector phase: scores, M, weights
     uint32_t poison = 0;                // groups of this row that are NaN
     auto softmax = [&](int i) __attribute__((always_inline)) {
         const uint8_t *t = lds + (i & (kRing - 1)) * I::BYTES;
-        const int ev_b = F32 ? __builtin_amdgcn_readlane(m_ev, i & 63) : m_ev;
-        const int ev = ev_b < kSomeBad / 2 ? ev_b : ev_b - kSomeBad;
+        const uint32_t bad = F32 ? __builtin_amdgcn_readlane(m_bad, i & 63) : m_bad;
         v16f &s = S[0];
+        if constexpr (!F32)
+            if (own_rf)
 #pragma unroll
-        for (int g = 0; g < GPD; g++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const v4f sc = *(const v4f *)((const float *)(t + I::KS) + 32 * g + 8 * k + 4 * h);
-#pragma unroll
-                for (int e = 0; e < 4; e++) s[4 * k + e] = fmaf(sc[e], S[1 + g][4 * k + e], s[4 * k + e]);
-            }
+                for (int k = 0; k < 16; k++) s[k] *= Q.rf;
         const bool masked = lo + 32 * (i + 1) > vis_min;
         if (masked) {
             const int n = vis - (lo + 32 * i + 4 * h);   // tokens seen from this lane's first on
@@ -330,24 +340,7 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
             for (int k = 0; k < 16; k++)
                 s[k] = 8 * (k >> 2) + (k & 3) < n ? s[k] : -__builtin_inff();
         }
-        float top = fmaxf(fmaxf(s[0], s[1]), s[2]);
-#pragma unroll
-        for (int k = 3; k < 16; k++) top = fmaxf(top, s[k]);
-        const float need = fmaf(half_max(top), Q.rf, (float)ev - kWinTop);
-        if (__ballot(need > M + kWinTau) != 0) {
-            const float mn = fmaxf(M, need);
-            const float al = __builtin_amdgcn_exp2f(M - mn);
-            M = mn;
-            L *= al;
-#pragma unroll
-            for (int f = 0; f < D / 32; f++)
-#pragma unroll
-                for (int k = 0; k < 16; k++) O[f][k] *= al;
-            if constexpr (F32)
-#pragma unroll
-                for (int g = 0; g < GPD; g++) C[g] *= al;
-        }
-        if (ev_b >= kSomeBad / 2) {
+        if (bad) {
             // rows that see a token with a non-finite V group
             uint32_t seen = 0;
 #pragma unroll
@@ -356,13 +349,8 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
             seen <<= 4 * h;
             poison |= (seen & mt[i].bad[0] ? 1u : 0u) | (seen & mt[i].bad[1] ? 2u : 0u);
         }
-        const float mr = F32 ? -M : (float)ev - M;
         float p[16];
-#pragma unroll
-        for (int k = 0; k < 16; k++) p[k] = __builtin_amdgcn_exp2f(fmaf(s[k], Q.rf, mr));
-        const float sum = (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]))) +
-                          (((p[8] + p[9]) + (p[10] + p[11])) + ((p[12] + p[13]) + (p[14] + p[15])));
-        L += F32 ? sum : scale2(sum, -ev);
+        R.weights(s, Q, (const float *)(t + I::W), h, p);
         if constexpr (F32) {
 #pragma unroll
             for (int g = 0; g < GPD; g++) {
@@ -385,7 +373,7 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
                         b[2 * k + e] = u_of(pk_rest(hi2, x[e], x[e + 2]));
                     }
                 }
-                C[g] += cs;
+                R.C[g] += cs;
 #pragma unroll
                 for (int ks = 0; ks < 2; ks++) {
                     P[2 * g][ks] = __builtin_bit_cast(
@@ -395,13 +383,7 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
                 }
             }
         } else {
-#pragma unroll
-            for (int ks = 0; ks < 2; ks++) {
-                const float *pp = p + 8 * ks;
-                P[0][ks] = __builtin_bit_cast(
-                    h8, uint4{u_of(pk_exp(pp[0], pp[2])), u_of(pk_exp(pp[1], pp[3])),
-                              u_of(pk_exp(pp[4], pp[6])), u_of(pk_exp(pp[5], pp[7]))});
-            }
+            Soft<D, F32>::operand(p, P[0]);
         }
     };
 
@@ -410,7 +392,8 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
     // read by none any more: their slots are filled again.
     auto sync = [&](int i) __attribute__((always_inline)) {
         __builtin_amdgcn_sched_barrier(0);
-        wait_loads<(kRing - 1 - 2 * kStep) * I::LOADS>();
+        if (w < I::MORE) wait_loads<(kRing - 1 - 2 * kStep) * (I::LOADS + 1)>();
+        else wait_loads<(kRing - 1 - 2 * kStep) * I::LOADS>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
 #pragma unroll
@@ -431,31 +414,9 @@ __global__ __launch_bounds__(64 * kPWaves, 2) void prompt_kernel(
         wait_loads<0>();
     }
 
-    const float l = L + __shfl_xor(L, 32, 64);
-    if constexpr (F32) {
-#pragma unroll
-        for (int g = 0; g < GPD; g++) {
-            const float cs = C[g] + __shfl_xor(C[g], 32, 64);
-#pragma unroll
-            for (int n = 0; n < 2; n++)
-#pragma unroll
-                for (int k = 0; k < 16; k++) O[2 * g + n][k] += cs;
-        }
-    } else {
-#pragma unroll
-        for (int f = 0; f < D / 32; f++)
-#pragma unroll
-            for (int k = 0; k < 16; k++) O[f][k] *= 0x1p-15f;          // V's operands carried 2^15
-    }
-    poison |= __shfl_xor(poison, 32, 64);
-    if (poison)
-#pragma unroll
-        for (int f = 0; f < D / 32; f++)
-            if (poison >> (f >> 1) & 1)
-#pragma unroll
-                for (int k = 0; k < 16; k++) O[f][k] = __builtin_nanf("");
+    const float l = R.finish(poison | __shfl_xor(poison, 32, 64));
     if (r0 + n32 < rows)
-        put_rows<D, F32>(row_out(job, c, chunk, tok, head, D, qrow, vec, part), O, l, M, h, out, part);
+        put_rows<D, F32>(row_out(job, c, chunk, tok, head, D, qrow, vec, part), R.O, l, R.M, h, out, part);
 }
 
 template <int D, bool F32>
@@ -465,7 +426,7 @@ int launch(const eakvd_geom &g, const WinJob &job, int64_t subtiles, const void 
     typedef Img<D, F32> I;
     Meta *meta = (Meta *)(img + subtiles * I::BYTES);
     hipLaunchKernelGGL((expand_kernel<D, F32>), dim3((unsigned)subtiles), dim3(64 * 4 * (D / 64)), 0, st,
-                       g, job, img, meta);
+                       g, job, img, meta, kKScale<F32> / sqrtf((float)D));
     constexpr int bytes = kRing * I::BYTES;
     static_assert(bytes <= 160 * 1024, "LDS");
     const unsigned blocks = (unsigned)job.pre[job.n_seq];
@@ -473,16 +434,16 @@ int launch(const eakvd_geom &g, const WinJob &job, int64_t subtiles, const void 
         const int e = allow_lds((const void *)kern, bytes, done);
         if (e) return e;
         hipLaunchKernelGGL(kern, dim3(blocks), dim3(64 * kPWaves), bytes, st, job, img, meta, q, out, part,
-                           1.0f / sqrtf((float)D), (int)vec);
+                           (int)vec);
         return (int)hipGetLastError();
     };
-    // d = 64 in bf16: without reading ahead two blocks fit a CU (116 registers against 149),
-    // which is worth more where there are two (4 x 1100 tokens at 5003 of 32Q/4KV 260 against
-    // 289 us, 4000 of 12Q/12KV 83 against 91; but 2000 at 30000, 252 blocks, 646 against 605)
+    // d = 64 in bf16: where no CU gets two blocks, one that reads ahead (2000 tokens at 30000 of
+    // 32Q/4KV, 252 blocks, 711 us against 758); at d = 128 that takes all registers (2048 at
+    // 30720 of 32Q/8KV 1231 against 1212)
     static std::atomic<uint64_t> done[2];
     if constexpr (D == 64 && !F32)
-        if (blocks > (unsigned)cu_count()) return run(prompt_kernel<D, F32, false>, done[0]);
-    return run(prompt_kernel<D, F32, !F32>, done[1]);
+        if (blocks <= (unsigned)cu_count()) return run(prompt_kernel<D, F32, true>, done[0]);
+    return run(prompt_kernel<D, F32, false>, done[1]);
 }
 
 }  // namespace

@@ -90,6 +90,70 @@ def test_keys_on_an_offset(E, rng, way, d, bf16):
 
 
 @pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("size", [1e3, 1e5, 1e8, 1e12, 1e18])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("way", WAYS)
+def test_magnitude_of_a_token_not_seen(E, rng, way, d, size, bf16):
+    """Later tokens of the window with K and V of `size`, in the same 32 tokens as those
+    that the earlier rows see: the same bits as with tokens of ordinary size."""
+    n_kv, n_q, wins = way
+    xs, q = data(rng, way, d)
+    plain = attend(E, way, d, xs, q, bf16)[0]
+    for x, (s, m) in zip(xs, wins):
+        x[:, 1, :, s + m - 4] *= size
+        x[:, :, :, s + m - 2] *= size
+    got, q, caches = attend(E, way, d, xs, q, bf16)
+    m = wins[0][1]
+    rows = np.arange(m) < m - 4
+    verify(way, got, q, caches, bf16, rows=rows)
+    every = np.tile(rows, len(wins))
+    assert np.array_equal(got[every].view(np.uint32), plain[every].view(np.uint32))
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("size", [1e5, 1e12])
+@pytest.mark.parametrize("d", [64, 128])
+def test_magnitude_of_another_branch(E, rng, d, size, bf16):
+    """A tree's node with K and V of `size`, seen by its own row alone."""
+    n_kv, n_q, wins = FEW
+    (s, m), = wins
+    words = [(1 << i + 1) - 1 & ~(1 << 5) for i in range(m)]
+    words[5] |= 1 << 5
+    xs, q = data(rng, FEW, d)
+    xs[0][:, :, :, s + 5] *= size
+    got, q, caches = attend(E, FEW, d, xs, q, bf16, words)
+    verify(FEW, got, q, caches, bf16, words, rows=np.arange(m) != 5)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("size", [1e5, 1e8, 1e12, 1e30])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("way", WAYS)
+def test_magnitude_of_a_token_without_weight(E, rng, way, d, size, bf16):
+    """A token with a score some 100 below the others' (weight e^-100) and V of `size`."""
+    xs, q = data(rng, way, d)
+    q += 1.0
+    for x in xs:
+        x[:, 0, :, 17] = -16.0 if d == 64 else -12.0
+        x[:, 1, :, 17] *= size
+    got, q, caches = attend(E, way, d, xs, q, bf16)
+    verify(way, got, q, caches, bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("size", [1e-3, 1e3])
+@pytest.mark.parametrize("way", WAYS)
+def test_magnitudes_that_vary(E, rng, way, size, bf16):
+    """V's size changes from token to token over 18 powers of ten around `size`; the
+    largest decide the outputs."""
+    xs, q = data(rng, way, 128)
+    for x in xs:
+        x[:, 1] *= (size * 10.0 ** rng.uniform(-9, 9, x.shape[3])).astype(np.float32)[:, None]
+    got, q, caches = attend(E, way, 128, xs, q, bf16)
+    verify(way, got, q, caches, bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("size", [0.0, 1e-30, 1e-3, 1.0])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("way", WAYS)
