@@ -82,8 +82,9 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WinJob job, const flo
     const float *po = part + first * D + sub * 4;
     for (int k0 = 0; k0 < most; k0 += W) {
         const float2 x = ml[min(k0 + sub, mc - 1) * per];
-        const float al = k0 + sub < mc && x.y != 0.0f ? __builtin_amdgcn_exp2f(x.x - m) : 0.0f;
-        l = fmaf(al, x.y, l);
+        // (-1: nothing there.  A factor that comes out 0 still takes its chunk's NaN along.)
+        const float al = k0 + sub < mc && x.y != 0.0f ? __builtin_amdgcn_exp2f(x.x - m) : -1.0f;
+        l = al < 0.0f ? l : fmaf(al, x.y, l);
         for (int k8 = k0; k8 < min(k0 + W, most); k8 += 8) {
             v4f v[8];
 #pragma unroll
@@ -92,7 +93,7 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WinJob job, const flo
             for (int k = 0; k < 8; k++) {
                 const float a = __shfl(al, lane - sub + k8 - k0 + k, 64);
 #pragma unroll
-                for (int e = 0; e < 4; e++) o4[e] = a != 0.0f ? fmaf(a, v[k][e], o4[e]) : o4[e];
+                for (int e = 0; e < 4; e++) o4[e] = a < 0.0f ? o4[e] : fmaf(a, v[k][e], o4[e]);
             }
         }
     }

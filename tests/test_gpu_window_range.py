@@ -197,3 +197,49 @@ def test_queries_near_the_end_of_the_range(E, rng, way, d):
     q *= np.float32(2.0 ** 120)
     got, q, caches = attend(E, way, d, xs, q, True)
     verify(way, got, q, caches, True)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("way", [(2, 8, [(9000, 6)]), (4, 64, [(1500, 512)])])
+def test_nonfinite_value_in_a_chunk_without_weight(E, rng, way, bf16):
+    """NaN in V of a token whose whole chunk lies hundreds of powers of two below the rows'
+    maximum: NaN in its 64 dims as anywhere else, and nowhere else."""
+    n_kv, n_q, ((s, m),) = way
+    d = 128
+    x = rng.standard_normal((1, 2, n_kv, s + m, d), dtype=np.float32)
+    x[:, 0, :, :s - 100] = -24.0
+    x[0, 1, 0, 33, 64] = np.nan                  # a group's first value: its scale and bias
+    c = E.Cache(1, n_kv, d, s + m)
+    c.load_raw(x, s + m)
+    call = W.Call(E, [c], [m], n_q, n_kv, bf16, [s])
+    call.put(rng.standard_normal((m, n_q, d), dtype=np.float32) * 0.5 + 1.0)
+    call.run()
+    nan = np.isnan(call.get())
+    want = np.zeros_like(nan)
+    want[:, :n_q // n_kv, 64:] = True
+    assert np.array_equal(nan, want)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("way", [(2, 8, [(9000, 6)]), (4, 64, [(1500, 512)])])
+def test_nonfinite_queries_over_chunks(E, rng, way, bf16):
+    """NaN and infinite queries: NaN in their own rows alone, whatever the chunks."""
+    n_kv, n_q, ((s, m),) = way
+    c = W.build(E, rng, [s + m], n_kv, 128, s + m)[0]
+    call = W.Call(E, [c], [m], n_q, n_kv, bf16, [s])
+    q = rng.standard_normal((m, n_q, 128), dtype=np.float32)
+    want = np.zeros(q.shape, bool)
+    for i, (row, head, x) in enumerate(((0, 1, np.nan), (3, 0, np.inf), (5, n_q - 1, -np.inf))):
+        q[row, head, 17 * i] = x
+        want[row, head] = True
+    if bf16:
+        bits = W.to_bf16(np.where(np.isnan(q), np.float32(1), q))
+        call.put(q)
+        bits[np.isnan(q)] = 0x7fc0
+        host = np.full(call.dq.nbytes, call.GUARD, np.uint8)
+        host[call.at:call.at + bits.nbytes] = bits.reshape(-1).view(np.uint8)
+        call.dq.upload(host)
+    else:
+        call.put(q)
+    call.run()
+    assert np.array_equal(np.isnan(call.get()), want)
