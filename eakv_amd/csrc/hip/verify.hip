@@ -45,6 +45,12 @@ __device__ __forceinline__ int count_of(const VerJob &J, int s)
     return n < 0 ? 0 : n > J.k ? J.k : n;
 }
 
+// Negative values and NaN as 0, in one instruction (the median takes NaN for the least).
+__device__ __forceinline__ float some(float x)
+{
+    return __builtin_amdgcn_fmed3f(x, 0.0f, __builtin_inff());
+}
+
 // The drafts of sequence s that are kept (every lane of a wave gets it).
 __device__ __forceinline__ int kept_of(const VerJob &J, int s, int n, int lane)
 {
@@ -56,7 +62,7 @@ __device__ __forceinline__ int kept_of(const VerJob &J, int s, int n, int lane)
             const int x = J.token[at];
             if (x >= 0 && x < J.vocab) {
                 const float p = J.target[((int64_t)s * (J.k + 1) + i) * J.ld_target + x];
-                const float q = J.draft ? J.draft[at * J.ld_draft + x] : 1.0f;
+                const float q = J.draft ? some(J.draft[at * J.ld_draft + x]) : 1.0f;
                 ok = (double)J.uniform[(int64_t)s * (J.k + 1) + i] * (double)q < (double)p;
             }
         }
@@ -70,9 +76,10 @@ __device__ __forceinline__ int kept_of(const VerJob &J, int s, int n, int lane)
 struct Row {
     const float *p, *q;         // q NULL: no draft row
     int less;                   // a token whose weight is 0 (one-hot draft), or -1
-    __device__ __forceinline__ double at(double p_, double q_, int j) const
+    // (negative values and NaN are 0 in both)
+    __device__ __forceinline__ double at(float p_, float q_, int j) const
     {
-        const double r = q ? p_ - q_ : p_;
+        const double r = q ? (double)p_ - (double)some(q_) : (double)p_;
         return j != less && r > 0.0 ? r : 0.0;
     }
 };
@@ -106,7 +113,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_sum_kernel(VerJob J)
     const int lo = b * J.seg, hi = min(J.vocab, lo + J.seg);
     double sr = 0.0, sp = 0.0;
     auto add = [&](float p, float q, int j) {
-        sr += R.at((double)p, (double)q, j);
+        sr += R.at(p, q, j);
         sp += p > 0.0f ? (double)p : 0.0;
     };
     int j = lo + 4 * lane;
@@ -215,7 +222,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerJob J)
         double r[4], sum = 0.0;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            r[e] = j + e < hi ? R.at((double)R.p[j + e], R.q ? (double)R.q[j + e] : 0.0, j + e) : 0.0;
+            r[e] = j + e < hi ? R.at(R.p[j + e], R.q ? R.q[j + e] : 0.0f, j + e) : 0.0;
             sum += r[e];
         }
         double all;
@@ -263,7 +270,7 @@ __global__ __launch_bounds__(1024) void verify_one_kernel(VerJob J)
         const v4f4 p = four(R.p, j), q = R.q ? four(R.q, j) : none;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            sr += R.at((double)p[e], (double)q[e], j + e);
+            sr += R.at(p[e], q[e], j + e);
             sp += p[e] > 0.0f ? (double)p[e] : 0.0;
         }
     }
@@ -314,7 +321,7 @@ __global__ __launch_bounds__(1024) void verify_one_kernel(VerJob J)
         double r[4], sum = 0.0;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            r[e] = R.at((double)p[e], (double)q[e], j + e);
+            r[e] = R.at(p[e], q[e], j + e);
             sum += r[e];
         }
         double v = sum;
