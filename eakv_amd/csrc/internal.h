@@ -50,6 +50,17 @@ int  eakvi_hip_fail(int hip_err, const char *what);
 int  eakvi_attn_check(const eakv_cache_t *c, int layer, int n_q, int n_kv);
 int  eakvi_same_batch(eakv_cache_t *const *caches, int n, const char *what);
 
+/* Bytes of a caller's buffer (NULL or none: overlaps nothing). */
+typedef struct {
+    const void *p;
+    size_t n;
+} eakvi_span;
+static inline int eakvi_overlap(eakvi_span a, eakvi_span b)
+{
+    const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+    return x && y && a.n && b.n && (x < y ? y - x < a.n : x - y < b.n);
+}
+
 /* Make the cache's device current; returns the previous device via *prev. */
 int  eakvi_enter(const eakv_cache_t *c, int *prev);
 void eakvi_leave(int prev);

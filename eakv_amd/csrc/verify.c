@@ -11,6 +11,11 @@ static int sizes_ok(int n_seqs, int n_drafts, int vocab)
            vocab >= 1 && vocab <= (1 << 30);
 }
 
+static size_t matrix(int64_t rows, int64_t ld, int cols)
+{
+    return rows > 0 ? ((size_t)(rows - 1) * (size_t)ld + (size_t)cols) * 4 : 0;
+}
+
 size_t eakv_verify_drafts_work_bytes(int n_seqs, int n_drafts, int vocab)
 {
     if (!sizes_ok(n_seqs, n_drafts, vocab)) {
@@ -40,6 +45,19 @@ int eakv_verify_drafts_device(int n_seqs, int n_drafts, int vocab, const int32_t
     if (work_bytes < need)
         return eakvi_set_error(EAKV_ERR_INVALID, "verify: %zu bytes of workspace, %zu needed",
                               work_bytes, need);
+    /* blocks write their results while others read */
+    const int64_t n = n_seqs, k = n_drafts;
+    const eakvi_span out[3] = {{d_accepted, (size_t)n * 4}, {d_next, (size_t)n * 4}, {d_work, need}};
+    const eakvi_span in[5] = {{d_counts, (size_t)n * 4},
+                        {d_tokens, (size_t)(n * k) * 4},
+                        {d_uniform, (size_t)(n * (k + 1)) * 4},
+                        {d_draft, matrix(n * k, ld_draft, vocab)},
+                        {d_target, matrix(n * (k + 1), ld_target, vocab)}};
+    for (int i = 0; i < 3; i++) {
+        int bad = eakvi_overlap(out[i], out[(i + 1) % 3]);
+        for (int j = 0; j < 5; j++) bad |= eakvi_overlap(out[i], in[j]);
+        if (bad) return eakvi_set_error(EAKV_ERR_INVALID, "verify: overlapping buffers");
+    }
     int e = eakvd_verify(n_seqs, n_drafts, vocab, d_counts, d_tokens, d_draft, ld_draft, d_target,
                          ld_target, d_uniform, d_accepted, d_next, d_work, stream);
     return e ? eakvi_hip_fail(e, "verify launch") : EAKV_OK;

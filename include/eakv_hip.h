@@ -209,6 +209,7 @@ size_t eakv_attention_window_work_bytes(eakv_cache_t *const *caches, int n_cache
  * holds nothing either; NaN and negative values count as 0 (infinite ones make d_next
  * some token of positive weight).  Products, differences and sums in f64.  d_work:
  * eakv_verify_drafts_work_bytes() of device scratch, 8-byte aligned, the call's own.
+ * The results and d_work overlap nothing else (refused).
  * Asynchronous; may be recorded in a graph. */
 int eakv_verify_drafts_device(int n_seqs, int n_drafts, int vocab, const int32_t *d_counts,
                               const int32_t *d_tokens, const float *d_draft, int64_t ld_draft,

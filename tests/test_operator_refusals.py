@@ -62,3 +62,30 @@ def test_move_arguments():
     assert E.last_error()[0] == E.EAKV_ERR_INVALID
     assert _code(L.eakv_cache_compact(None, 0, one, 1)) == E.EAKV_ERR_INVALID
     assert _code(L.eakv_cache_planes_device(None, 0, 0, None, None, None)) == E.EAKV_ERR_INVALID
+
+
+def test_verify_overlaps():
+    """Results on top of inputs, of one another or of the scratch (addresses alone: nothing
+    is launched)."""
+    L = E.lib()
+    n, k, v = 4, 3, 100
+    size = L.eakv_verify_drafts_work_bytes(n, k, v)
+    at, end = {}, 4096
+    for name, words in (("counts", n), ("tokens", n * k), ("draft", n * k * v), ("target", n * (k + 1) * v),
+                        ("u", n * (k + 1)), ("kept", n), ("next", n), ("work", size // 4)):
+        at[name], end = (end, 4 * words), end + (4 * words + 7) // 8 * 8
+
+    def call(**kw):
+        a = {x: kw.get(x, y[0]) for x, y in at.items()}
+        return L.eakv_verify_drafts_device(n, k, v, a["counts"], a["tokens"], a["draft"], v, a["target"], v,
+                                           a["u"], a["kept"], a["next"], a["work"], size, None)
+
+    for out in ("kept", "next", "work"):
+        for other, (p, m) in at.items():
+            if other == out:
+                continue
+            for q in (p, p + m - 4, p - at[out][1] + 4):
+                q = (q + 7) // 8 * 8 if out == "work" else q
+                if q + at[out][1] <= p or q >= p + m:
+                    continue
+                assert _code(call(**{out: q})) == E.EAKV_ERR_INVALID, (out, other, q - p)
