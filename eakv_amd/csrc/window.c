@@ -106,9 +106,15 @@ int eakv_attention_window_batch_device(eakv_cache_t *const *caches, int n_caches
                                                          dtype == EAKV_BF16);
     const int own = !d_work;
     int capturing = 0;
+    const size_t rows = (size_t)total * n_q * c0->head_dim * (dtype == EAKV_F32 ? 4 : 2);
+    const eakvi_span q = {d_q, rows}, out = {d_out, rows}, work_span = {d_work, need},
+                     words = {d_tree, (size_t)total * 8};
     if (d_work && work_bytes < need) {
         rc = eakvi_set_error(EAKV_ERR_INVALID, "window: %zu bytes of workspace, %zu needed",
                              work_bytes, need);
+    } else if (eakvi_overlap(out, words) || eakvi_overlap(work_span, q) ||
+               eakvi_overlap(work_span, out) || eakvi_overlap(work_span, words)) {
+        rc = eakvi_set_error(EAKV_ERR_INVALID, "window: overlapping buffers");
     } else {
         int e = eakvd_stream_capturing(stream ? stream : c0->stream, &capturing);
         if (e) rc = eakvi_hip_fail(e, "window");

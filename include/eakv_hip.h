@@ -156,7 +156,9 @@ int eakv_attention_fused_plan(eakv_cache_t *const *caches, int n_caches, int n_q
  *              are in the cache (appended, advanced or not).  starts[c] <= seq_len.
  *   n_tokens   host int32[n_caches]: queries of each cache, 0 or more
  *   d_q, d_out [sum of n_tokens][n_q_heads][head_dim] on the device, the caches'
- *              windows one after the other, of type dtype: EAKV_F32 or EAKV_BF16
+ *              windows one after the other, of type dtype: EAKV_F32 or EAKV_BF16; one
+ *              buffer, or two that do not overlap (a row is written when its own
+ *              query has been read, others may not have been)
  *   d_tree     NULL: query i sees the tokens up to its own.  Else one word for
  *              each query (device, 8-byte aligned, windows of at most
  *              EAKV_TREE_MAX tokens): bit j says that it sees token starts[c] + j
@@ -169,7 +171,8 @@ int eakv_attention_fused_plan(eakv_cache_t *const *caches, int n_caches, int n_q
  * weights are rounded to f16 (2^-12 relative), sums in f32, the result to bf16.  Scores
  * (q.k/sqrt(d)) are taken to be below 2^22 in size.
  * A non-finite scale or bias gives NaN in the scores of its token or in its 64 dims.
- *   d_work     device scratch of the call's own, 16-byte aligned and of at least
+ *   d_work     device scratch of the call's own, 16-byte aligned, over none of the
+ *              buffers (refused) and of at least
  *              eakv_attention_window_work_bytes() for the same arguments, or NULL:
  *              caches[0]'s workspace (grown when needed).  Calls that share one and
  *              overlap in time race.  A call on a stream that records a graph needs
