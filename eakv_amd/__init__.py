@@ -303,7 +303,7 @@ class Cache:
 
     def compact(self, keep, start=0):
         """Keep the tokens before start and, of the others, those at `keep`."""
-        k = np.ascontiguousarray(keep, dtype=np.int32)
+        k = np.frombuffer(ints(keep), np.int32) if len(keep) else np.zeros(0, np.int32)
         return _check(lib().eakv_cache_compact(self.h, start, _ptr(k), k.size))
 
     def sync(self):
@@ -330,6 +330,9 @@ def handles(caches):
 
 def ints(values):
     """ctypes int32 array for the batched entry points."""
+    values = [int(v) for v in values]
+    if any(not -2 ** 31 <= v < 2 ** 31 for v in values):
+        raise ValueError("a value beyond 32 bits")
     return (C.c_int32 * len(values))(*values)
 
 
@@ -340,6 +343,10 @@ class WindowPlan:
 
     def __init__(self, caches, n_tokens, n_q, n_kv, starts=None, dtype="f32"):
         self.caches = list(caches)
+        # the library reads one entry of each list per cache
+        for name, x in (("n_tokens", n_tokens), ("starts", starts)):
+            if x is not None and len(x) != len(self.caches):
+                raise ValueError(f"{name}: {len(x)} entries for {len(self.caches)} caches")
         self._h, self._n = handles(self.caches), ints(n_tokens)
         self._starts = None if starts is None else ints(starts)
         self._args = ({"f32": EAKV_F32, "bf16": EAKV_BF16}[dtype], n_q, n_kv)
