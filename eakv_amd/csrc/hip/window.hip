@@ -119,6 +119,8 @@ struct WinPlan {
     WinPart few, many;
 };
 
+constexpr size_t kManyMost = (size_t)4 << 30;
+
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // Tiles of a chunk, win_draft: an even share of the chip (4 tokens at 2048 of 32Q/8KV,
@@ -244,7 +246,9 @@ void plan_part(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv, bo
 }
 
 // Whether windows' K and V are expanded first: causal ones that no tree is allowed for,
-// of more than 512 rows per kv head, if both estimates say so.  Rates of the estimates
+// of more than 512 rows per kv head, if both estimates say so and the operands, 3.5 times
+// the packed planes at d = 128, stay below kManyMost (2.3 GB for 131072 tokens of 32 kv
+// heads).  Rates of the estimates
 // and what they choose between, in us, expanded / not: 8 of 264 rows at 10000 of
 // 32Q/8KV bf16 295 / 230, f32 436 / 320 (never asked); 768 rows at 30000 149 / 208,
 // 273 / 308; 2000 tokens at 2000 of 32Q/32KV 84 / 133, 161 / 167, of 8Q/8KV 46 / 35, 65 / 47;
@@ -262,7 +266,7 @@ void win_plan(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv, boo
     if (any) {
         plan_part(g, b, n_q, n_kv, bf16, false, many, &p->few);
         plan_part(g, b, n_q, n_kv, bf16, true, many, &p->many);
-        if (p->few.us < p->many.us) {
+        if (p->few.us < p->many.us || p->many.bytes > kManyMost) {
             memset(&p->many, 0, sizeof(p->many));
             for (int i = 0; i < b->n_seq; i++) few[i] = true;
         }

@@ -174,7 +174,10 @@ int eakv_attention_fused_plan(eakv_cache_t *const *caches, int n_caches, int n_q
  *   d_work     device scratch of the call's own, 16-byte aligned, over none of the
  *              buffers (refused) and of at least
  *              eakv_attention_window_work_bytes() for the same arguments, or NULL:
- *              caches[0]'s workspace (grown when needed).  Calls that share one and
+ *              caches[0]'s workspace (grown when needed, by a quarter more).  Windows of
+ *              more than 512 tokens x q heads per kv head may need operands of K and V
+ *              there, up to 18 KB (head_dim 64: 10) for each 32 tokens and kv head, but
+ *              no more than 4 GiB in all, beside partial results.  Calls that share one and
  *              overlap in time race.  A call on a stream that records a graph needs
  *              its own (unless 0 bytes are needed), allocates nothing and waits for
  *              nothing outside the graph: starts and n_tokens are recorded as they

@@ -44,3 +44,21 @@ def test_overlapping_buffers(E, rng, bf16):
     got = same.download()
     got = W.from_bf16(got) if bf16 else got
     assert np.array_equal(got.reshape(want.shape).view(np.uint32), want.view(np.uint32))
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("d,n_kv,ctx,seqs", [(128, 8, 1_000_000, 1), (64, 16, 120_000, 32)])
+def test_workspace_is_bounded(E, d, n_kv, ctx, seqs, bf16):
+    """Operands of every token would take more than 4 GiB: the call goes without them."""
+    caches = [E.Cache(1, n_kv, d, ctx) for _ in range(seqs)]
+    for c in caches:
+        c.advance(ctx)
+    for m in (130, 2000):
+        p = E.WindowPlan(caches, [m] * seqs, n_kv * 8, n_kv, starts=[ctx - m] * seqs,
+                         dtype="bf16" if bf16 else "f32")
+        assert p.work_bytes <= (4 << 30) + seqs * m * n_kv * 8 * (d + 2) * 4 * 64
+    short = E.WindowPlan(caches, [2000] * seqs, n_kv * 8, n_kv, starts=[0] * seqs,
+                         dtype="bf16" if bf16 else "f32")
+    assert short.work_bytes >= seqs * 2000 // 32 * n_kv * d * 128       # expanded
+    for c in caches:
+        c.free()
