@@ -299,7 +299,7 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
             h8 P[F32 ? 2 : 1][2];
             if constexpr (F32) {
                 uint32_t a[8], b[8];
-                float cs = 0.0f;
+                float cs = 0.0f, ls = 0.0f;
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const v4f sc = *(const v4f *)&S.vs[g][8 * k + 4 * h];
@@ -310,6 +310,11 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
                         x[e] = p[4 * k + e] * sc[e];
                         cs = fmaf(p[4 * k + e], cc[e], cs);
                     }
+                    if (g == GPD - 1) {
+                        const v4f w4 = *(const v4f *)&S.w[8 * k + 4 * h];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) ls = fmaf(p[4 * k + e], w4[e], ls);
+                    }
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const h2 hi2 = pk(x[e], x[e + 2]);
@@ -318,6 +323,7 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
                     }
                 }
                 R.C[g] += cs;
+                R.L += ls;
 #pragma unroll
                 for (int ks = 0; ks < 2; ks++) {
                     P[0][ks] = __builtin_bit_cast(h8, uint4{a[4 * ks], a[4 * ks + 1], a[4 * ks + 2],

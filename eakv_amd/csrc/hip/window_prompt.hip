@@ -355,7 +355,7 @@ __global__ __launch_bounds__(64 * kPWaves, D == 64 && !F32 && !PF ? 4 : 2) void 
 #pragma unroll
             for (int g = 0; g < GPD; g++) {
                 uint32_t a[8], b[8];
-                float cs = 0.0f;
+                float cs = 0.0f, ls = 0.0f;
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const v4f sc = *(const v4f *)((const float *)(t + I::VS) + 32 * g + 8 * k + 4 * h);
@@ -366,6 +366,11 @@ __global__ __launch_bounds__(64 * kPWaves, D == 64 && !F32 && !PF ? 4 : 2) void 
                         x[e] = p[4 * k + e] * sc[e];
                         cs = fmaf(p[4 * k + e], cc[e], cs);
                     }
+                    if (g == GPD - 1) {
+                        const v4f w4 = *(const v4f *)((const float *)(t + I::W) + 8 * k + 4 * h);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) ls = fmaf(p[4 * k + e], w4[e], ls);
+                    }
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const h2 hi2 = pk(x[e], x[e + 2]);
@@ -374,6 +379,7 @@ __global__ __launch_bounds__(64 * kPWaves, D == 64 && !F32 && !PF ? 4 : 2) void 
                     }
                 }
                 R.C[g] += cs;
+                R.L += ls;
 #pragma unroll
                 for (int ks = 0; ks < 2; ks++) {
                     P[2 * g][ks] = __builtin_bit_cast(
