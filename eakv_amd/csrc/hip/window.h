@@ -334,6 +334,13 @@ struct Soft {
     // no row's result depends on another's tokens.
     __device__ __forceinline__ void weights(v16f &s, QOp<D, F32> &Q, const float *w, int h, float *p)
     {
+        // (read here, their latency passes behind the maximum)
+        v4f w4[4];
+        if constexpr (!F32) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) w4[k] = *(const v4f *)(w + 8 * k + 4 * h);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         float top = fmaxf(fmaxf(s[0], s[1]), s[2]);
 #pragma unroll
         for (int k = 3; k < 16; k++) top = fmaxf(top, s[k]);
@@ -366,11 +373,10 @@ struct Soft {
         if constexpr (!F32) {
             float sum[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const v4f w4 = *(const v4f *)(w + 8 * k + 4 * h);
+            for (int k = 0; k < 4; k++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) sum[e] = k ? fmaf(p[4 * k + e], w4[e], sum[e]) : p[e] * w4[e];
-            }
+                for (int e = 0; e < 4; e++)
+                    sum[e] = k ? fmaf(p[4 * k + e], w4[k][e], sum[e]) : p[e] * w4[0][e];
             L += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
     }
