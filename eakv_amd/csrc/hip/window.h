@@ -1,4 +1,4 @@
-// window.h — what the window attention's kernels share (window.hip,
+// window.h — what the window attention's kernels share (window.hip, window_draft.hip,
 // window_prompt.hip; the mathematics stands in window.hip).
 #pragma once
 

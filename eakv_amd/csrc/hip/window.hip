@@ -248,12 +248,12 @@ void plan_part(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv, bo
 // Whether windows' K and V are expanded first: causal ones that no tree is allowed for,
 // of more than 512 rows per kv head, if both estimates say so and the operands, 3.5 times
 // the packed planes at d = 128, stay below kManyMost (2.3 GB for 131072 tokens of 32 kv
-// heads).  Rates of the estimates
-// and what they choose between, in us, expanded / not: 8 of 264 rows at 10000 of
-// 32Q/8KV bf16 295 / 230, f32 436 / 320 (never asked); 768 rows at 30000 149 / 208,
-// 273 / 308; 2000 tokens at 2000 of 32Q/32KV 84 / 133, 161 / 167, of 8Q/8KV 46 / 35, 65 / 47;
-// 3000 at 3000 of 40Q/8KV 122 / 258, 231 / 351; 4000 at 4000 of 12Q/12KV, d = 64, 90 / 89,
-// 140 / 116; 8 of 600 at 600 of 32Q/8KV 67 / 181, 114 / 223.
+// heads).  What the estimates choose between, in us, expanded / not: 2000 tokens at 2000 of
+// 32Q/32KV bf16 92 / 121, f32 156 / 164, of 8Q/8KV 49 / 36, 64 / 50; 3000 at 3000 of 40Q/8KV
+// 138 / 259, 238 / 365; 4000 at 4000 of 12Q/12KV, d = 64, 80 / 89, 134 / 116; 8 of 600 at
+// 600 of 32Q/8KV 76 / 187, 117 / 235; 512 at 8192 109 / 120, 177 / 188; 4 of 150 at 20000
+// 480 / 395, 690 / 627.  They are wrong by up to 40 % for some 800 rows at very long
+// contexts (70 tokens at 131072 of 64Q/8KV, not expanded: 729 / 817, 1084 / 1308).
 void win_plan(const eakvd_geom *g, const eakvd_window *b, int n_q, int n_kv, bool bf16, WinPlan *p)
 {
     bool few[EAKVD_MAX_BATCH], many[EAKVD_MAX_BATCH], any = false;

@@ -12,9 +12,10 @@
 //     operand order;
 // so no operand passes through LDS as f16, and no wave waits for another.
 //
-// Bound by vector instructions: per 32 tokens x 32 rows at d = 128 a wave issues about 380
-// (f32 530) beside 17 (33) matrix products and 5 KB of loads.  8 sequences of 8 tokens
-// at 32768 of 32Q/8KV (32 rows, 336 MB): bf16 76 us in the kernel, 4.4 TB/s; f32 116.
+// Bound by vector instructions: per 32 tokens x 32 rows at d = 128 a wave issues about 390
+// (f32 540) beside 17 (33) matrix products and 5 KB of loads.  8 sequences of 8 tokens
+// at 32768 of 32Q/8KV (32 rows, 336 MB): bf16 75 us in the kernel, 4.5 TB/s; f32 107-125.
+// Fewer rows cost the same: one bf16 token each 74.
 // Rows beyond 32 read the planes again, out of the caches: a block of 64 rows with
 // shared operands in LDS was slower at most sizes up to 512 rows (64 rows of 8 at 20000 of
 // 64Q/8KV bf16 158 against 164 us, but 192 rows of 6: 350 against 274; 64 of 4 at 4000,

@@ -8,9 +8,9 @@
 // vector instructions are the softmax's alone.
 //
 // K: n - z, exact, with the scales and biases beside them, as in window.hip.  (Values in
-// f16 instead save the scales' 32 instructions per 32 x 32 and a product, 1030 us against
-// 1206 for the prompt below; but their 2^-12 enters the scores times the scores' size:
-// K on an offset of 100 made outputs 2e-2 off.)  V, f32 queries: likewise; bf16 queries:
+// f16 instead save the scales' 32 instructions per 32 x 32 and a product, 1020-1080 us
+// against 1190-1250 for the prompt below; but their 2^-12 enters the scores times the
+// scores' size: K on an offset of 100 made outputs 2e-2 off.)  V, f32 queries: likewise; bf16 queries:
 // values n*s + b (f32) scaled by the token's power of two and rounded to f16, 2^-12
 // relative.
 //
@@ -19,10 +19,10 @@
 // sub-tile's scores and this one's weighted sum), then the softmax; a SIMD's two
 // waves are in different halves of it.
 //
-// Bound by the matrix cores and the vector ALUs together: 2048 tokens at 30720 of
-// 32Q/8KV, bf16 (1.07 Tflop): 1206 us, 884 Tflop/s, no more than one of the two busy at
-// most times.  f32, twice the products and 320 vector instructions for 32 x 32: 2.2 us
-// per 32 tokens of a block against 1.2.
+// Bound by the matrix cores and the vector ALUs in turn: 2048 tokens at 30720 of
+// 32Q/8KV, bf16 (1.07 Tflop): 1190-1250 us, 850-890 Tflop/s, with the matrix cores busy 45
+// and the vector ALUs 46 of 100 cycles at about 2.0 GHz.  f32, twice the products and 320
+// vector instructions for 32 x 32: 2.2 us per 32 tokens of a block against 1.2.
 #include <string.h>
 
 #include "window.h"
