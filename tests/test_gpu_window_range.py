@@ -34,7 +34,7 @@ def attend(E, way, d, xs, q, bf16, words=None):
         c.load_raw(x, x.shape[3])
         caches.append(c)
     call = W.Call(E, caches, [m for _, m in wins], n_q, n_kv, bf16, [s for s, _ in wins], words)
-    assert way is FEW or expanded(call, wins, n_kv)
+    assert way is not MANY or expanded(call, wins, n_kv)
     q = call.put(q)
     call.run()
     return call.get(), q, caches
@@ -243,3 +243,22 @@ def test_nonfinite_queries_over_chunks(E, rng, way, bf16):
         call.put(q)
     call.run()
     assert np.array_equal(np.isnan(call.get()), want)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("way", [(2, 8, [(33, 65)]), (2, 2, [(0, 300)]), (1, 16, [(100, 140)]),
+                                 (8, 128, [(16, 80), (0, 97), (200, 65)])])
+def test_k_is_exact_for_bf16_windows_of_many_rows(E, rng, way, d):
+    """The bound without a rounding of K, for windows of more than 256 rows per kv head, by
+    whichever way they go, with outlier channels in K."""
+    n_kv, n_q, wins = way
+    xs, q = data(rng, way, d)
+    for x in xs:
+        x[:, 0, ..., [3, d - 9]] *= 10.0
+    caches = [E.Cache(1, n_kv, d, max(s + m for s, m in wins)) for _ in wins]
+    for c, x in zip(caches, xs):
+        c.load_raw(x, x.shape[3])
+    call = W.Call(E, caches, [m for _, m in wins], n_q, n_kv, True, [s for s, _ in wins])
+    q = call.put(q)
+    call.run()
+    verify(way, call.get(), q, caches, True)
