@@ -109,6 +109,13 @@ __device__ __forceinline__ int exp_of(float a)
     const int e = (int)(__float_as_uint(a) >> 23) - 126;     // a < 2^e
     return e < kExpLow ? kExpLow : e;
 }
+// What a token's exponent is taken of, a group's scale and largest value given: f32, the
+// scale, or 2^-24 of the value where that is more (weights times biases stay in range).
+template <bool F32>
+__device__ __forceinline__ float v_size(float s, float top)
+{
+    return F32 ? fmaxf(fabsf(s), top * 0x1p-24f) : top;
+}
 // x * 2^e, one rounding, for any e
 __device__ __forceinline__ float scale2(float x, int e)
 {

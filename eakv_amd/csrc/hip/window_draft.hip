@@ -185,7 +185,7 @@ __global__ __launch_bounds__(64 * kDWaves, 2) void draft_kernel(eakvd_geom geo, 
         const float vs = live && fin ? st.vs : 0.0f, vb = live && fin ? st.vb : 0.0f;
         const float zv = zero_nibble(vs, vb), cv = fmaf(zv, vs, vb);
         // the token's exponent, of both groups
-        const float x = F32 ? fabsf(vs) : live && fin ? va : 0.0f;
+        const float x = live && fin ? v_size<F32>(vs, va) : 0.0f;
         const int ev = exp_of(GPD == 2 ? half_max(x) : x);
         // ---- scales to LDS
         S.w[n32] = scale2(1.0f, -ev);

@@ -94,7 +94,7 @@ __global__ __launch_bounds__(64 * 4 * (D / 64)) void expand_kernel(eakvd_geom ge
     const float vs = is_v ? s : Pv.s[gi], vb = is_v ? b : Pv.b[gi];
     const float a = fmaxf(fabsf(vb), fabsf(fmaf(15.0f, vs, vb)));
     const bool fin = a < __builtin_inff() && vs == vs;
-    const float top = !fin ? 0.0f : F32 ? fabsf(vs) : a;
+    const float top = fin ? v_size<F32>(vs, a) : 0.0f;
     const int e = exp_of(GPD == 2 ? half_max(top) : top);
     if (!is_v) {
         const uint2 by = *(const uint2 *)(P.w + (g0 + tn * GPD + g) * 32 + 16 * h + 8 * x);

@@ -166,7 +166,8 @@ int eakv_attention_fused_plan(eakv_cache_t *const *caches, int n_caches, int n_q
  *              the tokens before starts[c].
  * A query that sees no token gives zeros.  What a query does not see has no part in
  * its result, whatever its size, NaN and infinities included.  f32 queries: all sums in
- * f32, results 0.5e-6 to 2e-6 off the exact ones (norms); one token per sequence without
+ * f32, results 0.5e-6 to 2e-6 off the exact ones (norms; up to 1e-5 where V is near the
+ * ends of f32's range); one token per sequence without
  * a tree takes the launch of eakv_attention_fused_batch_device.  bf16 queries: V and the
  * weights are rounded to f16 (2^-12 relative), sums in f32, the result to bf16.  Scores
  * (q.k/sqrt(d)) are taken to be below 2^22 in size.

@@ -262,3 +262,33 @@ def test_k_is_exact_for_bf16_windows_of_many_rows(E, rng, way, d):
     q = call.put(q)
     call.run()
     verify(way, call.get(), q, caches, True)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("size", [1e19, 1e35])
+@pytest.mark.parametrize("way", WAYS)
+def test_constant_groups_of_any_size(E, rng, way, size, bf16):
+    """Groups of 64 equal values have scale 1 beside a bias of their size.  A token of such
+    groups near the end of f32's range leaves the rows that do not see it alone, and the rows
+    that do get their weight of it.
+
+    The token's exponent e (f32: of 2^-24 of its values) is added to its scores, so that the
+    3 roundings behind that are of sums of |e| + |score|, half a step each: up to 3 e 2^-24
+    in log2 units, ln 2 of which is the weight's error, and the normalisation's at most as
+    much again: 6 ln 2 e 2^-24 beside the norm's usual bound, 2.4e-5 at 1e35."""
+    n_kv, n_q, wins = way
+    xs, q = data(rng, way, 128)
+    for x, (s, m) in zip(xs, wins):
+        x[:, 1, :, s + m - 3] = size
+    got, q, caches = attend(E, way, 128, xs, q, bf16)
+    m = wins[0][1]
+    verify(way, got, q, caches, bf16, rows=np.arange(m) < m - 3)
+    bound = 2 * W.O16 / 3 if bf16 else 4e-6
+    bound += 6 * np.log(2) * (np.log2(abs(size)) + 1 - (0 if bf16 else 24)) * W.E32
+    at = 0
+    for c, (s, m) in zip(caches, wins):
+        for k, h in sample(n_kv, n_q):
+            want = exact(c, q[at:at + m, h], s, k)[0][m - 3:, 0]
+            rel = np.linalg.norm(got[at + m - 3:at + m, h] - want) / np.linalg.norm(want)
+            assert rel <= bound, rel
+        at += m
