@@ -322,9 +322,12 @@ struct Soft {
 #pragma unroll
         for (int g = 0; g < D / 64; g++) C[g] = 0.0f;
     }
-    __device__ __forceinline__ void rescale(float al)
+    // M rises by -d.  L by halves of it: where V's sizes differ by some 2^126 the rest of O is
+    // nothing beside what is to come, but the rest of L may be most of it.
+    __device__ __forceinline__ void rescale(float d)
     {
-        L *= al;
+        const float al = __builtin_amdgcn_exp2f(d), half = __builtin_amdgcn_exp2f(0.5f * d);
+        L = L * half * half;
 #pragma unroll
         for (int f = 0; f < D / 32; f++)
 #pragma unroll
@@ -356,7 +359,7 @@ struct Soft {
             const float need = fmaf(top, Q.rf, -kWinTop);
             if (__ballot(need > M + kWinTau) != 0) {
                 const float mn = need > M + kWinTau ? need : M;
-                rescale(__builtin_amdgcn_exp2f(M - mn));
+                rescale(M - mn);
                 M = mn;
             }
 #pragma unroll
@@ -368,7 +371,7 @@ struct Soft {
                 const float old = first ? 0.0f : M;
                 const float mn = hold_ref(Q, move ? old + (top - kWinTop) : old, h);
                 const float by = mn - old;
-                rescale(first ? 0.0f : __builtin_amdgcn_exp2f(-by));
+                rescale(first ? -__builtin_inff() : -by);
 #pragma unroll
                 for (int k = 0; k < 16; k++) s[k] -= by;
                 M = move ? mn : M;
@@ -516,8 +519,10 @@ __device__ __forceinline__ void join_put(float *lds, int wt, int lane,
     }
 #pragma unroll
     for (int t = 0; t < WT; t++) {
+        // (l by halves, as Soft::rescale)
+        const float half = __builtin_amdgcn_exp2f(0.5f * (a[t] - mm));
         a[t] = __builtin_amdgcn_exp2f(a[t] - mm);
-        ll = fmaf(a[t], ml[t * 128 + 64 + lane], ll);
+        ll = fmaf(half * ml[t * 128 + 64 + lane], half, ll);
     }
 #pragma unroll
     for (int k = 0; k < N / 4; k++) {

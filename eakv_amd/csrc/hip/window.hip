@@ -84,7 +84,8 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WinJob job, const flo
         const float2 x = ml[min(k0 + sub, mc - 1) * per];
         // (-1: nothing there.  A factor that comes out 0 still takes its chunk's NaN along.)
         const float al = k0 + sub < mc && x.y != 0.0f ? __builtin_amdgcn_exp2f(x.x - m) : -1.0f;
-        l = al < 0.0f ? l : fmaf(al, x.y, l);
+        const float half = __builtin_amdgcn_exp2f(0.5f * (x.x - m));     // (as Soft::rescale)
+        l = al < 0.0f ? l : fmaf(half * x.y, half, l);
         for (int k8 = k0; k8 < min(k0 + W, most); k8 += 8) {
             v4f v[8];
 #pragma unroll

@@ -265,7 +265,7 @@ def test_k_is_exact_for_bf16_windows_of_many_rows(E, rng, way, d):
 
 
 @pytest.mark.parametrize("bf16", [False, True])
-@pytest.mark.parametrize("size", [1e19, 1e35])
+@pytest.mark.parametrize("size", [1e19, 1e35, -3e38])
 @pytest.mark.parametrize("way", WAYS)
 def test_constant_groups_of_any_size(E, rng, way, size, bf16):
     """Groups of 64 equal values have scale 1 beside a bias of their size.  A token of such
