@@ -29,6 +29,8 @@ EAKV_ERR_DEVICE = -5
 EAKV_F32 = 0
 EAKV_BF16 = 1
 EAKV_TREE_MAX = 64
+EAKV_PAGE_MIN = 16
+EAKV_PAGED_SEQS = 4096
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libeakv.so")
@@ -90,6 +92,12 @@ SIGNATURES = {
     "eakv_cache_gather_batch_device": (C.c_int, [_vp, _vp, C.c_int, _vp, _vp, _vp, _vp]),
     "eakv_cache_fork": (_vp, [_vp, C.c_int, C.c_int]),
     "eakv_cache_compact": (C.c_int, [_vp, C.c_int, _vp, C.c_int]),
+    "eakv_append_paged_device": (
+        C.c_int, [_vp, _vp, C.c_int, _vp, _vp, C.c_int, C.c_int64, _vp]),
+    "eakv_attention_paged_device": (
+        C.c_int, [_vp, _vp, C.c_int, _vp, C.c_int64, C.c_int, C.c_int, C.c_int, _vp, C.c_int64, _vp,
+                  C.c_size_t, _vp]),
+    "eakv_attention_paged_work_bytes": (C.c_size_t, [_vp, _vp, C.c_int, C.c_int, C.c_int]),
     "eakv_cache_planes_device": (C.c_int, [_vp, C.c_int, C.c_int, _vp, _vp, _vp]),
     "eakv_attention_fused_plan": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp]),
     "eakv_dequantize_range_device": (
@@ -367,6 +375,58 @@ class WindowPlan:
         return _check(lib().eakv_attention_window_batch_device(
             self._h, len(self.caches), layer, self._starts, self._n, d_q, *self._args, d_tree,
             d_out, d_work, work_bytes, stream))
+
+
+_DTYPES = {"f32": EAKV_F32, "bf16": EAKV_BF16}
+
+
+class PagedBatchStruct(C.Structure):
+    """eakv_paged_batch_t"""
+    _fields_ = [("d_tables", _vp), ("ld_table", C.c_int64), ("d_lens", _vp), ("d_first", _vp),
+                ("n_seqs", C.c_int), ("page_tokens", C.c_int), ("n_new", C.c_int),
+                ("max_new", C.c_int), ("max_len", C.c_int)]
+
+
+class PagedBatch:
+    """Sequences in pages of a pool (a Cache) and their new tokens: eakv_paged_batch_t.
+    Buffers are device addresses; what they hold is read when a call runs.  d_first None:
+    max_new rows for each sequence."""
+
+    def __init__(self, pool, page_tokens, d_tables, ld_table, d_lens, n_seqs, max_len, max_new=1,
+                 d_first=None, n_new=None):
+        if n_new is None:
+            if d_first is not None:
+                raise ValueError("n_new: the rows that d_first divides")
+            n_new = n_seqs * max_new
+        self.pool = pool
+        self.args = PagedBatchStruct(d_tables, ld_table, d_lens, d_first, n_seqs, page_tokens, n_new,
+                                     max_new, max_len)
+        self._ref = C.addressof(self.args)
+
+    def append(self, layer, d_k, d_v, dtype="f32", ld=None, stream=None):
+        """K and V rows [n_new][n_kv][d] into their pages."""
+        if ld is None:
+            ld = self.pool.n_heads * self.pool.head_dim
+        return _check(lib().eakv_append_paged_device(self.pool.h, self._ref, layer, d_k, d_v,
+                                                     _DTYPES[dtype], ld, stream))
+
+    def work_bytes(self, n_q, n_kv, dtype="f32"):
+        """Bytes of scratch that attend() with a workspace of its own needs."""
+        L = lib()
+        L.eakv_clear_error()
+        n = L.eakv_attention_paged_work_bytes(self.pool.h, self._ref, _DTYPES[dtype], n_q, n_kv)
+        code, msg = last_error()
+        if code:
+            raise EakvError(code, msg)
+        return n
+
+    def attend(self, layer, d_q, d_out, n_q, n_kv, dtype="f32", d_work=None, work_bytes=0, ld_q=None,
+               ld_out=None, stream=None):
+        """Attention of the new tokens [n_new][n_q][d]."""
+        width = n_q * self.pool.head_dim
+        return _check(lib().eakv_attention_paged_device(
+            self.pool.h, self._ref, layer, d_q, width if ld_q is None else ld_q, _DTYPES[dtype], n_q, n_kv,
+            d_out, width if ld_out is None else ld_out, d_work, work_bytes, stream))
 
 
 FUSED_PLAN_KEYS = ("mfma", "chunks", "merge_levels", "tile_tokens", "waves_per_block",

@@ -207,6 +207,23 @@ int eakvd_verify(int n_seqs, int k, int vocab, const int32_t *count, const int32
                  const float *draft, int64_t ld_draft, const float *target, int64_t ld_target,
                  const float *uniform, int32_t *kept, int32_t *next, void *work, void *stream);
 
+/* ---- sequences in pages of a pool (hip/paged.hip, hip/pages.hip): eakv_paged_batch_t as
+ * the kernels take it.  Every value read from the device is held to the bounds here. */
+#define EAKVD_PAGED_SEQS 4096
+typedef struct {
+    int            n_seqs, page_tokens, n_new, max_new, max_len;
+    const int32_t *tables, *lens, *first;
+    int64_t        ld_table;
+} eakvd_pages;
+
+size_t eakvd_paged_work_bytes(const eakvd_geom *g, const eakvd_pages *b, int n_q, int n_kv);
+int eakvd_paged_attend(const eakvd_geom *g, const uint8_t *base, const eakvd_pages *b, int layer,
+                       const void *q, int64_t ld_q, int bf16, int n_q, int n_kv, void *out,
+                       int64_t ld_out, void *work, void *stream);
+/* K and V rows [n_new][n_kv][head_dim] (f32 or bf16), ld values from one token to the next */
+int eakvd_paged_append(const eakvd_geom *g, uint8_t *base, const eakvd_pages *b, int layer,
+                       const void *k, const void *v, int64_t ld, int bf16, void *stream);
+
 /* ---- whole-plane kernels (hip/planes.hip)
  * eakvd_dequantize: groups [g0, g0 + n) of block (layer, kv) to out
  * (f32[n][64], device).  eakvd_validate: the integrity check of the first n

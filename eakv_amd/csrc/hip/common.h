@@ -215,6 +215,35 @@ __device__ __forceinline__ void group_minmax8(const float4 &lo, const float4 &hi
     }
 }
 
+// One group: the reference's min/max, scale, bias and nibbles; lane j's
+// four packed bytes, and (lane 0) the scale and bias.
+struct QOut {
+    uint32_t word;
+    float scale, bias;
+};
+
+__device__ __forceinline__ QOut quantize_group8(const float4 &lo, const float4 &hi, int gbase)
+{
+    float mn, mx;
+    group_minmax8(lo, hi, gbase, mn, mx);
+    const float range = __fsub_rn(mx, mn);
+    QOut o;
+    o.scale = 1.0f;
+    o.bias = mn;
+    float inv = 0.0f;
+    if (range > 0.0f) {
+        o.scale = range / 15.0f;
+        inv = 15.0f / range;
+    }
+    const float f = q4_factor(inv);
+    const uint32_t b0 = q4(lo.x, mn, f) | (q4(hi.x, mn, f) << 4);
+    const uint32_t b1 = q4(lo.y, mn, f) | (q4(hi.y, mn, f) << 4);
+    const uint32_t b2 = q4(lo.z, mn, f) | (q4(hi.z, mn, f) << 4);
+    const uint32_t b3 = q4(lo.w, mn, f) | (q4(hi.w, mn, f) << 4);
+    o.word = b0 | (b1 << 8) | (b2 << 16) | (b3 << 24);
+    return o;
+}
+
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 

@@ -1,0 +1,902 @@
+// paged.hip — attention of new tokens over K and V in pages of a pool: position t of
+// sequence s is token table[s][t / P] * P + t % P of the pool, an ordinary cache, for
+// pages of P tokens.  Query i of n is at position len - n + i and sees the positions up to
+// its own:
+//
+//   out[i][h] = sum_t softmax_t(q[i][h].K[t] / sqrt(d)) V[t],
+//   K[t] = n*s + b per group of 64 dims (n the nibble), V likewise.
+//
+// Lengths, tables and rows are device data, so a recorded graph follows them; the host
+// knows bounds only.  The work is therefore split on the device: a unit is a row block (up
+// to 16 NR rows: new tokens x the q heads of one kv head) of one sequence and kv head, its
+// length the 256-token tiles that it sees.  All units stand in one line, which the blocks
+// share evenly, whatever the lengths; every block finds its part from the lengths' prefix
+// sum.  A unit that is cut leaves partial (O, M, l), at most two a block, which a second
+// launch joins.  No atomics: results are the same bits on every call.
+//
+// A block's 8 waves take 32-token sub-tiles in turn and join at the end.  A sub-tile is two
+// 16-token halves, each inside one page, so a page's address is scalar; pages of 64
+// sub-tiles are read at once, one to a lane.  Per sub-tile a wave computes
+//   S^T = K Q^T    v_mfma_f32_16x16x32_f16, 16 tokens x 16 rows of each half
+//   O^T = V^T P^T  16 dims x 16 rows; a lane's 8 scores belong to one row, and the
+//                  tokens of the step are numbered so that the scores' registers are P's
+//                  operand as they stand.
+//
+// K's operands: bf16 queries, the nibbles' own bits as subnormal f16 (2^-24 of them, which
+// the matrix cores take exactly); f32 queries, n - z with z the nibble nearest the value 0.
+// Scales are applied to the f32 dots; the biases c = b + z*s enter by one product of three
+// bf16 pieces each (24 bits).
+// V: the weights carry the scales, x = p s.
+//   bf16 queries  O[g] = sum_t x n + (p c - x z), nibbles as subnormals and the same rounded x
+//                 in both places, so that n - z cancels what it should; the second term is
+//                 one product with -z and one with c in every operand row.  x, p and c are
+//                 rounded to f16, 2^-12 each, against the output's 2^-9.  (A product with a
+//                 subnormal comes out to 2^-17 only, which f32 results would show.)
+//   f32 queries   O[g] = sum_t x (n - z) + p c, x a pair of f16 (24 bits), p c by f32 sums.
+// Softmax, V's exponents and the reference point M: as in window.hip.
+#include <string.h>
+
+#include "pages.h"
+#include "window.h"
+
+namespace {
+
+constexpr int kWaves = 8;
+constexpr int kTile = 32 * kWaves;      // tokens of a tile
+constexpr int kAhead = 3;               // V's slots: sub-tiles in flight and the one worked on
+// -z is held 2^11 times (30720 at most), as c with it, which f16 then holds to 2^-25
+constexpr float kZUp = 0x1p11f;
+
+typedef int v2i __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) v2i *lds_v2i;
+typedef __attribute__((address_space(3))) void *lds_v;
+typedef const __attribute__((address_space(1))) void *glb_v;
+
+struct PagedJob {
+    eakvd_pages b;
+    const uint8_t *base;
+    int layer, n_pages, log2p;
+    int n_q, n_kv, qpk;
+    int tb, hb;             // tokens of a row block; row blocks of a token (else 1)
+    int rbr;                // rows of a row block: 16 NR
+    int whole;              // units are not cut
+    const void *q;
+    void *out;
+    int64_t ld_q, ld_out;
+    float ksc;
+    int vec;
+    float *part;            // [grid][2][rbr][D], then [grid][2][rbr][2]
+    struct PagedCut *cut;   // [grid]
+};
+
+// A unit that begins in a block and ends in a later one.
+struct PagedCut {
+    int n;                  // blocks that hold a part of it, or 0
+    int tok, rows;          // its first row of q and out, and its rows
+    int head;               // its first q head
+};
+
+__device__ __forceinline__ int row_blocks(const PagedJob &J, int n)
+{
+    return n > 0 ? (n + J.tb - 1) / J.tb * J.hb : 0;
+}
+
+// Positions that row block rb of a sequence sees, and its length in the line.
+__device__ __forceinline__ int seen_by(const PagedJob &J, const Seq &q, int rb)
+{
+    const int k = J.hb == 1 ? rb : rb / J.hb;
+    return q.pos + min((k + 1) * J.tb, q.n);
+}
+__device__ __forceinline__ int length_of(const PagedJob &J, int seen)
+{
+    return J.whole || seen <= kTile ? 1 : (seen + kTile - 1) / kTile;
+}
+
+__device__ __forceinline__ int wave_sum_i(int v)
+{
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+__device__ __forceinline__ int wave_scan_i(int v, int lane)
+{
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(v, o, 64);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// pre[s]: the line's length before sequence s, s <= n_seqs.  All threads of the block.
+__device__ __forceinline__ void line_of(const PagedJob &J, int *pre, int *sums, int tid)
+{
+    const int lane = tid & 63, w = tid >> 6, n = J.b.n_seqs;
+    int carry = 0;
+    for (int s0 = 0; s0 < n; s0 += 64 * kWaves) {
+        const int s = s0 + tid;
+        Seq q = {0, 0, 0};
+        if (s < n) q = seq_at(J.b, s);
+        const int nrb = row_blocks(J, q.n);
+        int v = nrb ? length_of(J, seen_by(J, q, 0)) : 0;
+        // sequences of several row blocks one after the other, the wave's lanes on their blocks
+        uint64_t many = __ballot(nrb > 1);
+        while (many) {
+            const int k = __ffsll((unsigned long long)many) - 1;
+            many &= many - 1;
+            const Seq x = {0, __builtin_amdgcn_readlane(q.n, k), __builtin_amdgcn_readlane(q.pos, k)};
+            const int all = __builtin_amdgcn_readlane(nrb, k);
+            int sum = 0;
+            for (int r = lane; r < all; r += 64) sum += length_of(J, seen_by(J, x, r));
+            sum = wave_sum_i(sum);
+            if (lane == k) v = sum;
+        }
+        v *= J.n_kv;
+        const int upto = wave_scan_i(v, lane);
+        __syncthreads();
+        if (lane == 63) sums[w] = upto;
+        __syncthreads();
+        int before = carry;
+#pragma unroll
+        for (int i = 0; i < kWaves; i++) {
+            const int x = sums[i];
+            before += i < w ? x : 0;
+            carry += x;
+        }
+        if (s < n) pre[s] = before + upto - v;
+    }
+    if (tid == 0) pre[n] = carry;
+    __syncthreads();
+}
+
+// Where place x of the line is.
+struct Unit {
+    int s, kvh, rb;
+    int at, len;            // x's place in the unit and the unit's length
+    Seq q;
+    int seen;
+};
+
+__device__ __forceinline__ Unit unit_at(const PagedJob &J, const int *pre, int x, int lane)
+{
+    const int n = J.b.n_seqs;
+    Unit u;
+    // the last sequence that does not begin behind x, in two steps (n <= 4096)
+    int s = 0;
+    if (n > 64) {
+        const int i = lane * 64;
+        s = 64 * (uni((int)__popcll(__ballot(i < n && pre[min(i, n)] <= x))) - 1);
+    }
+    s += uni((int)__popcll(__ballot(s + lane < n && pre[min(s + lane, n)] <= x))) - 1;
+    u.s = s;
+    const Seq q = seq_at(J.b, s);
+    u.q.row = uni(q.row);
+    u.q.n = uni(q.n);
+    u.q.pos = uni(q.pos);
+    const int first = uni(pre[s]), per = (uni(pre[s + 1]) - first) / J.n_kv;
+    u.kvh = (x - first) / per;
+    int z = x - first - u.kvh * per;
+    const int nrb = row_blocks(J, u.q.n);
+    u.rb = 0;
+    if (nrb > 1) {
+        for (int r0 = 0; r0 < nrb; r0 += 64) {
+            const int v = r0 + lane < nrb ? length_of(J, seen_by(J, u.q, r0 + lane)) : 0;
+            const int upto = wave_scan_i(v, lane);
+            const uint64_t hit = __ballot(z < upto);
+            if (hit) {
+                const int k = __ffsll((unsigned long long)hit) - 1;
+                u.rb = r0 + k;
+                z -= __builtin_amdgcn_readlane(upto - v, k);
+                break;
+            }
+            z -= __builtin_amdgcn_readlane(upto, 63);
+        }
+    }
+    u.seen = seen_by(J, u.q, u.rb);
+    u.len = length_of(J, u.seen);
+    u.at = z;
+    return u;
+}
+
+// Blocks of one XCD (every eighth) take a contiguous part of the line, so that the row
+// blocks of a kv head share its planes in one L2.
+__device__ __forceinline__ int line_block(int b, int grid)
+{
+    return grid % 8 == 0 ? (b & 7) * (grid >> 3) + (b >> 3) : b;
+}
+
+template <int D, bool F32>
+struct __align__(16) PagedLds {
+    static constexpr int GPD = D / 64;
+    uint8_t v[kAhead][32 * 32 * GPD];   // V's bytes: rows of 32 GPD, their 16-byte units swizzled
+    float ks[GPD][32];                  // K's scales
+    float w[32];                        // 2^-e, e the exponent of a token's V
+    float vs[GPD][32];                  // V's scales, 2^-e of them
+    float vc[F32 ? GPD : 1][32];        // f32: V's biases c, 2^-e of them
+    float zk[F32 ? GPD : 1][32];        // f32: K's z
+    // of V's operands (block of 8 tokens, operand order), f32: -(1024 + z) and -(64 + z), bf16:
+    // -z and c
+    _Float16 zn[GPD][4][8];
+    _Float16 c16[GPD][4][8];
+};
+
+struct Stage {
+    uint2 k[2][2];                      // (half, group)
+    float ks, kb, vs, vb;
+    int at_a, at_b;                     // the halves' tokens in the pool, or -1
+};
+
+// the unit permutation of token row t
+template <int GPD>
+__device__ __forceinline__ int unit_swz(int t)
+{
+    return GPD == 2 ? ((t >> 2) & 1) | ((t >> 3) & 2) : (t >> 4) & 1;
+}
+
+// The maximum of a lane's value and those of the other three lanes of its row.
+__device__ __forceinline__ float row_max(float v)
+{
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return half_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float row_sum(float v)
+{
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// 16 rows' queries as the columns' operand, one lane's share: row lane % 16, of the
+// operand (g, nibble) the dims 64g + 32 nibble + 8b + 0..7, b = lane / 16, in nib2's order.
+// Rows are scaled by a power of two to below 2^15; against subnormals (bf16) the high
+// nibbles' dims to 2^-4 of that.
+template <int D, bool F32>
+struct Query {
+    h8 a[D / 32];
+    h8 b[F32 ? D / 32 : 1];             // f32: low parts
+    b8 bias;                            // pieces of the sum of q of group b / 2; b < 2: 1/rf
+    float rf;                           // score = dot * rf
+
+    __device__ __forceinline__ void load(const void *q, int64_t at, bool vec, int blk)
+    {
+        constexpr int GPD = D / 64;
+        float x[D / 32][8];
+        float top = 0.0f;
+#pragma unroll
+        for (int f = 0; f < D / 32; f++) {
+            const int64_t p = at + (f >> 1) * 64 + (f & 1) * 32 + 8 * blk;
+            if constexpr (F32) {
+                const float *s = (const float *)q + p;
+                if (vec) {
+                    const v4f lo = *(const v4f *)s, hi = *(const v4f *)(s + 4);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[f][j] = j < 4 ? lo[j & 3] : hi[j & 3];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[f][j] = s[j];
+                }
+            } else {
+                const uint16_t *s = (const uint16_t *)q + p;
+                if (vec) {
+                    const uint4 y = *(const uint4 *)s;
+                    const uint32_t ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        x[f][j] = __uint_as_float(j & 1 ? ys[j >> 1] & 0xffff0000u : ys[j >> 1] << 16);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[f][j] = __uint_as_float((uint32_t)s[j] << 16);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[f][j]));
+        }
+        const int up = 15 - exp_of(row_max(top));
+        const float scale = scale2(1.0f, up), less = F32 ? scale : scale * 0x1p-4f;
+        float sum[GPD];
+#pragma unroll
+        for (int f = 0; f < D / 32; f++) {
+            const float by = f & 1 ? less : scale;
+            float part = 0.0f;
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int j = (k >> 1) * 4 + (k & 1);
+                const float y0 = x[f][j] * by, y1 = x[f][j + 2] * by;
+                part += x[f][j] * scale + x[f][j + 2] * scale;
+                const h2 h = pk(y0, y1);
+                hi[k] = u_of(h);
+                if constexpr (F32) lo[k] = u_of(pk_rest(h, y0, y1));
+            }
+            a[f] = __builtin_bit_cast(h8, uint4{hi[0], hi[1], hi[2], hi[3]});
+            if constexpr (F32) b[f] = __builtin_bit_cast(h8, uint4{lo[0], lo[1], lo[2], lo[3]});
+            sum[f >> 1] = f & 1 ? sum[f >> 1] + part : part;
+        }
+#pragma unroll
+        for (int g = 0; g < GPD; g++) sum[g] = row_sum(sum[g]);
+        rf = scale2(1.0f, -up);
+        __bf16 p1, p2, p3;
+        pieces(GPD == 2 && blk >= 2 ? sum[GPD - 1] : sum[0], p1, p2, p3);
+        const __bf16 zero = (__bf16)0.0f;
+        bias = b8{p1, p2, p3, p1, p2, p1, blk < 2 ? (__bf16)scale : zero, zero};
+    }
+};
+
+template <int D, bool F32, int NR>
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(eakvd_geom geo, PagedJob J, int lds_line)
+{
+    constexpr int GPD = D / 64, RB = 32 * GPD, NF = D / 16, NP = F32 ? 2 : 1;
+    typedef PagedLds<D, F32> Lds;
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6);
+    const int n16 = lane & 15, blk = lane >> 4, n32 = lane & 31, h = lane >> 5;
+    Lds &S = ((Lds *)lds)[w];
+    int *pre = (int *)(lds + lds_line);
+    line_of(J, pre, (int *)lds, tid);
+    const int grid = (int)gridDim.x, total = uni(pre[J.b.n_seqs]);
+    const int share = max(1, (total + grid - 1) / grid);
+    const int bl = line_block((int)blockIdx.x, grid);
+    // (bl * share may pass 32 bits where there is little work for a large grid: no work then)
+    const int x1 = (int)min((int64_t)total, ((int64_t)bl + 1) * share);
+    int x = (int)min((int64_t)total, (int64_t)bl * share);
+    PagedCut cut = {0, 0, 0, 0};
+
+    const Planes K0 = planes_of(geo, J.base, J.layer, 0), V0 = planes_of(geo, J.base, J.layer, 1);
+    // where a lane's bytes of a half are: K, token n16, bytes 8 blk of each group; V, 16-byte
+    // unit `lane` of 1 KB of a slot is unit (lane % UPT) of row lane / UPT
+    constexpr int UPT = RB / 16, NV = RB * 32 / 1024, kLoads = NV + 2 * GPD + 4;
+    const uint32_t ok = n16 * RB + 8 * blk;
+    const int vt = lane / UPT;
+    const int pj = (n32 & 3) | ((n32 >> 4) << 2), pb = (n32 >> 2) & 3;
+    const int pos = (pj & 4) | ((pj & 1) << 1) | ((pj >> 1) & 1);
+    // transposed reads of V: lane supplies 8 bytes of row j = n16 / 2 of its block's tokens
+    const int jr = n16 >> 1, trow = 4 * blk + (jr & 3) + 16 * (jr >> 2);
+    int vrd[GPD][2];
+#pragma unroll
+    for (int g = 0; g < GPD; g++)
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+            vrd[g][c] = trow * RB + 16 * ((2 * g + c) ^ unit_swz<GPD>(trow)) + 8 * (lane & 1);
+    const bool owner = GPD == 2 || h == 0;
+    const int gh = GPD == 2 ? h : 0;
+    NibConst nc;
+    nc.hold();
+
+    while (x < x1) {
+        const Unit U = unit_at(J, pre, x, lane);
+        const int end = min(U.len, U.at + (x1 - x));
+        const bool whole = U.at == 0 && end == U.len;
+        const int hb = J.hb == 1 ? 0 : U.rb % J.hb, tb = J.hb == 1 ? U.rb : U.rb / J.hb;
+        const int tok0 = tb * J.tb;                              // of the sequence's new tokens
+        const int rows = J.hb == 1 ? min(J.tb, U.q.n - tok0) * J.qpk : min(J.rbr, J.qpk - hb * J.rbr);
+        const int head0 = U.kvh * J.qpk + hb * J.rbr;
+        const int lo = U.at * kTile;
+        const int hi = J.whole || end == U.len ? U.seen : end * kTile;
+        const int n_sub = hi > lo ? (hi - lo + 31) / 32 : 0;
+        const int n_i = n_sub > w ? (n_sub - w + kWaves - 1) / kWaves : 0;
+        const int32_t *table = J.b.tables + (int64_t)U.s * J.b.ld_table;
+        const int64_t g0 = (int64_t)U.kvh * geo.gph;
+        const uint8_t *kw = K0.w + g0 * 32, *vw = V0.w + g0 * 32;
+        const float *ks = K0.s + g0, *kb = K0.b + g0, *vs = V0.s + g0, *vb = V0.b + g0;
+
+        Query<D, F32> Q[NR];
+        int vis[NR];                                             // positions that the lane's row sees
+        int64_t orow[NR];
+#pragma unroll
+        for (int u = 0; u < NR; u++) {
+            const int r = min(16 * u + n16, rows - 1);
+            const int t = J.hb == 1 ? r / J.qpk : 0, hd = r - t * J.qpk;
+            vis[u] = U.q.pos + tok0 + t + 1;
+            const int64_t tok = U.q.row + tok0 + t;
+            orow[u] = tok * J.ld_out + (int64_t)(head0 + hd) * D;
+            Q[u].load(J.q, tok * J.ld_q + (int64_t)(head0 + hd) * D, J.vec & 1, blk);
+        }
+        const int vis_min = U.q.pos + tok0 + 1;
+
+        // pages of the wave's sub-tiles i, i + 1, .. i + 63: lane j holds where the halves of
+        // i + j are in the pool (-1: nowhere)
+        int pg_a = -1, pg_b = -1;
+        auto pages = [&](int i) __attribute__((always_inline)) {
+            const int t = min(lo + 32 * (w + kWaves * (i + lane)), hi - 1) & ~31;
+            const int at[2] = {t, min(t + 16, (hi - 1) & ~15)};
+            pg_a = place_of(table, at[0], J.log2p, J.n_pages);
+            pg_b = place_of(table, at[1], J.log2p, J.n_pages);
+        };
+        auto load = [&](int i, Stage &st) __attribute__((always_inline)) {
+            i = min(i, n_i - 1);
+            const int pa = __builtin_amdgcn_readlane(pg_a, i & 63), pb2 = __builtin_amdgcn_readlane(pg_b, i & 63);
+            st.at_a = pa;
+            st.at_b = pb2;
+            const int64_t a = max(pa, 0), b = max(pb2, 0);
+            uint8_t *slot = S.v[0] + (i % kAhead) * (32 * RB);
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                // d = 64: one load of both halves
+                const int t = vt + (NV == 2 ? 16 * j : 0);
+                const uint32_t off = (vt & 15) * RB + 16 * ((lane % UPT) ^ unit_swz<GPD>(t));
+                const uint8_t *p = NV == 2 ? vw + (j ? b : a) * RB : vw + (vt < 16 ? a : b) * RB;
+                __builtin_amdgcn_global_load_lds((glb_v)(p + off), (lds_v)(slot + 1024 * j), 16, 0, 2);
+            }
+#pragma unroll
+            for (int g = 0; g < GPD; g++) {
+                typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+                const u2 ya = __builtin_nontemporal_load((const u2 *)(kw + a * RB + (ok + 32 * g)));
+                const u2 yb = __builtin_nontemporal_load((const u2 *)(kw + b * RB + (ok + 32 * g)));
+                st.k[0][g] = uint2{ya[0], ya[1]};
+                st.k[1][g] = uint2{yb[0], yb[1]};
+            }
+            const uint32_t gi = (uint32_t)((n32 < 16 ? (int)a : (int)b) + (n32 & 15)) * GPD + gh;
+            st.ks = __builtin_nontemporal_load(ks + gi);
+            st.kb = __builtin_nontemporal_load(kb + gi);
+            st.vs = __builtin_nontemporal_load(vs + gi);
+            st.vb = __builtin_nontemporal_load(vb + gi);
+        };
+
+        v4f O[NR][NF], C[NR][F32 ? 1 : GPD];
+        float M[NR], L[NR], cs[NR][F32 ? GPD : 1];
+        uint32_t poison[NR];
+#pragma unroll
+        for (int u = 0; u < NR; u++) {
+#pragma unroll
+            for (int f = 0; f < NF; f++) O[u][f] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int g = 0; g < (F32 ? 1 : GPD); g++) C[u][g] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int g = 0; g < (F32 ? GPD : 1); g++) cs[u][g] = 0.0f;
+            M[u] = kMInit;
+            L[u] = 0.0f;
+            poison[u] = 0;
+        }
+
+        auto consume = [&](int i, const Stage &st) __attribute__((always_inline)) {
+            const int t0 = lo + 32 * (w + kWaves * i);
+            const bool half_ok = n32 < 16 ? st.at_a >= 0 : st.at_b >= 0;
+            // tokens behind the last, or in no page, have no part in this
+            const bool live = t0 + n32 < hi && half_ok;
+            const float zk = F32 ? zero_nibble(st.ks, st.kb) : 0.0f;
+            const float ck = (F32 ? fmaf(zk, st.ks, st.kb) : st.kb) * J.ksc;
+            // (a non-finite group counts as zeros and makes the rows that see it NaN)
+            const float va = fmaxf(fabsf(st.vb), fabsf(fmaf(15.0f, st.vs, st.vb)));
+            const bool fin = va < __builtin_inff() && st.vs == st.vs;
+            const uint64_t bad = __ballot(live && !fin);
+            const float sv = live && fin ? st.vs : 0.0f, bv = live && fin ? st.vb : 0.0f;
+            const float zv = zero_nibble(sv, bv), cv = fmaf(zv, sv, bv);
+            const float size = live && fin ? v_size<F32>(sv, va) : 0.0f;
+            const int ev = exp_of(GPD == 2 ? half_max(size) : size);
+            // ---- scales to LDS
+            S.w[n32] = scale2(1.0f, -ev);
+            if (owner) {
+                S.ks[gh][n32] = st.ks * (F32 ? J.ksc : J.ksc * 0x1p24f);
+                S.vs[gh][n32] = scale2(sv, -ev);
+                S.zn[gh][pb][pos] = (_Float16)(F32 ? -1024.0f - zv : -zv * kZUp);
+                if constexpr (F32) {
+                    S.c16[gh][pb][pos] = (_Float16)(-64.0f - zv);
+                    S.vc[gh][n32] = scale2(cv, -ev);
+                    S.zk[gh][n32] = zk;
+                } else {
+                    S.c16[gh][pb][pos] = (_Float16)scale2(cv, 11 - ev);
+                }
+            }
+            // K's operand of the bias product: a lane's own token, in its own block
+            __bf16 p1, p2, p3;
+            pieces(owner ? ck : 0.0f, p1, p2, p3);
+            const __bf16 none = (__bf16)0.0f;
+            const b8 kb8 = {p1, p1, p1, p2, p2, p3, h ? none : (__bf16)(float)ev, none};
+            const b8 kz8 = {none, none, none, none, none, none, none, none};
+            const b8 bias_a = n32 < 16 ? kb8 : kz8, bias_b = n32 < 16 ? kz8 : kb8;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            // ---- K's operands
+            h8 kl[2][GPD], kh[2][GPD];
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int g = 0; g < GPD; g++) {
+                    h2 off_l, off_h;
+                    if constexpr (F32) {
+                        const float z = S.zk[g][16 * k + n16];
+                        off_l = nib_off<false>(z, z);
+                        off_h = nib_off<true>(z, z);
+                    }
+                    const uint32_t xs[2] = {st.k[k][g].x, st.k[k][g].y};
+                    uint32_t a[4], b[4];
+#pragma unroll
+                    for (int d = 0; d < 2; d++) {
+                        const uint32_t y0 = xs[d], y1 = y0 >> 8;
+                        a[2 * d] = F32 ? u_of(nib2<false>(y0, off_l, nc)) : nib_sub<false>(y0);
+                        a[2 * d + 1] = F32 ? u_of(nib2<false>(y1, off_l, nc)) : nib_sub<false>(y1);
+                        b[2 * d] = F32 ? u_of(nib2<true>(y0, off_h, nc)) : nib_sub<true>(y0);
+                        b[2 * d + 1] = F32 ? u_of(nib2<true>(y1, off_h, nc)) : nib_sub<true>(y1);
+                    }
+                    kl[k][g] = __builtin_bit_cast(h8, uint4{a[0], a[1], a[2], a[3]});
+                    kh[k][g] = __builtin_bit_cast(h8, uint4{b[0], b[1], b[2], b[3]});
+                }
+            // ---- V's bytes, transposed (their loads are done: K's of the same sub-tile,
+            // issued behind them, are)
+            v2i vx[GPD][2];
+            const uint8_t *slot = S.v[0] + (i % kAhead) * (32 * RB);
+#pragma unroll
+            for (int g = 0; g < GPD; g++)
+#pragma unroll
+                for (int c = 0; c < 2; c++)
+                    vx[g][c] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i)(slot + vrd[g][c]));
+            const bool masked = t0 + 32 > vis_min || st.at_a < 0 || st.at_b < 0;
+            h8 X[NR][NP][GPD], P[F32 ? 1 : NR];
+#pragma unroll
+            for (int u = 0; u < NR; u++) {
+                if (u > 0 && 16 * u >= rows) break;
+                // ---- scores
+                v4f s[2];
+                s[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bias_a, Q[u].bias, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+                s[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bias_b, Q[u].bias, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+                for (int g = 0; g < GPD; g++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+                        if constexpr (F32) {
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[k][g], Q[u].b[F32 ? 2 * g : 0], acc, 0, 0, 0);
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[k][g], Q[u].b[F32 ? 2 * g + 1 : 0], acc, 0, 0, 0);
+                        }
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[k][g], Q[u].a[2 * g], acc, 0, 0, 0);
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[k][g], Q[u].a[2 * g + 1], acc, 0, 0, 0);
+                        const v4f sc = *(const v4f *)&S.ks[g][16 * k + 4 * blk];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) s[k][e] = fmaf(sc[e], acc[e], s[k][e]);
+                    }
+                // ---- softmax
+                if (masked) {
+#pragma unroll
+                    for (int k = 0; k < 2; k++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int t = t0 + 16 * k + 4 * blk + e;
+                            const bool see = t < vis[u] && (k ? st.at_b : st.at_a) >= 0;
+                            s[k][e] = see ? s[k][e] : -__builtin_inff();
+                        }
+                }
+                if (bad) {
+                    // rows that see a token with a non-finite V group
+                    uint32_t seen = 0;
+#pragma unroll
+                    for (int k = 0; k < 2; k++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            seen |= s[k][e] != -__builtin_inff() ? 1u << (16 * k + e) : 0u;
+                    seen <<= 4 * blk;
+                    poison[u] |= (seen & (uint32_t)bad ? 1u : 0u) |
+                                 (GPD == 2 && (seen & (uint32_t)(bad >> 32)) ? 2u : 0u);
+                }
+                const float top = row_max(fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                                                fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))));
+                const float need = fmaf(top, Q[u].rf, -kWinTop);
+                if (__ballot(need > M[u] + kWinTau) != 0) {
+                    const float mn = need > M[u] + kWinTau ? need : M[u], d = M[u] - mn;
+                    // (L by halves, as in window.h)
+                    const float al = __builtin_amdgcn_exp2f(d), half = __builtin_amdgcn_exp2f(0.5f * d);
+                    L[u] = L[u] * half * half;
+#pragma unroll
+                    for (int f = 0; f < NF; f++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) O[u][f][e] *= al;
+#pragma unroll
+                    for (int g = 0; g < (F32 ? 1 : GPD); g++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) C[u][g][e] *= al;
+                    if constexpr (F32)
+#pragma unroll
+                        for (int g = 0; g < GPD; g++) cs[u][g] *= al;
+                    M[u] = mn;
+                }
+                float p[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    p[j] = __builtin_amdgcn_exp2f(fmaf(s[j >> 2][j & 3], Q[u].rf, -M[u]));
+                float ls = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const v4f w4 = *(const v4f *)&S.w[16 * k + 4 * blk];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) ls = fmaf(p[4 * k + e], w4[e], ls);
+                }
+                L[u] += ls;
+                // ---- weights as operands
+#pragma unroll
+                for (int g = 0; g < GPD; g++) {
+                    uint32_t xh[4], xl[4];
+                    float c = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const v4f sc = *(const v4f *)&S.vs[g][16 * k + 4 * blk];
+                        float y[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) y[e] = p[4 * k + e] * sc[e];
+                        if constexpr (F32) {
+                            const v4f cc = *(const v4f *)&S.vc[g][16 * k + 4 * blk];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) c = fmaf(p[4 * k + e], cc[e], c);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const h2 hi2 = pk(y[e], y[e + 2]);
+                            xh[2 * k + e] = u_of(hi2);
+                            if constexpr (F32) xl[2 * k + e] = u_of(pk_rest(hi2, y[e], y[e + 2]));
+                        }
+                    }
+                    X[u][0][g] = __builtin_bit_cast(h8, uint4{xh[0], xh[1], xh[2], xh[3]});
+                    if constexpr (F32) {
+                        X[u][NP - 1][g] = __builtin_bit_cast(h8, uint4{xl[0], xl[1], xl[2], xl[3]});
+                        cs[u][F32 ? g : 0] += c;
+                    }
+                }
+                if constexpr (!F32)
+                    P[F32 ? 0 : u] = __builtin_bit_cast(h8, uint4{u_of(pk_exp(p[0], p[2])), u_of(pk_exp(p[1], p[3])),
+                                                                  u_of(pk_exp(p[4], p[6])), u_of(pk_exp(p[5], p[7]))});
+            }
+            // ---- weighted sums
+#pragma unroll
+            for (int g = 0; g < GPD; g++) {
+                const uint4 zn = *(const uint4 *)S.zn[g][blk], c8 = *(const uint4 *)S.c16[g][blk];
+                const uint32_t zs[4] = {zn.x, zn.y, zn.z, zn.w}, cz[4] = {c8.x, c8.y, c8.z, c8.w};
+                if constexpr (!F32) {
+#pragma unroll
+                    for (int u = 0; u < NR; u++) {
+                        if (u > 0 && 16 * u >= rows) break;
+                        C[u][F32 ? 0 : g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            __builtin_bit_cast(h8, zn), X[u][0][g], C[u][F32 ? 0 : g], 0, 0, 0);
+                        C[u][F32 ? 0 : g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            __builtin_bit_cast(h8, c8), P[F32 ? 0 : u], C[u][F32 ? 0 : g], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    uint32_t a[4], b[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint32_t y = (uint32_t)vx[g][c][k >> 1] >> (8 * (k & 1));
+                        a[k] = F32 ? u_of(nib2<false>(y, h_of(zs[k]), nc)) : nib_sub<false>(y);
+                        b[k] = F32 ? u_of(nib2<true>(y, h_of(cz[k]), nc)) : nib_sub<true>(y);
+                    }
+                    const h8 vl = __builtin_bit_cast(h8, uint4{a[0], a[1], a[2], a[3]});
+                    const h8 vh = __builtin_bit_cast(h8, uint4{b[0], b[1], b[2], b[3]});
+#pragma unroll
+                    for (int u = 0; u < NR; u++) {
+                        if (u > 0 && 16 * u >= rows) break;
+                        const int f = 4 * g + 2 * c;
+#pragma unroll
+                        for (int k = NP - 1; k >= 0; k--) {
+                            O[u][f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, X[u][k][g], O[u][f], 0, 0, 0);
+                            O[u][f + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, X[u][k][g], O[u][f + 1], 0, 0, 0);
+                        }
+                    }
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        };
+
+        if (n_i > 0) {
+            Stage st[kAhead];
+            pages(0);
+#pragma unroll
+            for (int k = 0; k < kAhead - 1; k++) load(k, st[k]);
+            for (int i = 0; i < n_i; i += kAhead) {
+#pragma unroll
+                for (int k = 0; k < kAhead; k++) {
+                    if (i + k >= n_i) break;
+                    const int next = i + k + kAhead - 1;
+                    if ((next & 63) == 0 && next < n_i) pages(next);
+                    load(next, st[(k + kAhead - 1) % kAhead]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    // all loads but those of the sub-tiles behind this one
+                    wait_loads<(kAhead - 1) * kLoads>();
+                    __builtin_amdgcn_sched_barrier(0);
+                    consume(i + k, st[k]);
+                }
+            }
+            wait_loads<0>();
+        }
+
+        // ---- the waves joined, 16 rows at a time
+        float *jo = (float *)lds;                                // [wave][NF][64][4]
+        float2 *jml = (float2 *)(lds + (size_t)kWaves * NF * 64 * 16);   // [wave][16]
+        const int slot = 2 * bl + (U.at == 0 ? 1 : 0);
+#pragma unroll
+        for (int u = 0; u < NR; u++) {
+            if (u > 0 && 16 * u >= rows) break;
+            // a lane has its row's sums of its own tokens only
+            const float l = row_sum(L[u]);
+            poison[u] |= __shfl_xor(poison[u], 16, 64);
+            poison[u] |= __shfl_xor(poison[u], 32, 64);
+            __syncthreads();
+#pragma unroll
+            for (int g = 0; g < GPD; g++) {
+                const float c = F32 ? row_sum(cs[u][F32 ? g : 0]) : 0.0f;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int f = 4 * g + k;
+                    v4f o;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        o[e] = F32 ? O[u][f][e] + c
+                                   : fmaf(O[u][f][e], k & 1 ? 0x1p20f : 0x1p24f,
+                                          C[u][F32 ? 0 : g][e] * (1.0f / kZUp));
+                        if (poison[u] >> g & 1) o[e] = __builtin_nanf("");
+                    }
+                    *((v4f *)jo + (w * NF + f) * 64 + lane) = o;
+                }
+            }
+            if (blk == 0) jml[w * 16 + n16] = float2{M[u], l};
+            __syncthreads();
+            float al[kWaves], m = kMInit, ll = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kWaves; k++) {
+                al[k] = jml[k * 16 + n16].x;
+                m = fmaxf(m, al[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < kWaves; k++) {
+                const float half = __builtin_amdgcn_exp2f(0.5f * (al[k] - m));
+                al[k] = __builtin_amdgcn_exp2f(al[k] - m);
+                ll = fmaf(half * jml[k * 16 + n16].y, half, ll);
+            }
+            const bool row_ok = 16 * u + n16 < rows;
+            if (w < NF) {
+                v4f y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int k = 0; k < kWaves; k++) {
+                    const v4f o = *((const v4f *)jo + (k * NF + w) * 64 + lane);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) y[e] = fmaf(al[k], o[e], y[e]);
+                }
+                const int dim = (w >> 2) * 64 + (w & 1) * 32 + ((w >> 1) & 1) * 16 + 4 * blk;
+                if (row_ok && whole) {
+                    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+                    const float o4[4] = {y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv};
+                    store4<F32>(J.out, orow[u] + dim, J.vec & 2, o4);
+                } else if (row_ok) {
+                    *(v4f *)(J.part + ((int64_t)slot * J.rbr + 16 * u + n16) * D + dim) = y;
+                }
+            }
+            if (!whole && row_ok && blk == 0 && w == 0) {
+                float *ml = J.part + (int64_t)grid * 2 * J.rbr * D + ((int64_t)slot * J.rbr + 16 * u + n16) * 2;
+                ml[0] = m;
+                ml[1] = ll;
+            }
+        }
+        __syncthreads();
+        if (U.at == 0 && !whole) {
+            cut.n = (x + U.len - 1) / share - bl + 1;
+            cut.tok = U.q.row + tok0;
+            cut.rows = rows;
+            cut.head = head0;
+        }
+        x += end - U.at;
+    }
+    if (!J.whole && tid == 0) J.cut[bl] = cut;
+}
+
+// The parts of units that were cut, joined: a block for each 16 rows of a cut, 4 dims
+// and a row to a thread.
+template <int D, bool F32>
+__global__ __launch_bounds__(D * 4) void paged_join_kernel(PagedJob J, int grid)
+{
+    const int b = blockIdx.x, j = 16 * (int)blockIdx.y + (int)threadIdx.x / (D / 4);
+    const int dim = (int)threadIdx.x % (D / 4) * 4;
+    const PagedCut c = J.cut[b];
+    if (c.n == 0 || j >= c.rows) return;
+    const float *po = J.part, *pm = J.part + (int64_t)grid * 2 * J.rbr * D;
+    auto row = [&](int k) { return (int64_t)(k ? 2 * (b + k) : 2 * b + 1) * J.rbr + j; };
+    float m = kMInit;
+    for (int k = 0; k < c.n; k++) {
+        const float2 x = *(const float2 *)(pm + row(k) * 2);
+        if (x.y != 0.0f) m = fmaxf(m, x.x);
+    }
+    float l = 0.0f;
+    v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = 0; k < c.n; k++) {
+        const float2 x = *(const float2 *)(pm + row(k) * 2);
+        const v4f v = *(const v4f *)(po + row(k) * D + dim);
+        if (x.y == 0.0f) continue;                               // (nothing seen there)
+        const float al = __builtin_amdgcn_exp2f(x.x - m), half = __builtin_amdgcn_exp2f(0.5f * (x.x - m));
+        l = fmaf(half * x.y, half, l);
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = fmaf(al, v[e], o[e]);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float y[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+    const int t = J.hb == 1 ? j / J.qpk : 0;
+    store4<F32>(J.out, (int64_t)(c.tok + t) * J.ld_out + (int64_t)(c.head + j - t * J.qpk) * D + dim,
+                J.vec & 2, y);
+}
+
+struct PagedPlan {
+    int nr, grid, whole;
+    size_t part, bytes;
+};
+
+// 16 rows to a unit where no sequence has more, else 32.
+PagedPlan paged_plan(const eakvd_geom *g, const eakvd_pages *b, int n_q, int n_kv)
+{
+    PagedPlan p;
+    const int qpk = n_q / n_kv;
+    p.nr = (int64_t)b->max_new * qpk <= 16 ? 1 : 2;
+    const int rbr = 16 * p.nr, tb = qpk < rbr ? rbr / qpk : 1, hb = (qpk + rbr - 1) / rbr;
+    // units at most
+    const int64_t units = (b->n_new / tb + (int64_t)(b->n_seqs < b->n_new ? b->n_seqs : b->n_new)) *
+                          hb * n_kv;
+    const int64_t tiles = (b->max_len + kTile - 1) / kTile;
+    // (two tiles stay together: the joining launch costs more)
+    p.whole = tiles <= 2;
+    const int64_t most = units * (p.whole ? 1 : tiles > 1 ? tiles : 1), cus = cu_count();
+    p.grid = (int)(most < cus ? most : cus);
+    p.part = ((size_t)p.grid * 2 * rbr * (g->head_dim + 2) * sizeof(float) + 255) & ~(size_t)255;
+    p.bytes = p.whole ? 0 : p.part + (size_t)p.grid * sizeof(PagedCut);
+    return p;
+}
+
+template <int D, bool F32, int NR>
+int launch(const eakvd_geom &g, PagedJob &J, const PagedPlan &p, hipStream_t st)
+{
+    constexpr size_t tiles = kWaves * sizeof(PagedLds<D, F32>);
+    constexpr size_t join = (size_t)kWaves * (D / 16) * 64 * 16 + kWaves * 16 * sizeof(float2);
+    constexpr size_t line = tiles > join ? tiles : join;
+    static_assert(line + (EAKVD_PAGED_SEQS + 1) * 4 <= 160 * 1024, "LDS");
+    auto *kern = paged_kernel<D, F32, NR>;
+    static std::atomic<uint64_t> done;
+    const int e = allow_lds((const void *)kern, line + (EAKVD_PAGED_SEQS + 1) * 4, done);
+    if (e) return e;
+    hipLaunchKernelGGL(kern, dim3((unsigned)p.grid), dim3(64 * kWaves), line + (J.b.n_seqs + 1) * 4, st, g,
+                       J, (int)line);
+    if (!p.whole)
+        hipLaunchKernelGGL((paged_join_kernel<D, F32>), dim3((unsigned)p.grid, NR), dim3(D * 4), 0, st, J,
+                           p.grid);
+    return (int)hipGetLastError();
+}
+
+}  // namespace
+
+extern "C" size_t eakvd_paged_work_bytes(const eakvd_geom *g, const eakvd_pages *b, int n_q, int n_kv)
+{
+    return paged_plan(g, b, n_q, n_kv).bytes;
+}
+
+extern "C" int eakvd_paged_attend(const eakvd_geom *g, const uint8_t *base, const eakvd_pages *b,
+                                  int layer, const void *q, int64_t ld_q, int bf16, int n_q, int n_kv,
+                                  void *out, int64_t ld_out, void *work, void *stream)
+{
+    const PagedPlan p = paged_plan(g, b, n_q, n_kv);
+    if (p.grid == 0) return 0;
+    PagedJob J;
+    memset(&J, 0, sizeof(J));
+    J.b = *b;
+    J.base = base;
+    J.layer = layer;
+    J.log2p = __builtin_ctz((unsigned)b->page_tokens);
+    J.n_pages = g->max_seq_len >> J.log2p;
+    J.n_q = n_q;
+    J.n_kv = n_kv;
+    J.qpk = n_q / n_kv;
+    J.rbr = 16 * p.nr;
+    J.tb = J.qpk < J.rbr ? J.rbr / J.qpk : 1;
+    J.hb = (J.qpk + J.rbr - 1) / J.rbr;
+    J.whole = p.whole;
+    J.q = q;
+    J.out = out;
+    J.ld_q = ld_q;
+    J.ld_out = ld_out;
+    J.ksc = EAKV_LOG2E / sqrtf((float)g->head_dim);
+    // 16-byte loads of q, 16- or 8-byte stores of out
+    const int64_t per = bf16 ? 8 : 4;
+    J.vec = ((uintptr_t)q % 16 == 0 && ld_q % per == 0 ? 1 : 0) |
+            ((uintptr_t)out % 16 == 0 && ld_out % per == 0 ? 2 : 0);
+    J.part = (float *)work;
+    J.cut = (PagedCut *)((uint8_t *)work + p.part);
+    const hipStream_t st = (hipStream_t)stream;
+    if (g->head_dim == 64) {
+        if (bf16) return p.nr == 1 ? launch<64, false, 1>(*g, J, p, st) : launch<64, false, 2>(*g, J, p, st);
+        return p.nr == 1 ? launch<64, true, 1>(*g, J, p, st) : launch<64, true, 2>(*g, J, p, st);
+    }
+    if (bf16) return p.nr == 1 ? launch<128, false, 1>(*g, J, p, st) : launch<128, false, 2>(*g, J, p, st);
+    return p.nr == 1 ? launch<128, true, 1>(*g, J, p, st) : launch<128, true, 2>(*g, J, p, st);
+}

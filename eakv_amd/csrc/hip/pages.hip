@@ -1,0 +1,131 @@
+// pages.hip — K and V of new tokens quantized into the pages that the sequences' tables
+// name, both in one launch.  Rows are [token][kv head][dim], f32 or bf16, as a model's
+// projections leave them; codes, scales and biases are bit for bit those of quantize.hip.
+//
+// A block takes 16 tokens of one kv head (d = 64: 32): its groups are contiguous in a page,
+// where it writes, and 256 to 512 bytes a token where it reads.  First its waves find each
+// token's sequence and place, 64 row numbers at a time (two loads for up to 4096 sequences),
+// then 8 lanes quantize a group.  Bound by a launch's latency for a decode step, by HBM
+// for prompts.
+#include "pages.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+
+struct AppendJob {
+    eakvd_pages b;
+    uint8_t *base;
+    int layer, n_pages, log2p;
+    const void *src[2];
+    int64_t ld;
+    int vec;
+};
+
+template <bool BF16, bool VEC>
+__device__ __forceinline__ float4 load4(const void *src, int64_t at)
+{
+    if constexpr (BF16) {
+        const uint16_t *p = (const uint16_t *)src + at;
+        uint32_t x, y;
+        if constexpr (VEC) {
+            const uint2 v = *(const uint2 *)p;
+            x = v.x;
+            y = v.y;
+        } else {
+            x = p[0] | (uint32_t)p[1] << 16;
+            y = p[2] | (uint32_t)p[3] << 16;
+        }
+        return make_float4(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u),
+                           __uint_as_float(y << 16), __uint_as_float(y & 0xffff0000u));
+    } else {
+        const float *p = (const float *)src + at;
+        if constexpr (VEC) {
+            const v4f v = __builtin_nontemporal_load((const v4f *)p);
+            return make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+            return make_float4(p[0], p[1], p[2], p[3]);
+        }
+    }
+}
+
+template <int GPD, bool BF16, bool VEC>
+__global__ __launch_bounds__(kThreads) void append_kernel(eakvd_geom g, AppendJob J)
+{
+    constexpr int T = kThreads / 8 / GPD;            // tokens of a block
+    __shared__ int place[T];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int r0 = (int)blockIdx.x * T, n = J.b.n_seqs;
+    // the last sequence that does not begin behind row r
+    auto begin = [&](int s) { return s < n ? seq_at(J.b, s).row : INT32_MAX; };
+    const int coarse = n > 64 ? begin(lane * 64) : 0;
+    for (int k = w; k < T; k += kThreads / 64) {
+        const int r = r0 + k;
+        if (r >= J.b.n_new) break;
+        int s = n > 64 ? 64 * ((int)__popcll(__ballot(coarse <= r)) - 1) : 0;
+        if (s < 0) s = 0;
+        s += (int)__popcll(__ballot(begin(s + lane) <= r)) - 1;
+        int at = -1;
+        if (s >= 0) {
+            const Seq q = seq_at(J.b, s);
+            const int i = r - q.row, t = q.pos + i;
+            if (i < q.n && t >= 0) at = place_of(J.b.tables + (int64_t)s * J.b.ld_table, t, J.log2p, J.n_pages);
+        }
+        if (lane == 0) place[k] = at;
+    }
+    __syncthreads();
+    const int l8 = tid & 7, gbase = lane & ~7, slot = tid >> 3;
+    const int k = slot / GPD, gd = slot % GPD;
+    const int at = r0 + k < J.b.n_new ? place[k] : -1;
+    for (int y = blockIdx.y; y < 2 * g.n_kv_heads; y += gridDim.y) {
+        const int kv = y >= g.n_kv_heads, hd = y - kv * g.n_kv_heads;
+        // (rows behind the last are read as the last: the 8 lanes of a group, and the wave, go on
+        // together)
+        const int r = min(r0 + k, J.b.n_new - 1);
+        const int64_t from = r * J.ld + (int64_t)hd * g.head_dim + gd * 64 + l8 * 4;
+        const float4 lo = load4<BF16, VEC>(J.src[kv], from), hi = load4<BF16, VEC>(J.src[kv], from + 32);
+        const QOut o = quantize_group8(lo, hi, gbase);
+        if (at >= 0) {
+            uint8_t *blk = J.base + (int64_t)(J.layer * 2 + kv) * g.block_bytes;
+            const int64_t gi = hd * g.gph + (int64_t)at * GPD + gd;
+            __builtin_nontemporal_store(o.word, (uint32_t *)(blk + gi * 32 + l8 * 4));
+            if (l8 == 0) {
+                __builtin_nontemporal_store(o.scale, (float *)(blk + g.s_off) + gi);
+                __builtin_nontemporal_store(o.bias, (float *)(blk + g.b_off) + gi);
+            }
+        }
+    }
+}
+
+}  // namespace
+
+extern "C" int eakvd_paged_append(const eakvd_geom *g, uint8_t *base, const eakvd_pages *b, int layer,
+                                  const void *k, const void *v, int64_t ld, int bf16, void *stream)
+{
+    if (b->n_new <= 0) return 0;
+    AppendJob J;
+    J.b = *b;
+    J.base = base;
+    J.layer = layer;
+    J.log2p = __builtin_ctz((unsigned)b->page_tokens);
+    J.n_pages = g->max_seq_len >> J.log2p;
+    J.src[0] = k;
+    J.src[1] = v;
+    J.ld = ld;
+    // 16-byte loads (bf16: 8)
+    const uintptr_t odd = bf16 ? 7 : 15;
+    const bool vec = (((uintptr_t)k | (uintptr_t)v) & odd) == 0 && ld % 4 == 0;
+    const int t = kThreads / 8 / (int)g->gpd;
+    const dim3 grid((unsigned)((b->n_new + t - 1) / t),
+                    (unsigned)(2 * g->n_kv_heads < 65535 ? 2 * g->n_kv_heads : 65535));
+    auto run = [&](auto *kern) {
+        hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, (hipStream_t)stream, *g, J);
+        return (int)hipGetLastError();
+    };
+    if (g->gpd == 2) {
+        if (bf16) return vec ? run(append_kernel<2, true, true>) : run(append_kernel<2, true, false>);
+        return vec ? run(append_kernel<2, false, true>) : run(append_kernel<2, false, false>);
+    }
+    if (bf16) return vec ? run(append_kernel<1, true, true>) : run(append_kernel<1, true, false>);
+    return vec ? run(append_kernel<1, false, true>) : run(append_kernel<1, false, false>);
+}

@@ -256,6 +256,65 @@ int eakv_cache_gather_batch_device(eakv_cache_t *const *srcs, eakv_cache_t *cons
 eakv_cache_t *eakv_cache_fork(const eakv_cache_t *src, int n_tokens, int max_seq_len);
 int eakv_cache_compact(eakv_cache_t *cache, int start, const int32_t *keep, int n_keep);
 
+/* Sequences in pages (no counterpart in the reference): K and V of many sequences in one
+ * cache, the pool, whose room is cut into pages of page_tokens tokens.  Position t of
+ * sequence s is token d_tables[s * ld_table + t / page_tokens] * page_tokens + t %
+ * page_tokens of the pool, in every layer.  The pool is an ordinary cache (its seq_len
+ * has no part in this); which pages are free is the caller's to know, and
+ * pages may stand in several tables.
+ *   page_tokens  a power of two, EAKV_PAGE_MIN or more; pages are numbered below
+ *                max_seq_len / page_tokens.  A page outside that (-1: none) holds nothing:
+ *                nobody sees its positions and nothing is written there.
+ *   d_lens       int32[n_seqs]: the tokens of each sequence, its new ones included
+ *   d_first      int32[n_seqs + 1], not falling: the rows of sequence s in the buffers of
+ *                new tokens are d_first[s] to d_first[s + 1]; NULL: max_new rows each.
+ *                The last of n rows is position d_lens[s] - 1, the first d_lens[s] - n
+ *                (rows before position 0, of sequences shorter than n, see nothing and
+ *                are not appended).  Rows of no sequence are left alone.
+ *   n_new        rows of those buffers
+ *   max_new, max_len  the most rows and tokens that a sequence has.  Values on the device that
+ *                pass these bounds are held to them.
+ * d_tables, d_lens and d_first are device memory, read when the call runs: a recorded graph
+ * follows what they hold at each replay.  At most EAKV_PAGED_SEQS sequences. */
+#define EAKV_PAGE_MIN 16
+#define EAKV_PAGED_SEQS 4096
+typedef struct eakv_paged_batch {
+    const int32_t *d_tables;
+    int64_t        ld_table;
+    const int32_t *d_lens;
+    const int32_t *d_first;
+    int            n_seqs, page_tokens, n_new, max_new, max_len;
+} eakv_paged_batch_t;
+
+/* K and V of the new tokens quantized into their pages of one layer, both in one launch: the
+ * bits of eakv_cache_append.  d_k, d_v: [n_new][n_kv_heads][head_dim] of type dtype
+ * (EAKV_F32 or EAKV_BF16), ld values from one token to the next (n_kv_heads * head_dim or
+ * more).  Where one place is written twice in a call (a page in two tables), what is left
+ * there is unspecified.  Streams: as eakv_append_batch_device; on a stream that records a
+ * graph nothing outside the graph is waited for, and what later reads the pages must wait
+ * for the replay. */
+int eakv_append_paged_device(eakv_cache_t *pool, const eakv_paged_batch_t *batch, int layer,
+                             const void *d_k, const void *d_v, int dtype, int64_t ld, void *stream);
+
+/* Attention of the new tokens over their sequences' pages, softmax(q.k/sqrt(d)).v, causal: a
+ * row sees the positions up to its own (appended before, in this layer).  d_q, d_out:
+ * [n_new][n_q_heads][head_dim] of type dtype, ld_q and ld_out values from one token to
+ * the next (n_q_heads * head_dim or more); one buffer with one ld, or two that do not overlap.
+ * Rows that see nothing give zeros.  What a row does not see has no part in its
+ * result.  Precision, non-finite values and ranges: as eakv_attention_window_batch_device.
+ *   d_work  device scratch of the call's own, 16-byte aligned, over none of the buffers and
+ *           of eakv_attention_paged_work_bytes() for the same batch (some MB at most), or
+ *           NULL: the pool's workspace.  Calls that share one and overlap in time race.  A
+ *           call on a stream that records a graph needs its own (unless 0 bytes are needed).
+ * Streams: as eakv_attention_fused_batch_device. */
+int eakv_attention_paged_device(const eakv_cache_t *pool, const eakv_paged_batch_t *batch, int layer,
+                                const void *d_q, int64_t ld_q, int dtype, int n_q_heads,
+                                int n_kv_heads, void *d_out, int64_t ld_out, void *d_work,
+                                size_t work_bytes, void *stream);
+/* 0 also for invalid arguments (recorded). */
+size_t eakv_attention_paged_work_bytes(const eakv_cache_t *pool, const eakv_paged_batch_t *batch,
+                                       int dtype, int n_q_heads, int n_kv_heads);
+
 /* Device addresses of the planes of block (layer, kv_idx): packed codes, scales and
  * biases in the group order of eakv_dequantize_range_device.  Any may be NULL. */
 int eakv_cache_planes_device(const eakv_cache_t *cache, int layer, int kv_idx,
