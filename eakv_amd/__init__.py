@@ -31,6 +31,7 @@ EAKV_BF16 = 1
 EAKV_TREE_MAX = 64
 EAKV_PAGE_MIN = 16
 EAKV_PAGED_SEQS = 4096
+EAKV_TOP_MAX = 32
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libeakv.so")
@@ -98,6 +99,19 @@ SIGNATURES = {
         C.c_int, [_vp, _vp, C.c_int, _vp, C.c_int64, C.c_int, C.c_int, C.c_int, _vp, C.c_int64, _vp,
                   C.c_size_t, _vp]),
     "eakv_attention_paged_work_bytes": (C.c_size_t, [_vp, _vp, C.c_int, C.c_int, C.c_int]),
+    "eakv_attention_weights_batch_device": (
+        C.c_int, [_vp, C.c_int, C.c_int, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_float, _vp,
+                  C.c_int64, _vp, C.c_size_t, _vp]),
+    "eakv_attention_weights_work_bytes": (
+        C.c_size_t, [_vp, C.c_int, _vp, _vp, C.c_int, C.c_int, C.c_int]),
+    "eakv_evict_select_device": (
+        C.c_int, [C.c_int, C.c_int, _vp, C.c_int64, _vp, C.c_int, C.c_int, _vp, _vp, _vp, C.c_int64, _vp,
+                  C.c_size_t, _vp]),
+    "eakv_evict_select_work_bytes": (C.c_size_t, [C.c_int, _vp]),
+    "eakv_token_logprobs_device": (
+        C.c_int, [C.c_int, C.c_int, _vp, C.c_int, C.c_int64, _vp, C.c_int, _vp, _vp, _vp, _vp, _vp,
+                  C.c_size_t, _vp]),
+    "eakv_token_logprobs_work_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
     "eakv_cache_planes_device": (C.c_int, [_vp, C.c_int, C.c_int, _vp, _vp, _vp]),
     "eakv_attention_fused_plan": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp]),
     "eakv_dequantize_range_device": (
@@ -362,10 +376,11 @@ class WindowPlan:
     @property
     def work_bytes(self):
         """Bytes of scratch that a run with a workspace of its own needs."""
-        L = lib()
-        L.eakv_clear_error()
-        n = L.eakv_attention_window_work_bytes(self._h, len(self.caches), self._starts, self._n,
-                                               *self._args)
+        return self._work_bytes(lib().eakv_attention_window_work_bytes)
+
+    def _work_bytes(self, fn):
+        lib().eakv_clear_error()
+        n = fn(self._h, len(self.caches), self._starts, self._n, *self._args)
         code, msg = last_error()
         if code:
             raise EakvError(code, msg)
@@ -375,6 +390,21 @@ class WindowPlan:
         return _check(lib().eakv_attention_window_batch_device(
             self._h, len(self.caches), layer, self._starts, self._n, d_q, *self._args, d_tree,
             d_out, d_work, work_bytes, stream))
+
+
+class WeightsPlan(WindowPlan):
+    """One shape of eakv_attention_weights_batch_device: the arguments of a WindowPlan."""
+
+    @property
+    def work_bytes(self):
+        """Bytes of scratch that a run with a workspace of its own needs."""
+        return self._work_bytes(lib().eakv_attention_weights_work_bytes)
+
+    def run(self, layer, d_q, d_weights, ld, keep=1.0, d_work=None, work_bytes=0, stream=None):
+        """d_weights [caches][n_kv][ld]: keep of what it holds, plus the window's weights."""
+        return _check(lib().eakv_attention_weights_batch_device(
+            self._h, len(self.caches), layer, self._starts, self._n, d_q, *self._args, keep, d_weights, ld,
+            d_work, work_bytes, stream))
 
 
 _DTYPES = {"f32": EAKV_F32, "bf16": EAKV_BF16}

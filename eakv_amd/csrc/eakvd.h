@@ -224,6 +224,28 @@ int eakvd_paged_attend(const eakvd_geom *g, const uint8_t *base, const eakvd_pag
 int eakvd_paged_append(const eakvd_geom *g, uint8_t *base, const eakvd_pages *b, int layer,
                        const void *k, const void *v, int64_t ld, int bf16, void *stream);
 
+/* ---- eviction by attention weight (hip/weights.hip, hip/evict.hip)
+ * eakvd_weights: out [b->n_seq][n_kv][ld]; work: eakvd_weights_work_bytes(). */
+size_t eakvd_weights_work_bytes(const eakvd_window *b, int n_q, int n_kv);
+int eakvd_weights(const eakvd_geom *g, const eakvd_window *b, int layer, const void *q, int bf16, int n_q,
+                  int n_kv, float keep, float *out, int64_t ld, void *work, void *stream);
+/* See eakv_evict_select_device; first[i]: where sequence i's list begins in index. */
+typedef struct {
+    int     n_seq, n_heads, n_first, n_recent;
+    int     n_tokens[EAKVD_MAX_BATCH], n_keep[EAKVD_MAX_BATCH];
+    int64_t first[EAKVD_MAX_BATCH];
+} eakvd_evict;
+size_t eakvd_evict_work_bytes(int n_seq, const int32_t *n_tokens);
+int eakvd_evict_select(const eakvd_evict *job, const float *weights, int64_t ld, int32_t *index,
+                       float *kept, int64_t ld_kept, void *work, void *stream);
+
+/* ---- log probabilities (hip/logprobs.hip); see eakv_token_logprobs_device */
+#define EAKVD_TOP_MAX 32
+size_t eakvd_logprobs_work_bytes(int n_rows, int vocab, int n_top);
+int eakvd_logprobs(int n_rows, int vocab, const void *logits, int bf16, int64_t ld, const int32_t *tokens,
+                   int n_top, float *logprobs, float *entropy, int32_t *top_tokens, float *top_logprobs,
+                   void *work, void *stream);
+
 /* ---- whole-plane kernels (hip/planes.hip)
  * eakvd_dequantize: groups [g0, g0 + n) of block (layer, kv) to out
  * (f32[n][64], device).  eakvd_validate: the integrity check of the first n

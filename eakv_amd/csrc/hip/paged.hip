@@ -37,7 +37,7 @@
 #include <string.h>
 
 #include "pages.h"
-#include "window.h"
+#include "rows16.h"
 
 namespace {
 
@@ -234,96 +234,6 @@ __device__ __forceinline__ int unit_swz(int t)
     return GPD == 2 ? ((t >> 2) & 1) | ((t >> 3) & 2) : (t >> 4) & 1;
 }
 
-// The maximum of a lane's value and those of the other three lanes of its row.
-__device__ __forceinline__ float row_max(float v)
-{
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return half_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
-}
-__device__ __forceinline__ float row_sum(float v)
-{
-    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
-// 16 rows' queries as the columns' operand, one lane's share: row lane % 16, of the
-// operand (g, nibble) the dims 64g + 32 nibble + 8b + 0..7, b = lane / 16, in nib2's order.
-// Rows are scaled by a power of two to below 2^15; against subnormals (bf16) the high
-// nibbles' dims to 2^-4 of that.
-template <int D, bool F32>
-struct Query {
-    h8 a[D / 32];
-    h8 b[F32 ? D / 32 : 1];             // f32: low parts
-    b8 bias;                            // pieces of the sum of q of group b / 2; b < 2: 1/rf
-    float rf;                           // score = dot * rf
-
-    __device__ __forceinline__ void load(const void *q, int64_t at, bool vec, int blk)
-    {
-        constexpr int GPD = D / 64;
-        float x[D / 32][8];
-        float top = 0.0f;
-#pragma unroll
-        for (int f = 0; f < D / 32; f++) {
-            const int64_t p = at + (f >> 1) * 64 + (f & 1) * 32 + 8 * blk;
-            if constexpr (F32) {
-                const float *s = (const float *)q + p;
-                if (vec) {
-                    const v4f lo = *(const v4f *)s, hi = *(const v4f *)(s + 4);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) x[f][j] = j < 4 ? lo[j & 3] : hi[j & 3];
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) x[f][j] = s[j];
-                }
-            } else {
-                const uint16_t *s = (const uint16_t *)q + p;
-                if (vec) {
-                    const uint4 y = *(const uint4 *)s;
-                    const uint32_t ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        x[f][j] = __uint_as_float(j & 1 ? ys[j >> 1] & 0xffff0000u : ys[j >> 1] << 16);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) x[f][j] = __uint_as_float((uint32_t)s[j] << 16);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[f][j]));
-        }
-        const int up = 15 - exp_of(row_max(top));
-        const float scale = scale2(1.0f, up), less = F32 ? scale : scale * 0x1p-4f;
-        float sum[GPD];
-#pragma unroll
-        for (int f = 0; f < D / 32; f++) {
-            const float by = f & 1 ? less : scale;
-            float part = 0.0f;
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int j = (k >> 1) * 4 + (k & 1);
-                const float y0 = x[f][j] * by, y1 = x[f][j + 2] * by;
-                part += x[f][j] * scale + x[f][j + 2] * scale;
-                const h2 h = pk(y0, y1);
-                hi[k] = u_of(h);
-                if constexpr (F32) lo[k] = u_of(pk_rest(h, y0, y1));
-            }
-            a[f] = __builtin_bit_cast(h8, uint4{hi[0], hi[1], hi[2], hi[3]});
-            if constexpr (F32) b[f] = __builtin_bit_cast(h8, uint4{lo[0], lo[1], lo[2], lo[3]});
-            sum[f >> 1] = f & 1 ? sum[f >> 1] + part : part;
-        }
-#pragma unroll
-        for (int g = 0; g < GPD; g++) sum[g] = row_sum(sum[g]);
-        rf = scale2(1.0f, -up);
-        __bf16 p1, p2, p3;
-        pieces(GPD == 2 && blk >= 2 ? sum[GPD - 1] : sum[0], p1, p2, p3);
-        const __bf16 zero = (__bf16)0.0f;
-        bias = b8{p1, p2, p3, p1, p2, p1, blk < 2 ? (__bf16)scale : zero, zero};
-    }
-};
-
 template <int D, bool F32, int NR>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(eakvd_geom geo, PagedJob J, int lds_line)
 {
@@ -381,7 +291,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(eakvd_geom geo, P
         const uint8_t *kw = K0.w + g0 * 32, *vw = V0.w + g0 * 32;
         const float *ks = K0.s + g0, *kb = K0.b + g0, *vs = V0.s + g0, *vb = V0.b + g0;
 
-        Query<D, F32> Q[NR];
+        Query<D, F32, !F32> Q[NR];
         int vis[NR];                                             // positions that the lane's row sees
         int64_t orow[NR];
 #pragma unroll
@@ -479,39 +389,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(eakvd_geom geo, P
                     S.c16[gh][pb][pos] = (_Float16)scale2(cv, 11 - ev);
                 }
             }
-            // K's operand of the bias product: a lane's own token, in its own block
-            __bf16 p1, p2, p3;
-            pieces(owner ? ck : 0.0f, p1, p2, p3);
-            const __bf16 none = (__bf16)0.0f;
-            const b8 kb8 = {p1, p1, p1, p2, p2, p3, h ? none : (__bf16)(float)ev, none};
-            const b8 kz8 = {none, none, none, none, none, none, none, none};
-            const b8 bias_a = n32 < 16 ? kb8 : kz8, bias_b = n32 < 16 ? kz8 : kb8;
+            b8 bias[2];
+            bias_operands(owner ? ck : 0.0f, (float)ev, h == 0, bias, n32);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             // ---- K's operands
             h8 kl[2][GPD], kh[2][GPD];
 #pragma unroll
             for (int k = 0; k < 2; k++)
 #pragma unroll
-                for (int g = 0; g < GPD; g++) {
-                    h2 off_l, off_h;
-                    if constexpr (F32) {
-                        const float z = S.zk[g][16 * k + n16];
-                        off_l = nib_off<false>(z, z);
-                        off_h = nib_off<true>(z, z);
-                    }
-                    const uint32_t xs[2] = {st.k[k][g].x, st.k[k][g].y};
-                    uint32_t a[4], b[4];
-#pragma unroll
-                    for (int d = 0; d < 2; d++) {
-                        const uint32_t y0 = xs[d], y1 = y0 >> 8;
-                        a[2 * d] = F32 ? u_of(nib2<false>(y0, off_l, nc)) : nib_sub<false>(y0);
-                        a[2 * d + 1] = F32 ? u_of(nib2<false>(y1, off_l, nc)) : nib_sub<false>(y1);
-                        b[2 * d] = F32 ? u_of(nib2<true>(y0, off_h, nc)) : nib_sub<true>(y0);
-                        b[2 * d + 1] = F32 ? u_of(nib2<true>(y1, off_h, nc)) : nib_sub<true>(y1);
-                    }
-                    kl[k][g] = __builtin_bit_cast(h8, uint4{a[0], a[1], a[2], a[3]});
-                    kh[k][g] = __builtin_bit_cast(h8, uint4{b[0], b[1], b[2], b[3]});
-                }
+                for (int g = 0; g < GPD; g++)
+                    k_operands<!F32>(st.k[k][g], F32 ? S.zk[F32 ? g : 0][16 * k + n16] : 0.0f, nc, kl[k][g], kh[k][g]);
             // ---- V's bytes, transposed (their loads are done: K's of the same sub-tile,
             // issued behind them, are)
             v2i vx[GPD][2];
@@ -528,19 +415,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(eakvd_geom geo, P
                 if (u > 0 && 16 * u >= rows) break;
                 // ---- scores
                 v4f s[2];
-                s[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bias_a, Q[u].bias, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-                s[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bias_b, Q[u].bias, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+                    s[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bias[k], Q[u].bias, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0,
+                                                                   0, 0);
 #pragma unroll
                 for (int g = 0; g < GPD; g++)
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
-                        v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
-                        if constexpr (F32) {
-                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[k][g], Q[u].b[F32 ? 2 * g : 0], acc, 0, 0, 0);
-                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[k][g], Q[u].b[F32 ? 2 * g + 1 : 0], acc, 0, 0, 0);
-                        }
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[k][g], Q[u].a[2 * g], acc, 0, 0, 0);
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[k][g], Q[u].a[2 * g + 1], acc, 0, 0, 0);
+                        const v4f acc = group_dots(kl[k][g], kh[k][g], Q[u], g);
                         const v4f sc = *(const v4f *)&S.ks[g][16 * k + 4 * blk];
 #pragma unroll
                         for (int e = 0; e < 4; e++) s[k][e] = fmaf(sc[e], acc[e], s[k][e]);

@@ -50,6 +50,12 @@ int  eakvi_hip_fail(int hip_err, const char *what);
 int  eakvi_attn_check(const eakv_cache_t *c, int layer, int n_q, int n_kv);
 int  eakvi_same_batch(eakv_cache_t *const *caches, int n, const char *what);
 
+/* Checks a call over windows of new tokens (window.c) and fills *b and the sum of the
+ * windows; the window of cache i begins at starts[i], or (NULL) at its seq_len. */
+int  eakvi_window_check(eakv_cache_t *const *caches, int n, int layer, const int32_t *starts,
+                        const int32_t *n_tokens, int dtype, int n_q, int n_kv, int tree,
+                        eakvd_window *b, int64_t *total);
+
 /* Bytes of a caller's buffer (NULL or none: overlaps nothing). */
 typedef struct {
     const void *p;

@@ -5,11 +5,9 @@
 
 #include "internal.h"
 
-/* Fills *b and the sum of the windows; the window of cache i begins at starts[i],
- * or (NULL) at its seq_len. */
-static int window_check(eakv_cache_t *const *caches, int n, int layer, const int32_t *starts,
-                        const int32_t *n_tokens, int dtype, int n_q, int n_kv, int tree,
-                        eakvd_window *b, int64_t *total)
+int eakvi_window_check(eakv_cache_t *const *caches, int n, int layer, const int32_t *starts,
+                       const int32_t *n_tokens, int dtype, int n_q, int n_kv, int tree,
+                       eakvd_window *b, int64_t *total)
 {
     if (!caches || n <= 0 || n > EAKVD_MAX_BATCH || !n_tokens)
         return eakvi_set_error(EAKV_ERR_INVALID, "window: invalid argument");
@@ -64,7 +62,7 @@ size_t eakv_attention_window_work_bytes(eakv_cache_t *const *caches, int n_cache
     eakvd_window b;
     eakvd_batch d;
     int64_t total;
-    if (window_check(caches, n_caches, 0, starts, n_tokens, dtype, n_q, n_kv, 0, &b, &total))
+    if (eakvi_window_check(caches, n_caches, 0, starts, n_tokens, dtype, n_q, n_kv, 0, &b, &total))
         return 0;
     int prev;
     if (eakvi_enter(caches[0], &prev)) return 0;
@@ -88,8 +86,8 @@ int eakv_attention_window_batch_device(eakv_cache_t *const *caches, int n_caches
     eakvd_window b;
     eakvd_batch d;
     int64_t total;
-    int rc = window_check(caches, n_caches, layer, starts, n_tokens, dtype, n_q, n_kv,
-                          d_tree != NULL, &b, &total);
+    int rc = eakvi_window_check(caches, n_caches, layer, starts, n_tokens, dtype, n_q, n_kv,
+                                d_tree != NULL, &b, &total);
     if (rc) return rc;
     if (total == 0) return EAKV_OK;
     const uintptr_t odd = dtype == EAKV_F32 ? 3 : 1;

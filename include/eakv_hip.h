@@ -315,6 +315,71 @@ int eakv_attention_paged_device(const eakv_cache_t *pool, const eakv_paged_batch
 size_t eakv_attention_paged_work_bytes(const eakv_cache_t *pool, const eakv_paged_batch_t *batch,
                                        int dtype, int n_q_heads, int n_kv_heads);
 
+/* The attention weight of every cached token, for eviction (no counterpart in the
+ * reference): for cache c, kv head h and t < starts[c] + n_tokens[c]
+ *   d_weights[(c * n_kv_heads + h) * ld + t] = keep * itself + the sum, over the window's
+ *   queries that see t and the q heads of h, of softmax(q.k/sqrt(d))[t]
+ * with the windows, queries and types of eakv_attention_window_batch_device (causal, without
+ * a tree; only K is read).  keep 0: what was there is not read.  Entries from starts[c] +
+ * n_tokens[c] on, and those of a cache without queries, are left alone.
+ *   ld       at least the most starts[c] + n_tokens[c]
+ *   d_work   as there: eakv_attention_weights_work_bytes() of scratch, or NULL
+ * A token that a query does not see has no part in its softmax, whatever its size.
+ * Streams and graphs: as eakv_attention_window_batch_device. */
+int eakv_attention_weights_batch_device(eakv_cache_t *const *caches, int n_caches, int layer,
+                                        const int32_t *starts, const int32_t *n_tokens, const void *d_q,
+                                        int dtype, int n_q_heads, int n_kv_heads, float keep,
+                                        float *d_weights, int64_t ld, void *d_work, size_t work_bytes,
+                                        void *stream);
+/* 0 also for invalid arguments (recorded). */
+size_t eakv_attention_weights_work_bytes(eakv_cache_t *const *caches, int n_caches, const int32_t *starts,
+                                         const int32_t *n_tokens, int dtype, int n_q_heads,
+                                         int n_kv_heads);
+
+/* Which tokens of n_seqs sequences stay (no counterpart in the reference), on the current
+ * HIP device and the given stream (NULL: the default stream): of sequence i's n_tokens[i]
+ * the first n_first and the last n_recent, and of the others those of largest score,
+ * n_keep[i] in all; ties to the lower position.  A token's score is the sum of its weights
+ * d_weights[(i * n_heads + h) * ld + t] over the n_heads rows h (kv heads, or layers x kv heads),
+ * summed in 64 bits and rounded to 32; NaN is below every number.
+ *   n_tokens, n_keep  host int32[n_seqs]; min(n_first + n_recent, n_tokens[i]) <= n_keep[i] <=
+ *                     n_tokens[i]; at most 32 sequences
+ *   d_index  int32[sum of n_keep]: each sequence's positions, ascending, one list after the
+ *            other: what eakv_cache_gather_batch_device takes
+ *   d_kept   NULL, or f32[n_seqs][n_heads][ld_kept]: the weights of the tokens that stay, in
+ *            their new places, and 0 from n_keep[i] on (tokens to come have none)
+ *   d_work   eakv_evict_select_work_bytes() of device scratch, 4-byte aligned, the call's own
+ *            (0 bytes up to 16384 tokens)
+ * The results and d_work overlap nothing else (refused).  Asynchronous; may be recorded in a
+ * graph. */
+int eakv_evict_select_device(int n_seqs, int n_heads, const float *d_weights, int64_t ld,
+                             const int32_t *n_tokens, int n_first, int n_recent, const int32_t *n_keep,
+                             int32_t *d_index, float *d_kept, int64_t ld_kept, void *d_work,
+                             size_t work_bytes, void *stream);
+size_t eakv_evict_select_work_bytes(int n_seqs, const int32_t *n_tokens);
+
+/* Log probabilities of given tokens (no counterpart in the reference), on the current HIP
+ * device and the given stream (NULL: the default stream).  For each of n_rows rows of
+ * logits, ld values apart, of type dtype (EAKV_F32 or EAKV_BF16), p = softmax of the row:
+ *   d_logprobs      f32[n_rows]: ln p of token d_tokens[row]; -inf for one outside the
+ *                   vocabulary.  NULL: not wanted (d_tokens too)
+ *   d_entropy       f32[n_rows]: -sum p ln p, or NULL
+ *   d_top_tokens, d_top_logprobs  int32 and f32 [n_rows][n_top]: the n_top (at most EAKV_TOP_MAX)
+ *                   most likely tokens, ties to the lower one, and their ln p; -1 and -inf
+ *                   where fewer have a logit above -inf
+ * Logits of -inf have p = 0.  Rows with NaN or +inf, or nothing but -inf, give NaN where a ln p is
+ * taken; NaN is no alternative.  Sums in f32, results 1e-6 or less off.
+ *   d_work  eakv_token_logprobs_work_bytes() of device scratch, 16-byte aligned, the call's
+ *           own (0 bytes up to 16377 tokens)
+ * The results and d_work overlap nothing else (refused).  Asynchronous; may be recorded in a
+ * graph. */
+#define EAKV_TOP_MAX 32
+int eakv_token_logprobs_device(int n_rows, int vocab, const void *d_logits, int dtype, int64_t ld,
+                               const int32_t *d_tokens, int n_top, float *d_logprobs, float *d_entropy,
+                               int32_t *d_top_tokens, float *d_top_logprobs, void *d_work,
+                               size_t work_bytes, void *stream);
+size_t eakv_token_logprobs_work_bytes(int n_rows, int vocab, int n_top);
+
 /* Device addresses of the planes of block (layer, kv_idx): packed codes, scales and
  * biases in the group order of eakv_dequantize_range_device.  Any may be NULL. */
 int eakv_cache_planes_device(const eakv_cache_t *cache, int layer, int kv_idx,
