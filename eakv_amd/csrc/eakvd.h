@@ -216,7 +216,7 @@ typedef struct {
     int64_t        ld_table;
 } eakvd_pages;
 
-size_t eakvd_paged_work_bytes(const eakvd_geom *g, const eakvd_pages *b, int n_q, int n_kv);
+size_t eakvd_paged_work_bytes(const eakvd_geom *g, const eakvd_pages *b, int n_q, int n_kv, int bf16);
 int eakvd_paged_attend(const eakvd_geom *g, const uint8_t *base, const eakvd_pages *b, int layer,
                        const void *q, int64_t ld_q, int bf16, int n_q, int n_kv, void *out,
                        int64_t ld_out, void *work, void *stream);

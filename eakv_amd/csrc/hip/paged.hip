@@ -41,16 +41,18 @@
 
 namespace {
 
-constexpr int kWaves = 8;
-constexpr int kTile = 32 * kWaves;      // tokens of a tile
-constexpr int kAhead = 3;               // V's slots: sub-tiles in flight and the one worked on
+constexpr int kTile = 256;              // tokens of a tile
 // -z is held 2^11 times (30720 at most), as c with it, which f16 then holds to 2^-25
 constexpr float kZUp = 0x1p11f;
 
 typedef int v2i __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) v2i *lds_v2i;
-typedef __attribute__((address_space(3))) void *lds_v;
-typedef const __attribute__((address_space(1))) void *glb_v;
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void *p, int64_t bytes)
+{
+    // dword3 0x00020000: raw 32-bit buffer; reads beyond `bytes` return 0
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, (int)(uint32_t)bytes, 0x00020000);
+}
 
 struct PagedJob {
     eakvd_pages b;
@@ -110,6 +112,7 @@ __device__ __forceinline__ int wave_scan_i(int v, int lane)
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // pre[s]: the line's length before sequence s, s <= n_seqs.  All threads of the block.
+template <int kWaves>
 __device__ __forceinline__ void line_of(const PagedJob &J, int *pre, int *sums, int tid)
 {
     const int lane = tid & 63, w = tid >> 6, n = J.b.n_seqs;
@@ -206,23 +209,49 @@ __device__ __forceinline__ int line_block(int b, int grid)
     return grid % 8 == 0 ? (b & 7) * (grid >> 3) + (b >> 3) : b;
 }
 
-template <int D, bool F32>
-struct __align__(16) PagedLds {
+// What a variant of the kernel holds where.  NR row tiles of 16 share a wave's operands of K and V.
+// One (decode): queries in registers, 4 waves to a block and 3 to a SIMD.  More: queries in LDS,
+// which all 8 waves of the block share.  Four (bf16 alone): V's operands are its values in
+// f16, made once for 64 rows, and weights are operands as they stand (with the scales in the
+// weights each row tile takes 28 instructions more and V's operands 64 less).
+template <int NR>
+constexpr int kWavesOf = NR > 1 ? 8 : 4;
+
+template <int D, bool F32, int NR>
+struct Form {
     static constexpr int GPD = D / 64;
-    uint8_t v[kAhead][32 * 32 * GPD];   // V's bytes: rows of 32 GPD, their 16-byte units swizzled
-    float ks[GPD][32];                  // K's scales
-    float w[32];                        // 2^-e, e the exponent of a token's V
-    float vs[GPD][32];                  // V's scales, 2^-e of them
-    float vc[F32 ? GPD : 1][32];        // f32: V's biases c, 2^-e of them
-    float zk[F32 ? GPD : 1][32];        // f32: K's z
-    // of V's operands (block of 8 tokens, operand order), f32: -(1024 + z) and -(64 + z), bf16:
-    // -z and c
-    _Float16 zn[GPD][4][8];
-    _Float16 c16[GPD][4][8];
+    static constexpr int kWaves = kWavesOf<NR>;
+    static constexpr bool kShared = NR > 1;             // queries in LDS
+    static constexpr bool kValues = !F32 && NR > 2;    // V's operands are values
+    static constexpr int NQ = D / 32 * (F32 ? 2 : 1) + 1;
+
+    struct __align__(16) Wave {
+        uint8_t v[32 * 32 * GPD];               // V's bytes: rows of 32 GPD, their 16-byte units swizzled
+        float ks[GPD][32];                      // K's scales
+        float w[32];                            // 2^-e, e the exponent of a token's V
+        float vs[kValues ? 1 : GPD][32];        // V's scales, 2^-e of them
+        float vc[F32 ? GPD : 1][32];            // f32: V's biases c, 2^-e of them
+        float zk[F32 ? GPD : 1][32];            // f32: K's z
+        // of V's operands (block of 8 tokens, operand order): -(1024 + z) and -(64 + z), or
+        // (scales in the weights, subnormals) -z and c; values: their scales and biases
+        _Float16 z0[GPD][4][8], z1[GPD][4][8];
+        _Float16 s16[kValues ? GPD : 1][4][8], c16[kValues ? GPD : 1][4][8];
+    };
+    struct Rows {
+        uint4 q[NR][NQ][64];
+        float rf[NR][16];
+        int vis[NR][16];
+    };
+    static constexpr size_t kWaveBytes = kWaves * sizeof(Wave);
+    static constexpr size_t kJoin = (size_t)kWaves * (D / 16) * 64 * 16 + kWaves * 16 * sizeof(float2);
+    static constexpr size_t kRows = kWaveBytes > kJoin ? kWaveBytes : kJoin;    // where the rows are
+    static constexpr size_t kLine = kRows + (kShared ? sizeof(Rows) : 0);       // and the line
 };
 
+template <int GPD>
 struct Stage {
-    uint2 k[2][2];                      // (half, group)
+    uint2 k[2][GPD];                    // (half, group)
+    uint32_t v[2][2 * GPD];             // of each half, in order
     float ks, kb, vs, vb;
     int at_a, at_b;                     // the halves' tokens in the pool, or -1
 };
@@ -235,16 +264,20 @@ __device__ __forceinline__ int unit_swz(int t)
 }
 
 template <int D, bool F32, int NR>
-__global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(eakvd_geom geo, PagedJob J, int lds_line)
+__global__ __launch_bounds__(64 * kWavesOf<NR>, NR > 1 ? 2 : 3) void paged_kernel(eakvd_geom geo, PagedJob J)
 {
+    typedef Form<D, F32, NR> Fm;
     constexpr int GPD = D / 64, RB = 32 * GPD, NF = D / 16, NP = F32 ? 2 : 1;
-    typedef PagedLds<D, F32> Lds;
+    constexpr int kWaves = Fm::kWaves;
+    constexpr bool kValues = Fm::kValues, kSub = !F32 && !kValues;
+    constexpr int NC = kSub ? GPD : 1;
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6);
     const int n16 = lane & 15, blk = lane >> 4, n32 = lane & 31, h = lane >> 5;
-    Lds &S = ((Lds *)lds)[w];
-    int *pre = (int *)(lds + lds_line);
-    line_of(J, pre, (int *)lds, tid);
+    typename Fm::Wave &S = ((typename Fm::Wave *)lds)[w];
+    typename Fm::Rows &R = *(typename Fm::Rows *)(lds + Fm::kRows);
+    int *pre = (int *)(lds + Fm::kLine);
+    line_of<kWaves>(J, pre, (int *)lds, tid);
     const int grid = (int)gridDim.x, total = uni(pre[J.b.n_seqs]);
     const int share = max(1, (total + grid - 1) / grid);
     const int bl = line_block((int)blockIdx.x, grid);
@@ -254,11 +287,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(eakvd_geom geo, P
     PagedCut cut = {0, 0, 0, 0};
 
     const Planes K0 = planes_of(geo, J.base, J.layer, 0), V0 = planes_of(geo, J.base, J.layer, 1);
-    // where a lane's bytes of a half are: K, token n16, bytes 8 blk of each group; V, 16-byte
-    // unit `lane` of 1 KB of a slot is unit (lane % UPT) of row lane / UPT
-    constexpr int UPT = RB / 16, NV = RB * 32 / 1024, kLoads = NV + 2 * GPD + 4;
-    const uint32_t ok = n16 * RB + 8 * blk;
-    const int vt = lane / UPT;
+    // a lane's bytes of a half: K, token n16, bytes 8 blk of each group; V, 8 GPD bytes in order,
+    // which are part lane % 4 of row lane / 4
+    const int ok = n16 * RB + 8 * blk;
+    int vwr[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int t = 16 * k + (lane >> 2), at = 8 * GPD * (lane & 3);
+        vwr[k] = t * RB + 16 * ((at >> 4) ^ unit_swz<GPD>(t)) + (at & 15);
+    }
     const int pj = (n32 & 3) | ((n32 >> 4) << 2), pb = (n32 >> 2) & 3;
     const int pos = (pj & 4) | ((pj & 1) << 1) | ((pj >> 1) & 1);
     // transposed reads of V: lane supplies 8 bytes of row j = n16 / 2 of its block's tokens
@@ -289,20 +326,45 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(eakvd_geom geo, P
         const int32_t *table = J.b.tables + (int64_t)U.s * J.b.ld_table;
         const int64_t g0 = (int64_t)U.kvh * geo.gph;
         const uint8_t *kw = K0.w + g0 * 32, *vw = V0.w + g0 * 32;
-        const float *ks = K0.s + g0, *kb = K0.b + g0, *vs = V0.s + g0, *vb = V0.b + g0;
+        const int64_t plane = geo.gph * 4;
+        const auto rks = rsrc(K0.s + g0, plane), rkb = rsrc(K0.b + g0, plane);
+        const auto rvs = rsrc(V0.s + g0, plane), rvb = rsrc(V0.b + g0, plane);
 
-        Query<D, F32, !F32> Q[NR];
-        int vis[NR];                                             // positions that the lane's row sees
-        int64_t orow[NR];
+        // row 16 u + n16: its token (of the unit's) and q head
+        auto row_at = [&](int u, int &t, int &hd) __attribute__((always_inline)) {
+            const int r = min(16 * u + n16, rows - 1);
+            t = J.hb == 1 ? r / J.qpk : 0;
+            hd = r - t * J.qpk;
+        };
+        Query<D, F32, kSub || kValues> Q[Fm::kShared ? 1 : NR];
+        int vis1 = 0;
+        float rf1 = 0.0f;
 #pragma unroll
         for (int u = 0; u < NR; u++) {
-            const int r = min(16 * u + n16, rows - 1);
-            const int t = J.hb == 1 ? r / J.qpk : 0, hd = r - t * J.qpk;
-            vis[u] = U.q.pos + tok0 + t + 1;
-            const int64_t tok = U.q.row + tok0 + t;
-            orow[u] = tok * J.ld_out + (int64_t)(head0 + hd) * D;
-            Q[u].load(J.q, tok * J.ld_q + (int64_t)(head0 + hd) * D, J.vec & 1, blk);
+            int t, hd;
+            row_at(u, t, hd);
+            const int vis = U.q.pos + tok0 + t + 1;              // positions that the row sees
+            if (!Fm::kShared || (u == w && 16 * u < rows)) {
+                auto &q = Q[Fm::kShared ? 0 : u];
+                q.load(J.q, (int64_t)(U.q.row + tok0 + t) * J.ld_q + (int64_t)(head0 + hd) * D, J.vec & 1, blk);
+                if constexpr (Fm::kShared) {
+#pragma unroll
+                    for (int f = 0; f < D / 32; f++) {
+                        R.q[u][f][lane] = __builtin_bit_cast(uint4, q.a[f]);
+                        if constexpr (F32) R.q[u][D / 32 + (F32 ? f : 0)][lane] = __builtin_bit_cast(uint4, q.b[F32 ? f : 0]);
+                    }
+                    R.q[u][Fm::NQ - 1][lane] = __builtin_bit_cast(uint4, q.bias);
+                    if (blk == 0) {
+                        R.rf[u][n16] = q.rf;
+                        R.vis[u][n16] = vis;
+                    }
+                } else {
+                    vis1 = vis;
+                    rf1 = q.rf;
+                }
+            }
         }
+        if constexpr (Fm::kShared) __syncthreads();
         const int vis_min = U.q.pos + tok0 + 1;
 
         // pages of the wave's sub-tiles i, i + 1, .. i + 63: lane j holds where the halves of
@@ -310,61 +372,67 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(eakvd_geom geo, P
         int pg_a = -1, pg_b = -1;
         auto pages = [&](int i) __attribute__((always_inline)) {
             const int t = min(lo + 32 * (w + kWaves * (i + lane)), hi - 1) & ~31;
-            const int at[2] = {t, min(t + 16, (hi - 1) & ~15)};
-            pg_a = place_of(table, at[0], J.log2p, J.n_pages);
-            pg_b = place_of(table, at[1], J.log2p, J.n_pages);
+            pg_a = place_of(table, t, J.log2p, J.n_pages);
+            pg_b = place_of(table, min(t + 16, (hi - 1) & ~15), J.log2p, J.n_pages);
         };
-        auto load = [&](int i, Stage &st) __attribute__((always_inline)) {
+        // sub-tile i (the last one again behind it): K, the scales; then V.  A half's bytes by
+        // buffers of its own: pages are anywhere in the plane.
+        constexpr int aux = NR == 1 ? 2 : 0;                     // (read once, or again by other rows)
+        auto load = [&](int i, Stage<GPD> &st) __attribute__((always_inline)) {
             i = min(i, n_i - 1);
-            const int pa = __builtin_amdgcn_readlane(pg_a, i & 63), pb2 = __builtin_amdgcn_readlane(pg_b, i & 63);
-            st.at_a = pa;
-            st.at_b = pb2;
-            const int64_t a = max(pa, 0), b = max(pb2, 0);
-            uint8_t *slot = S.v[0] + (i % kAhead) * (32 * RB);
+            st.at_a = __builtin_amdgcn_readlane(pg_a, i & 63);
+            st.at_b = __builtin_amdgcn_readlane(pg_b, i & 63);
+            const int a = max(st.at_a, 0), b = max(st.at_b, 0);
 #pragma unroll
-            for (int j = 0; j < NV; j++) {
-                // d = 64: one load of both halves
-                const int t = vt + (NV == 2 ? 16 * j : 0);
-                const uint32_t off = (vt & 15) * RB + 16 * ((lane % UPT) ^ unit_swz<GPD>(t));
-                const uint8_t *p = NV == 2 ? vw + (j ? b : a) * RB : vw + (vt < 16 ? a : b) * RB;
-                __builtin_amdgcn_global_load_lds((glb_v)(p + off), (lds_v)(slot + 1024 * j), 16, 0, 2);
-            }
+            for (int k = 0; k < 2; k++) {
+                const auto r = rsrc(kw + (int64_t)(k ? b : a) * RB, 16 * RB);
 #pragma unroll
-            for (int g = 0; g < GPD; g++) {
-                typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-                const u2 ya = __builtin_nontemporal_load((const u2 *)(kw + a * RB + (ok + 32 * g)));
-                const u2 yb = __builtin_nontemporal_load((const u2 *)(kw + b * RB + (ok + 32 * g)));
-                st.k[0][g] = uint2{ya[0], ya[1]};
-                st.k[1][g] = uint2{yb[0], yb[1]};
+                for (int g = 0; g < GPD; g++) {
+                    const auto y = __builtin_amdgcn_raw_buffer_load_b64(r, ok + 32 * g, 0, aux);
+                    st.k[k][g] = uint2{y[0], y[1]};
+                }
             }
-            const uint32_t gi = (uint32_t)((n32 < 16 ? (int)a : (int)b) + (n32 & 15)) * GPD + gh;
-            st.ks = __builtin_nontemporal_load(ks + gi);
-            st.kb = __builtin_nontemporal_load(kb + gi);
-            st.vs = __builtin_nontemporal_load(vs + gi);
-            st.vb = __builtin_nontemporal_load(vb + gi);
+            const uint32_t at = (uint32_t)((n32 < 16 ? a : b) + (n32 & 15)) * (4 * GPD) + 4 * gh;
+            st.ks = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rks, at, 0, aux));
+            st.kb = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rkb, at, 0, aux));
+            st.vs = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rvs, at, 0, aux));
+            st.vb = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rvb, at, 0, aux));
+        };
+        auto load_v = [&](Stage<GPD> &st) __attribute__((always_inline)) {
+            const int a = max(st.at_a, 0), b = max(st.at_b, 0);
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const auto r = rsrc(vw + (int64_t)(k ? b : a) * RB, 16 * RB);
+                if constexpr (GPD == 2) {
+                    const auto y = __builtin_amdgcn_raw_buffer_load_b128(r, 16 * lane, 0, aux);
+                    st.v[k][0] = y[0], st.v[k][1] = y[1], st.v[k][GPD] = y[2], st.v[k][2 * GPD - 1] = y[3];
+                } else {
+                    const auto y = __builtin_amdgcn_raw_buffer_load_b64(r, 8 * lane, 0, aux);
+                    st.v[k][0] = y[0], st.v[k][1] = y[1];
+                }
+            }
         };
 
-        v4f O[NR][NF], C[NR][F32 ? 1 : GPD];
+        v4f O[NR][NF], C[NR][NC];
         float M[NR], L[NR], cs[NR][F32 ? GPD : 1];
-        uint32_t poison[NR];
+        uint32_t poison = 0;                                     // two bits of each row tile: NaN groups
 #pragma unroll
         for (int u = 0; u < NR; u++) {
 #pragma unroll
             for (int f = 0; f < NF; f++) O[u][f] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int g = 0; g < (F32 ? 1 : GPD); g++) C[u][g] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int g = 0; g < NC; g++) C[u][g] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int g = 0; g < (F32 ? GPD : 1); g++) cs[u][g] = 0.0f;
             M[u] = kMInit;
             L[u] = 0.0f;
-            poison[u] = 0;
         }
 
-        auto consume = [&](int i, const Stage &st) __attribute__((always_inline)) {
+        auto consume = [&](int i, Stage<GPD> &st) __attribute__((always_inline)) {
             const int t0 = lo + 32 * (w + kWaves * i);
-            const bool half_ok = n32 < 16 ? st.at_a >= 0 : st.at_b >= 0;
+            const bool ok_a = st.at_a >= 0, ok_b = st.at_b >= 0;
             // tokens behind the last, or in no page, have no part in this
-            const bool live = t0 + n32 < hi && half_ok;
+            const bool live = t0 + n32 < hi && (n32 < 16 ? ok_a : ok_b);
             const float zk = F32 ? zero_nibble(st.ks, st.kb) : 0.0f;
             const float ck = (F32 ? fmaf(zk, st.ks, st.kb) : st.kb) * J.ksc;
             // (a non-finite group counts as zeros and makes the rows that see it NaN)
@@ -379,63 +447,95 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(eakvd_geom geo, P
             S.w[n32] = scale2(1.0f, -ev);
             if (owner) {
                 S.ks[gh][n32] = st.ks * (F32 ? J.ksc : J.ksc * 0x1p24f);
-                S.vs[gh][n32] = scale2(sv, -ev);
-                S.zn[gh][pb][pos] = (_Float16)(F32 ? -1024.0f - zv : -zv * kZUp);
-                if constexpr (F32) {
-                    S.c16[gh][pb][pos] = (_Float16)(-64.0f - zv);
-                    S.vc[gh][n32] = scale2(cv, -ev);
-                    S.zk[gh][n32] = zk;
+                S.z0[gh][pb][pos] = (_Float16)(kSub ? -zv * kZUp : -1024.0f - zv);
+                S.z1[gh][pb][pos] = (_Float16)(kSub ? scale2(cv, 11 - ev) : -64.0f - zv);
+                if constexpr (kValues) {
+                    S.s16[kValues ? gh : 0][pb][pos] = (_Float16)scale2(sv, 15 - ev);
+                    S.c16[kValues ? gh : 0][pb][pos] = (_Float16)scale2(cv, 15 - ev);
                 } else {
-                    S.c16[gh][pb][pos] = (_Float16)scale2(cv, 11 - ev);
+                    S.vs[kValues ? 0 : gh][n32] = scale2(sv, -ev);
+                }
+                if constexpr (F32) {
+                    S.vc[F32 ? gh : 0][n32] = scale2(cv, -ev);
+                    S.zk[F32 ? gh : 0][n32] = zk;
                 }
             }
             b8 bias[2];
             bias_operands(owner ? ck : 0.0f, (float)ev, h == 0, bias, n32);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            // V's bytes through LDS, transposed
+            v2i vx[GPD][2];
+            auto turn_v = [&]() __attribute__((always_inline)) {
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    if constexpr (GPD == 2)
+                        *(uint4 *)(S.v + vwr[k]) = uint4{st.v[k][0], st.v[k][1], st.v[k][GPD], st.v[k][2 * GPD - 1]};
+                    else
+                        *(uint2 *)(S.v + vwr[k]) = uint2{st.v[k][0], st.v[k][1]};
+                }
+#pragma unroll
+                for (int g = 0; g < GPD; g++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++)
+                        vx[g][c] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i)(S.v + vrd[g][c]));
+            };
+            if constexpr (NR == 1) turn_v();
+            // ---- the next sub-tile
+            __builtin_amdgcn_sched_barrier(0);
+            if (((i + 1) & 63) == 0 && i + 1 < n_i) pages(i + 1);
+            uint2 kx[2][GPD];
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int g = 0; g < GPD; g++) kx[k][g] = st.k[k][g];
+            load(i + 1, st);
+            if constexpr (NR == 1) load_v(st);
+            __builtin_amdgcn_sched_barrier(0);
             // ---- K's operands
             h8 kl[2][GPD], kh[2][GPD];
 #pragma unroll
             for (int k = 0; k < 2; k++)
 #pragma unroll
                 for (int g = 0; g < GPD; g++)
-                    k_operands<!F32>(st.k[k][g], F32 ? S.zk[F32 ? g : 0][16 * k + n16] : 0.0f, nc, kl[k][g], kh[k][g]);
-            // ---- V's bytes, transposed (their loads are done: K's of the same sub-tile,
-            // issued behind them, are)
-            v2i vx[GPD][2];
-            const uint8_t *slot = S.v[0] + (i % kAhead) * (32 * RB);
-#pragma unroll
-            for (int g = 0; g < GPD; g++)
-#pragma unroll
-                for (int c = 0; c < 2; c++)
-                    vx[g][c] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i)(slot + vrd[g][c]));
-            const bool masked = t0 + 32 > vis_min || st.at_a < 0 || st.at_b < 0;
-            h8 X[NR][NP][GPD], P[F32 ? 1 : NR];
+                    k_operands<!F32>(kx[k][g], F32 ? S.zk[F32 ? g : 0][16 * k + n16] : 0.0f, nc, kl[k][g], kh[k][g]);
+            const bool masked = t0 + 32 > vis_min || !ok_a || !ok_b;
+            h8 X[kValues ? 1 : NR][NP][GPD], P[F32 ? 1 : NR];
 #pragma unroll
             for (int u = 0; u < NR; u++) {
                 if (u > 0 && 16 * u >= rows) break;
+                if constexpr (NR > 1) __builtin_amdgcn_sched_barrier(0);
                 // ---- scores
+                auto &q = Q[Fm::kShared ? 0 : u];
+                if constexpr (Fm::kShared) {
+#pragma unroll
+                    for (int f = 0; f < D / 32; f++) {
+                        q.a[f] = __builtin_bit_cast(h8, R.q[u][f][lane]);
+                        if constexpr (F32) q.b[F32 ? f : 0] = __builtin_bit_cast(h8, R.q[u][D / 32 + (F32 ? f : 0)][lane]);
+                    }
+                    q.bias = __builtin_bit_cast(b8, R.q[u][Fm::NQ - 1][lane]);
+                }
+                const float rf = Fm::kShared ? R.rf[u][n16] : rf1;
                 v4f s[2];
 #pragma unroll
                 for (int k = 0; k < 2; k++)
-                    s[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bias[k], Q[u].bias, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0,
-                                                                   0, 0);
+                    s[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bias[k], q.bias, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
 #pragma unroll
                 for (int g = 0; g < GPD; g++)
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
-                        const v4f acc = group_dots(kl[k][g], kh[k][g], Q[u], g);
+                        const v4f acc = group_dots(kl[k][g], kh[k][g], q, g);
                         const v4f sc = *(const v4f *)&S.ks[g][16 * k + 4 * blk];
 #pragma unroll
                         for (int e = 0; e < 4; e++) s[k][e] = fmaf(sc[e], acc[e], s[k][e]);
                     }
                 // ---- softmax
                 if (masked) {
+                    const int n = (Fm::kShared ? R.vis[u][n16] : vis1) - t0 - 4 * blk;
 #pragma unroll
                     for (int k = 0; k < 2; k++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            const int t = t0 + 16 * k + 4 * blk + e;
-                            const bool see = t < vis[u] && (k ? st.at_b : st.at_a) >= 0;
+                            const bool see = 16 * k + e < n && (k ? ok_b : ok_a);
                             s[k][e] = see ? s[k][e] : -__builtin_inff();
                         }
                 }
@@ -448,12 +548,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(eakvd_geom geo, P
                         for (int e = 0; e < 4; e++)
                             seen |= s[k][e] != -__builtin_inff() ? 1u << (16 * k + e) : 0u;
                     seen <<= 4 * blk;
-                    poison[u] |= (seen & (uint32_t)bad ? 1u : 0u) |
-                                 (GPD == 2 && (seen & (uint32_t)(bad >> 32)) ? 2u : 0u);
+                    poison |= (seen & (uint32_t)bad ? 1u << 2 * u : 0u) |
+                              (GPD == 2 && (seen & (uint32_t)(bad >> 32)) ? 2u << 2 * u : 0u);
                 }
                 const float top = row_max(fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                                                 fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))));
-                const float need = fmaf(top, Q[u].rf, -kWinTop);
+                const float need = fmaf(top, rf, -kWinTop);
                 if (__ballot(need > M[u] + kWinTau) != 0) {
                     const float mn = need > M[u] + kWinTau ? need : M[u], d = M[u] - mn;
                     // (L by halves, as in window.h)
@@ -463,10 +563,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(eakvd_geom geo, P
                     for (int f = 0; f < NF; f++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) O[u][f][e] *= al;
+                    if constexpr (kSub)
 #pragma unroll
-                    for (int g = 0; g < (F32 ? 1 : GPD); g++)
+                        for (int g = 0; g < NC; g++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) C[u][g][e] *= al;
+                            for (int e = 0; e < 4; e++) C[u][g][e] *= al;
                     if constexpr (F32)
 #pragma unroll
                         for (int g = 0; g < GPD; g++) cs[u][g] *= al;
@@ -475,7 +576,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(eakvd_geom geo, P
                 float p[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++)
-                    p[j] = __builtin_amdgcn_exp2f(fmaf(s[j >> 2][j & 3], Q[u].rf, -M[u]));
+                    p[j] = __builtin_amdgcn_exp2f(fmaf(s[j >> 2][j & 3], rf, -M[u]));
                 float ls = 0.0f;
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
@@ -485,61 +586,85 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(eakvd_geom geo, P
                 }
                 L[u] += ls;
                 // ---- weights as operands
+                if constexpr (!kValues)
 #pragma unroll
-                for (int g = 0; g < GPD; g++) {
-                    uint32_t xh[4], xl[4];
-                    float c = 0.0f;
+                    for (int g = 0; g < GPD; g++) {
+                        uint32_t xh[4], xl[4];
+                        float c = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const v4f sc = *(const v4f *)&S.vs[g][16 * k + 4 * blk];
-                        float y[4];
+                        for (int k = 0; k < 2; k++) {
+                            const v4f sc = *(const v4f *)&S.vs[kValues ? 0 : g][16 * k + 4 * blk];
+                            float y[4];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) y[e] = p[4 * k + e] * sc[e];
+                            for (int e = 0; e < 4; e++) y[e] = p[4 * k + e] * sc[e];
+                            if constexpr (F32) {
+                                const v4f cc = *(const v4f *)&S.vc[F32 ? g : 0][16 * k + 4 * blk];
+#pragma unroll
+                                for (int e = 0; e < 4; e++) c = fmaf(p[4 * k + e], cc[e], c);
+                            }
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                const h2 hi2 = pk(y[e], y[e + 2]);
+                                xh[2 * k + e] = u_of(hi2);
+                                if constexpr (F32) xl[2 * k + e] = u_of(pk_rest(hi2, y[e], y[e + 2]));
+                            }
+                        }
+                        X[kValues ? 0 : u][0][g] = __builtin_bit_cast(h8, uint4{xh[0], xh[1], xh[2], xh[3]});
                         if constexpr (F32) {
-                            const v4f cc = *(const v4f *)&S.vc[g][16 * k + 4 * blk];
-#pragma unroll
-                            for (int e = 0; e < 4; e++) c = fmaf(p[4 * k + e], cc[e], c);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const h2 hi2 = pk(y[e], y[e + 2]);
-                            xh[2 * k + e] = u_of(hi2);
-                            if constexpr (F32) xl[2 * k + e] = u_of(pk_rest(hi2, y[e], y[e + 2]));
+                            X[kValues ? 0 : u][NP - 1][g] = __builtin_bit_cast(h8, uint4{xl[0], xl[1], xl[2], xl[3]});
+                            cs[u][F32 ? g : 0] += c;
                         }
                     }
-                    X[u][0][g] = __builtin_bit_cast(h8, uint4{xh[0], xh[1], xh[2], xh[3]});
-                    if constexpr (F32) {
-                        X[u][NP - 1][g] = __builtin_bit_cast(h8, uint4{xl[0], xl[1], xl[2], xl[3]});
-                        cs[u][F32 ? g : 0] += c;
-                    }
-                }
                 if constexpr (!F32)
                     P[F32 ? 0 : u] = __builtin_bit_cast(h8, uint4{u_of(pk_exp(p[0], p[2])), u_of(pk_exp(p[1], p[3])),
                                                                   u_of(pk_exp(p[4], p[6])), u_of(pk_exp(p[5], p[7]))});
             }
+            if constexpr (NR > 1) {
+                __builtin_amdgcn_sched_barrier(0);
+                turn_v();
+                load_v(st);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             // ---- weighted sums
 #pragma unroll
             for (int g = 0; g < GPD; g++) {
-                const uint4 zn = *(const uint4 *)S.zn[g][blk], c8 = *(const uint4 *)S.c16[g][blk];
-                const uint32_t zs[4] = {zn.x, zn.y, zn.z, zn.w}, cz[4] = {c8.x, c8.y, c8.z, c8.w};
-                if constexpr (!F32) {
+                if constexpr (NR > 1) __builtin_amdgcn_sched_barrier(0);
+                const uint4 z0 = *(const uint4 *)S.z0[g][blk], z1 = *(const uint4 *)S.z1[g][blk];
+                const uint32_t zl[4] = {z0.x, z0.y, z0.z, z0.w}, zh[4] = {z1.x, z1.y, z1.z, z1.w};
+                uint32_t ss[4], cc[4];
+                if constexpr (kValues) {
+                    const uint4 a = *(const uint4 *)S.s16[kValues ? g : 0][blk], b = *(const uint4 *)S.c16[kValues ? g : 0][blk];
+                    ss[0] = a.x, ss[1] = a.y, ss[2] = a.z, ss[3] = a.w;
+                    cc[0] = b.x, cc[1] = b.y, cc[2] = b.z, cc[3] = b.w;
+                }
+                if constexpr (kSub) {
 #pragma unroll
                     for (int u = 0; u < NR; u++) {
                         if (u > 0 && 16 * u >= rows) break;
-                        C[u][F32 ? 0 : g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            __builtin_bit_cast(h8, zn), X[u][0][g], C[u][F32 ? 0 : g], 0, 0, 0);
-                        C[u][F32 ? 0 : g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            __builtin_bit_cast(h8, c8), P[F32 ? 0 : u], C[u][F32 ? 0 : g], 0, 0, 0);
+                        v4f &c = C[u][kSub ? g : 0];
+                        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, z0), X[kValues ? 0 : u][0][g], c, 0, 0, 0);
+                        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, z1), P[F32 ? 0 : u], c, 0, 0, 0);
                     }
                 }
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
+                    if constexpr (NR > 1) __builtin_amdgcn_sched_barrier(0);
                     uint32_t a[4], b[4];
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
                         const uint32_t y = (uint32_t)vx[g][c][k >> 1] >> (8 * (k & 1));
-                        a[k] = F32 ? u_of(nib2<false>(y, h_of(zs[k]), nc)) : nib_sub<false>(y);
-                        b[k] = F32 ? u_of(nib2<true>(y, h_of(cz[k]), nc)) : nib_sub<true>(y);
+                        if constexpr (kSub) {
+                            a[k] = nib_sub<false>(y);
+                            b[k] = nib_sub<true>(y);
+                        } else {
+                            h2 lo2 = nib2<false>(y, h_of(zl[k]), nc), hi2 = nib2<true>(y, h_of(zh[k]), nc);
+                            if constexpr (kValues) {
+                                lo2 = __builtin_elementwise_fma(lo2, h_of(ss[k]), h_of(cc[k]));
+                                hi2 = __builtin_elementwise_fma(hi2, h_of(ss[k]), h_of(cc[k]));
+                            }
+                            a[k] = u_of(lo2);
+                            b[k] = u_of(hi2);
+                        }
                     }
                     const h8 vl = __builtin_bit_cast(h8, uint4{a[0], a[1], a[2], a[3]});
                     const h8 vh = __builtin_bit_cast(h8, uint4{b[0], b[1], b[2], b[3]});
@@ -549,8 +674,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(eakvd_geom geo, P
                         const int f = 4 * g + 2 * c;
 #pragma unroll
                         for (int k = NP - 1; k >= 0; k--) {
-                            O[u][f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, X[u][k][g], O[u][f], 0, 0, 0);
-                            O[u][f + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, X[u][k][g], O[u][f + 1], 0, 0, 0);
+                            const h8 &y = kValues ? P[F32 ? 0 : u] : X[kValues ? 0 : u][kValues ? 0 : k][kValues ? 0 : g];
+                            O[u][f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, y, O[u][f], 0, 0, 0);
+                            O[u][f + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, y, O[u][f + 1], 0, 0, 0);
                         }
                     }
                 }
@@ -559,38 +685,24 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(eakvd_geom geo, P
         };
 
         if (n_i > 0) {
-            Stage st[kAhead];
             pages(0);
-#pragma unroll
-            for (int k = 0; k < kAhead - 1; k++) load(k, st[k]);
-            for (int i = 0; i < n_i; i += kAhead) {
-#pragma unroll
-                for (int k = 0; k < kAhead; k++) {
-                    if (i + k >= n_i) break;
-                    const int next = i + k + kAhead - 1;
-                    if ((next & 63) == 0 && next < n_i) pages(next);
-                    load(next, st[(k + kAhead - 1) % kAhead]);
-                    __builtin_amdgcn_sched_barrier(0);
-                    // all loads but those of the sub-tiles behind this one
-                    wait_loads<(kAhead - 1) * kLoads>();
-                    __builtin_amdgcn_sched_barrier(0);
-                    consume(i + k, st[k]);
-                }
-            }
-            wait_loads<0>();
+            Stage<GPD> st;
+            load(0, st);
+            load_v(st);
+            for (int i = 0; i < n_i; i++) consume(i, st);
         }
 
         // ---- the waves joined, 16 rows at a time
         float *jo = (float *)lds;                                // [wave][NF][64][4]
         float2 *jml = (float2 *)(lds + (size_t)kWaves * NF * 64 * 16);   // [wave][16]
         const int slot = 2 * bl + (U.at == 0 ? 1 : 0);
+        poison |= __shfl_xor(poison, 16, 64);
+        poison |= __shfl_xor(poison, 32, 64);
 #pragma unroll
         for (int u = 0; u < NR; u++) {
             if (u > 0 && 16 * u >= rows) break;
             // a lane has its row's sums of its own tokens only
             const float l = row_sum(L[u]);
-            poison[u] |= __shfl_xor(poison[u], 16, 64);
-            poison[u] |= __shfl_xor(poison[u], 32, 64);
             __syncthreads();
 #pragma unroll
             for (int g = 0; g < GPD; g++) {
@@ -602,9 +714,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(eakvd_geom geo, P
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         o[e] = F32 ? O[u][f][e] + c
-                                   : fmaf(O[u][f][e], k & 1 ? 0x1p20f : 0x1p24f,
-                                          C[u][F32 ? 0 : g][e] * (1.0f / kZUp));
-                        if (poison[u] >> g & 1) o[e] = __builtin_nanf("");
+                               : kValues ? O[u][f][e] * 0x1p-15f
+                                         : fmaf(O[u][f][e], k & 1 ? 0x1p20f : 0x1p24f,
+                                                C[u][kSub ? g : 0][e] * (1.0f / kZUp));
+                        if (poison >> (2 * u + g) & 1) o[e] = __builtin_nanf("");
                     }
                     *((v4f *)jo + (w * NF + f) * 64 + lane) = o;
                 }
@@ -624,19 +737,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_kernel(eakvd_geom geo, P
                 ll = fmaf(half * jml[k * 16 + n16].y, half, ll);
             }
             const bool row_ok = 16 * u + n16 < rows;
-            if (w < NF) {
+            for (int f = w; f < NF; f += kWaves) {
                 v4f y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int k = 0; k < kWaves; k++) {
-                    const v4f o = *((const v4f *)jo + (k * NF + w) * 64 + lane);
+                    const v4f o = *((const v4f *)jo + (k * NF + f) * 64 + lane);
 #pragma unroll
                     for (int e = 0; e < 4; e++) y[e] = fmaf(al[k], o[e], y[e]);
                 }
-                const int dim = (w >> 2) * 64 + (w & 1) * 32 + ((w >> 1) & 1) * 16 + 4 * blk;
+                const int dim = (f >> 2) * 64 + (f & 1) * 32 + ((f >> 1) & 1) * 16 + 4 * blk;
                 if (row_ok && whole) {
                     const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
                     const float o4[4] = {y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv};
-                    store4<F32>(J.out, orow[u] + dim, J.vec & 2, o4);
+                    int t, hd;
+                    row_at(u, t, hd);
+                    store4<F32>(J.out, (int64_t)(U.q.row + tok0 + t) * J.ld_out + (int64_t)(head0 + hd) * D + dim,
+                                J.vec & 2, o4);
                 } else if (row_ok) {
                     *(v4f *)(J.part + ((int64_t)slot * J.rbr + 16 * u + n16) * D + dim) = y;
                 }
@@ -698,12 +814,13 @@ struct PagedPlan {
     size_t part, bytes;
 };
 
-// 16 rows to a unit where no sequence has more, else 32.
-PagedPlan paged_plan(const eakvd_geom *g, const eakvd_pages *b, int n_q, int n_kv)
+// 16 rows to a unit where no sequence has more, else 32, and 64 for bf16 beyond 32.
+PagedPlan paged_plan(const eakvd_geom *g, const eakvd_pages *b, int n_q, int n_kv, bool bf16)
 {
     PagedPlan p;
     const int qpk = n_q / n_kv;
-    p.nr = (int64_t)b->max_new * qpk <= 16 ? 1 : 2;
+    const int64_t rows = (int64_t)b->max_new * qpk;
+    p.nr = rows <= 16 ? 1 : rows <= 32 || !bf16 ? 2 : g->head_dim == 64 ? 4 : 3;
     const int rbr = 16 * p.nr, tb = qpk < rbr ? rbr / qpk : 1, hb = (qpk + rbr - 1) / rbr;
     // units at most
     const int64_t units = (b->n_new / tb + (int64_t)(b->n_seqs < b->n_new ? b->n_seqs : b->n_new)) *
@@ -711,8 +828,8 @@ PagedPlan paged_plan(const eakvd_geom *g, const eakvd_pages *b, int n_q, int n_k
     const int64_t tiles = (b->max_len + kTile - 1) / kTile;
     // (two tiles stay together: the joining launch costs more)
     p.whole = tiles <= 2;
-    const int64_t most = units * (p.whole ? 1 : tiles > 1 ? tiles : 1), cus = cu_count();
-    p.grid = (int)(most < cus ? most : cus);
+    const int64_t most = units * (p.whole ? 1 : tiles > 1 ? tiles : 1), slots = (p.nr == 1 ? 3 : 1) * cu_count();
+    p.grid = (int)(most < slots ? most : slots);
     p.part = ((size_t)p.grid * 2 * rbr * (g->head_dim + 2) * sizeof(float) + 255) & ~(size_t)255;
     p.bytes = p.whole ? 0 : p.part + (size_t)p.grid * sizeof(PagedCut);
     return p;
@@ -721,16 +838,14 @@ PagedPlan paged_plan(const eakvd_geom *g, const eakvd_pages *b, int n_q, int n_k
 template <int D, bool F32, int NR>
 int launch(const eakvd_geom &g, PagedJob &J, const PagedPlan &p, hipStream_t st)
 {
-    constexpr size_t tiles = kWaves * sizeof(PagedLds<D, F32>);
-    constexpr size_t join = (size_t)kWaves * (D / 16) * 64 * 16 + kWaves * 16 * sizeof(float2);
-    constexpr size_t line = tiles > join ? tiles : join;
-    static_assert(line + (EAKVD_PAGED_SEQS + 1) * 4 <= 160 * 1024, "LDS");
+    typedef Form<D, F32, NR> Fm;
+    static_assert(Fm::kLine + (EAKVD_PAGED_SEQS + 1) * 4 <= 160 * 1024, "LDS");
     auto *kern = paged_kernel<D, F32, NR>;
     static std::atomic<uint64_t> done;
-    const int e = allow_lds((const void *)kern, line + (EAKVD_PAGED_SEQS + 1) * 4, done);
+    const int e = allow_lds((const void *)kern, Fm::kLine + (EAKVD_PAGED_SEQS + 1) * 4, done);
     if (e) return e;
-    hipLaunchKernelGGL(kern, dim3((unsigned)p.grid), dim3(64 * kWaves), line + (J.b.n_seqs + 1) * 4, st, g,
-                       J, (int)line);
+    hipLaunchKernelGGL(kern, dim3((unsigned)p.grid), dim3(64 * Fm::kWaves), Fm::kLine + (J.b.n_seqs + 1) * 4, st, g,
+                       J);
     if (!p.whole)
         hipLaunchKernelGGL((paged_join_kernel<D, F32>), dim3((unsigned)p.grid, NR), dim3(D * 4), 0, st, J,
                            p.grid);
@@ -739,16 +854,16 @@ int launch(const eakvd_geom &g, PagedJob &J, const PagedPlan &p, hipStream_t st)
 
 }  // namespace
 
-extern "C" size_t eakvd_paged_work_bytes(const eakvd_geom *g, const eakvd_pages *b, int n_q, int n_kv)
+extern "C" size_t eakvd_paged_work_bytes(const eakvd_geom *g, const eakvd_pages *b, int n_q, int n_kv, int bf16)
 {
-    return paged_plan(g, b, n_q, n_kv).bytes;
+    return paged_plan(g, b, n_q, n_kv, bf16).bytes;
 }
 
 extern "C" int eakvd_paged_attend(const eakvd_geom *g, const uint8_t *base, const eakvd_pages *b,
                                   int layer, const void *q, int64_t ld_q, int bf16, int n_q, int n_kv,
                                   void *out, int64_t ld_out, void *work, void *stream)
 {
-    const PagedPlan p = paged_plan(g, b, n_q, n_kv);
+    const PagedPlan p = paged_plan(g, b, n_q, n_kv, bf16);
     if (p.grid == 0) return 0;
     PagedJob J;
     memset(&J, 0, sizeof(J));
@@ -776,10 +891,12 @@ extern "C" int eakvd_paged_attend(const eakvd_geom *g, const uint8_t *base, cons
     J.part = (float *)work;
     J.cut = (PagedCut *)((uint8_t *)work + p.part);
     const hipStream_t st = (hipStream_t)stream;
-    if (g->head_dim == 64) {
-        if (bf16) return p.nr == 1 ? launch<64, false, 1>(*g, J, p, st) : launch<64, false, 2>(*g, J, p, st);
-        return p.nr == 1 ? launch<64, true, 1>(*g, J, p, st) : launch<64, true, 2>(*g, J, p, st);
-    }
-    if (bf16) return p.nr == 1 ? launch<128, false, 1>(*g, J, p, st) : launch<128, false, 2>(*g, J, p, st);
-    return p.nr == 1 ? launch<128, true, 1>(*g, J, p, st) : launch<128, true, 2>(*g, J, p, st);
+    auto run = [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        if (!bf16) return p.nr == 1 ? launch<D, true, 1>(*g, J, p, st) : launch<D, true, 2>(*g, J, p, st);
+        return p.nr == 1   ? launch<D, false, 1>(*g, J, p, st)
+               : p.nr == 2 ? launch<D, false, 2>(*g, J, p, st)
+                           : launch<D, false, D == 64 ? 4 : 3>(*g, J, p, st);
+    };
+    return g->head_dim == 64 ? run(std::integral_constant<int, 64>()) : run(std::integral_constant<int, 128>());
 }

@@ -123,7 +123,7 @@ size_t eakv_attention_paged_work_bytes(const eakv_cache_t *pool, const eakv_page
         return 0;
     int prev;
     if (eakvi_enter(pool, &prev)) return 0;
-    const size_t need = eakvd_paged_work_bytes(&pool->geom, &d, n_q, n_kv);
+    const size_t need = eakvd_paged_work_bytes(&pool->geom, &d, n_q, n_kv, dtype == EAKV_BF16);
     eakvi_leave(prev);
     return need;
 }
@@ -149,7 +149,7 @@ int eakv_attention_paged_device(const eakv_cache_t *cpool, const eakv_paged_batc
     int prev;
     rc = eakvi_enter(pool, &prev);
     if (rc) return rc;
-    const size_t need = eakvd_paged_work_bytes(&pool->geom, &d, n_q, n_kv);
+    const size_t need = eakvd_paged_work_bytes(&pool->geom, &d, n_q, n_kv, dtype == EAKV_BF16);
     const size_t size = dtype == EAKV_F32 ? 4 : 2;
     const int own = !d_work && need;
     const eakvi_span q = {d_q, rows_bytes(d.n_new, ld_q, width, size)},
