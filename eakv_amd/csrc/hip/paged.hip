@@ -42,6 +42,13 @@
 namespace {
 
 constexpr int kTile = 256;              // tokens of a tile
+// M's distance from the maximum when it is set, and the headroom of a lazy M (log2 units): weights
+// stay below 2^15.  A small distance moves M less often (every move scales O); weights keep f16's
+// precision down to 2^-18 (f32: of their pairs, 2^-21) of the largest, and 2^-29 (2^-32) of it below.
+template <bool F32>
+constexpr float kTop = F32 ? 7.0f : 4.0f;
+template <bool F32>
+constexpr float kTau = F32 ? 8.0f : 11.0f;
 // -z is held 2^11 times (30720 at most), as c with it, which f16 then holds to 2^-25
 constexpr float kZUp = 0x1p11f;
 
@@ -428,7 +435,9 @@ __global__ __launch_bounds__(64 * kWavesOf<NR>, NR > 1 ? 2 : 3) void paged_kerne
             L[u] = 0.0f;
         }
 
-        auto consume = [&](int i, Stage<GPD> &st) __attribute__((always_inline)) {
+        // N: row tiles that the unit has (1, or NR)
+        auto consume = [&](auto count, int i, Stage<GPD> &st) __attribute__((always_inline)) {
+            constexpr int N = decltype(count)::value;
             const int t0 = lo + 32 * (w + kWaves * i);
             const bool ok_a = st.at_a >= 0, ok_b = st.at_b >= 0;
             // tokens behind the last, or in no page, have no part in this
@@ -499,14 +508,13 @@ __global__ __launch_bounds__(64 * kWavesOf<NR>, NR > 1 ? 2 : 3) void paged_kerne
                 for (int g = 0; g < GPD; g++)
                     k_operands<!F32>(kx[k][g], F32 ? S.zk[F32 ? g : 0][16 * k + n16] : 0.0f, nc, kl[k][g], kh[k][g]);
             const bool masked = t0 + 32 > vis_min || !ok_a || !ok_b;
-            h8 X[kValues ? 1 : NR][NP][GPD], P[F32 ? 1 : NR];
+            // ---- scores
+            float s[N][8];
 #pragma unroll
-            for (int u = 0; u < NR; u++) {
-                if (u > 0 && 16 * u >= rows) break;
-                if constexpr (NR > 1) __builtin_amdgcn_sched_barrier(0);
-                // ---- scores
-                auto &q = Q[Fm::kShared ? 0 : u];
+            for (int u = 0; u < N; u++) {
+                auto &q = Q[0];
                 if constexpr (Fm::kShared) {
+                    if constexpr (N > 1) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int f = 0; f < D / 32; f++) {
                         q.a[f] = __builtin_bit_cast(h8, R.q[u][f][lane]);
@@ -514,11 +522,10 @@ __global__ __launch_bounds__(64 * kWavesOf<NR>, NR > 1 ? 2 : 3) void paged_kerne
                     }
                     q.bias = __builtin_bit_cast(b8, R.q[u][Fm::NQ - 1][lane]);
                 }
-                const float rf = Fm::kShared ? R.rf[u][n16] : rf1;
-                v4f s[2];
+                v4f t[2];
 #pragma unroll
                 for (int k = 0; k < 2; k++)
-                    s[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bias[k], q.bias, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+                    t[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bias[k], q.bias, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
 #pragma unroll
                 for (int g = 0; g < GPD; g++)
 #pragma unroll
@@ -526,36 +533,52 @@ __global__ __launch_bounds__(64 * kWavesOf<NR>, NR > 1 ? 2 : 3) void paged_kerne
                         const v4f acc = group_dots(kl[k][g], kh[k][g], q, g);
                         const v4f sc = *(const v4f *)&S.ks[g][16 * k + 4 * blk];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) s[k][e] = fmaf(sc[e], acc[e], s[k][e]);
+                        for (int e = 0; e < 4; e++) t[k][e] = fmaf(sc[e], acc[e], t[k][e]);
                     }
-                // ---- softmax
-                if (masked) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) s[u][j] = t[j >> 2][j & 3];
+            }
+            if constexpr (N > 1) __builtin_amdgcn_sched_barrier(0);
+            // ---- softmax, all row tiles side by side
+            if (masked) {
+#pragma unroll
+                for (int u = 0; u < N; u++) {
                     const int n = (Fm::kShared ? R.vis[u][n16] : vis1) - t0 - 4 * blk;
 #pragma unroll
-                    for (int k = 0; k < 2; k++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const bool see = 16 * k + e < n && (k ? ok_b : ok_a);
-                            s[k][e] = see ? s[k][e] : -__builtin_inff();
-                        }
+                    for (int j = 0; j < 8; j++) {
+                        const bool see = 16 * (j >> 2) + (j & 3) < n && (j >> 2 ? ok_b : ok_a);
+                        s[u][j] = see ? s[u][j] : -__builtin_inff();
+                    }
                 }
-                if (bad) {
-                    // rows that see a token with a non-finite V group
+            }
+            if (bad) {
+                // rows that see a token with a non-finite V group
+#pragma unroll
+                for (int u = 0; u < N; u++) {
                     uint32_t seen = 0;
 #pragma unroll
-                    for (int k = 0; k < 2; k++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            seen |= s[k][e] != -__builtin_inff() ? 1u << (16 * k + e) : 0u;
+                    for (int j = 0; j < 8; j++)
+                        seen |= s[u][j] != -__builtin_inff() ? 1u << (16 * (j >> 2) + (j & 3)) : 0u;
                     seen <<= 4 * blk;
                     poison |= (seen & (uint32_t)bad ? 1u << 2 * u : 0u) |
                               (GPD == 2 && (seen & (uint32_t)(bad >> 32)) ? 2u << 2 * u : 0u);
                 }
-                const float top = row_max(fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                                                fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))));
-                const float need = fmaf(top, rf, -kWinTop);
-                if (__ballot(need > M[u] + kWinTau) != 0) {
-                    const float mn = need > M[u] + kWinTau ? need : M[u], d = M[u] - mn;
+            }
+            float rf[N], need[N];
+            bool move = false;
+#pragma unroll
+            for (int u = 0; u < N; u++) {
+                rf[u] = Fm::kShared ? R.rf[u][n16] : rf1;
+                const float top = row_max(max3(max3(max3(s[u][0], s[u][1], s[u][2]), s[u][3], s[u][4]),
+                                               max3(s[u][5], s[u][6], s[u][7]), s[u][7]));
+                need[u] = fmaf(top, rf[u], -kTop<F32>);
+                move |= need[u] > M[u] + kTau<F32>;
+            }
+            if (__ballot(move) != 0) {
+#pragma unroll
+                for (int u = 0; u < N; u++) {
+                    if (N > 1 && __ballot(need[u] > M[u] + kTau<F32>) == 0) continue;
+                    const float mn = need[u] > M[u] + kTau<F32> ? need[u] : M[u], d = M[u] - mn;
                     // (L by halves, as in window.h)
                     const float al = __builtin_amdgcn_exp2f(d), half = __builtin_amdgcn_exp2f(0.5f * d);
                     L[u] = L[u] * half * half;
@@ -573,19 +596,19 @@ __global__ __launch_bounds__(64 * kWavesOf<NR>, NR > 1 ? 2 : 3) void paged_kerne
                         for (int g = 0; g < GPD; g++) cs[u][g] *= al;
                     M[u] = mn;
                 }
+            }
+            h8 X[kValues ? 1 : N][NP][GPD], P[F32 ? 1 : N];
+            const v4f w0 = *(const v4f *)&S.w[4 * blk], w1 = *(const v4f *)&S.w[16 + 4 * blk];
+#pragma unroll
+            for (int u = 0; u < N; u++) {
                 float p[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-                    p[j] = __builtin_amdgcn_exp2f(fmaf(s[j >> 2][j & 3], rf, -M[u]));
+                for (int j = 0; j < 8; j++) p[j] = __builtin_amdgcn_exp2f(fmaf(s[u][j], rf[u], -M[u]));
                 float ls = 0.0f;
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const v4f w4 = *(const v4f *)&S.w[16 * k + 4 * blk];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) ls = fmaf(p[4 * k + e], w4[e], ls);
-                }
+                for (int j = 0; j < 8; j++) ls = fmaf(p[j], j < 4 ? w0[j & 3] : w1[j & 3], ls);
                 L[u] += ls;
-                // ---- weights as operands
+                // weights as operands
                 if constexpr (!kValues)
 #pragma unroll
                     for (int g = 0; g < GPD; g++) {
@@ -639,8 +662,7 @@ __global__ __launch_bounds__(64 * kWavesOf<NR>, NR > 1 ? 2 : 3) void paged_kerne
                 }
                 if constexpr (kSub) {
 #pragma unroll
-                    for (int u = 0; u < NR; u++) {
-                        if (u > 0 && 16 * u >= rows) break;
+                    for (int u = 0; u < N; u++) {
                         v4f &c = C[u][kSub ? g : 0];
                         c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, z0), X[kValues ? 0 : u][0][g], c, 0, 0, 0);
                         c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, z1), P[F32 ? 0 : u], c, 0, 0, 0);
@@ -669,8 +691,7 @@ __global__ __launch_bounds__(64 * kWavesOf<NR>, NR > 1 ? 2 : 3) void paged_kerne
                     const h8 vl = __builtin_bit_cast(h8, uint4{a[0], a[1], a[2], a[3]});
                     const h8 vh = __builtin_bit_cast(h8, uint4{b[0], b[1], b[2], b[3]});
 #pragma unroll
-                    for (int u = 0; u < NR; u++) {
-                        if (u > 0 && 16 * u >= rows) break;
+                    for (int u = 0; u < N; u++) {
                         const int f = 4 * g + 2 * c;
 #pragma unroll
                         for (int k = NP - 1; k >= 0; k--) {
@@ -689,7 +710,10 @@ __global__ __launch_bounds__(64 * kWavesOf<NR>, NR > 1 ? 2 : 3) void paged_kerne
             Stage<GPD> st;
             load(0, st);
             load_v(st);
-            for (int i = 0; i < n_i; i++) consume(i, st);
+            if (NR > 1 && rows > 16)
+                for (int i = 0; i < n_i; i++) consume(std::integral_constant<int, NR>(), i, st);
+            else
+                for (int i = 0; i < n_i; i++) consume(std::integral_constant<int, 1>(), i, st);
         }
 
         // ---- the waves joined, 16 rows at a time

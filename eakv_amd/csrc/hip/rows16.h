@@ -11,11 +11,20 @@
 
 namespace {
 
+// One instruction (the compiler puts another before each input that it cannot prove quiet).
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 // The maximum of a lane's value and those of the other three lanes of its row.
 __device__ __forceinline__ float row_max(float v)
 {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return half_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = max3(__uint_as_float(r[0]), __uint_as_float(r[1]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return max3(__uint_as_float(r[0]), __uint_as_float(r[1]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float row_sum(float v)
 {
