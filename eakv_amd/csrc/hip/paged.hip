@@ -41,6 +41,7 @@
 
 namespace {
 
+constexpr int kWaves = 4;
 constexpr int kTile = 256;              // tokens of a tile
 // M's distance from the maximum when it is set, and the headroom of a lazy M (log2 units): weights
 // stay below 2^15.  A small distance moves M less often (every move scales O); weights keep f16's
@@ -119,7 +120,6 @@ __device__ __forceinline__ int wave_scan_i(int v, int lane)
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // pre[s]: the line's length before sequence s, s <= n_seqs.  All threads of the block.
-template <int kWaves>
 __device__ __forceinline__ void line_of(const PagedJob &J, int *pre, int *sums, int tid)
 {
     const int lane = tid & 63, w = tid >> 6, n = J.b.n_seqs;
@@ -217,17 +217,13 @@ __device__ __forceinline__ int line_block(int b, int grid)
 }
 
 // What a variant of the kernel holds where.  NR row tiles of 16 share a wave's operands of K and V.
-// One (decode): queries in registers, 4 waves to a block and 3 to a SIMD.  More: queries in LDS,
-// which all 8 waves of the block share.  Four (bf16 alone): V's operands are its values in
+// One (decode): queries in registers, 3 blocks to a CU.  More: queries in LDS, which the waves of
+// the block share, 2 blocks to a CU, so that one computes while the other begins or ends a unit.  Four (bf16 alone): V's operands are its values in
 // f16, made once for 64 rows, and weights are operands as they stand (with the scales in the
 // weights each row tile takes 28 instructions more and V's operands 64 less).
-template <int NR>
-constexpr int kWavesOf = NR > 1 ? 8 : 4;
-
 template <int D, bool F32, int NR>
 struct Form {
     static constexpr int GPD = D / 64;
-    static constexpr int kWaves = kWavesOf<NR>;
     static constexpr bool kShared = NR > 1;             // queries in LDS
     static constexpr bool kValues = !F32 && NR > 2;    // V's operands are values
     static constexpr int NQ = D / 32 * (F32 ? 2 : 1) + 1;
@@ -250,7 +246,9 @@ struct Form {
         int vis[NR][16];
     };
     static constexpr size_t kWaveBytes = kWaves * sizeof(Wave);
-    static constexpr size_t kJoin = (size_t)kWaves * (D / 16) * 64 * 16 + kWaves * 16 * sizeof(float2);
+    static constexpr size_t kJoinRows = (size_t)kWaves * (D / 16) * 64 * 16;    // a row tile's sums
+    static constexpr int kBuffers = NR > 1 && D == 64 ? 2 : 1;  // (two at d = 128 and one block is all that fits)
+    static constexpr size_t kJoin = kBuffers * (kJoinRows + kWaves * 16 * sizeof(float2));
     static constexpr size_t kRows = kWaveBytes > kJoin ? kWaveBytes : kJoin;    // where the rows are
     static constexpr size_t kLine = kRows + (kShared ? sizeof(Rows) : 0);       // and the line
 };
@@ -271,11 +269,10 @@ __device__ __forceinline__ int unit_swz(int t)
 }
 
 template <int D, bool F32, int NR>
-__global__ __launch_bounds__(64 * kWavesOf<NR>, NR > 1 ? 2 : 3) void paged_kernel(eakvd_geom geo, PagedJob J)
+__global__ __launch_bounds__(64 * kWaves, NR > 1 ? 2 : 3) void paged_kernel(eakvd_geom geo, PagedJob J)
 {
     typedef Form<D, F32, NR> Fm;
     constexpr int GPD = D / 64, RB = 32 * GPD, NF = D / 16, NP = F32 ? 2 : 1;
-    constexpr int kWaves = Fm::kWaves;
     constexpr bool kValues = Fm::kValues, kSub = !F32 && !kValues;
     constexpr int NC = kSub ? GPD : 1;
     extern __shared__ __align__(16) uint8_t lds[];
@@ -284,7 +281,7 @@ __global__ __launch_bounds__(64 * kWavesOf<NR>, NR > 1 ? 2 : 3) void paged_kerne
     typename Fm::Wave &S = ((typename Fm::Wave *)lds)[w];
     typename Fm::Rows &R = *(typename Fm::Rows *)(lds + Fm::kRows);
     int *pre = (int *)(lds + Fm::kLine);
-    line_of<kWaves>(J, pre, (int *)lds, tid);
+    line_of(J, pre, (int *)lds, tid);
     const int grid = (int)gridDim.x, total = uni(pre[J.b.n_seqs]);
     const int share = max(1, (total + grid - 1) / grid);
     const int bl = line_block((int)blockIdx.x, grid);
@@ -717,17 +714,18 @@ __global__ __launch_bounds__(64 * kWavesOf<NR>, NR > 1 ? 2 : 3) void paged_kerne
         }
 
         // ---- the waves joined, 16 rows at a time
-        float *jo = (float *)lds;                                // [wave][NF][64][4]
-        float2 *jml = (float2 *)(lds + (size_t)kWaves * NF * 64 * 16);   // [wave][16]
+        // (two buffers: one is read while the next is written)
         const int slot = 2 * bl + (U.at == 0 ? 1 : 0);
         poison |= __shfl_xor(poison, 16, 64);
         poison |= __shfl_xor(poison, 32, 64);
 #pragma unroll
         for (int u = 0; u < NR; u++) {
             if (u > 0 && 16 * u >= rows) break;
+            float *jo = (float *)(lds + u % Fm::kBuffers * Fm::kJoinRows);            // [wave][NF][64][4]
+            float2 *jml = (float2 *)(lds + Fm::kBuffers * Fm::kJoinRows) + u % Fm::kBuffers * kWaves * 16;   // [wave][16]
             // a lane has its row's sums of its own tokens only
             const float l = row_sum(L[u]);
-            __syncthreads();
+            if (u == 0 || Fm::kBuffers == 1) __syncthreads();
 #pragma unroll
             for (int g = 0; g < GPD; g++) {
                 const float c = F32 ? row_sum(cs[u][F32 ? g : 0]) : 0.0f;
@@ -852,7 +850,7 @@ PagedPlan paged_plan(const eakvd_geom *g, const eakvd_pages *b, int n_q, int n_k
     const int64_t tiles = (b->max_len + kTile - 1) / kTile;
     // (two tiles stay together: the joining launch costs more)
     p.whole = tiles <= 2;
-    const int64_t most = units * (p.whole ? 1 : tiles > 1 ? tiles : 1), slots = (p.nr == 1 ? 3 : 1) * cu_count();
+    const int64_t most = units * (p.whole ? 1 : tiles > 1 ? tiles : 1), slots = (p.nr == 1 ? 3 : 2) * cu_count();
     p.grid = (int)(most < slots ? most : slots);
     p.part = ((size_t)p.grid * 2 * rbr * (g->head_dim + 2) * sizeof(float) + 255) & ~(size_t)255;
     p.bytes = p.whole ? 0 : p.part + (size_t)p.grid * sizeof(PagedCut);
@@ -868,7 +866,7 @@ int launch(const eakvd_geom &g, PagedJob &J, const PagedPlan &p, hipStream_t st)
     static std::atomic<uint64_t> done;
     const int e = allow_lds((const void *)kern, Fm::kLine + (EAKVD_PAGED_SEQS + 1) * 4, done);
     if (e) return e;
-    hipLaunchKernelGGL(kern, dim3((unsigned)p.grid), dim3(64 * Fm::kWaves), Fm::kLine + (J.b.n_seqs + 1) * 4, st, g,
+    hipLaunchKernelGGL(kern, dim3((unsigned)p.grid), dim3(64 * kWaves), Fm::kLine + (J.b.n_seqs + 1) * 4, st, g,
                        J);
     if (!p.whole)
         hipLaunchKernelGGL((paged_join_kernel<D, F32>), dim3((unsigned)p.grid, NR), dim3(D * 4), 0, st, J,
