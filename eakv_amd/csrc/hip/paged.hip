@@ -218,9 +218,16 @@ __device__ __forceinline__ int line_block(int b, int grid)
 
 // What a variant of the kernel holds where.  NR row tiles of 16 share a wave's operands of K and V.
 // One (decode): queries in registers, 3 blocks to a CU.  More: queries in LDS, which the waves of
-// the block share, 2 blocks to a CU, so that one computes while the other begins or ends a unit.  Four (bf16 alone): V's operands are its values in
-// f16, made once for 64 rows, and weights are operands as they stand (with the scales in the
-// weights each row tile takes 28 instructions more and V's operands 64 less).
+// the block share, 2 blocks to a CU, so that one computes while the other begins or ends a unit.
+// bf16, more than two: V's operands are its values in f16, made once for all rows, and weights are
+// operands as they stand (with the scales in the weights each row tile takes 28 instructions
+// more and V's operands 64 less).
+// Row tiles for prompts: what 256 registers hold.  (bf16, 1500 x 4 at up to 6001 of 32Q/4KV, d = 64: 3
+// 394 us, 4 404, 5 392, 6 365, 7 380; 2048 at 30720 of 32Q/8KV, d = 128: 2 2018 us, 3 1742, 4 2645.
+// f32, the first of these: 2 634 us, 4 536.)
+template <int D, bool F32>
+constexpr int kMany = D == 64 ? (F32 ? 4 : 6) : (F32 ? 2 : 3);
+
 template <int D, bool F32, int NR>
 struct Form {
     static constexpr int GPD = D / 64;
@@ -348,7 +355,7 @@ __global__ __launch_bounds__(64 * kWaves, NR > 1 ? 2 : 3) void paged_kernel(eakv
             int t, hd;
             row_at(u, t, hd);
             const int vis = U.q.pos + tok0 + t + 1;              // positions that the row sees
-            if (!Fm::kShared || (u == w && 16 * u < rows)) {
+            if (!Fm::kShared || (u % kWaves == w && 16 * u < rows)) {
                 auto &q = Q[Fm::kShared ? 0 : u];
                 q.load(J.q, (int64_t)(U.q.row + tok0 + t) * J.ld_q + (int64_t)(head0 + hd) * D, J.vec & 1, blk);
                 if constexpr (Fm::kShared) {
@@ -836,13 +843,15 @@ struct PagedPlan {
     size_t part, bytes;
 };
 
-// 16 rows to a unit where no sequence has more, else 32, and 64 for bf16 beyond 32.
+// 16 rows to a unit where no sequence has more, 32 likewise, else kMany tiles.
 PagedPlan paged_plan(const eakvd_geom *g, const eakvd_pages *b, int n_q, int n_kv, bool bf16)
 {
     PagedPlan p;
     const int qpk = n_q / n_kv;
     const int64_t rows = (int64_t)b->max_new * qpk;
-    p.nr = rows <= 16 ? 1 : rows <= 32 || !bf16 ? 2 : g->head_dim == 64 ? 4 : 3;
+    const int many = g->head_dim == 64 ? (bf16 ? kMany<64, false> : kMany<64, true>)
+                                       : (bf16 ? kMany<128, false> : kMany<128, true>);
+    p.nr = rows <= 16 ? 1 : rows <= 32 ? 2 : many;
     const int rbr = 16 * p.nr, tb = qpk < rbr ? rbr / qpk : 1, hb = (qpk + rbr - 1) / rbr;
     // units at most
     const int64_t units = (b->n_new / tb + (int64_t)(b->n_seqs < b->n_new ? b->n_seqs : b->n_new)) *
@@ -915,10 +924,13 @@ extern "C" int eakvd_paged_attend(const eakvd_geom *g, const uint8_t *base, cons
     const hipStream_t st = (hipStream_t)stream;
     auto run = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        if (!bf16) return p.nr == 1 ? launch<D, true, 1>(*g, J, p, st) : launch<D, true, 2>(*g, J, p, st);
-        return p.nr == 1   ? launch<D, false, 1>(*g, J, p, st)
-               : p.nr == 2 ? launch<D, false, 2>(*g, J, p, st)
-                           : launch<D, false, D == 64 ? 4 : 3>(*g, J, p, st);
+        auto by_type = [&](auto f32) {
+            constexpr bool F = decltype(f32)::value;
+            return p.nr == 1   ? launch<D, F, 1>(*g, J, p, st)
+                   : p.nr == 2 ? launch<D, F, 2>(*g, J, p, st)
+                               : launch<D, F, kMany<D, F>>(*g, J, p, st);
+        };
+        return bf16 ? by_type(std::false_type()) : by_type(std::true_type());
     };
     return g->head_dim == 64 ? run(std::integral_constant<int, 64>()) : run(std::integral_constant<int, 128>());
 }
