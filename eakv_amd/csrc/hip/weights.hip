@@ -4,21 +4,23 @@
 //   w[h][t] = keep * w[h][t] + sum_{i, q heads of h} exp(s_i[t] - M_i) / L_i,
 //   s_i[t] = q_i.K[t] / sqrt(d) where query i sees t, M_i = max_t s_i, L_i = sum_t exp(s_i - M_i).
 //
-// Two passes over K, the scores made on the matrix cores in both (rows16.h; the arithmetic
-// of window.hip): the first leaves each row's (M, L) of a chunk of tokens, the second joins
-// them and sums the weights.  Rows (window tokens x q heads) are taken 128 at a time, their
-// operands in LDS; a wave holds 32 tokens' operands of K in registers and goes through the
-// rows.  A token's sum is one wave's: no atomics, the same bits on every call.
+// The scores are made on the matrix cores (rows16.h; the arithmetic of window.hip, K's operands
+// exact for both types).  A first pass over K leaves each row's (M, L) of a chunk of tokens.
+// Few rows (up to kStore to a kv head, a decode step): it also leaves the scores, and the
+// second launch adds their weights up: 8 bytes a row and token more against K's 80, and no
+// products.  More: the second pass makes the scores again.  Rows (window tokens x q heads) are
+// taken kRowTiles row tiles at a time, their operands in LDS; a wave holds 32 tokens'
+// operands of K in registers and goes through the rows.  A token's sum is one thread's or one
+// wave's: no atomics, the same bits on every call.
 #include <string.h>
 
 #include "rows16.h"
 
 namespace {
 
-constexpr int kWaves = 8;
-constexpr int kTile = 32 * kWaves;
-constexpr int kRowTiles = 8;                    // of a pass over a chunk's tokens
-constexpr int kGroupRows = 16 * kRowTiles;
+constexpr int kTile = 256;
+constexpr int kRowTiles = 8;                    // of a pass over a chunk's tokens, at most
+constexpr int kStore = 8;
 
 struct WeightsJob {
     int n_seq, n_q, n_kv, qpk, layer;
@@ -27,32 +29,65 @@ struct WeightsJob {
     int seq[EAKVD_MAX_BATCH];                   // its number in the call
     int mc[EAKVD_MAX_BATCH], clen[EAKVD_MAX_BATCH];
     int pre[EAKVD_MAX_BATCH + 1];               // blocks before this sequence's
+    int add[EAKVD_MAX_BATCH + 1];               // weights_add_kernel: likewise
     int64_t stat[EAKVD_MAX_BATCH];              // its rows' first (M, L)
+    int64_t score[EAKVD_MAX_BATCH], ld_s[EAKVD_MAX_BATCH];      // its scores, and from row to row
 };
 
-template <int D, bool F32>
-struct __align__(16) WLds {
-    static constexpr int NQ = D / 32 * (F32 ? 2 : 1) + 1;       // operands of a row tile
-    uint4 q[kRowTiles][NQ][64];
-    float rf[kRowTiles][16];
-    float2 ml[kRowTiles][16];                   // second pass: M and 1/L of the rows
-    struct {
-        float ks[D / 64][32], zk[D / 64][32];
-    } w[kWaves];
-    float2 run[kWaves][kRowTiles][64];          // first pass: a lane's running M and L
+// LDS: the waves' scales, then a Tile for each row tile of a pass.
+struct Scales {
+    float ks[2][32], zk[2][32];
+};
+template <int D, bool F32, int W>
+struct __align__(16) Tile {
+    static constexpr int NQ = D / 32 * (F32 ? 2 : 1) + 1;       // operands
+    uint4 q[NQ][64];
+    float rf[16];
+    int vis[16];                                // positions that the row sees
+    float2 ml[16];                              // second pass: M and 1/L
+    float2 run[W][64];                          // first pass: a lane's running M and L
 };
 
-// SUM: the second pass.
-template <int D, bool F32, bool SUM>
-__global__ __launch_bounds__(64 * kWaves, 2) void weights_kernel(eakvd_geom geo, WeightsJob job,
-                                                                 const void *q, float2 *stat, float *out,
-                                                                 int64_t ld, float keep, float ksc, int vec)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void *p, int64_t bytes)
+{
+    // dword3 0x00020000: raw 32-bit buffer; reads beyond `bytes` return 0
+    const int64_t most = 0xfffffff0ll;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0,
+                                             (int)(uint32_t)(bytes < most ? bytes : most), 0x00020000);
+}
+
+// The chunks' (M, L) of a row joined, 4 lanes to a row (sub): M and 1/L, 0 where nothing is seen.
+__device__ __forceinline__ float2 join_row(const float2 *st, int mc, int sub, bool live)
+{
+    float mm = kMInit;
+    for (int k = sub; live && k < mc; k += 4) {
+        const float2 x = st[k];
+        if (x.y != 0.0f) mm = fmaxf(mm, x.x);
+    }
+    mm = fmaxf(mm, __shfl_xor(mm, 1, 64));
+    mm = fmaxf(mm, __shfl_xor(mm, 2, 64));
+    float l = 0.0f;
+    for (int k = sub; live && k < mc; k += 4) {
+        const float2 x = st[k];
+        if (x.y != 0.0f) l = fmaf(__builtin_amdgcn_exp2f(x.x - mm), x.y, l);
+    }
+    l += __shfl_xor(l, 1, 64);
+    l += __shfl_xor(l, 2, 64);
+    return float2{mm, l == 0.0f ? 0.0f : 1.0f / l};
+}
+
+// W waves.  SUM: the second pass; STORE: the first pass leaves the scores, log2, [kv head][row][ld_s].
+template <int D, bool F32, int W, bool SUM, bool STORE>
+__global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void weights_kernel(
+    eakvd_geom geo, WeightsJob job, const void *q, float2 *stat, float *score, float *out, int64_t ld,
+    float keep, float ksc, int vec, int tiles)
 {
     constexpr int GPD = D / 64, RB = 32 * GPD;
-    typedef WLds<D, F32> Lds;
+    typedef Tile<D, F32, W> Tl;
     extern __shared__ __align__(16) uint8_t lds[];
-    Lds &S = *(Lds *)lds;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    Scales &S = ((Scales *)lds)[w];
+    Tl *T = (Tl *)(lds + W * sizeof(Scales));
     const int n16 = lane & 15, blk = lane >> 4, n32 = lane & 31, h = lane >> 5;
     const bool owner = GPD == 2 || h == 0;
     const int gh = GPD == 2 ? h : 0;
@@ -65,77 +100,68 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weights_kernel(eakvd_geom geo,
     const int lo = chunk * job.clen[c];
     const int hi = t_end - lo > job.clen[c] ? lo + job.clen[c] : t_end;
     const int n_sub = hi > lo ? (hi - lo + 31) / 32 : 0;
-    const int n_i = n_sub > w ? (n_sub - w + kWaves - 1) / kWaves : 0;
+    const int n_i = n_sub > w ? (n_sub - w + W - 1) / W : 0;
     float2 *st = stat + job.stat[c] + (int64_t)kvh * rows * mc;          // [row][chunk]
 
+    // (offsets from the chunk's first token are 32 bits; behind the plane's end loads give 0)
     const Planes K = planes_of(geo, job.base[c], job.layer, 0);
     const int64_t g0 = (int64_t)kvh * geo.gph + (int64_t)lo * GPD;
-    const uint8_t *kw = K.w + g0 * 32;
-    const float *ks = K.s + g0, *kb = K.b + g0;
-    const int last = hi - 1 - lo;                               // the chunk's last token
+    const int64_t room = (int64_t)(geo.max_seq_len - lo) * GPD;
+    const auto rk = rsrc(K.w + g0 * 32, room * 32), rks = rsrc(K.s + g0, room * 4), rkb = rsrc(K.b + g0, room * 4);
     NibConst nc;
     nc.hold();
 
-    for (int r0 = 0; r0 < rows; r0 += kGroupRows) {
-        const int nu = min(kRowTiles, (rows - r0 + 15) / 16);
+    for (int r0 = 0; r0 < rows; r0 += 16 * tiles) {
+        const int nu = min(tiles, (rows - r0 + 15) / 16);
         __syncthreads();
-        if (w < nu) {
-            const int row = min(r0 + 16 * w + n16, rows - 1), tok = row / qpk;
+        for (int u = w; u < nu; u += W) {
+            const int at = r0 + 16 * u + n16, row = min(at, rows - 1), tok = row / qpk;
             Query<D, F32, false> Q;
             Q.load(q, ((int64_t)(job.tok0[c] + tok) * job.n_q + kvh * qpk + row - tok * qpk) * D, vec, blk);
 #pragma unroll
             for (int f = 0; f < D / 32; f++) {
-                S.q[w][f][lane] = __builtin_bit_cast(uint4, Q.a[f]);
-                if constexpr (F32) S.q[w][D / 32 + (F32 ? f : 0)][lane] = __builtin_bit_cast(uint4, Q.b[F32 ? f : 0]);
+                T[u].q[f][lane] = __builtin_bit_cast(uint4, Q.a[f]);
+                if constexpr (F32) T[u].q[D / 32 + (F32 ? f : 0)][lane] = __builtin_bit_cast(uint4, Q.b[F32 ? f : 0]);
             }
-            S.q[w][Lds::NQ - 1][lane] = __builtin_bit_cast(uint4, Q.bias);
-            if (blk == 0) S.rf[w][n16] = Q.rf;
+            T[u].q[Tl::NQ - 1][lane] = __builtin_bit_cast(uint4, Q.bias);
+            if (blk == 0) {
+                T[u].rf[n16] = Q.rf;
+                T[u].vis[n16] = at < rows ? start + tok + 1 : 0;
+            }
+            if constexpr (!SUM)
+                for (int k = 0; k < W; k++) T[u].run[k][lane] = float2{kMInit, 0.0f};
         }
-        if constexpr (SUM) {
-            // the chunks' (M, L) of a row, 4 lanes to each of 128 rows
-            const int r = tid >> 2, row = r0 + r;
-            float mm = kMInit;
-            if (row < rows)
-                for (int k = tid & 3; k < mc; k += 4) {
-                    const float2 x = st[(int64_t)row * mc + k];
-                    if (x.y != 0.0f) mm = fmaxf(mm, x.x);
-                }
-            mm = fmaxf(mm, __shfl_xor(mm, 1, 64));
-            mm = fmaxf(mm, __shfl_xor(mm, 2, 64));
-            float l = 0.0f;
-            if (row < rows)
-                for (int k = tid & 3; k < mc; k += 4) {
-                    const float2 x = st[(int64_t)row * mc + k];
-                    if (x.y != 0.0f) l = fmaf(__builtin_amdgcn_exp2f(x.x - mm), x.y, l);
-                }
-            l += __shfl_xor(l, 1, 64);
-            l += __shfl_xor(l, 2, 64);
-            if ((tid & 3) == 0) S.ml[r >> 4][r & 15] = float2{mm, l == 0.0f ? 0.0f : 1.0f / l};
-        } else {
-            for (int u = 0; u < nu; u++) S.run[w][u][lane] = float2{kMInit, 0.0f};
-        }
+        if constexpr (SUM)
+            for (int r = tid >> 2; r < 16 * nu; r += 16 * W) {
+                const float2 x = join_row(st + (int64_t)(r0 + r) * mc, mc, tid & 3, r0 + r < rows);
+                if ((tid & 3) == 0) T[r >> 4].ml[r & 15] = x;
+            }
         __syncthreads();
 
         uint2 kx[2][GPD];
         float s0 = 0.0f, b0 = 0.0f;
-        auto load = [&](int i) {
-            const int t = 32 * (w + kWaves * i);
+        auto load = [&](int i) __attribute__((always_inline)) {
+            const int t = 32 * (w + W * i);
+            constexpr int aux = W == 4 && !SUM ? 2 : 0;
 #pragma unroll
             for (int k = 0; k < 2; k++)
 #pragma unroll
-                for (int g = 0; g < GPD; g++)
-                    kx[k][g] = *(const uint2 *)(kw + (int64_t)min(t + 16 * k + n16, last) * RB + 32 * g + 8 * blk);
-            const int64_t gi = (int64_t)min(t + n32, last) * GPD + gh;
-            s0 = ks[gi];
-            b0 = kb[gi];
+                for (int g = 0; g < GPD; g++) {
+                    const auto y = __builtin_amdgcn_raw_buffer_load_b64(rk, n16 * RB + 8 * blk, (t + 16 * k) * RB + 32 * g,
+                                                                        aux);
+                    kx[k][g] = uint2{y[0], y[1]};
+                }
+            const int at = (n32 * GPD + gh) * 4;
+            s0 = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rks, at, t * GPD * 4, aux));
+            b0 = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rkb, at, t * GPD * 4, aux));
         };
         if (n_i > 0) load(0);
         for (int i = 0; i < n_i; i++) {
-            const int t0 = lo + 32 * (w + kWaves * i);
+            const int t0 = lo + 32 * (w + W * i);
             const float zk = zero_nibble(s0, b0), ck = fmaf(zk, s0, b0) * ksc;
             if (owner) {
-                S.w[w].ks[gh][n32] = s0 * ksc;
-                S.w[w].zk[gh][n32] = zk;
+                S.ks[gh][n32] = s0 * ksc;
+                S.zk[gh][n32] = zk;
             }
             b8 bias[2];
             bias_operands(owner ? ck : 0.0f, 0.0f, false, bias, n32);
@@ -146,8 +172,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weights_kernel(eakvd_geom geo,
             for (int k = 0; k < 2; k++)
 #pragma unroll
                 for (int g = 0; g < GPD; g++) {
-                    k_operands<false>(kx[k][g], S.w[w].zk[g][16 * k + n16], nc, kl[k][g], kh[k][g]);
-                    sc[k][g] = *(const v4f *)&S.w[w].ks[g][16 * k + 4 * blk];
+                    k_operands<false>(kx[k][g], S.zk[g][16 * k + n16], nc, kl[k][g], kh[k][g]);
+                    sc[k][g] = *(const v4f *)&S.ks[g][16 * k + 4 * blk];
                 }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             if (i + 1 < n_i) load(i + 1);
@@ -159,14 +185,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weights_kernel(eakvd_geom geo,
                 Query<D, F32, false> Q;
 #pragma unroll
                 for (int f = 0; f < D / 32; f++) {
-                    Q.a[f] = __builtin_bit_cast(h8, S.q[u][f][lane]);
-                    if constexpr (F32) Q.b[F32 ? f : 0] = __builtin_bit_cast(h8, S.q[u][D / 32 + (F32 ? f : 0)][lane]);
+                    Q.a[f] = __builtin_bit_cast(h8, T[u].q[f][lane]);
+                    if constexpr (F32) Q.b[F32 ? f : 0] = __builtin_bit_cast(h8, T[u].q[D / 32 + (F32 ? f : 0)][lane]);
                 }
-                const b8 qb = __builtin_bit_cast(b8, S.q[u][Lds::NQ - 1][lane]);
-                const float rf = S.rf[u][n16];
-                const int row = r0 + 16 * u + n16;
-                // positions that the row sees (rows behind the last: none)
-                const int vis = row < rows ? start + row / qpk + 1 : 0;
+                const b8 qb = __builtin_bit_cast(b8, T[u].q[Tl::NQ - 1][lane]);
+                const float rf = T[u].rf[n16];
+                const int vis = T[u].vis[n16];
                 float x[8];
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
@@ -183,30 +207,44 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weights_kernel(eakvd_geom geo,
                 const bool masked = __ballot(t0 + 32 > vis) != 0;
                 const int seen = vis - t0 - 4 * blk;            // of the lane's first half on
                 if constexpr (SUM) {
-                    const float2 ml = S.ml[u][n16];
+                    const float2 ml = T[u].ml[n16];
+                    if (masked) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const float y = __builtin_amdgcn_exp2f(fmaf(x[j], rf, -ml.x)) * ml.y;
-                        acc[j] += !masked || 16 * (j >> 2) + (j & 3) < seen ? y : 0.0f;
+                        for (int j = 0; j < 8; j++) {
+                            const float y = __builtin_amdgcn_exp2f(fmaf(x[j], rf, -ml.x)) * ml.y;
+                            acc[j] += 16 * (j >> 2) + (j & 3) < seen ? y : 0.0f;
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            acc[j] = fmaf(__builtin_amdgcn_exp2f(fmaf(x[j], rf, -ml.x)), ml.y, acc[j]);
                     }
                 } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[j] *= rf;
                     if (masked)
 #pragma unroll
                         for (int j = 0; j < 8; j++)
                             x[j] = 16 * (j >> 2) + (j & 3) < seen ? x[j] : -__builtin_inff();
-                    float2 run = S.run[w][u][lane];
-                    float top = fmaxf(x[0], x[1]);
-#pragma unroll
-                    for (int j = 2; j < 8; j++) top = fmaxf(top, x[j]);
-                    const float mn = fmaxf(run.x, top * rf);
+                    if constexpr (STORE) {
+                        if (r0 + 16 * u + n16 < rows) {
+                            float *o = score + job.score[c] + ((int64_t)kvh * rows + r0 + 16 * u + n16) * job.ld_s[c] + t0 +
+                                       4 * blk;
+                            *(v4f *)o = v4f{x[0], x[1], x[2], x[3]};
+                            *(v4f *)(o + 16) = v4f{x[4], x[5], x[6], x[7]};
+                        }
+                    }
+                    float2 run = T[u].run[w][lane];
+                    const float top = max3(max3(max3(x[0], x[1], x[2]), x[3], x[4]), max3(x[5], x[6], x[7]), x[7]);
+                    const float mn = fmaxf(run.x, top);
                     float l = run.y * __builtin_amdgcn_exp2f(run.x - mn);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) l += __builtin_amdgcn_exp2f(fmaf(x[j], rf, -mn));
-                    S.run[w][u][lane] = float2{mn, l};
+                    for (int j = 0; j < 8; j++) l += __builtin_amdgcn_exp2f(x[j] - mn);
+                    T[u].run[w][lane] = float2{mn, l};
                 }
             }
             if constexpr (SUM) {
-                // over the 16 rows of the tile: lanes with one blk
+                // over the 16 rows of the tiles: lanes with one blk
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     acc[j] += dpp_f<0x128>(acc[j]);             // row_ror 8, 4, 2, 1
@@ -228,29 +266,73 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weights_kernel(eakvd_geom geo,
         if constexpr (!SUM) {
             // rows' (M, L) of the chunk: over the lanes of a row and the waves
             __syncthreads();
-            const int r = tid >> 2, row = r0 + r;
-            float mm = kMInit;
-            for (int k = 0; k < kWaves; k++) mm = fmaxf(mm, S.run[k][r >> 4][(r & 15) + 16 * (tid & 3)].x);
-            mm = fmaxf(mm, __shfl_xor(mm, 1, 64));
-            mm = fmaxf(mm, __shfl_xor(mm, 2, 64));
-            float l = 0.0f;
-            for (int k = 0; k < kWaves; k++) {
-                const float2 x = S.run[k][r >> 4][(r & 15) + 16 * (tid & 3)];
-                l = x.y == 0.0f ? l : fmaf(__builtin_amdgcn_exp2f(x.x - mm), x.y, l);
+            for (int r = tid >> 2; r < 16 * nu; r += 16 * W) {
+                const int row = r0 + r;
+                float mm = kMInit;
+                for (int k = 0; k < W; k++) mm = fmaxf(mm, T[r >> 4].run[k][(r & 15) + 16 * (tid & 3)].x);
+                mm = fmaxf(mm, __shfl_xor(mm, 1, 64));
+                mm = fmaxf(mm, __shfl_xor(mm, 2, 64));
+                float l = 0.0f;
+                for (int k = 0; k < W; k++) {
+                    const float2 x = T[r >> 4].run[k][(r & 15) + 16 * (tid & 3)];
+                    l = x.y == 0.0f ? l : fmaf(__builtin_amdgcn_exp2f(x.x - mm), x.y, l);
+                }
+                l += __shfl_xor(l, 1, 64);
+                l += __shfl_xor(l, 2, 64);
+                if ((tid & 3) == 0 && row < rows) st[(int64_t)row * mc + chunk] = float2{mm, l};
             }
-            l += __shfl_xor(l, 1, 64);
-            l += __shfl_xor(l, 2, 64);
-            if ((tid & 3) == 0 && row < rows) st[(int64_t)row * mc + chunk] = float2{mm, l};
         }
     }
 }
 
+// The scores that the first pass left, as weights: 4 tokens to a thread, the unit's rows one
+// after the other.
+constexpr int kAddThreads = 256;
+__global__ __launch_bounds__(kAddThreads) void weights_add_kernel(WeightsJob job, const float2 *stat,
+                                                                  const float *score, float *out, int64_t ld,
+                                                                  float keep)
+{
+    __shared__ float2 ml[kStore];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int c = seq_of(job.add, job.n_seq, (int)blockIdx.x, lane);
+    const int rem = (int)blockIdx.x - job.add[c];
+    const int kvh = rem % job.n_kv, t0 = (rem / job.n_kv) * 4 * kAddThreads + 4 * tid;
+    const int rows = job.ntok[c] * job.qpk, mc = job.mc[c], hi = job.start[c] + job.ntok[c];
+    if (tid < 4 * kStore) {
+        const int r = tid >> 2;
+        const float2 x = join_row(stat + job.stat[c] + ((int64_t)kvh * rows + min(r, rows - 1)) * mc, mc, tid & 3,
+                                  r < rows);
+        if ((tid & 3) == 0) ml[r] = x;
+    }
+    __syncthreads();
+    if (t0 >= hi) return;
+    // (rows of scores are whole tiles; those that a row does not see are -inf, and what is
+    // there has no part in the sum where its 1/L is NaN)
+    const float *s = score + job.score[c] + (int64_t)kvh * rows * job.ld_s[c] + t0;
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int r = 0; r < rows; r++) {
+        const v4f x = __builtin_nontemporal_load((const v4f *)(s + (int64_t)r * job.ld_s[c]));
+        const float2 y = ml[r];
+        const int vis = job.start[c] + r / job.qpk + 1;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            acc[e] += t0 + e < vis ? __builtin_amdgcn_exp2f(x[e] - y.x) * y.y : 0.0f;
+    }
+    float *o = out + ((int64_t)job.seq[c] * job.n_kv + kvh) * ld + t0;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (t0 + e < hi) o[e] = keep == 0.0f ? acc[e] : fmaf(keep, o[e], acc[e]);
+}
+
 struct WeightsPlan {
     WeightsJob job;
-    size_t bytes;
+    int waves, tiles;
+    bool store;
+    size_t stat_bytes, bytes;
 };
 
-// Chunks of an even share of the tiles for two blocks per CU.
+// Chunks of an even share of the tiles: 3 blocks of 4 waves to a CU for up to two row tiles, else
+// one of 8.
 void weights_plan(const eakvd_window *b, int n_q, int n_kv, WeightsPlan *p)
 {
     memset(p, 0, sizeof(*p));
@@ -258,7 +340,7 @@ void weights_plan(const eakvd_window *b, int n_q, int n_kv, WeightsPlan *p)
     j.n_q = n_q;
     j.n_kv = n_kv;
     j.qpk = n_q / n_kv;
-    int64_t tiles = 0, stat = 0;
+    int64_t tiles = 0, stat = 0, score = 0, rows = 0;
     int tok0 = 0;
     for (int i = 0; i < b->n_seq; i++) {
         if (b->ntok[i]) {
@@ -269,40 +351,70 @@ void weights_plan(const eakvd_window *b, int n_q, int n_kv, WeightsPlan *p)
             j.tok0[k] = tok0;
             j.seq[k] = i;
             tiles += ((int64_t)b->start[i] + b->ntok[i] + kTile - 1) / kTile * n_kv;
+            const int64_t r = (int64_t)b->ntok[i] * j.qpk;
+            rows = r > rows ? r : rows;
         }
         tok0 += b->ntok[i];
     }
-    const int64_t slots = 2 * cu_count(), share = (tiles + slots - 1) / slots;
+    p->store = rows <= kStore;
+    p->tiles = (int)((rows + 15) / 16 < kRowTiles ? (rows + 15) / 16 : kRowTiles);
+    p->waves = p->tiles <= 2 ? 4 : 8;
+    const int64_t slots = (p->waves == 4 ? 3 : 1) * cu_count(), share = (tiles + slots - 1) / slots;
     for (int i = 0; i < j.n_seq; i++) {
-        const int64_t n_t = ((int64_t)j.start[i] + j.ntok[i] + kTile - 1) / kTile;
+        const int64_t t = (int64_t)j.start[i] + j.ntok[i], n_t = (t + kTile - 1) / kTile;
         int64_t mc = (n_t + share - 1) / share;
+        // (offsets from a chunk's first token are 32 bits)
+        if (mc < (n_t >> 16) + 1) mc = (n_t >> 16) + 1;
         const int64_t per = (n_t + mc - 1) / mc;
         mc = (n_t + per - 1) / per;
         j.mc[i] = (int)mc;
-        j.clen[i] = (int)(per * kTile < INT32_MAX ? per * kTile : INT32_MAX);
+        j.clen[i] = (int)(per * kTile);
         j.pre[i + 1] = j.pre[i] + (int)mc * n_kv;
+        j.add[i + 1] = j.add[i] + (int)((t + 4 * kAddThreads - 1) / (4 * kAddThreads)) * n_kv;
         j.stat[i] = stat;
         stat += (int64_t)j.ntok[i] * n_q * mc;
+        j.ld_s[i] = n_t * kTile;
+        j.score[i] = score;
+        score += (int64_t)j.ntok[i] * n_q * j.ld_s[i];
     }
-    p->bytes = (size_t)stat * sizeof(float2);
+    p->stat_bytes = ((size_t)stat * sizeof(float2) + 255) & ~(size_t)255;
+    p->bytes = p->stat_bytes + (p->store ? (size_t)score * sizeof(float) : 0);
 }
 
 template <int D, bool F32>
-int launch(const eakvd_geom &g, const WeightsJob &job, const void *q, float2 *stat, float *out, int64_t ld,
+int launch(const eakvd_geom &g, const WeightsPlan &p, const void *q, void *work, float *out, int64_t ld,
            float keep, int vec, hipStream_t st)
 {
-    constexpr size_t bytes = sizeof(WLds<D, F32>);
-    static_assert(bytes <= 160 * 1024, "LDS");
-    auto run = [&](auto *kern, std::atomic<uint64_t> &done) {
-        const int e = allow_lds((const void *)kern, bytes, done);
+    const WeightsJob &job = p.job;
+    float2 *stat = (float2 *)work;
+    float *score = (float *)((uint8_t *)work + p.stat_bytes);
+    auto run = [&](auto *kern, int waves, size_t tile, int most, std::atomic<uint64_t> &done) {
+        const int e = allow_lds((const void *)kern, waves * sizeof(Scales) + most * tile, done);
         if (e) return e;
-        hipLaunchKernelGGL(kern, dim3((unsigned)job.pre[job.n_seq]), dim3(64 * kWaves), bytes, st, g, job, q,
-                           stat, out, ld, keep, EAKV_LOG2E / sqrtf((float)D), vec);
+        hipLaunchKernelGGL(kern, dim3((unsigned)job.pre[job.n_seq]), dim3(64 * waves),
+                           waves * sizeof(Scales) + p.tiles * tile, st, g, job, q, stat, score, out, ld, keep,
+                           EAKV_LOG2E / sqrtf((float)D), vec, p.tiles);
         return (int)hipGetLastError();
     };
-    static std::atomic<uint64_t> done[2];
-    const int e = run(weights_kernel<D, F32, false>, done[0]);
-    return e ? e : run(weights_kernel<D, F32, true>, done[1]);
+    static std::atomic<uint64_t> done[5];
+    constexpr size_t t4 = sizeof(Tile<D, F32, 4>), t8 = sizeof(Tile<D, F32, 8>);
+    static_assert(8 * sizeof(Scales) + kRowTiles * t8 <= 160 * 1024, "LDS");
+    int e;
+    if (p.store) {
+        e = run(weights_kernel<D, F32, 4, false, true>, 4, t4, 2, done[0]);
+        if (!e) {
+            hipLaunchKernelGGL(weights_add_kernel, dim3((unsigned)job.add[job.n_seq]), dim3(kAddThreads), 0, st, job,
+                               stat, score, out, ld, keep);
+            e = (int)hipGetLastError();
+        }
+    } else if (p.waves == 4) {
+        e = run(weights_kernel<D, F32, 4, false, false>, 4, t4, 2, done[1]);
+        if (!e) e = run(weights_kernel<D, F32, 4, true, false>, 4, t4, 2, done[2]);
+    } else {
+        e = run(weights_kernel<D, F32, 8, false, false>, 8, t8, kRowTiles, done[3]);
+        if (!e) e = run(weights_kernel<D, F32, 8, true, false>, 8, t8, kRowTiles, done[4]);
+    }
+    return e;
 }
 
 }  // namespace
@@ -323,10 +435,9 @@ extern "C" int eakvd_weights(const eakvd_geom *g, const eakvd_window *b, int lay
     p.job.layer = layer;
     const hipStream_t st = (hipStream_t)stream;
     const int vec = (uintptr_t)q % 16 == 0;
-    float2 *stat = (float2 *)work;
     if (g->head_dim == 64)
-        return bf16 ? launch<64, false>(*g, p.job, q, stat, out, ld, keep, vec, st)
-                    : launch<64, true>(*g, p.job, q, stat, out, ld, keep, vec, st);
-    return bf16 ? launch<128, false>(*g, p.job, q, stat, out, ld, keep, vec, st)
-                : launch<128, true>(*g, p.job, q, stat, out, ld, keep, vec, st);
+        return bf16 ? launch<64, false>(*g, p, q, work, out, ld, keep, vec, st)
+                    : launch<64, true>(*g, p, q, work, out, ld, keep, vec, st);
+    return bf16 ? launch<128, false>(*g, p, q, work, out, ld, keep, vec, st)
+                : launch<128, true>(*g, p, q, work, out, ld, keep, vec, st);
 }
