@@ -226,7 +226,7 @@ int eakvd_paged_append(const eakvd_geom *g, uint8_t *base, const eakvd_pages *b,
 
 /* ---- eviction by attention weight (hip/weights.hip, hip/evict.hip)
  * eakvd_weights: out [b->n_seq][n_kv][ld]; work: eakvd_weights_work_bytes(). */
-size_t eakvd_weights_work_bytes(const eakvd_window *b, int n_q, int n_kv);
+size_t eakvd_weights_work_bytes(const eakvd_window *b, int n_q, int n_kv, int bf16);
 int eakvd_weights(const eakvd_geom *g, const eakvd_window *b, int layer, const void *q, int bf16, int n_q,
                   int n_kv, float keep, float *out, int64_t ld, void *work, void *stream);
 /* See eakv_evict_select_device; first[i]: where sequence i's list begins in index. */

@@ -13,7 +13,7 @@ size_t eakv_attention_weights_work_bytes(eakv_cache_t *const *caches, int n_cach
     if (eakvi_window_check(caches, n_caches, 0, starts, n_tokens, dtype, n_q, n_kv, 0, &b, &total)) return 0;
     int prev;
     if (eakvi_enter(caches[0], &prev)) return 0;
-    const size_t need = eakvd_weights_work_bytes(&b, n_q, n_kv);
+    const size_t need = eakvd_weights_work_bytes(&b, n_q, n_kv, dtype == EAKV_BF16);
     eakvi_leave(prev);
     return need;
 }
@@ -39,7 +39,7 @@ int eakv_attention_weights_batch_device(eakv_cache_t *const *caches, int n_cache
     int prev;
     rc = eakvi_enter(c0, &prev);
     if (rc) return rc;
-    const size_t need = eakvd_weights_work_bytes(&b, n_q, n_kv);
+    const size_t need = eakvd_weights_work_bytes(&b, n_q, n_kv, dtype == EAKV_BF16);
     const int own = !d_work;
     const eakvi_span q = {d_q, (size_t)total * n_q * c0->head_dim * (dtype == EAKV_F32 ? 4 : 2)},
                      out = {d_weights, (size_t)n_caches * n_kv * (size_t)ld * 4}, work = {d_work, need};

@@ -57,28 +57,34 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void *p, int64_t by
 }
 
 // The chunks' (M, L) of a row joined, 4 lanes to a row (sub): M and 1/L, 0 where nothing is seen.
+// (Eight loads in flight: a chunk at a time this was most of a small launch.)
 __device__ __forceinline__ float2 join_row(const float2 *st, int mc, int sub, bool live)
 {
-    float mm = kMInit;
-    for (int k = sub; live && k < mc; k += 4) {
-        const float2 x = st[k];
-        if (x.y != 0.0f) mm = fmaxf(mm, x.x);
+    float mm = kMInit, l = 0.0f;
+    for (int k0 = sub; live && k0 < mc; k0 += 32) {
+        float2 x[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = st[min(k0 + 4 * k, mc - 1)];
+        float top = mm;
+#pragma unroll
+        for (int k = 0; k < 8; k++) top = x[k].y != 0.0f ? fmaxf(top, x[k].x) : top;
+        l *= __builtin_amdgcn_exp2f(mm - top);
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            l = k0 + 4 * k < mc && x[k].y != 0.0f ? fmaf(__builtin_amdgcn_exp2f(x[k].x - top), x[k].y, l) : l;
+        mm = top;
     }
-    mm = fmaxf(mm, __shfl_xor(mm, 1, 64));
-    mm = fmaxf(mm, __shfl_xor(mm, 2, 64));
-    float l = 0.0f;
-    for (int k = sub; live && k < mc; k += 4) {
-        const float2 x = st[k];
-        if (x.y != 0.0f) l = fmaf(__builtin_amdgcn_exp2f(x.x - mm), x.y, l);
-    }
+    float top = fmaxf(mm, __shfl_xor(mm, 1, 64));
+    top = fmaxf(top, __shfl_xor(top, 2, 64));
+    l *= __builtin_amdgcn_exp2f(mm - top);
     l += __shfl_xor(l, 1, 64);
     l += __shfl_xor(l, 2, 64);
-    return float2{mm, l == 0.0f ? 0.0f : 1.0f / l};
+    return float2{top, l == 0.0f ? 0.0f : 1.0f / l};
 }
 
 // W waves.  SUM: the second pass; STORE: the first pass leaves the scores, log2, [kv head][row][ld_s].
 template <int D, bool F32, int W, bool SUM, bool STORE>
-__global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void weights_kernel(
+__global__ __launch_bounds__(64 * W, W == 4 ? 3 : F32 ? 2 : 4) void weights_kernel(
     eakvd_geom geo, WeightsJob job, const void *q, float2 *stat, float *score, float *out, int64_t ld,
     float keep, float ksc, int vec, int tiles)
 {
@@ -220,8 +226,6 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void weights_kernel(
                             acc[j] = fmaf(__builtin_amdgcn_exp2f(fmaf(x[j], rf, -ml.x)), ml.y, acc[j]);
                     }
                 } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) x[j] *= rf;
                     if (masked)
 #pragma unroll
                         for (int j = 0; j < 8; j++)
@@ -230,16 +234,16 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 2) void weights_kernel(
                         if (r0 + 16 * u + n16 < rows) {
                             float *o = score + job.score[c] + ((int64_t)kvh * rows + r0 + 16 * u + n16) * job.ld_s[c] + t0 +
                                        4 * blk;
-                            *(v4f *)o = v4f{x[0], x[1], x[2], x[3]};
-                            *(v4f *)(o + 16) = v4f{x[4], x[5], x[6], x[7]};
+                            *(v4f *)o = v4f{x[0] * rf, x[1] * rf, x[2] * rf, x[3] * rf};
+                            *(v4f *)(o + 16) = v4f{x[4] * rf, x[5] * rf, x[6] * rf, x[7] * rf};
                         }
                     }
                     float2 run = T[u].run[w][lane];
                     const float top = max3(max3(max3(x[0], x[1], x[2]), x[3], x[4]), max3(x[5], x[6], x[7]), x[7]);
-                    const float mn = fmaxf(run.x, top);
+                    const float mn = fmaxf(run.x, top * rf);
                     float l = run.y * __builtin_amdgcn_exp2f(run.x - mn);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) l += __builtin_amdgcn_exp2f(x[j] - mn);
+                    for (int j = 0; j < 8; j++) l += __builtin_amdgcn_exp2f(fmaf(x[j], rf, -mn));
                     T[u].run[w][lane] = float2{mn, l};
                 }
             }
@@ -332,8 +336,8 @@ struct WeightsPlan {
 };
 
 // Chunks of an even share of the tiles: 3 blocks of 4 waves to a CU for up to two row tiles, else
-// one of 8.
-void weights_plan(const eakvd_window *b, int n_q, int n_kv, WeightsPlan *p)
+// one of 8 (bf16: two).
+void weights_plan(const eakvd_window *b, int n_q, int n_kv, bool bf16, WeightsPlan *p)
 {
     memset(p, 0, sizeof(*p));
     WeightsJob &j = p->job;
@@ -359,7 +363,7 @@ void weights_plan(const eakvd_window *b, int n_q, int n_kv, WeightsPlan *p)
     p->store = rows <= kStore;
     p->tiles = (int)((rows + 15) / 16 < kRowTiles ? (rows + 15) / 16 : kRowTiles);
     p->waves = p->tiles <= 2 ? 4 : 8;
-    const int64_t slots = (p->waves == 4 ? 3 : 1) * cu_count(), share = (tiles + slots - 1) / slots;
+    const int64_t slots = (p->waves == 4 ? 3 : bf16 ? 2 : 1) * cu_count(), share = (tiles + slots - 1) / slots;
     for (int i = 0; i < j.n_seq; i++) {
         const int64_t t = (int64_t)j.start[i] + j.ntok[i], n_t = (t + kTile - 1) / kTile;
         int64_t mc = (n_t + share - 1) / share;
@@ -419,10 +423,10 @@ int launch(const eakvd_geom &g, const WeightsPlan &p, const void *q, void *work,
 
 }  // namespace
 
-extern "C" size_t eakvd_weights_work_bytes(const eakvd_window *b, int n_q, int n_kv)
+extern "C" size_t eakvd_weights_work_bytes(const eakvd_window *b, int n_q, int n_kv, int bf16)
 {
     WeightsPlan p;
-    weights_plan(b, n_q, n_kv, &p);
+    weights_plan(b, n_q, n_kv, bf16, &p);
     return p.bytes;
 }
 
@@ -430,7 +434,7 @@ extern "C" int eakvd_weights(const eakvd_geom *g, const eakvd_window *b, int lay
                              int n_q, int n_kv, float keep, float *out, int64_t ld, void *work, void *stream)
 {
     WeightsPlan p;
-    weights_plan(b, n_q, n_kv, &p);
+    weights_plan(b, n_q, n_kv, bf16, &p);
     if (p.job.n_seq == 0) return 0;
     p.job.layer = layer;
     const hipStream_t st = (hipStream_t)stream;
