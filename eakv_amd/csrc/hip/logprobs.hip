@@ -7,14 +7,20 @@
 // Both terms of H are positive, so that sharp distributions cancel nothing.
 //
 // The logits are read once.  A block takes a segment of kSeg values of a row in registers, 64
-// to a lane: first the maximum, then S and the sum of H in its terms, and the segment's
-// alternatives.  These are found by a bound that at least k values reach (of the lanes'
-// maxima, k reach it in some wave): the few values that do go to LDS and are ranked by
+// to a lane (bf16: two to a register): first the maximum, then S and the sum of H in its terms,
+// and the segment's alternatives.  These are found by a bound that at least k values reach (in
+// every wave the maxima of k / 4 lanes do): the few values that do go to LDS and are ranked by
 // counting.  Where more reach it than LDS holds (many equal values), they are taken one
 // after the other.  Order: larger first, equal ones by position, a whole number of both.
 // A second launch joins the segments of a row (one segment: none).
+//
+// Exponents are z = x log2(e) - c, one instruction, c = M log2(e) rounded: all are off by the
+// same r = M log2(e) - c, which S, T and H are rid of at the end (S 2^-r).  (From 2^20 on r is
+// not small: differences first.)
 #include <math.h>
 #include <string.h>
+
+#include <type_traits>
 
 #include "common.h"
 
@@ -23,7 +29,10 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kEach = 64;
 constexpr int kSeg = kThreads * kEach;
-constexpr int kCand = 1024;             // candidates that LDS holds
+static_assert(kThreads == 256, "four waves");
+constexpr int kCand = 256;              // candidates that LDS holds for each wave
+constexpr int kGroups = 128;            // and groups of 8 values with one
+constexpr int kHeld = 512;              // keys of a row's segments that its joining wave holds
 
 struct LpJob {
     int vocab, k, n_seg;
@@ -32,7 +41,7 @@ struct LpJob {
     const int32_t *token;
     float *lp, *entropy, *top_lp;
     int32_t *top;
-    float *part;                        // [row][seg][4]: M, S, T
+    float *part;                        // [row][seg][4]: M, S, T, r
     uint64_t *list;                     // [row][seg][k]
 };
 
@@ -69,19 +78,16 @@ __device__ __forceinline__ float logit(const void *x, int64_t at)
     else return ((const float *)x)[at];
 }
 
-// A row's results from M, S, T (in units of ln 2) and its sorted alternatives.
-template <bool BF16>
-__device__ __forceinline__ void finish(const LpJob &J, int64_t row, float m, double s, double t,
-                                       const u64 *best, int tid)
+// A row's results from M, S, T (in units of ln 2), the given token's logit and the sorted
+// alternatives.
+__device__ __forceinline__ void finish(const LpJob &J, int64_t row, float m, double s, double t, int token,
+                                       float given, const u64 *best, int tid)
 {
     const double ln_s = log(s);
     if (tid == 0) {
-        if (J.lp) {
-            const int x = J.token[row];
-            const bool in = x >= 0 && x < J.vocab;
-            J.lp[row] = in ? (float)((double)logit<BF16>(J.x, row * J.ld + x) - (double)m - ln_s)
-                           : -__builtin_inff();
-        }
+        if (J.lp)
+            J.lp[row] = token >= 0 && token < J.vocab ? (float)((double)given - (double)m - ln_s)
+                                                      : -__builtin_inff();
         if (J.entropy) J.entropy[row] = (float)(ln_s - 0.6931471805599453 * (t / s));
     }
     if (tid < J.k) {
@@ -92,28 +98,62 @@ __device__ __forceinline__ void finish(const LpJob &J, int64_t row, float m, dou
     }
 }
 
-// best[0..k): the largest of n keys in order, 0 where there are fewer.  n <= kCand (all the
-// block's threads; the keys differ).
-__device__ __forceinline__ void rank(const u64 *cand, int n, u64 *best, int k, int tid)
+// S and T of terms whose exponents are all off by r
+__device__ __forceinline__ void put_right(double r, double &s, double &t)
 {
+    t = exp2(-r) * (t - r * s);
+    s = exp2(-r) * s;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+// best[0..k): the largest of the keys in order, 0 where there are fewer.  cand: a list for each wave,
+// n[w] <= kCand keys, all different.  All the block's threads.
+__device__ __forceinline__ void rank(const u64 (*cand)[kCand], const int *n, u64 *best, int k, int tid)
+{
+    const int lane = tid & 63, w = tid >> 6;
     if (tid < k) best[tid] = 0;
     __syncthreads();
-    for (int i = tid; i < n; i += kThreads) {
-        const u64 mine = cand[i];
+    for (int i = lane; i < n[w]; i += 64) {
+        const u64 mine = cand[w][i];
         int r = 0;
-        for (int j = 0; j < n; j++) r += cand[j] > mine;
+        for (int v = 0; v < kThreads / 64; v++) {
+            const int m = n[v];
+#pragma unroll 4
+            for (int j = 0; j < m; j++) r += cand[v][j] > mine;
+        }
         if (r < k && mine) best[r] = mine;
     }
     __syncthreads();
 }
 
-template <bool BF16>
+// A bound that the maxima of k lanes of a wave reach, in 16 bits of a float's order (-inf: fewer
+// lanes have one).
+__device__ __forceinline__ float reached(float top, int k)
+{
+    const uint32_t b = __float_as_uint(top + 0.0f);
+    const uint32_t key = top > -__builtin_inff() ? b ^ (b >> 31 ? 0xffffffffu : 0x80000000u) : 0;
+    uint32_t t = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 16; bit--)
+        if ((int)__popcll(__ballot(key >= (t | 1u << bit))) >= k) t |= 1u << bit;
+    return t ? __uint_as_float(t >> 31 ? t ^ 0x80000000u : ~t) : -__builtin_inff();
+}
+
+// TOP, ENT: whether alternatives and entropies are wanted.
+template <bool BF16, bool TOP, bool ENT>
 __global__ __launch_bounds__(kThreads, 4) void logprob_kernel(LpJob J)
 {
-    constexpr int V = BF16 ? 8 : 4, NV = kEach / V;
-    __shared__ u64 cand[kCand], best[EAKVD_TOP_MAX], wbest[kThreads / 64];
+    constexpr int V = BF16 ? 8 : 4, NV = kEach / V, NX = BF16 ? kEach / 2 : kEach;
+    __shared__ u64 cand[kThreads / 64][TOP ? kCand : 1], best[EAKVD_TOP_MAX], wbest[kThreads / 64];
     __shared__ float red[3][kThreads / 64];
-    __shared__ int n_cand;
+    __shared__ int n_cand[kThreads / 64], n_group[kThreads / 64];
+    __shared__ uint16_t groups[kThreads / 64][TOP ? kGroups : 1];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int64_t row = blockIdx.x / J.n_seg;
     const int seg = (int)(blockIdx.x - row * J.n_seg);
@@ -122,96 +162,141 @@ __global__ __launch_bounds__(kThreads, 4) void logprob_kernel(LpJob J)
     const int shift = (int)(((uintptr_t)J.x / (BF16 ? 2 : 4) + (uint64_t)at) % V);
     const int i0 = seg * kSeg + V * tid - shift;        // of the lane's first vector
     const float none = -__builtin_inff();
-    float x[kEach];
+    uint32_t raw[NX];
+    auto x = [&](int e) __attribute__((always_inline)) {
+        if constexpr (BF16) return __uint_as_float(e & 1 ? raw[e >> 1] & 0xffff0000u : raw[e >> 1] << 16);
+        else return __uint_as_float(raw[e]);
+    };
+    typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int i = i0 + j * kThreads * V;
+        v4u y;
         if (i >= 0 && i + V <= J.vocab) {
-            if constexpr (BF16) {
-                typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-                const v4u y = __builtin_nontemporal_load((const v4u *)((const uint16_t *)J.x + at + i));
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    x[j * V + e] = __uint_as_float(e & 1 ? y[e >> 1] & 0xffff0000u : y[e >> 1] << 16);
-            } else {
-                const v4f y = __builtin_nontemporal_load((const v4f *)((const float *)J.x + at + i));
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[j * V + e] = y[e];
-            }
+            y = __builtin_nontemporal_load((const v4u *)((const uint8_t *)J.x + (at + i) * (BF16 ? 2 : 4)));
         } else {
 #pragma unroll
-            for (int e = 0; e < V; e++)
-                x[j * V + e] = i + e >= 0 && i + e < J.vocab ? logit<BF16>(J.x, at + i + e) : none;
+            for (int e = 0; e < 4; e++) {
+                auto word = [&](int k) {
+                    return i + k >= 0 && i + k < J.vocab ? __float_as_uint(logit<BF16>(J.x, at + i + k)) : 0xff800000u;
+                };
+                if constexpr (BF16) y[e] = word(2 * e) >> 16 | word(2 * e + 1);
+                else y[e] = word(e);
+            }
         }
-    }
-    if (tid == 0) n_cand = 0;
-    float top = x[0];
 #pragma unroll
-    for (int e = 1; e < kEach; e++) top = fmaxf(top, x[e]);
-    // the wave's bound: the largest top half of a float's order that k lanes reach
-    float thr = none;
-    if (J.k) {
-        const uint32_t b = __float_as_uint(top + 0.0f);
-        const uint32_t key = top > none ? b ^ (b >> 31 ? 0xffffffffu : 0x80000000u) : 0;
-        uint32_t t = 0;
-        for (int bit = 31; bit >= 12; bit--)
-            if ((int)__popcll(__ballot(key >= (t | 1u << bit))) >= J.k) t |= 1u << bit;
-        thr = t ? __uint_as_float(t >> 31 ? t ^ 0x80000000u : ~t) : none;
+        for (int e = 0; e < 4; e++) raw[j * 4 + e] = y[e];
     }
+    // (two values of a register are taken apart where they are used, not kept apart)
+    auto hold = [&]() __attribute__((always_inline)) {
+        if constexpr (BF16)
+#pragma unroll
+            for (int k = 0; k < NX; k++) asm("" : "+v"(raw[k]));
+    };
+    float high[kEach / 8];                              // of 8 values each
+#pragma unroll
+    for (int j = 0; j < kEach / 8; j++)
+        high[j] = max3(max3(max3(x(8 * j), x(8 * j + 1), x(8 * j + 2)), x(8 * j + 3), x(8 * j + 4)),
+                       max3(x(8 * j + 5), x(8 * j + 6), x(8 * j + 7)), x(8 * j + 7));
+    const float top = max3(max3(max3(high[0], high[1], high[2]), high[3], high[4]), max3(high[5], high[6], high[7]),
+                           high[7]);
+    hold();
+    const float bound = TOP ? reached(top, (J.k + 3) / 4) : none;
     float m = wave_max(top);
     if (lane == 0) {
         red[0][w] = m;
-        red[1][w] = thr;
+        red[1][w] = bound;
     }
     __syncthreads();
     m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    thr = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+    float thr = fminf(fminf(red[1][0], red[1][1]), fminf(red[1][2], red[1][3]));
     __syncthreads();
+    if (TOP && thr == none) {
+        // a wave has too few: what k lanes of one reach
+        const float b = reached(top, J.k);
+        if (lane == 0) red[2][w] = b;
+        __syncthreads();
+        thr = fmaxf(fmaxf(red[2][0], red[2][1]), fmaxf(red[2][2], red[2][3]));
+    }
     // (nothing but -inf: every term is 0)
     const float from = m == none ? 0.0f : m;
-    float s = 0.0f, t = 0.0f;
+    const float c = from * EAKV_LOG2E;
+    float r = fmaf(from, EAKV_LOG2E, -c), s = 0.0f, t = 0.0f;
 #pragma unroll
     for (int e = 0; e < kEach; e++) {
-        const float z = (x[e] - from) * EAKV_LOG2E, p = __builtin_amdgcn_exp2f(z);
+        const float z = fmaf(x(e), EAKV_LOG2E, -c), p = __builtin_amdgcn_exp2f(z);
         s += p;
-        t = fmaf(p, fmaxf(z, -1000.0f), t);     // (a term of 0, not NaN, for -inf)
+        if constexpr (ENT) t = fmaf(p, fmaxf(z, -1000.0f), t);      // (a term of 0, not NaN, for -inf)
     }
+    if (!(fabsf(from) < 0x1p20f)) {
+        // r is not small: from differences, read again
+        s = t = r = 0.0f;
+        for (int i = max(seg * kSeg - shift, 0) + tid; i < min((seg + 1) * kSeg - shift, J.vocab); i += kThreads) {
+            const float z = (logit<BF16>(J.x, at + i) - from) * EAKV_LOG2E, p = __builtin_amdgcn_exp2f(z);
+            s += p;
+            t = fmaf(p, fmaxf(z, -1000.0f), t);
+        }
+    }
+    hold();
     s = wave_sum(s);
-    t = wave_sum(t);
+    if constexpr (ENT) t = wave_sum(t);
     if (lane == 0) {
         red[0][w] = s;
         red[1][w] = t;
     }
-    if (J.k && top >= thr) {
+    // groups of 8 with a value that reaches the bound
+    if constexpr (TOP) {
+        int found = 0;
 #pragma unroll
-        for (int j = 0; j < kEach; j += 8) {
-            float most = x[j];
-#pragma unroll
-            for (int e = 1; e < 8; e++) most = fmaxf(most, x[j + e]);
-            if (most >= thr)
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (x[j + e] >= thr && x[j + e] > none) {
-                        const int p = atomicAdd(&n_cand, 1);
-                        const int v = (j + e) / V;
-                        if (p < kCand) cand[p] = key_of(x[j + e], i0 + v * kThreads * V + (j + e) % V);
-                    }
+        for (int j = 0; j < kEach / 8; j++) {
+            const bool in = high[j] >= thr && high[j] > none;
+            const uint64_t b = __ballot(in);
+            if (b == 0) continue;
+            const int p = found + (int)__popcll(b & ((1ull << lane) - 1));
+            if (in && p < kGroups) groups[w][p] = (uint16_t)(tid * (kEach / 8) + j);
+            found += (int)__popcll(b);
         }
+        if (lane == 0) n_group[w] = found;
     }
     __syncthreads();
     s = (red[0][0] + red[0][1]) + (red[0][2] + red[0][3]);
     t = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-    if (J.k) {
-        if (n_cand <= kCand) {
+    if constexpr (TOP) {
+        // their values, one to a thread, read again
+        const int g0 = n_group[0], g1 = g0 + n_group[1], g2 = g1 + n_group[2], all = g2 + n_group[3];
+        bool fits = max(max(n_group[0], n_group[1]), max(n_group[2], n_group[3])) <= kGroups && all <= 4 * kGroups;
+        if (fits) {
+            int found = 0;
+            for (int q0 = 0; q0 < 8 * all; q0 += kThreads) {
+                const int q = q0 + tid, g = q >> 3;
+                u64 key = 0;
+                if (g < all) {
+                    const int v = (g >= g0) + (g >= g1) + (g >= g2);
+                    const int id = groups[v][g - (v == 0 ? 0 : v == 1 ? g0 : v == 2 ? g1 : g2)];
+                    const int e = id % (kEach / 8) * 8 + (q & 7);
+                    const int i = seg * kSeg + V * (id / (kEach / 8)) - shift + e / V * kThreads * V + e % V;
+                    if (i >= 0 && i < J.vocab) {
+                        const float y = logit<BF16>(J.x, at + i);
+                        key = y >= thr ? key_of(y, i) : 0;
+                    }
+                }
+                const uint64_t b = __ballot(key != 0);
+                const int p = found + (int)__popcll(b & ((1ull << lane) - 1));
+                if (key && p < kCand) cand[w][p] = key;
+                found += (int)__popcll(b);
+            }
+            if (lane == 0) n_cand[w] = found;
+            fits = !__syncthreads_or(found > kCand);
+        }
+        if (fits) {
             rank(cand, n_cand, best, J.k, tid);
         } else {
-            // one after the other
+            // one after the other, read again
             u64 prev = ~0ull;
             for (int r = 0; r < J.k; r++) {
                 u64 mine = 0;
-#pragma unroll
-                for (int e = 0; e < kEach; e++) {
-                    const u64 key = key_of(x[e], i0 + e / V * kThreads * V + e % V);
+                for (int i = max(seg * kSeg - shift, 0) + tid; i < min((seg + 1) * kSeg - shift, J.vocab); i += kThreads) {
+                    const u64 key = key_of(logit<BF16>(J.x, at + i), i);
                     mine = key < prev && key > mine ? key : mine;
                 }
                 mine = wave_max64(mine);
@@ -225,51 +310,110 @@ __global__ __launch_bounds__(kThreads, 4) void logprob_kernel(LpJob J)
         }
     }
     if (J.n_seg == 1) {
-        finish<BF16>(J, row, from, s, t, best, tid);
+        double sd = s, td = t;
+        put_right(r, sd, td);
+        const int token = J.lp ? J.token[row] : -1;
+        const float given = token >= 0 && token < J.vocab ? logit<BF16>(J.x, at + token) : none;
+        finish(J, row, from, sd, td, token, given, best, tid);
         return;
     }
     const int64_t p = row * J.n_seg + seg;
-    if (tid == 0) *(v4f *)(J.part + p * 4) = v4f{m, s, t, 0.0f};
+    if (tid == 0) *(v4f *)(J.part + p * 4) = v4f{m, s, t, r};
     if (tid < J.k) J.list[p * J.k + tid] = best[tid];
 }
 
-// A row's segments joined, a block to a row.
+// A row's segments joined, a wave to a row.  Alternatives: every segment's list is sorted, so the
+// least of the lists' n-th entries, n = k / segments, is reached by k keys; those that do are
+// ranked by counting (or, where the lists are more than LDS holds, taken one after the other).
 template <bool BF16>
-__global__ __launch_bounds__(kThreads) void logprob_join_kernel(LpJob J)
+__global__ __launch_bounds__(kThreads) void logprob_join_kernel(LpJob J, int n_rows)
 {
-    __shared__ u64 cand[kCand], best[EAKVD_TOP_MAX];
-    const int64_t row = blockIdx.x;
-    const int tid = threadIdx.x;
-    const float *part = J.part + row * J.n_seg * 4;
-    float m = -__builtin_inff();
-    for (int i = 0; i < J.n_seg; i++) m = fmaxf(m, part[4 * i]);
-    const float from = m == -__builtin_inff() ? 0.0f : m;
+    __shared__ u64 cands[kThreads / 64][kHeld], bests[kThreads / 64][EAKVD_TOP_MAX];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, k = J.k, n_seg = J.n_seg;
+    const int64_t row = (int64_t)blockIdx.x * (kThreads / 64) + w;
+    if (row >= n_rows) return;
+    u64 *cand = cands[w], *best = bests[w];
+    const float none = -__builtin_inff();
+    const v4f *part = (const v4f *)J.part + row * n_seg;
+    // all loads at once: the lists, the segments' sums, the given token's logit
+    const u64 *list = J.list + row * n_seg * k;
+    const int all = n_seg * k;
+    u64 key[kHeld / 64];
+#pragma unroll
+    for (int i = 0; i < kHeld / 64; i++) key[i] = lane + 64 * i < all ? list[lane + 64 * i] : 0;
+    const int token = J.lp ? J.token[row] : -1;
+    const v4f first = part[min(lane, n_seg - 1)];
+    const float given = token >= 0 && token < J.vocab ? logit<BF16>(J.x, row * J.ld + token) : none;
+    float m = lane < n_seg ? first[0] : none;
+    for (int i = lane + 64; i < n_seg; i += 64) m = fmaxf(m, part[i][0]);
+    m = wave_max(m);
+    const float from = m == none ? 0.0f : m;
     double s = 0.0, t = 0.0;
-    for (int i = 0; i < J.n_seg; i++) {
-        const v4f x = *(const v4f *)(part + 4 * i);
-        const float mine = x[0] == -__builtin_inff() ? 0.0f : x[0];
+    for (int i = lane; i < n_seg; i += 64) {
+        const v4f x = i < 64 ? first : part[i];
+        const float mine = x[0] == none ? 0.0f : x[0];
         // (a segment of -inf has S = 0, at any M)
-        const double d = ((double)mine - (double)from) * 1.4426950408889634, f = exp2(d);
         if (x[1] == 0.0f) continue;
-        s += f * (double)x[1];
-        if (f != 0.0) t += f * ((double)x[2] + (double)x[1] * d);
+        double si = x[1], ti = x[2];
+        put_right(x[3], si, ti);
+        const double d = ((double)mine - (double)from) * 1.4426950408889634, f = exp2(d);
+        s += f * si;
+        if (f != 0.0) t += f * (ti + si * d);
     }
-    if (J.k) {
-        // the lists' keys, kCand at a time, beside the best so far
-        const int all = J.n_seg * J.k;
-        int n = 0;
-        for (int a = 0; a < all;) {
-            const int more = min(kCand - n, all - a);
-            __syncthreads();
-            for (int i = tid; i < n; i += kThreads) cand[i] = best[i];
-            for (int i = tid; i < more; i += kThreads) cand[n + i] = J.list[row * all + a + i];
-            __syncthreads();
-            rank(cand, n + more, best, J.k, tid);
-            a += more;
-            n = J.k;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        s += __shfl_xor(s, o, 64);
+        t += __shfl_xor(t, o, 64);
+    }
+    if (k) {
+        const int n = (k + n_seg - 1) / n_seg;
+        int found = kHeld + 1;
+        if (all <= kHeld) {
+#pragma unroll
+            for (int i = 0; i < kHeld / 64; i++) cand[lane + 64 * i] = key[i];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            u64 least = ~0ull;
+            for (int i = lane; i < n_seg; i += 64) {
+                const u64 x = cand[i * k + n - 1];
+                least = x < least ? x : least;
+            }
+            least = ~wave_max64(~least);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            found = 0;
+#pragma unroll
+            for (int i = 0; i < kHeld / 64; i++) {
+                const bool in = key[i] != 0 && key[i] >= least;
+                const uint64_t b = __ballot(in);
+                const int p = found + (int)__popcll(b & ((1ull << lane) - 1));
+                if (in) cand[p] = key[i];
+                found += (int)__popcll(b);
+            }
         }
+        if (lane < k) best[lane] = 0;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (found <= kHeld) {
+            for (int i = lane; i < found; i += 64) {
+                const u64 mine = cand[i];
+                int r = 0;
+#pragma unroll 4
+                for (int j = 0; j < found; j++) r += cand[j] > mine;
+                if (r < k) best[r] = mine;
+            }
+        } else {
+            u64 prev = ~0ull;
+            for (int r = 0; r < k; r++) {
+                u64 mine = 0;
+                for (int i = lane; i < all; i += 64) {
+                    const u64 x = list[i];
+                    mine = x < prev && x > mine ? x : mine;
+                }
+                prev = wave_max64(mine);
+                if (lane == 0) best[r] = prev;
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    finish<BF16>(J, row, from, s, t, best, tid);
+    finish(J, row, from, s, t, token, given, best, lane);
 }
 
 // (a row's first vector may begin up to 7 places before it)
@@ -301,10 +445,17 @@ extern "C" int eakvd_logprobs(int n_rows, int vocab, const void *logits, int bf1
     J.part = (float *)work;
     J.list = (u64 *)((uint8_t *)work + (size_t)n_rows * J.n_seg * 16);
     const hipStream_t st = (hipStream_t)stream;
-    const dim3 grid((unsigned)((int64_t)n_rows * J.n_seg)), rows((unsigned)n_rows), nt(kThreads);
-    auto *kern = bf16 ? logprob_kernel<true> : logprob_kernel<false>;
+    const dim3 grid((unsigned)((int64_t)n_rows * J.n_seg)), nt(kThreads);
+    const dim3 rows((unsigned)((n_rows + kThreads / 64 - 1) / (kThreads / 64)));
+    const bool top = n_top > 0, ent = entropy != nullptr;
+    auto pick = [&](auto b) {
+        constexpr bool B = decltype(b)::value;
+        return top ? (ent ? logprob_kernel<B, true, true> : logprob_kernel<B, true, false>)
+                   : (ent ? logprob_kernel<B, false, true> : logprob_kernel<B, false, false>);
+    };
+    auto *kern = bf16 ? pick(std::true_type()) : pick(std::false_type());
     auto *join = bf16 ? logprob_join_kernel<true> : logprob_join_kernel<false>;
     hipLaunchKernelGGL(kern, grid, nt, 0, st, J);
-    if (J.n_seg > 1) hipLaunchKernelGGL(join, rows, nt, 0, st, J);
+    if (J.n_seg > 1) hipLaunchKernelGGL(join, rows, nt, 0, st, J, n_rows);
     return (int)hipGetLastError();
 }
