@@ -2,8 +2,8 @@
 // the others those of largest score, ties to the lower position; positions ascending, as a
 // gather takes them.  score[t] = the heads' weights, summed in f64 and rounded to f32.
 //
-// Scores become whole numbers in their order (u32); the keep-th largest is found bit by
-// bit, then every token knows its place from counts of the tokens before it.  Counts alone are
+// Scores become whole numbers in their order (u32); the keep-th largest is found by
+// histograms of 8 to 11 of its bits at a time, then every token knows its place from counts of the tokens before it.  Counts alone are
 // shared between blocks: the same list on every call.
 //
 // Up to kOneMost tokens: one launch, a block to a sequence, the numbers in registers.
@@ -16,10 +16,9 @@
 namespace {
 
 constexpr int kOneThreads = 1024;
-constexpr int kOneEach = 16;
-constexpr int kOneMost = kOneThreads * kOneEach;
+constexpr int kOneMost = kOneThreads * 8;
 constexpr int kPartThreads = 256;
-constexpr int kPartEach = 16;
+constexpr int kPartEach = 8;
 constexpr int kPart = kPartThreads * kPartEach;
 
 struct EvictJob {
@@ -35,27 +34,70 @@ struct EvictJob {
     int parts;
 };
 
-// Positions in the order of their scores; NaN below everything, the tokens that stay anyway
-// above.
-__device__ __forceinline__ uint32_t key_of(const EvictJob &J, int s, int t, int n)
+// Scores in their order: NaN below everything, the tokens that stay anyway above.
+__device__ __forceinline__ uint32_t key_of(const EvictJob &J, int t, int n, double sum)
 {
     if (t < J.e.n_first || t >= n - J.e.n_recent) return 0xffffffffu;
-    const float *w = J.weights + (int64_t)s * J.e.n_heads * J.ld + t;
-    double sum = 0.0;
-    for (int h = 0; h < J.e.n_heads; h++) sum += (double)w[h * J.ld];
     const float x = (float)sum + 0.0f;          // (-0 as 0)
     const uint32_t b = __float_as_uint(x);
     return x != x ? 0u : b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
 }
 
-// Token t of sequence s stays, as the rank-th.
-__device__ __forceinline__ void put(const EvictJob &J, int s, int t, int rank)
+// Keys of E tokens `step` apart from t0 on (0 from `end` on) of a sequence of n: heads H at a time, all their loads
+// in flight.  A head's sum is in its order, whatever H.  x: the last H heads' weights.
+template <int E>
+constexpr int kHeadsOf = E > 8 ? 2 : 32 / E > 8 ? 8 : 32 / E;
+template <int E>
+__device__ __forceinline__ void load_heads(const EvictJob &J, int s, int t0, int step, int n, int h0,
+                                           float (&x)[E][kHeadsOf<E>])
 {
-    J.index[J.e.first[s] + rank] = t;
-    if (J.kept) {
-        const float *w = J.weights + (int64_t)s * J.e.n_heads * J.ld + t;
-        float *k = J.kept + (int64_t)s * J.e.n_heads * J.ld_kept + rank;
-        for (int h = 0; h < J.e.n_heads; h++) k[h * J.ld_kept] = w[h * J.ld];
+    const float *w = J.weights + (int64_t)s * J.e.n_heads * J.ld;
+#pragma unroll
+    for (int h = 0; h < kHeadsOf<E>; h++)
+#pragma unroll
+        for (int i = 0; i < E; i++)
+            x[i][h] = w[(int64_t)min(h0 + h, J.e.n_heads - 1) * J.ld + min(t0 + i * step, n - 1)];
+}
+template <int E>
+__device__ __forceinline__ void keys_of(const EvictJob &J, int s, int t0, int step, int end, int n, uint32_t *key,
+                                        float (&x)[E][kHeadsOf<E>])
+{
+    constexpr int H = kHeadsOf<E>;
+    double sum[E];
+#pragma unroll
+    for (int i = 0; i < E; i++) sum[i] = 0.0;
+    for (int h0 = 0; h0 < J.e.n_heads; h0 += H) {
+        load_heads<E>(J, s, t0, step, n, h0, x);
+#pragma unroll
+        for (int h = 0; h < H; h++)
+#pragma unroll
+            for (int i = 0; i < E; i++)
+                if (h0 + h < J.e.n_heads) sum[i] += (double)x[i][h];
+    }
+#pragma unroll
+    for (int i = 0; i < E; i++) key[i] = t0 + i * step < end ? key_of(J, t0 + i * step, n, sum[i]) : 0u;
+}
+
+// Tokens t0 + i * step of sequence s stay, as the rank[i]-th (-1: do not): x holds their weights of
+// up to kHeadsOf heads, else they are read again, all tokens' loads of some heads in flight.
+template <int E>
+__device__ __forceinline__ void put_all(const EvictJob &J, int s, int t0, int step, int n, const int *rank,
+                                        float (&x)[E][kHeadsOf<E>])
+{
+    constexpr int H = kHeadsOf<E>;
+    int32_t *index = J.index + J.e.first[s];
+#pragma unroll
+    for (int i = 0; i < E; i++)
+        if (rank[i] >= 0) index[rank[i]] = t0 + i * step;
+    if (!J.kept) return;
+    float *k = J.kept + (int64_t)s * J.e.n_heads * J.ld_kept;
+    for (int h0 = 0; h0 < J.e.n_heads; h0 += H) {
+        if (J.e.n_heads > H) load_heads<E>(J, s, t0, step, n, h0, x);
+#pragma unroll
+        for (int h = 0; h < H; h++)
+#pragma unroll
+            for (int i = 0; i < E; i++)
+                if (rank[i] >= 0 && h0 + h < J.e.n_heads) k[(h0 + h) * J.ld_kept + rank[i]] = x[i][h];
     }
 }
 
@@ -70,9 +112,22 @@ __device__ __forceinline__ void clear_rest(const EvictJob &J, int s, int i, int 
     }
 }
 
+// The sum of the lanes 4 apart: two rotations in a row of 16, two exchanges between rows.
+__device__ __forceinline__ int over_waves(int v)
+{
+    v += __builtin_amdgcn_mov_dpp(v, 0x124, 0xf, 0xf, true);
+    v += __builtin_amdgcn_mov_dpp(v, 0x128, 0xf, 0xf, true);
+    auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = (int)(r[0] + r[1]);
+    r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return (int)(r[0] + r[1]);
+}
+
+template <int E>
 __global__ __launch_bounds__(kOneThreads) void evict_one_kernel(EvictJob J)
 {
-    __shared__ int sums[2][16][3];
+    __shared__ int sums[64];                    // [wave][4]
+    __shared__ __align__(16) uint32_t hist[4][1024];
     const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int n = J.e.n_tokens[s], keep = J.e.n_keep[s];
     clear_rest(J, s, tid, kOneThreads);
@@ -80,73 +135,77 @@ __global__ __launch_bounds__(kOneThreads) void evict_one_kernel(EvictJob J)
     // token (w * each + i) * 64 + lane
     const int each = (n + kOneThreads - 1) / kOneThreads;
     const int t0 = w * each * 64 + lane;
-    uint32_t key[kOneEach];
-#pragma unroll
-    for (int i = 0; i < kOneEach; i++) {
-        const int t = t0 + 64 * i;
-        key[i] = i < each && t < n ? key_of(J, s, t, n) : 0u;
-    }
-    // the largest threshold that at least `keep` keys reach, two bits at a time.  (Tokens behind
-    // the last have key 0, as the lowest have: they count for threshold 0 alone.)
+    uint32_t key[E];
+    float x[E][kHeadsOf<E>];
+    *(uint4 *)&hist[tid >> 8][(tid & 255) * 4] = uint4{0, 0, 0, 0};
+    __syncthreads();
+    keys_of<E>(J, s, t0, 64, min(n, (w + 1) * each * 64), n, key, x);
+    // the keep-th largest key, 8 bits at a time: a histogram in LDS (four copies, as neighbouring lanes
+    // often meet in one bin), which every wave searches for itself
     uint32_t thr = 0;
-    int reach = INT32_MAX, it = 0;              // keys that reach thr, where known
-    for (int bit = 30; bit >= 0; bit -= 2, it ^= 1) {
-        int c[3] = {0, 0, 0};
+    int ties = keep;                            // of the keys that have the bits known
 #pragma unroll
-        for (int i = 0; i < kOneEach; i++) {
-            if (i < each)
+    for (int p = 0; p < 4; p++) {
+        const int shift = 24 - 8 * p;
 #pragma unroll
-                for (int k = 0; k < 3; k++)
-                    c[k] += (int)__popcll(__ballot(key[i] >= thr + ((uint32_t)(k + 1) << bit)));
-        }
-        if (lane < 3) sums[it][w][lane] = lane == 0 ? c[0] : lane == 1 ? c[1] : c[2];
+        for (int i = 0; i < E; i++)
+            if (i < each && t0 + 64 * i < n && (p == 0 || key[i] >> (32 - 8 * p) == thr))
+                atomicAdd(&hist[p][(key[i] >> shift & 255) * 4 + (lane & 3)], 1u);
         __syncthreads();
-        int all[3] = {0, 0, 0};
-        for (int i = 0; i < 16; i++)
+        // lane l: digits 255 - 4 l down to 252 - 4 l
+        int c[4], sum = 0;
 #pragma unroll
-            for (int k = 0; k < 3; k++) all[k] += sums[it][i][k];
+        for (int k = 0; k < 4; k++) {
+            const uint4 x = *(const uint4 *)&hist[p][(255 - 4 * lane - k) * 4];
+            c[k] = (int)(x.x + x.y + x.z + x.w);
+            sum += c[k];
+        }
+        int upto = sum;
 #pragma unroll
-        for (int k = 2; k >= 0; k--)
-            if (all[k] >= keep) {
-                thr += (uint32_t)(k + 1) << bit;
-                reach = all[k];
-                break;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(upto, o, 64);
+            if (lane >= o) upto += u;
+        }
+        const int at = __ffsll((unsigned long long)__ballot(upto >= ties)) - 1;
+        int before = __builtin_amdgcn_readlane(upto - sum, at), d = 255 - 4 * at;
+#pragma unroll
+        for (int k = 0; k < 3; k++) {
+            const int n_k = __builtin_amdgcn_readlane(c[k], at);
+            if (d == 255 - 4 * at - k && before + n_k < ties) {
+                before += n_k;
+                d--;
             }
-        if (reach == keep) break;
+        }
+        ties -= before;
+        thr = thr << 8 | (uint32_t)d;
     }
     // larger than thr: all; equal: the first `ties`
-    __syncthreads();
     int gt = 0, eq = 0;
 #pragma unroll
-    for (int i = 0; i < kOneEach; i++) {
+    for (int i = 0; i < E; i++) {
         const bool in = i < each && t0 + 64 * i < n;
         gt += (int)__popcll(__ballot(in && key[i] > thr));
         eq += (int)__popcll(__ballot(in && key[i] == thr));
     }
-    if (lane == 0) {
-        sums[0][w][0] = gt;
-        sums[0][w][1] = eq;
-    }
+    if (lane < 2) sums[4 * w + lane] = lane ? eq : gt;
     __syncthreads();
-    int gt_all = 0, gt_before = 0, eq_before = 0;
-    for (int i = 0; i < 16; i++) {
-        gt_all += sums[0][i][0];
-        gt_before += i < w ? sums[0][i][0] : 0;
-        eq_before += i < w ? sums[0][i][1] : 0;
-    }
-    const int ties = keep - gt_all;
+    const int mine4 = sums[lane];
+    const int before = over_waves(lane >> 2 < w ? mine4 : 0);
+    int gt_before = __builtin_amdgcn_readlane(before, 0), eq_before = __builtin_amdgcn_readlane(before, 1);
+    int rank[E];
 #pragma unroll
-    for (int i = 0; i < kOneEach; i++) {
+    for (int i = 0; i < E; i++) {
         const int t = t0 + 64 * i;
         const bool in = i < each && t < n;
         const uint64_t below = (1ull << lane) - 1;
         const uint64_t g = __ballot(in && key[i] > thr), e = __ballot(in && key[i] == thr);
         const int eq_at = eq_before + (int)__popcll(e & below);
         const bool mine = (g >> lane & 1) || ((e >> lane & 1) && eq_at < ties);
-        if (mine) put(J, s, t, gt_before + (int)__popcll(g & below) + min(eq_at, ties));
+        rank[i] = mine ? gt_before + (int)__popcll(g & below) + min(eq_at, ties) : -1;
         gt_before += (int)__popcll(g);
         eq_before += (int)__popcll(e);
     }
+    put_all<E>(J, s, t0, 64, n, rank, x);
 }
 
 __global__ __launch_bounds__(256) void evict_clear_kernel(uint32_t *p, int n)
@@ -155,14 +214,19 @@ __global__ __launch_bounds__(256) void evict_clear_kernel(uint32_t *p, int n)
     if (i < n) p[i] = 0;
 }
 
-// The digit that the keep-th largest key has, of `bins` (a multiple of kPartThreads): hist[d] keys have
+// The digit that the keep-th largest key has, of BINS: hist[d] keys have
 // digit d; *above gets the keys with larger ones.  All threads of the block.
-__device__ __forceinline__ int digit_of(const uint32_t *hist, int bins, int keep, int *above, int *sh, int tid)
+template <int BINS>
+__device__ __forceinline__ int digit_of(const uint32_t *hist, int keep, int *above, int *sh, int tid)
 {
-    const int lane = tid & 63, w = tid >> 6, per = bins / kPartThreads;
+    constexpr int per = BINS / kPartThreads;
+    const int lane = tid & 63, w = tid >> 6;
     // thread 0 has the largest digits
-    int sum = 0;
-    for (int i = 0; i < per; i++) sum += (int)hist[bins - 1 - (tid * per + i)];
+    int c[BINS / kPartThreads], sum = 0;
+#pragma unroll
+    for (int i = 0; i < per; i++) c[i] = (int)hist[BINS - 1 - (tid * per + i)];
+#pragma unroll
+    for (int i = 0; i < per; i++) sum += c[i];
     int upto = sum;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -175,14 +239,13 @@ __device__ __forceinline__ int digit_of(const uint32_t *hist, int bins, int keep
     int before = upto - sum;
     for (int i = 0; i < w; i++) before += sh[i];
     if (before < keep && keep <= before + sum)
+#pragma unroll
         for (int i = 0; i < per; i++) {
-            const int d = bins - 1 - (tid * per + i), c = (int)hist[d];
-            if (keep <= before + c) {
-                sh[4] = d;
+            if (before < keep && keep <= before + c[i]) {
+                sh[4] = BINS - 1 - (tid * per + i);
                 sh[5] = before;
-                break;
             }
-            before += c;
+            before += c[i];
         }
     __syncthreads();
     *above = sh[5];
@@ -191,20 +254,22 @@ __device__ __forceinline__ int digit_of(const uint32_t *hist, int bins, int keep
     return d;
 }
 
-// What is known of the threshold after `level` histograms: its top bits, and how many keys
+// What is known of the threshold after LEVEL histograms: its top bits, and how many keys
 // with them stay.
 struct Known {
     uint32_t top;
     int keep;
 };
-__device__ __forceinline__ Known known(const EvictJob &J, int s, int level, int *sh, int tid)
+template <int LEVEL>
+__device__ __forceinline__ Known known(const EvictJob &J, int s, int *sh, int tid)
 {
     Known k = {0, J.e.n_keep[s]};
-    for (int l = 0; l < level; l++) {
+#pragma unroll
+    for (int l = 0; l < LEVEL; l++) {
         int above;
-        const int bins = l < 2 ? 2048 : 1024;
-        const int d = digit_of(J.hist + ((int64_t)s * 3 + l) * 2048, bins, k.keep, &above, sh, tid);
-        k.top = k.top * (uint32_t)bins + (uint32_t)d;
+        const uint32_t *hist = J.hist + ((int64_t)s * 3 + l) * 2048;
+        const int d = l < 2 ? digit_of<2048>(hist, k.keep, &above, sh, tid) : digit_of<1024>(hist, k.keep, &above, sh, tid);
+        k.top = k.top * (l < 2 ? 2048u : 1024u) + (uint32_t)d;
         k.keep -= above;
     }
     return k;
@@ -220,24 +285,26 @@ __global__ __launch_bounds__(kPartThreads) void evict_part_kernel(EvictJob J)
     const int s = blockIdx.y, tid = threadIdx.x, t0 = (int)blockIdx.x * kPart;
     const int n = J.e.n_tokens[s];
     if (t0 >= n || J.e.n_keep[s] == 0) return;
-    const Known k = known(J, s, LEVEL, sh, tid);
-    uint32_t *keys = J.key + (int64_t)s * J.most;
+    uint32_t *keys = J.key + (int64_t)s * J.most, key[kPartEach];
+    if constexpr (LEVEL > 0)
+#pragma unroll
+        for (int i = 0; i < kPartEach; i++) key[i] = keys[min(t0 + i * kPartThreads + tid, n - 1)];
+    const Known k = known<LEVEL>(J, s, sh, tid);
     if constexpr (LEVEL < 3) {
         for (int i = tid; i < 2048; i += kPartThreads) bins[i] = 0;
         __syncthreads();
     }
     int gt = 0, eq = 0;
+    if constexpr (LEVEL == 0) {
+        float x[kPartEach][kHeadsOf<kPartEach>];
+        keys_of<kPartEach>(J, s, t0 + tid, kPartThreads, n, n, key, x);
+    }
 #pragma unroll
     for (int i = 0; i < kPartEach; i++) {
         const int t = t0 + i * kPartThreads + tid;
-        if (t >= n) break;
-        uint32_t x;
-        if constexpr (LEVEL == 0) {
-            x = key_of(J, s, t, n);
-            keys[t] = x;
-        } else {
-            x = keys[t];
-        }
+        if (t >= n) continue;
+        const uint32_t x = key[i];
+        if constexpr (LEVEL == 0) keys[t] = x;
         if constexpr (LEVEL == 0) atomicAdd(&bins[x >> 21], 1u);
         if constexpr (LEVEL == 1) {
             if (x >> 21 == k.top) atomicAdd(&bins[x >> 10 & 2047], 1u);
@@ -272,7 +339,11 @@ __global__ __launch_bounds__(kPartThreads) void evict_write_kernel(EvictJob J)
     const int n = J.e.n_tokens[s];
     clear_rest(J, s, (int)blockIdx.x * kPartThreads + tid, (int)gridDim.x * kPartThreads);
     if (t0 >= n || J.e.n_keep[s] == 0) return;
-    const Known k = known(J, s, 3, sh, tid);
+    const uint32_t *keys = J.key + (int64_t)s * J.most;
+    uint32_t key[kPartEach];
+#pragma unroll
+    for (int i = 0; i < kPartEach; i++) key[i] = keys[min(t0 + i * kPartThreads + tid, n - 1)];
+    const Known k = known<3>(J, s, sh, tid);
     // (k.keep of the keys at the threshold stay)
     if (tid < 2) sh[tid] = 0;
     __syncthreads();
@@ -288,11 +359,12 @@ __global__ __launch_bounds__(kPartThreads) void evict_write_kernel(EvictJob J)
     }
     __syncthreads();
     int gt_before = sh[0], eq_before = sh[1];
-    const uint32_t *keys = J.key + (int64_t)s * J.most;
     const uint64_t below = (1ull << lane) - 1;
+    int rank[kPartEach];
+#pragma unroll
     for (int i = 0; i < kPartEach; i++) {
         const int t = t0 + i * kPartThreads + tid;
-        const uint32_t x = t < n ? keys[t] : 0;
+        const uint32_t x = key[i];
         const uint64_t g = __ballot(t < n && x > k.top), e = __ballot(t < n && x == k.top);
         if (lane == 0) {
             sums[i & 1][w][0] = (int)__popcll(g);
@@ -308,8 +380,11 @@ __global__ __launch_bounds__(kPartThreads) void evict_write_kernel(EvictJob J)
             gt_before += a;
             eq_before += b;
         }
-        if ((g >> lane & 1) || ((e >> lane & 1) && e_at < k.keep)) put(J, s, t, g_at + min(e_at, k.keep));
+        rank[i] = (g >> lane & 1) || ((e >> lane & 1) && e_at < k.keep) ? g_at + min(e_at, k.keep) : -1;
     }
+    float w4[kPartEach][kHeadsOf<kPartEach>];
+    if (J.kept && J.e.n_heads <= kHeadsOf<kPartEach>) load_heads<kPartEach>(J, s, t0 + tid, kPartThreads, n, 0, w4);
+    put_all<kPartEach>(J, s, t0 + tid, kPartThreads, n, rank, w4);
 }
 
 int most_of(int n_seq, const int32_t *n)
@@ -344,7 +419,8 @@ extern "C" int eakvd_evict_select(const eakvd_evict *job, const float *weights, 
     const hipStream_t st = (hipStream_t)stream;
     const unsigned n = (unsigned)job->n_seq;
     if (J.most <= kOneMost) {
-        hipLaunchKernelGGL(evict_one_kernel, dim3(n), dim3(kOneThreads), 0, st, J);
+        auto *kern = J.most <= 4 * kOneThreads ? evict_one_kernel<4> : evict_one_kernel<8>;
+        hipLaunchKernelGGL(kern, dim3(n), dim3(kOneThreads), 0, st, J);
         return (int)hipGetLastError();
     }
     J.parts = (J.most + kPart - 1) / kPart;

@@ -349,7 +349,7 @@ size_t eakv_attention_weights_work_bytes(eakv_cache_t *const *caches, int n_cach
  *   d_kept   NULL, or f32[n_seqs][n_heads][ld_kept]: the weights of the tokens that stay, in
  *            their new places, and 0 from n_keep[i] on (tokens to come have none)
  *   d_work   eakv_evict_select_work_bytes() of device scratch, 4-byte aligned, the call's own
- *            (0 bytes up to 16384 tokens)
+ *            (0 bytes up to 8192 tokens)
  * The results and d_work overlap nothing else (refused).  Asynchronous; may be recorded in a
  * graph. */
 int eakv_evict_select_device(int n_seqs, int n_heads, const float *d_weights, int64_t ld,
