@@ -2,16 +2,17 @@
 // name, both in one launch.  Rows are [token][kv head][dim], f32 or bf16, as a model's
 // projections leave them; codes, scales and biases are bit for bit those of quantize.hip.
 //
-// A block takes 16 tokens of one kv head (d = 64: 32): its groups are contiguous in a page,
-// where it writes, and 256 to 512 bytes a token where it reads.  First its waves find each
-// token's sequence and place, 64 row numbers at a time (two loads for up to 4096 sequences),
-// then 8 lanes quantize a group.  Bound by a launch's latency for a decode step, by HBM
+// A block takes 16 tokens (d = 64: 32) of some kv heads: a head's groups are contiguous in a page,
+// where it writes, and 256 to 512 bytes a token where it reads.  While the first head's values
+// are on their way its waves find each token's sequence and place, 64 row numbers at a time
+// (two loads for up to 4096 sequences); 8 lanes quantize a group.  Bound by a launch's latency for a decode step, by HBM
 // for prompts.
 #include "pages.h"
 
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int64_t kBlocks = 8192;
 
 struct AppendJob {
     eakvd_pages b;
@@ -19,7 +20,7 @@ struct AppendJob {
     int layer, n_pages, log2p;
     const void *src[2];
     int64_t ld;
-    int vec;
+    int heads, parts;       // heads (K's, then V's) of a block, blocks of a chunk of tokens
 };
 
 template <bool BF16, bool VEC>
@@ -55,7 +56,21 @@ __global__ __launch_bounds__(kThreads) void append_kernel(eakvd_geom g, AppendJo
     constexpr int T = kThreads / 8 / GPD;            // tokens of a block
     __shared__ int place[T];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int r0 = (int)blockIdx.x * T, n = J.b.n_seqs;
+    const int chunk = (int)blockIdx.x / J.parts, part = (int)blockIdx.x - chunk * J.parts;
+    const int r0 = chunk * T, n = J.b.n_seqs;
+    const int l8 = tid & 7, gbase = lane & ~7, slot = tid >> 3;
+    const int k8 = slot / GPD, gd = slot % GPD;
+    const int y0 = part * J.heads, y1 = min(y0 + J.heads, 2 * g.n_kv_heads);
+    // (rows behind the last are read as the last: the 8 lanes of a group, and the wave, go on together)
+    const int64_t from = min(r0 + k8, J.b.n_new - 1) * J.ld + gd * 64 + l8 * 4;
+    auto load = [&](int y, float4 &lo, float4 &hi) {
+        const int kv = y >= g.n_kv_heads;
+        const int64_t at = from + (int64_t)(y - kv * g.n_kv_heads) * g.head_dim;
+        lo = load4<BF16, VEC>(J.src[kv], at);
+        hi = load4<BF16, VEC>(J.src[kv], at + 32);
+    };
+    float4 lo, hi;
+    load(y0, lo, hi);
     // the last sequence that does not begin behind row r
     auto begin = [&](int s) { return s < n ? seq_at(J.b, s).row : INT32_MAX; };
     const int coarse = n > 64 ? begin(lane * 64) : 0;
@@ -74,26 +89,23 @@ __global__ __launch_bounds__(kThreads) void append_kernel(eakvd_geom g, AppendJo
         if (lane == 0) place[k] = at;
     }
     __syncthreads();
-    const int l8 = tid & 7, gbase = lane & ~7, slot = tid >> 3;
-    const int k = slot / GPD, gd = slot % GPD;
-    const int at = r0 + k < J.b.n_new ? place[k] : -1;
-    for (int y = blockIdx.y; y < 2 * g.n_kv_heads; y += gridDim.y) {
-        const int kv = y >= g.n_kv_heads, hd = y - kv * g.n_kv_heads;
-        // (rows behind the last are read as the last: the 8 lanes of a group, and the wave, go on
-        // together)
-        const int r = min(r0 + k, J.b.n_new - 1);
-        const int64_t from = r * J.ld + (int64_t)hd * g.head_dim + gd * 64 + l8 * 4;
-        const float4 lo = load4<BF16, VEC>(J.src[kv], from), hi = load4<BF16, VEC>(J.src[kv], from + 32);
+    const int at = r0 + k8 < J.b.n_new ? place[k8] : -1;
+    for (int y = y0; y < y1; y++) {
+        float4 nlo = lo, nhi = hi;
+        if (y + 1 < y1) load(y + 1, nlo, nhi);
         const QOut o = quantize_group8(lo, hi, gbase);
         if (at >= 0) {
+            const int kv = y >= g.n_kv_heads;
             uint8_t *blk = J.base + (int64_t)(J.layer * 2 + kv) * g.block_bytes;
-            const int64_t gi = hd * g.gph + (int64_t)at * GPD + gd;
+            const int64_t gi = (y - kv * g.n_kv_heads) * g.gph + (int64_t)at * GPD + gd;
             __builtin_nontemporal_store(o.word, (uint32_t *)(blk + gi * 32 + l8 * 4));
             if (l8 == 0) {
                 __builtin_nontemporal_store(o.scale, (float *)(blk + g.s_off) + gi);
                 __builtin_nontemporal_store(o.bias, (float *)(blk + g.b_off) + gi);
             }
         }
+        lo = nlo;
+        hi = nhi;
     }
 }
 
@@ -116,8 +128,15 @@ extern "C" int eakvd_paged_append(const eakvd_geom *g, uint8_t *base, const eakv
     const uintptr_t odd = bf16 ? 7 : 15;
     const bool vec = (((uintptr_t)k | (uintptr_t)v) & odd) == 0 && ld % 4 == 0;
     const int t = kThreads / 8 / (int)g->gpd;
-    const dim3 grid((unsigned)((b->n_new + t - 1) / t),
-                    (unsigned)(2 * g->n_kv_heads < 65535 ? 2 * g->n_kv_heads : 65535));
+    // about kBlocks blocks, heads of the same tokens side by side
+    const int64_t chunks = (b->n_new + t - 1) / t;
+    const int all = 2 * g->n_kv_heads;
+    int64_t parts = (kBlocks + chunks - 1) / chunks;
+    if (parts > all) parts = all;
+    J.heads = (int)((all + parts - 1) / parts);
+    J.parts = (all + J.heads - 1) / J.heads;
+    if (chunks * J.parts > INT32_MAX) return (int)hipErrorInvalidValue;
+    const dim3 grid((unsigned)(chunks * J.parts));
     auto run = [&](auto *kern) {
         hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, (hipStream_t)stream, *g, J);
         return (int)hipGetLastError();
