@@ -76,7 +76,9 @@ int eakv_attention_weights_batch_device(eakv_cache_t *const *caches, int n_cache
 
 size_t eakv_evict_select_work_bytes(int n_seqs, const int32_t *n_tokens)
 {
-    if (n_seqs < 0 || n_seqs > EAKVD_MAX_BATCH || (n_seqs && !n_tokens)) {
+    int bad = n_seqs < 0 || n_seqs > EAKVD_MAX_BATCH || (n_seqs && !n_tokens);
+    for (int i = 0; !bad && i < n_seqs; i++) bad = n_tokens[i] < 0;
+    if (bad) {
         eakvi_set_error(EAKV_ERR_INVALID, "evict: invalid argument");
         return 0;
     }

@@ -4,9 +4,9 @@
 
 static int sizes_ok(int n_rows, int vocab, int n_top)
 {
-    /* one block for each 16384 values of a row */
+    /* a block of 256 threads for each 16384 values of a row; a launch has fewer than 2^32 threads */
     return n_rows >= 0 && vocab >= 1 && vocab <= (1 << 30) && n_top >= 0 && n_top <= EAKV_TOP_MAX &&
-           (int64_t)n_rows * ((int64_t)vocab / 16384 + 2) <= INT32_MAX;
+           (int64_t)n_rows * ((int64_t)vocab / 16384 + 2) < 1 << 24;
 }
 
 size_t eakv_token_logprobs_work_bytes(int n_rows, int vocab, int n_top)
