@@ -44,7 +44,8 @@ struct __align__(16) Tile {
     uint4 q[NQ][64];
     float rf[16];
     int vis[16];                                // positions that the row sees
-    float2 ml[16];                              // second pass: M and 1/L
+    int all, pad[3];                            // that all of them see
+    float off[16];                              // second pass: M + log2 L
     float2 run[W][64];                          // first pass: a lane's running M and L
 };
 
@@ -56,9 +57,11 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void *p, int64_t by
                                              (int)(uint32_t)(bytes < most ? bytes : most), 0x00020000);
 }
 
-// The chunks' (M, L) of a row joined, 4 lanes to a row (sub): M and 1/L, 0 where nothing is seen.
+// The chunks' (M, L) of a row joined, 4 lanes to a row (sub): M + log2 L, whose power is taken off a
+// score's: one exponential is the weight.  (Its rounding is half a step of M's, which M's own has
+// as well; the logarithm is off by 2 steps at most.)
 // (Eight loads in flight: a chunk at a time this was most of a small launch.)
-__device__ __forceinline__ float2 join_row(const float2 *st, int mc, int sub, bool live)
+__device__ __forceinline__ float join_row(const float2 *st, int mc, int sub, bool live)
 {
     float mm = kMInit, l = 0.0f;
     for (int k0 = sub; live && k0 < mc; k0 += 32) {
@@ -79,7 +82,32 @@ __device__ __forceinline__ float2 join_row(const float2 *st, int mc, int sub, bo
     l *= __builtin_amdgcn_exp2f(mm - top);
     l += __shfl_xor(l, 1, 64);
     l += __shfl_xor(l, 2, 64);
-    return float2{top, l == 0.0f ? 0.0f : 1.0f / l};
+    return top + __builtin_amdgcn_logf(l);
+}
+
+// A row tile's operands from LDS; the bias's is the result.
+template <int D, bool F32>
+__device__ __forceinline__ b8 load_query(const uint4 (*q)[64], int lane, Query<D, F32, false> &Q)
+{
+#pragma unroll
+    for (int f = 0; f < D / 32; f++) {
+        Q.a[f] = __builtin_bit_cast(h8, q[f][lane]);
+        if constexpr (F32) Q.b[F32 ? f : 0] = __builtin_bit_cast(h8, q[D / 32 + (F32 ? f : 0)][lane]);
+    }
+    return __builtin_bit_cast(b8, q[D / 32 * (F32 ? 2 : 1)][lane]);
+}
+
+// group_dots with tokens across: a lane has one token's of four rows.
+template <int D, bool F32>
+__device__ __forceinline__ v4f row_dots(const h8 &lo, const h8 &hi, const Query<D, F32, false> &Q, int g)
+{
+    v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (F32) {
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(Q.b[F32 ? 2 * g : 0], lo, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(Q.b[F32 ? 2 * g + 1 : 0], hi, acc, 0, 0, 0);
+    }
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(Q.a[2 * g], lo, acc, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(Q.a[2 * g + 1], hi, acc, 0, 0, 0);
 }
 
 // W waves.  SUM: the second pass; STORE: the first pass leaves the scores, log2, [kv head][row][ld_s].
@@ -133,14 +161,15 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : F32 ? 2 : 4) void weights_kern
             if (blk == 0) {
                 T[u].rf[n16] = Q.rf;
                 T[u].vis[n16] = at < rows ? start + tok + 1 : 0;
+                if (n16 == 0) T[u].all = r0 + 16 * u + 15 < rows ? start + tok + 1 : 0;
             }
             if constexpr (!SUM)
                 for (int k = 0; k < W; k++) T[u].run[k][lane] = float2{kMInit, 0.0f};
         }
         if constexpr (SUM)
             for (int r = tid >> 2; r < 16 * nu; r += 16 * W) {
-                const float2 x = join_row(st + (int64_t)(r0 + r) * mc, mc, tid & 3, r0 + r < rows);
-                if ((tid & 3) == 0) T[r >> 4].ml[r & 15] = x;
+                const float x = join_row(st + (int64_t)(r0 + r) * mc, mc, tid & 3, r0 + r < rows);
+                if ((tid & 3) == 0) T[r >> 4].off[r & 15] = x;
             }
         __syncthreads();
 
@@ -173,63 +202,89 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : F32 ? 2 : 4) void weights_kern
             bias_operands(owner ? ck : 0.0f, 0.0f, false, bias, n32);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             h8 kl[2][GPD], kh[2][GPD];
-            v4f sc[2][GPD];
 #pragma unroll
             for (int k = 0; k < 2; k++)
 #pragma unroll
-                for (int g = 0; g < GPD; g++) {
+                for (int g = 0; g < GPD; g++)
                     k_operands<false>(kx[k][g], S.zk[g][16 * k + n16], nc, kl[k][g], kh[k][g]);
-                    sc[k][g] = *(const v4f *)&S.ks[g][16 * k + 4 * blk];
-                }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             if (i + 1 < n_i) load(i + 1);
-            float acc[8];
+            if constexpr (SUM) {
+                // a lane: token n16 of each half, rows 4 blk to 4 blk + 3, so that the rows add up in
+                // its own registers
+                float acc[2] = {0.0f, 0.0f}, ks[2][GPD];
 #pragma unroll
-            for (int j = 0; j < 8; j++) acc[j] = 0.0f;
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int g = 0; g < GPD; g++) ks[k][g] = S.ks[g][16 * k + n16];
 #pragma unroll 1
-            for (int u = 0; u < nu; u++) {
-                Query<D, F32, false> Q;
+                for (int u = 0; u < nu; u++) {
+                    Query<D, F32, false> Q;
+                    const b8 qb = load_query<D, F32>(T[u].q, lane, Q);
+                    const v4f rf = *(const v4f *)&T[u].rf[4 * blk], off = *(const v4f *)&T[u].off[4 * blk];
+                    float y[2][4];
 #pragma unroll
-                for (int f = 0; f < D / 32; f++) {
-                    Q.a[f] = __builtin_bit_cast(h8, T[u].q[f][lane]);
-                    if constexpr (F32) Q.b[F32 ? f : 0] = __builtin_bit_cast(h8, T[u].q[D / 32 + (F32 ? f : 0)][lane]);
-                }
-                const b8 qb = __builtin_bit_cast(b8, T[u].q[Tl::NQ - 1][lane]);
-                const float rf = T[u].rf[n16];
-                const int vis = T[u].vis[n16];
-                float x[8];
+                    for (int k = 0; k < 2; k++) {
+                        v4f s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qb, bias[k], v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    v4f s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bias[k], qb, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+                        for (int g = 0; g < GPD; g++) {
+                            const v4f dot = row_dots(kl[k][g], kh[k][g], Q, g);
 #pragma unroll
-                    for (int g = 0; g < GPD; g++) {
-                        const v4f dot = group_dots(kl[k][g], kh[k][g], Q, g);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) s[e] = fmaf(sc[k][g][e], dot[e], s[e]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; e++) x[4 * k + e] = s[e];
-                }
-                const bool masked = __ballot(t0 + 32 > vis) != 0;
-                const int seen = vis - t0 - 4 * blk;            // of the lane's first half on
-                if constexpr (SUM) {
-                    const float2 ml = T[u].ml[n16];
-                    if (masked) {
-#pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            const float y = __builtin_amdgcn_exp2f(fmaf(x[j], rf, -ml.x)) * ml.y;
-                            acc[j] += 16 * (j >> 2) + (j & 3) < seen ? y : 0.0f;
+                            for (int e = 0; e < 4; e++) s[e] = fmaf(ks[k][g], dot[e], s[e]);
                         }
-                    } else {
 #pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            acc[j] = fmaf(__builtin_amdgcn_exp2f(fmaf(x[j], rf, -ml.x)), ml.y, acc[j]);
+                        for (int e = 0; e < 4; e++) y[k][e] = __builtin_amdgcn_exp2f(fmaf(s[e], rf[e], -off[e]));
                     }
-                } else {
-                    if (masked)
+                    if (t0 + 32 > T[u].all) {
+                        const int4 vis = *(const int4 *)&T[u].vis[4 * blk];
+                        const int seen[4] = {vis.x, vis.y, vis.z, vis.w};
+#pragma unroll
+                        for (int k = 0; k < 2; k++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) y[k][e] = t0 + 16 * k + n16 < seen[e] ? y[k][e] : 0.0f;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; k++) acc[k] += (y[k][0] + y[k][1]) + (y[k][2] + y[k][3]);
+                }
+                // over the lanes of one token: one half's sums to lanes 0-15, the other's to 16-31
+                float v = row_sum(acc[0]);
+                const float v1 = row_sum(acc[1]);
+                v = blk == 1 ? v1 : v;
+                const int t = t0 + n32;
+                if (h == 0 && t < hi) {
+                    float *o = out + ((int64_t)job.seq[c] * job.n_kv + kvh) * ld + t;
+                    const float by = r0 == 0 ? keep : 1.0f;
+                    *o = by == 0.0f ? v : fmaf(by, *o, v);
+                }
+            } else {
+                v4f sc[2][GPD];
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int g = 0; g < GPD; g++) sc[k][g] = *(const v4f *)&S.ks[g][16 * k + 4 * blk];
+#pragma unroll 1
+                for (int u = 0; u < nu; u++) {
+                    Query<D, F32, false> Q;
+                    const b8 qb = load_query<D, F32>(T[u].q, lane, Q);
+                    const float rf = T[u].rf[n16];
+                    float x[8];
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        v4f s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bias[k], qb, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+                        for (int g = 0; g < GPD; g++) {
+                            const v4f dot = group_dots(kl[k][g], kh[k][g], Q, g);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) s[e] = fmaf(sc[k][g][e], dot[e], s[e]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x[4 * k + e] = s[e];
+                    }
+                    if (t0 + 32 > T[u].all) {
+                        const int seen = T[u].vis[n16] - t0 - 4 * blk;          // of the lane's first half on
 #pragma unroll
                         for (int j = 0; j < 8; j++)
                             x[j] = 16 * (j >> 2) + (j & 3) < seen ? x[j] : -__builtin_inff();
+                    }
                     if constexpr (STORE) {
                         if (r0 + 16 * u + n16 < rows) {
                             float *o = score + job.score[c] + ((int64_t)kvh * rows + r0 + 16 * u + n16) * job.ld_s[c] + t0 +
@@ -247,25 +302,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : F32 ? 2 : 4) void weights_kern
                     T[u].run[w][lane] = float2{mn, l};
                 }
             }
-            if constexpr (SUM) {
-                // over the 16 rows of the tiles: lanes with one blk
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    acc[j] += dpp_f<0x128>(acc[j]);             // row_ror 8, 4, 2, 1
-                    acc[j] += dpp_f<0x124>(acc[j]);
-                    acc[j] += dpp_f<0x122>(acc[j]);
-                    acc[j] += dpp_f<0x121>(acc[j]);
-                }
-                float v = acc[0];
-#pragma unroll
-                for (int j = 1; j < 8; j++) v = n16 == j ? acc[j] : v;
-                const int t = t0 + 16 * ((n16 >> 2) & 1) + 4 * blk + (n16 & 3);
-                if (n16 < 8 && t < hi) {
-                    float *o = out + ((int64_t)job.seq[c] * job.n_kv + kvh) * ld + t;
-                    const float by = r0 == 0 ? keep : 1.0f;
-                    *o = by == 0.0f ? v : fmaf(by, *o, v);
-                }
-            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
         if constexpr (!SUM) {
             // rows' (M, L) of the chunk: over the lanes of a row and the waves
@@ -296,7 +333,7 @@ __global__ __launch_bounds__(kAddThreads) void weights_add_kernel(WeightsJob job
                                                                   const float *score, float *out, int64_t ld,
                                                                   float keep)
 {
-    __shared__ float2 ml[kStore];
+    __shared__ float off[kStore];
     const int tid = threadIdx.x, lane = tid & 63;
     const int c = seq_of(job.add, job.n_seq, (int)blockIdx.x, lane);
     const int rem = (int)blockIdx.x - job.add[c];
@@ -304,23 +341,23 @@ __global__ __launch_bounds__(kAddThreads) void weights_add_kernel(WeightsJob job
     const int rows = job.ntok[c] * job.qpk, mc = job.mc[c], hi = job.start[c] + job.ntok[c];
     if (tid < 4 * kStore) {
         const int r = tid >> 2;
-        const float2 x = join_row(stat + job.stat[c] + ((int64_t)kvh * rows + min(r, rows - 1)) * mc, mc, tid & 3,
-                                  r < rows);
-        if ((tid & 3) == 0) ml[r] = x;
+        const float x = join_row(stat + job.stat[c] + ((int64_t)kvh * rows + min(r, rows - 1)) * mc, mc, tid & 3,
+                                 r < rows);
+        if ((tid & 3) == 0) off[r] = x;
     }
     __syncthreads();
     if (t0 >= hi) return;
     // (rows of scores are whole tiles; those that a row does not see are -inf, and what is
-    // there has no part in the sum where its 1/L is NaN)
+    // there has no part in the sum where the row's is NaN)
     const float *s = score + job.score[c] + (int64_t)kvh * rows * job.ld_s[c] + t0;
     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int r = 0; r < rows; r++) {
         const v4f x = __builtin_nontemporal_load((const v4f *)(s + (int64_t)r * job.ld_s[c]));
-        const float2 y = ml[r];
+        const float y = off[r];
         const int vis = job.start[c] + r / job.qpk + 1;
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            acc[e] += t0 + e < vis ? __builtin_amdgcn_exp2f(x[e] - y.x) * y.y : 0.0f;
+            acc[e] += t0 + e < vis ? __builtin_amdgcn_exp2f(x[e] - y) : 0.0f;
     }
     float *o = out + ((int64_t)job.seq[c] * job.n_kv + kvh) * ld + t0;
 #pragma unroll
