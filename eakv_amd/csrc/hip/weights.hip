@@ -19,7 +19,8 @@
 namespace {
 
 constexpr int kTile = 256;
-constexpr int kRowTiles = 8;                    // of a pass over a chunk's tokens, at most
+constexpr int kRowTiles = 8;                    // of a block of the first pass, at most
+constexpr int kSumTiles = 16;                   // of a pass over a chunk's tokens in the second
 constexpr int kStore = 8;
 
 struct WeightsJob {
@@ -27,18 +28,20 @@ struct WeightsJob {
     const uint8_t *base[EAKVD_MAX_BATCH];
     int start[EAKVD_MAX_BATCH], ntok[EAKVD_MAX_BATCH], tok0[EAKVD_MAX_BATCH];
     int seq[EAKVD_MAX_BATCH];                   // its number in the call
-    int mc[EAKVD_MAX_BATCH], clen[EAKVD_MAX_BATCH];
-    int pre[EAKVD_MAX_BATCH + 1];               // blocks before this sequence's
+    int mc[EAKVD_MAX_BATCH];                    // chunks of the first pass
+    int clen[2][EAKVD_MAX_BATCH];               // a chunk's tokens, either pass
+    int pre[2][EAKVD_MAX_BATCH + 1];            // blocks before this sequence's
     int add[EAKVD_MAX_BATCH + 1];               // weights_add_kernel: likewise
     int64_t stat[EAKVD_MAX_BATCH];              // its rows' first (M, L)
     int64_t score[EAKVD_MAX_BATCH], ld_s[EAKVD_MAX_BATCH];      // its scores, and from row to row
 };
 
-// LDS: the waves' scales, then a Tile for each row tile of a pass.
+// LDS: the waves' scales, a Tile for each row tile of a pass, then (first pass) the waves' running
+// M and L, a lane's each, [tile][wave][64].
 struct Scales {
     float ks[2][32], zk[2][32];
 };
-template <int D, bool F32, int W>
+template <int D, bool F32>
 struct __align__(16) Tile {
     static constexpr int NQ = D / 32 * (F32 ? 2 : 1) + 1;       // operands
     uint4 q[NQ][64];
@@ -46,7 +49,6 @@ struct __align__(16) Tile {
     int vis[16];                                // positions that the row sees
     int all, pad[3];                            // that all of them see
     float off[16];                              // second pass: M + log2 L
-    float2 run[W][64];                          // first pass: a lane's running M and L
 };
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void *p, int64_t bytes)
@@ -112,27 +114,31 @@ __device__ __forceinline__ v4f row_dots(const h8 &lo, const h8 &hi, const Query<
 
 // W waves.  SUM: the second pass; STORE: the first pass leaves the scores, log2, [kv head][row][ld_s].
 template <int D, bool F32, int W, bool SUM, bool STORE>
-__global__ __launch_bounds__(64 * W, W == 4 ? 3 : F32 ? 2 : 4) void weights_kernel(
+__global__ __launch_bounds__(64 * W, W == 4 ? 3 : W == 8 && F32 ? 2 : 4) void weights_kernel(
     eakvd_geom geo, WeightsJob job, const void *q, float2 *stat, float *score, float *out, int64_t ld,
     float keep, float ksc, int vec, int tiles)
 {
     constexpr int GPD = D / 64, RB = 32 * GPD;
-    typedef Tile<D, F32, W> Tl;
+    typedef Tile<D, F32> Tl;
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     Scales &S = ((Scales *)lds)[w];
     Tl *T = (Tl *)(lds + W * sizeof(Scales));
+    float2 (*run)[W][64] = (float2 (*)[W][64])(T + tiles);
     const int n16 = lane & 15, blk = lane >> 4, n32 = lane & 31, h = lane >> 5;
     const bool owner = GPD == 2 || h == 0;
     const int gh = GPD == 2 ? h : 0;
 
-    const int c = seq_of(job.pre, job.n_seq, (int)blockIdx.x, lane);
-    const int rem = (int)blockIdx.x - job.pre[c];
-    const int kvh = rem % job.n_kv, chunk = rem / job.n_kv;
-    const int m = job.ntok[c], start = job.start[c], qpk = job.qpk, mc = job.mc[c];
-    const int rows = m * qpk, t_end = start + m;
-    const int lo = chunk * job.clen[c];
-    const int hi = t_end - lo > job.clen[c] ? lo + job.clen[c] : t_end;
+    const int c = seq_of(job.pre[SUM], job.n_seq, (int)blockIdx.x, lane);
+    const int rem = (int)blockIdx.x - job.pre[SUM][c];
+    const int m = job.ntok[c], start = job.start[c], qpk = job.qpk, mc = job.mc[c], clen = job.clen[SUM][c];
+    const int kvh = rem % job.n_kv;
+    const int chunk = SUM ? rem / job.n_kv : rem / job.n_kv % mc;
+    // the block's rows: tiles of them in the first pass, all in the second
+    const int row0 = SUM ? 0 : rem / job.n_kv / mc * 16 * tiles;
+    const int rows = m * qpk, row1 = SUM ? rows : min(rows, row0 + 16 * tiles), t_end = start + m;
+    const int lo = chunk * clen;
+    const int hi = t_end - lo > clen ? lo + clen : t_end;
     const int n_sub = hi > lo ? (hi - lo + 31) / 32 : 0;
     const int n_i = n_sub > w ? (n_sub - w + W - 1) / W : 0;
     float2 *st = stat + job.stat[c] + (int64_t)kvh * rows * mc;          // [row][chunk]
@@ -145,7 +151,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : F32 ? 2 : 4) void weights_kern
     NibConst nc;
     nc.hold();
 
-    for (int r0 = 0; r0 < rows; r0 += 16 * tiles) {
+    for (int r0 = row0; r0 < row1; r0 += 16 * tiles) {
         const int nu = min(tiles, (rows - r0 + 15) / 16);
         __syncthreads();
         for (int u = w; u < nu; u += W) {
@@ -164,7 +170,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : F32 ? 2 : 4) void weights_kern
                 if (n16 == 0) T[u].all = r0 + 16 * u + 15 < rows ? start + tok + 1 : 0;
             }
             if constexpr (!SUM)
-                for (int k = 0; k < W; k++) T[u].run[k][lane] = float2{kMInit, 0.0f};
+                for (int k = 0; k < W; k++) run[u][k][lane] = float2{kMInit, 0.0f};
         }
         if constexpr (SUM)
             for (int r = tid >> 2; r < 16 * nu; r += 16 * W) {
@@ -293,13 +299,13 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : F32 ? 2 : 4) void weights_kern
                             *(v4f *)(o + 16) = v4f{x[4] * rf, x[5] * rf, x[6] * rf, x[7] * rf};
                         }
                     }
-                    float2 run = T[u].run[w][lane];
+                    const float2 old = run[u][w][lane];
                     const float top = max3(max3(max3(x[0], x[1], x[2]), x[3], x[4]), max3(x[5], x[6], x[7]), x[7]);
-                    const float mn = fmaxf(run.x, top * rf);
-                    float l = run.y * __builtin_amdgcn_exp2f(run.x - mn);
+                    const float mn = fmaxf(old.x, top * rf);
+                    float l = old.y * __builtin_amdgcn_exp2f(old.x - mn);
 #pragma unroll
                     for (int j = 0; j < 8; j++) l += __builtin_amdgcn_exp2f(fmaf(x[j], rf, -mn));
-                    T[u].run[w][lane] = float2{mn, l};
+                    run[u][w][lane] = float2{mn, l};
                 }
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -310,12 +316,12 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : F32 ? 2 : 4) void weights_kern
             for (int r = tid >> 2; r < 16 * nu; r += 16 * W) {
                 const int row = r0 + r;
                 float mm = kMInit;
-                for (int k = 0; k < W; k++) mm = fmaxf(mm, T[r >> 4].run[k][(r & 15) + 16 * (tid & 3)].x);
+                for (int k = 0; k < W; k++) mm = fmaxf(mm, run[r >> 4][k][(r & 15) + 16 * (tid & 3)].x);
                 mm = fmaxf(mm, __shfl_xor(mm, 1, 64));
                 mm = fmaxf(mm, __shfl_xor(mm, 2, 64));
                 float l = 0.0f;
                 for (int k = 0; k < W; k++) {
-                    const float2 x = T[r >> 4].run[k][(r & 15) + 16 * (tid & 3)];
+                    const float2 x = run[r >> 4][k][(r & 15) + 16 * (tid & 3)];
                     l = x.y == 0.0f ? l : fmaf(__builtin_amdgcn_exp2f(x.x - mm), x.y, l);
                 }
                 l += __shfl_xor(l, 1, 64);
@@ -367,13 +373,14 @@ __global__ __launch_bounds__(kAddThreads) void weights_add_kernel(WeightsJob job
 
 struct WeightsPlan {
     WeightsJob job;
-    int waves, tiles;
+    int waves, tiles[2];
     bool store;
     size_t stat_bytes, bytes;
 };
 
-// Chunks of an even share of the tiles: 3 blocks of 4 waves to a CU for up to two row tiles, else
-// one of 8 (bf16: two).
+// Chunks of an even share of the tiles: 3 blocks of 4 waves to a CU for up to two row tiles.  More:
+// blocks of 8 waves and up to kRowTiles row tiles in the first pass (bf16: two to a CU); in
+// the second one of 16 waves, all rows after one another.
 void weights_plan(const eakvd_window *b, int n_q, int n_kv, bool bf16, WeightsPlan *p)
 {
     memset(p, 0, sizeof(*p));
@@ -381,7 +388,7 @@ void weights_plan(const eakvd_window *b, int n_q, int n_kv, bool bf16, WeightsPl
     j.n_q = n_q;
     j.n_kv = n_kv;
     j.qpk = n_q / n_kv;
-    int64_t tiles = 0, stat = 0, score = 0, rows = 0;
+    int64_t tiles[2] = {0, 0}, stat = 0, score = 0, rows = 0;
     int tok0 = 0;
     for (int i = 0; i < b->n_seq; i++) {
         if (b->ntok[i]) {
@@ -391,71 +398,84 @@ void weights_plan(const eakvd_window *b, int n_q, int n_kv, bool bf16, WeightsPl
             j.ntok[k] = b->ntok[i];
             j.tok0[k] = tok0;
             j.seq[k] = i;
-            tiles += ((int64_t)b->start[i] + b->ntok[i] + kTile - 1) / kTile * n_kv;
             const int64_t r = (int64_t)b->ntok[i] * j.qpk;
             rows = r > rows ? r : rows;
         }
         tok0 += b->ntok[i];
     }
+    const int64_t row_tiles = (rows + 15) / 16;
     p->store = rows <= kStore;
-    p->tiles = (int)((rows + 15) / 16 < kRowTiles ? (rows + 15) / 16 : kRowTiles);
-    p->waves = p->tiles <= 2 ? 4 : 8;
-    const int64_t slots = (p->waves == 4 ? 3 : bf16 ? 2 : 1) * cu_count(), share = (tiles + slots - 1) / slots;
+    p->tiles[0] = (int)(row_tiles < kRowTiles ? row_tiles : kRowTiles);
+    p->tiles[1] = (int)(row_tiles < kSumTiles ? row_tiles : kSumTiles);
+    p->waves = row_tiles <= 2 ? 4 : 8;
+    const auto groups = [&](int i) { return ((int64_t)j.ntok[i] * j.qpk + 16 * p->tiles[0] - 1) / (16 * p->tiles[0]); };
     for (int i = 0; i < j.n_seq; i++) {
-        const int64_t t = (int64_t)j.start[i] + j.ntok[i], n_t = (t + kTile - 1) / kTile;
-        int64_t mc = (n_t + share - 1) / share;
-        // (offsets from a chunk's first token are 32 bits)
-        if (mc < (n_t >> 16) + 1) mc = (n_t >> 16) + 1;
-        const int64_t per = (n_t + mc - 1) / mc;
-        mc = (n_t + per - 1) / per;
-        j.mc[i] = (int)mc;
-        j.clen[i] = (int)(per * kTile);
-        j.pre[i + 1] = j.pre[i] + (int)mc * n_kv;
-        j.add[i + 1] = j.add[i] + (int)((t + 4 * kAddThreads - 1) / (4 * kAddThreads)) * n_kv;
-        j.stat[i] = stat;
-        stat += (int64_t)j.ntok[i] * n_q * mc;
-        j.ld_s[i] = n_t * kTile;
-        j.score[i] = score;
-        score += (int64_t)j.ntok[i] * n_q * j.ld_s[i];
+        const int64_t n = ((int64_t)j.start[i] + j.ntok[i] + kTile - 1) / kTile * n_kv;
+        tiles[0] += n * groups(i);
+        tiles[1] += n;
+    }
+    for (int pass = 0; pass < 2; pass++) {
+        const int64_t slots = (p->waves == 4 ? 3 : bf16 && pass == 0 ? 2 : 1) * cu_count();
+        const int64_t share = (tiles[pass] + slots - 1) / slots;
+        for (int i = 0; i < j.n_seq; i++) {
+            const int64_t t = (int64_t)j.start[i] + j.ntok[i], n_t = (t + kTile - 1) / kTile;
+            int64_t mc = (n_t + share - 1) / share;
+            // (offsets from a chunk's first token are 32 bits)
+            if (mc < (n_t >> 16) + 1) mc = (n_t >> 16) + 1;
+            const int64_t per = (n_t + mc - 1) / mc;
+            mc = (n_t + per - 1) / per;
+            j.clen[pass][i] = (int)(per * kTile);
+            j.pre[pass][i + 1] = j.pre[pass][i] + (int)(mc * n_kv * (pass ? 1 : groups(i)));
+            if (pass) continue;
+            j.mc[i] = (int)mc;
+            j.add[i + 1] = j.add[i] + (int)((t + 4 * kAddThreads - 1) / (4 * kAddThreads)) * n_kv;
+            j.stat[i] = stat;
+            stat += (int64_t)j.ntok[i] * n_q * mc;
+            j.ld_s[i] = n_t * kTile;
+            j.score[i] = score;
+            score += (int64_t)j.ntok[i] * n_q * j.ld_s[i];
+        }
     }
     p->stat_bytes = ((size_t)stat * sizeof(float2) + 255) & ~(size_t)255;
     p->bytes = p->stat_bytes + (p->store ? (size_t)score * sizeof(float) : 0);
+}
+
+template <int D, bool F32, int W, bool SUM, bool STORE>
+int pass(const eakvd_geom &g, const WeightsPlan &p, const void *q, void *work, float *out, int64_t ld,
+         float keep, int vec, hipStream_t st)
+{
+    constexpr size_t tile = sizeof(Tile<D, F32>) + (SUM ? 0 : W * 64 * sizeof(float2));
+    constexpr int most = W == 4 ? 2 : SUM ? kSumTiles : kRowTiles;
+    static_assert(W * sizeof(Scales) + most * tile <= 160 * 1024, "LDS");
+    static std::atomic<uint64_t> done;
+    auto *kern = weights_kernel<D, F32, W, SUM, STORE>;
+    const int e = allow_lds((const void *)kern, W * sizeof(Scales) + most * tile, done);
+    if (e) return e;
+    hipLaunchKernelGGL(kern, dim3((unsigned)p.job.pre[SUM][p.job.n_seq]), dim3(64 * W),
+                       W * sizeof(Scales) + p.tiles[SUM] * tile, st, g, p.job, q, (float2 *)work,
+                       (float *)((uint8_t *)work + p.stat_bytes), out, ld, keep, EAKV_LOG2E / sqrtf((float)D), vec,
+                       p.tiles[SUM]);
+    return (int)hipGetLastError();
 }
 
 template <int D, bool F32>
 int launch(const eakvd_geom &g, const WeightsPlan &p, const void *q, void *work, float *out, int64_t ld,
            float keep, int vec, hipStream_t st)
 {
-    const WeightsJob &job = p.job;
-    float2 *stat = (float2 *)work;
-    float *score = (float *)((uint8_t *)work + p.stat_bytes);
-    auto run = [&](auto *kern, int waves, size_t tile, int most, std::atomic<uint64_t> &done) {
-        const int e = allow_lds((const void *)kern, waves * sizeof(Scales) + most * tile, done);
-        if (e) return e;
-        hipLaunchKernelGGL(kern, dim3((unsigned)job.pre[job.n_seq]), dim3(64 * waves),
-                           waves * sizeof(Scales) + p.tiles * tile, st, g, job, q, stat, score, out, ld, keep,
-                           EAKV_LOG2E / sqrtf((float)D), vec, p.tiles);
-        return (int)hipGetLastError();
-    };
-    static std::atomic<uint64_t> done[5];
-    constexpr size_t t4 = sizeof(Tile<D, F32, 4>), t8 = sizeof(Tile<D, F32, 8>);
-    static_assert(8 * sizeof(Scales) + kRowTiles * t8 <= 160 * 1024, "LDS");
     int e;
     if (p.store) {
-        e = run(weights_kernel<D, F32, 4, false, true>, 4, t4, 2, done[0]);
-        if (!e) {
-            hipLaunchKernelGGL(weights_add_kernel, dim3((unsigned)job.add[job.n_seq]), dim3(kAddThreads), 0, st, job,
-                               stat, score, out, ld, keep);
-            e = (int)hipGetLastError();
-        }
-    } else if (p.waves == 4) {
-        e = run(weights_kernel<D, F32, 4, false, false>, 4, t4, 2, done[1]);
-        if (!e) e = run(weights_kernel<D, F32, 4, true, false>, 4, t4, 2, done[2]);
-    } else {
-        e = run(weights_kernel<D, F32, 8, false, false>, 8, t8, kRowTiles, done[3]);
-        if (!e) e = run(weights_kernel<D, F32, 8, true, false>, 8, t8, kRowTiles, done[4]);
+        e = pass<D, F32, 4, false, true>(g, p, q, work, out, ld, keep, vec, st);
+        if (e) return e;
+        hipLaunchKernelGGL(weights_add_kernel, dim3((unsigned)p.job.add[p.job.n_seq]), dim3(kAddThreads), 0, st, p.job,
+                           (float2 *)work, (float *)((uint8_t *)work + p.stat_bytes), out, ld, keep);
+        return (int)hipGetLastError();
     }
-    return e;
+    if (p.waves == 4) {
+        e = pass<D, F32, 4, false, false>(g, p, q, work, out, ld, keep, vec, st);
+        return e ? e : pass<D, F32, 4, true, false>(g, p, q, work, out, ld, keep, vec, st);
+    }
+    e = pass<D, F32, 8, false, false>(g, p, q, work, out, ld, keep, vec, st);
+    return e ? e : pass<D, F32, 16, true, false>(g, p, q, work, out, ld, keep, vec, st);
 }
 
 }  // namespace
