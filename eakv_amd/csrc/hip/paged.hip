@@ -568,21 +568,25 @@ __global__ __launch_bounds__(64 * kWaves, NR > 1 ? 2 : 3) void paged_kernel(eakv
                               (GPD == 2 && (seen & (uint32_t)(bad >> 32)) ? 2u << 2 * u : 0u);
                 }
             }
-            float rf[N], need[N];
+            // (a lane looks at its own scores; a row's lanes join where one of them moves M)
+            float rf[N], top[N];
             bool move = false;
+            auto moves = [&](int u) __attribute__((always_inline)) {
+                return fmaf(top[u], rf[u], -(kTop<F32> + kTau<F32>)) > M[u];
+            };
 #pragma unroll
             for (int u = 0; u < N; u++) {
                 rf[u] = Fm::kShared ? R.rf[u][n16] : rf1;
-                const float top = row_max(max3(max3(max3(s[u][0], s[u][1], s[u][2]), s[u][3], s[u][4]),
-                                               max3(s[u][5], s[u][6], s[u][7]), s[u][7]));
-                need[u] = fmaf(top, rf[u], -kTop<F32>);
-                move |= need[u] > M[u] + kTau<F32>;
+                top[u] = max3(max3(max3(s[u][0], s[u][1], s[u][2]), s[u][3], s[u][4]),
+                              max3(s[u][5], s[u][6], s[u][7]), s[u][7]);
+                move |= moves(u);
             }
             if (__ballot(move) != 0) {
 #pragma unroll
                 for (int u = 0; u < N; u++) {
-                    if (N > 1 && __ballot(need[u] > M[u] + kTau<F32>) == 0) continue;
-                    const float mn = need[u] > M[u] + kTau<F32> ? need[u] : M[u], d = M[u] - mn;
+                    if (N > 1 && __ballot(moves(u)) == 0) continue;
+                    top[u] = row_max(top[u]);
+                    const float mn = moves(u) ? fmaf(top[u], rf[u], -kTop<F32>) : M[u], d = M[u] - mn;
                     // (L by halves, as in window.h)
                     const float al = __builtin_amdgcn_exp2f(d), half = __builtin_amdgcn_exp2f(0.5f * d);
                     L[u] = L[u] * half * half;
