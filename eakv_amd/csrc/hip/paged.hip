@@ -764,8 +764,11 @@ __global__ __launch_bounds__(64 * kWaves, NR > 1 ? 2 : 3) void paged_kernel(eakv
         // ---- the waves joined, 16 rows at a time
         // (two buffers: one is read while the next is written)
         const int slot = 2 * bl + (U.at == 0 ? 1 : 0);
-        poison |= __shfl_xor(poison, 16, 64);
-        poison |= __shfl_xor(poison, 32, 64);
+        const bool poisoned = __ballot(poison != 0) != 0;
+        if (poisoned) {
+            poison |= __shfl_xor(poison, 16, 64);
+            poison |= __shfl_xor(poison, 32, 64);
+        }
 #pragma unroll
         for (int u = 0; u < NR; u++) {
             if (u > 0 && 16 * u >= rows) break;
@@ -787,8 +790,9 @@ __global__ __launch_bounds__(64 * kWaves, NR > 1 ? 2 : 3) void paged_kernel(eakv
                                : kValues ? O[u][f][e] * 0x1p-15f
                                          : fmaf(O[u][f][e], k & 1 ? 0x1p20f : 0x1p24f,
                                                 C[u][kSub ? g : 0][e] * (1.0f / kZUp));
-                        if (poison >> (2 * u + g) & 1) o[e] = __builtin_nanf("");
                     }
+                    if (poisoned && (poison >> (2 * u + g) & 1))
+                        o = v4f{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
                     *((v4f *)jo + (w * NF + f) * 64 + lane) = o;
                 }
             }
