@@ -30,7 +30,7 @@ constexpr int kThreads = 256;
 constexpr int kEach = 64;
 constexpr int kSeg = kThreads * kEach;
 static_assert(kThreads == 256, "four waves");
-constexpr int kCand = 256;              // candidates that LDS holds for each wave
+constexpr int kCand = 512;              // candidates that LDS holds for a block
 constexpr int kGroups = 128;            // and groups of 8 values with one
 constexpr int kHeld = 512;              // keys of a row's segments that its joining wave holds
 
@@ -78,17 +78,29 @@ __device__ __forceinline__ float logit(const void *x, int64_t at)
     else return ((const float *)x)[at];
 }
 
+// ln s of a sum: its exponent and the logarithm of what is left of it, of 1 to 2, each in one
+// instruction (2^-23 off; with the library's in 64 bits a launch took 0.3 us more).
+__device__ __forceinline__ double ln_of(double s)
+{
+    const uint64_t b = (uint64_t)__double_as_longlong(s);
+    const int e = (int)(b >> 52);               // (0, infinite and NaN sums: 0, 0x7ff, above)
+    const bool plain = e > 0 && e < 0x7ff;
+    const double f = plain ? __longlong_as_double((long long)((b & 0xfffffffffffffull) | 0x3ff0000000000000ull)) : s;
+    return fma(0.6931471805599453, (double)__builtin_amdgcn_logf((float)f),
+               plain ? 0.6931471805599453 * (double)(e - 1023) : 0.0);
+}
+
 // A row's results from M, S, T (in units of ln 2), the given token's logit and the sorted
 // alternatives.
 __device__ __forceinline__ void finish(const LpJob &J, int64_t row, float m, double s, double t, int token,
                                        float given, const u64 *best, int tid)
 {
-    const double ln_s = log(s);
+    const double ln_s = ln_of(s);
     if (tid == 0) {
         if (J.lp)
             J.lp[row] = token >= 0 && token < J.vocab ? (float)((double)given - (double)m - ln_s)
                                                       : -__builtin_inff();
-        if (J.entropy) J.entropy[row] = (float)(ln_s - 0.6931471805599453 * (t / s));
+        if (J.entropy) J.entropy[row] = (float)(ln_s - 0.6931471805599453 * (double)((float)t * __builtin_amdgcn_rcpf((float)s)));
     }
     if (tid < J.k) {
         const u64 key = best[tid];
@@ -101,8 +113,9 @@ __device__ __forceinline__ void finish(const LpJob &J, int64_t row, float m, dou
 // S and T of terms whose exponents are all off by r
 __device__ __forceinline__ void put_right(double r, double &s, double &t)
 {
-    t = exp2(-r) * (t - r * s);
-    s = exp2(-r) * s;
+    const double f = (double)__builtin_amdgcn_exp2f(-(float)r);
+    t = f * (t - r * s);
+    s = f * s;
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c)
@@ -112,24 +125,25 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return r;
 }
 
-// best[0..k): the largest of the keys in order, 0 where there are fewer.  cand: a list for each wave,
-// n[w] <= kCand keys, all different.  All the block's threads.
-__device__ __forceinline__ void rank(const u64 (*cand)[kCand], const int *n, u64 *best, int k, int tid)
+// (the compiler makes a number of __ballot's argument first)
+__device__ __forceinline__ uint64_t ballot(bool b) { return __builtin_amdgcn_ballot_w64(b); }
+
+// best[0..k): the largest of n different keys in order, 0 where there are fewer (as best is).
+// cand: 16-byte aligned, 8 zeros behind the keys.  Thread tid of `threads`.
+__device__ __forceinline__ void rank(u64 *cand, int n, u64 *best, int k, int tid, int threads)
 {
-    const int lane = tid & 63, w = tid >> 6;
-    if (tid < k) best[tid] = 0;
-    __syncthreads();
-    for (int i = lane; i < n[w]; i += 64) {
-        const u64 mine = cand[w][i];
+    for (int i = tid; i < n; i += threads) {
+        const u64 mine = cand[i];
         int r = 0;
-        for (int v = 0; v < kThreads / 64; v++) {
-            const int m = n[v];
-#pragma unroll 4
-            for (int j = 0; j < m; j++) r += cand[v][j] > mine;
+        for (int j = 0; j < n; j += 8) {
+            u64 y[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = cand[j + e];
+#pragma unroll
+            for (int e = 0; e < 8; e++) r += y[e] > mine;
         }
         if (r < k && mine) best[r] = mine;
     }
-    __syncthreads();
 }
 
 // A bound that the maxima of k lanes of a wave reach, in 16 bits of a float's order (-inf: fewer
@@ -141,7 +155,7 @@ __device__ __forceinline__ float reached(float top, int k)
     uint32_t t = 0;
 #pragma unroll
     for (int bit = 31; bit >= 16; bit--)
-        if ((int)__popcll(__ballot(key >= (t | 1u << bit))) >= k) t |= 1u << bit;
+        if ((int)__popcll(ballot(key >= (t | 1u << bit))) >= k) t |= 1u << bit;
     return t ? __uint_as_float(t >> 31 ? t ^ 0x80000000u : ~t) : -__builtin_inff();
 }
 
@@ -150,11 +164,17 @@ template <bool BF16, bool TOP, bool ENT>
 __global__ __launch_bounds__(kThreads, 4) void logprob_kernel(LpJob J)
 {
     constexpr int V = BF16 ? 8 : 4, NV = kEach / V, NX = BF16 ? kEach / 2 : kEach;
-    __shared__ u64 cand[kThreads / 64][TOP ? kCand : 1], best[EAKVD_TOP_MAX], wbest[kThreads / 64];
+    __shared__ __align__(16) u64 cand[TOP ? kCand + 8 : 1];
+    __shared__ u64 best[EAKVD_TOP_MAX], wbest[kThreads / 64];
     __shared__ float red[3][kThreads / 64];
-    __shared__ int n_cand[kThreads / 64], n_group[kThreads / 64];
+    __shared__ int n_cand, n_group[kThreads / 64];
     __shared__ uint16_t groups[kThreads / 64][TOP ? kGroups : 1];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    if constexpr (TOP) {
+        for (int i = tid; i < kCand + 8; i += kThreads) cand[i] = 0;
+        if (tid < EAKVD_TOP_MAX) best[tid] = 0;
+        if (tid == 0) n_cand = 0;
+    }
     const int64_t row = blockIdx.x / J.n_seg;
     const int seg = (int)(blockIdx.x - row * J.n_seg);
     // vectors are aligned: value i of the row is at place i + shift
@@ -250,7 +270,7 @@ __global__ __launch_bounds__(kThreads, 4) void logprob_kernel(LpJob J)
 #pragma unroll
         for (int j = 0; j < kEach / 8; j++) {
             const bool in = high[j] >= thr && high[j] > none;
-            const uint64_t b = __ballot(in);
+            const uint64_t b = ballot(in);
             if (b == 0) continue;
             const int p = found + (int)__popcll(b & ((1ull << lane) - 1));
             if (in && p < kGroups) groups[w][p] = (uint16_t)(tid * (kEach / 8) + j);
@@ -266,7 +286,6 @@ __global__ __launch_bounds__(kThreads, 4) void logprob_kernel(LpJob J)
         const int g0 = n_group[0], g1 = g0 + n_group[1], g2 = g1 + n_group[2], all = g2 + n_group[3];
         bool fits = max(max(n_group[0], n_group[1]), max(n_group[2], n_group[3])) <= kGroups && all <= 4 * kGroups;
         if (fits) {
-            int found = 0;
             for (int q0 = 0; q0 < 8 * all; q0 += kThreads) {
                 const int q = q0 + tid, g = q >> 3;
                 u64 key = 0;
@@ -280,16 +299,19 @@ __global__ __launch_bounds__(kThreads, 4) void logprob_kernel(LpJob J)
                         key = y >= thr ? key_of(y, i) : 0;
                     }
                 }
-                const uint64_t b = __ballot(key != 0);
-                const int p = found + (int)__popcll(b & ((1ull << lane) - 1));
-                if (key && p < kCand) cand[w][p] = key;
-                found += (int)__popcll(b);
+                // (places in any order: the keys' own order decides)
+                const uint64_t b = ballot(key != 0);
+                int p = 0;
+                if (lane == 0 && b) p = atomicAdd(&n_cand, (int)__popcll(b));
+                p = __builtin_amdgcn_readfirstlane(p) + (int)__popcll(b & ((1ull << lane) - 1));
+                if (key && p < kCand) cand[p] = key;
             }
-            if (lane == 0) n_cand[w] = found;
-            fits = !__syncthreads_or(found > kCand);
+            __syncthreads();
+            fits = n_cand <= kCand;
         }
         if (fits) {
-            rank(cand, n_cand, best, J.k, tid);
+            rank(cand, n_cand, best, J.k, tid, kThreads);
+            __syncthreads();
         } else {
             // one after the other, read again
             u64 prev = ~0ull;
@@ -328,7 +350,8 @@ __global__ __launch_bounds__(kThreads, 4) void logprob_kernel(LpJob J)
 template <bool BF16>
 __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LpJob J, int n_rows)
 {
-    __shared__ u64 cands[kThreads / 64][kHeld], bests[kThreads / 64][EAKVD_TOP_MAX];
+    __shared__ __align__(16) u64 cands[kThreads / 64][kHeld + 8];
+    __shared__ u64 bests[kThreads / 64][EAKVD_TOP_MAX];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, k = J.k, n_seg = J.n_seg;
     const int64_t row = (int64_t)blockIdx.x * (kThreads / 64) + w;
     if (row >= n_rows) return;
@@ -356,7 +379,8 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LpJob J, int n_r
         if (x[1] == 0.0f) continue;
         double si = x[1], ti = x[2];
         put_right(x[3], si, ti);
-        const double d = ((double)mine - (double)from) * 1.4426950408889634, f = exp2(d);
+        const double d = ((double)mine - (double)from) * 1.4426950408889634,
+                     f = (double)__builtin_amdgcn_exp2f((float)d);
         s += f * si;
         if (f != 0.0) t += f * (ti + si * d);
     }
@@ -383,22 +407,17 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LpJob J, int n_r
 #pragma unroll
             for (int i = 0; i < kHeld / 64; i++) {
                 const bool in = key[i] != 0 && key[i] >= least;
-                const uint64_t b = __ballot(in);
+                const uint64_t b = ballot(in);
                 const int p = found + (int)__popcll(b & ((1ull << lane) - 1));
                 if (in) cand[p] = key[i];
                 found += (int)__popcll(b);
             }
         }
         if (lane < k) best[lane] = 0;
+        if (found <= kHeld && lane < 8) cand[found + lane] = 0;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (found <= kHeld) {
-            for (int i = lane; i < found; i += 64) {
-                const u64 mine = cand[i];
-                int r = 0;
-#pragma unroll 4
-                for (int j = 0; j < found; j++) r += cand[j] > mine;
-                if (r < k) best[r] = mine;
-            }
+            rank(cand, found, best, k, lane, 64);
         } else {
             u64 prev = ~0ull;
             for (int r = 0; r < k; r++) {
