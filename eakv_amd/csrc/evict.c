@@ -74,10 +74,13 @@ int eakv_attention_weights_batch_device(eakv_cache_t *const *caches, int n_cache
     return rc;
 }
 
+/* the kernels' positions are 32 bits, with room for a block's behind the last */
+#define MOST_TOKENS (1 << 30)
+
 size_t eakv_evict_select_work_bytes(int n_seqs, const int32_t *n_tokens)
 {
     int bad = n_seqs < 0 || n_seqs > EAKVD_MAX_BATCH || (n_seqs && !n_tokens);
-    for (int i = 0; !bad && i < n_seqs; i++) bad = n_tokens[i] < 0;
+    for (int i = 0; !bad && i < n_seqs; i++) bad = n_tokens[i] < 0 || n_tokens[i] > MOST_TOKENS;
     if (bad) {
         eakvi_set_error(EAKV_ERR_INVALID, "evict: invalid argument");
         return 0;
@@ -102,7 +105,7 @@ int eakv_evict_select_device(int n_seqs, int n_heads, const float *d_weights, in
     int64_t total = 0;
     for (int i = 0; i < n_seqs; i++) {
         const int64_t n = n_tokens[i], stay = (int64_t)n_first + n_recent;
-        if (n < 0 || n_keep[i] < (stay < n ? stay : n) || n_keep[i] > n || ld < n ||
+        if (n < 0 || n > MOST_TOKENS || n_keep[i] < (stay < n ? stay : n) || n_keep[i] > n || ld < n ||
             (d_kept && ld_kept < n_keep[i]))
             return eakvi_set_error(EAKV_ERR_INVALID,
                                    "evict: %d of %lld tokens, %lld of them the first and last", n_keep[i],

@@ -21,6 +21,11 @@ constexpr int kPartThreads = 256;
 constexpr int kPartEach = 8;
 constexpr int kPart = kPartThreads * kPartEach;
 
+struct Known {
+    uint32_t top;
+    int keep;
+};
+
 struct EvictJob {
     eakvd_evict e;
     const float *weights;
@@ -31,6 +36,7 @@ struct EvictJob {
     uint32_t *key;          // [n_seq][most]
     uint32_t *hist;         // [n_seq][3][2048]
     uint32_t *count;        // [n_seq][parts][2]: larger than the threshold, equal to it
+    Known *known;           // [n_seq][3]: what 1, 2 and 3 histograms say
     int parts;
 };
 
@@ -160,12 +166,7 @@ __global__ __launch_bounds__(kOneThreads) void evict_one_kernel(EvictJob J)
             c[k] = (int)(x.x + x.y + x.z + x.w);
             sum += c[k];
         }
-        int upto = sum;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int u = __shfl_up(upto, o, 64);
-            if (lane >= o) upto += u;
-        }
+        const int upto = wave_scan_i(sum);
         const int at = __ffsll((unsigned long long)__ballot(upto >= ties)) - 1;
         int before = __builtin_amdgcn_readlane(upto - sum, at), d = 255 - 4 * at;
 #pragma unroll
@@ -184,8 +185,8 @@ __global__ __launch_bounds__(kOneThreads) void evict_one_kernel(EvictJob J)
 #pragma unroll
     for (int i = 0; i < E; i++) {
         const bool in = i < each && t0 + 64 * i < n;
-        gt += (int)__popcll(__ballot(in && key[i] > thr));
-        eq += (int)__popcll(__ballot(in && key[i] == thr));
+        gt += (int)__popcll(__builtin_amdgcn_ballot_w64(in && key[i] > thr));
+        eq += (int)__popcll(__builtin_amdgcn_ballot_w64(in && key[i] == thr));
     }
     if (lane < 2) sums[4 * w + lane] = lane ? eq : gt;
     __syncthreads();
@@ -198,7 +199,8 @@ __global__ __launch_bounds__(kOneThreads) void evict_one_kernel(EvictJob J)
         const int t = t0 + 64 * i;
         const bool in = i < each && t < n;
         const uint64_t below = (1ull << lane) - 1;
-        const uint64_t g = __ballot(in && key[i] > thr), e = __ballot(in && key[i] == thr);
+        const uint64_t g = __builtin_amdgcn_ballot_w64(in && key[i] > thr),
+                       e = __builtin_amdgcn_ballot_w64(in && key[i] == thr);
         const int eq_at = eq_before + (int)__popcll(e & below);
         const bool mine = (g >> lane & 1) || ((e >> lane & 1) && eq_at < ties);
         rank[i] = mine ? gt_before + (int)__popcll(g & below) + min(eq_at, ties) : -1;
@@ -227,12 +229,7 @@ __device__ __forceinline__ int digit_of(const uint32_t *hist, int keep, int *abo
     for (int i = 0; i < per; i++) c[i] = (int)hist[BINS - 1 - (tid * per + i)];
 #pragma unroll
     for (int i = 0; i < per; i++) sum += c[i];
-    int upto = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(upto, o, 64);
-        if (lane >= o) upto += u;
-    }
+    const int upto = wave_scan_i(sum);
     __syncthreads();
     if (lane == 63) sh[w] = upto;
     __syncthreads();
@@ -255,23 +252,17 @@ __device__ __forceinline__ int digit_of(const uint32_t *hist, int keep, int *abo
 }
 
 // What is known of the threshold after LEVEL histograms: its top bits, and how many keys
-// with them stay.
-struct Known {
-    uint32_t top;
-    int keep;
-};
+// with them stay.  The launch before left it after LEVEL - 1 of them.
 template <int LEVEL>
 __device__ __forceinline__ Known known(const EvictJob &J, int s, int *sh, int tid)
 {
-    Known k = {0, J.e.n_keep[s]};
-#pragma unroll
-    for (int l = 0; l < LEVEL; l++) {
-        int above;
-        const uint32_t *hist = J.hist + ((int64_t)s * 3 + l) * 2048;
-        const int d = l < 2 ? digit_of<2048>(hist, k.keep, &above, sh, tid) : digit_of<1024>(hist, k.keep, &above, sh, tid);
-        k.top = k.top * (l < 2 ? 2048u : 1024u) + (uint32_t)d;
-        k.keep -= above;
-    }
+    if constexpr (LEVEL == 0) return Known{0, J.e.n_keep[s]};
+    Known k = LEVEL == 1 ? Known{0, J.e.n_keep[s]} : J.known[3 * s + LEVEL - 2];
+    int above;
+    const uint32_t *hist = J.hist + ((int64_t)s * 3 + LEVEL - 1) * 2048;
+    const int d = LEVEL < 3 ? digit_of<2048>(hist, k.keep, &above, sh, tid) : digit_of<1024>(hist, k.keep, &above, sh, tid);
+    k.top = k.top * (LEVEL < 3 ? 2048u : 1024u) + (uint32_t)d;
+    k.keep -= above;
     return k;
 }
 
@@ -290,6 +281,7 @@ __global__ __launch_bounds__(kPartThreads) void evict_part_kernel(EvictJob J)
 #pragma unroll
         for (int i = 0; i < kPartEach; i++) key[i] = keys[min(t0 + i * kPartThreads + tid, n - 1)];
     const Known k = known<LEVEL>(J, s, sh, tid);
+    if (LEVEL > 0 && blockIdx.x == 0 && tid == 0) J.known[3 * s + LEVEL - 1] = k;
     if constexpr (LEVEL < 3) {
         for (int i = tid; i < 2048; i += kPartThreads) bins[i] = 0;
         __syncthreads();
@@ -334,7 +326,7 @@ __global__ __launch_bounds__(kPartThreads) void evict_part_kernel(EvictJob J)
 
 __global__ __launch_bounds__(kPartThreads) void evict_write_kernel(EvictJob J)
 {
-    __shared__ int sh[8], sums[2][kPartThreads / 64][2];
+    __shared__ int sh[2], sums[kPartEach][kPartThreads / 64][2];
     const int s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, t0 = (int)blockIdx.x * kPart;
     const int n = J.e.n_tokens[s];
     clear_rest(J, s, (int)blockIdx.x * kPartThreads + tid, (int)gridDim.x * kPartThreads);
@@ -343,8 +335,7 @@ __global__ __launch_bounds__(kPartThreads) void evict_write_kernel(EvictJob J)
     uint32_t key[kPartEach];
 #pragma unroll
     for (int i = 0; i < kPartEach; i++) key[i] = keys[min(t0 + i * kPartThreads + tid, n - 1)];
-    const Known k = known<3>(J, s, sh, tid);
-    // (k.keep of the keys at the threshold stay)
+    const Known k = J.known[3 * s + 2];         // (k.keep of the keys at the threshold stay)
     if (tid < 2) sh[tid] = 0;
     __syncthreads();
     {
@@ -357,30 +348,33 @@ __global__ __launch_bounds__(kPartThreads) void evict_write_kernel(EvictJob J)
         if (g) atomicAdd(&sh[0], g);
         if (e) atomicAdd(&sh[1], e);
     }
-    __syncthreads();
-    int gt_before = sh[0], eq_before = sh[1];
     const uint64_t below = (1ull << lane) - 1;
-    int rank[kPartEach];
+    uint64_t gs[kPartEach], es[kPartEach];
 #pragma unroll
     for (int i = 0; i < kPartEach; i++) {
         const int t = t0 + i * kPartThreads + tid;
-        const uint32_t x = key[i];
-        const uint64_t g = __ballot(t < n && x > k.top), e = __ballot(t < n && x == k.top);
+        gs[i] = __builtin_amdgcn_ballot_w64(t < n && key[i] > k.top);
+        es[i] = __builtin_amdgcn_ballot_w64(t < n && key[i] == k.top);
         if (lane == 0) {
-            sums[i & 1][w][0] = (int)__popcll(g);
-            sums[i & 1][w][1] = (int)__popcll(e);
+            sums[i][w][0] = (int)__popcll(gs[i]);
+            sums[i][w][1] = (int)__popcll(es[i]);
         }
-        __syncthreads();
-        int g_at = gt_before + (int)__popcll(g & below), e_at = eq_before + (int)__popcll(e & below);
+    }
+    __syncthreads();
+    int gt_before = sh[0], eq_before = sh[1];
+    int rank[kPartEach];
+#pragma unroll
+    for (int i = 0; i < kPartEach; i++) {
+        int g_at = gt_before + (int)__popcll(gs[i] & below), e_at = eq_before + (int)__popcll(es[i] & below);
 #pragma unroll
         for (int j = 0; j < kPartThreads / 64; j++) {
-            const int a = sums[i & 1][j][0], b = sums[i & 1][j][1];
+            const int a = sums[i][j][0], b = sums[i][j][1];
             g_at += j < w ? a : 0;
             e_at += j < w ? b : 0;
             gt_before += a;
             eq_before += b;
         }
-        rank[i] = (g >> lane & 1) || ((e >> lane & 1) && e_at < k.keep) ? g_at + min(e_at, k.keep) : -1;
+        rank[i] = (gs[i] >> lane & 1) || ((es[i] >> lane & 1) && e_at < k.keep) ? g_at + min(e_at, k.keep) : -1;
     }
     float w4[kPartEach][kHeadsOf<kPartEach>];
     if (J.kept && J.e.n_heads <= kHeadsOf<kPartEach>) load_heads<kPartEach>(J, s, t0 + tid, kPartThreads, n, 0, w4);
@@ -401,7 +395,7 @@ extern "C" size_t eakvd_evict_work_bytes(int n_seq, const int32_t *n_tokens)
     const int most = most_of(n_seq, n_tokens);
     if (most <= kOneMost) return 0;
     const size_t parts = ((size_t)most + kPart - 1) / kPart;
-    return (size_t)n_seq * ((size_t)most + 3 * 2048 + 2 * parts) * 4;
+    return (size_t)n_seq * ((size_t)most + 3 * 2048 + 3 * 2 + 2 * parts) * 4;
 }
 
 extern "C" int eakvd_evict_select(const eakvd_evict *job, const float *weights, int64_t ld, int32_t *index,
@@ -425,7 +419,8 @@ extern "C" int eakvd_evict_select(const eakvd_evict *job, const float *weights, 
     }
     J.parts = (J.most + kPart - 1) / kPart;
     J.hist = (uint32_t *)work;
-    J.count = J.hist + (size_t)n * 3 * 2048;
+    J.known = (Known *)(J.hist + (size_t)n * 3 * 2048);
+    J.count = (uint32_t *)(J.known + (size_t)n * 3);
     J.key = J.count + (size_t)n * J.parts * 2;
     const int zero = (int)n * 3 * 2048;
     const dim3 grid((unsigned)J.parts, n), nt(kPartThreads);

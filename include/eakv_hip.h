@@ -343,7 +343,7 @@ size_t eakv_attention_weights_work_bytes(eakv_cache_t *const *caches, int n_cach
  * d_weights[(i * n_heads + h) * ld + t] over the n_heads rows h (kv heads, or layers x kv heads),
  * summed in 64 bits and rounded to 32; NaN is below every number.
  *   n_tokens, n_keep  host int32[n_seqs]; min(n_first + n_recent, n_tokens[i]) <= n_keep[i] <=
- *                     n_tokens[i]; at most 32 sequences
+ *                     n_tokens[i]; at most 32 sequences of 2^30 tokens
  *   d_index  int32[sum of n_keep]: each sequence's positions, ascending, one list after the
  *            other: what eakv_cache_gather_batch_device takes
  *   d_kept   NULL, or f32[n_seqs][n_heads][ld_kept]: the weights of the tokens that stay, in

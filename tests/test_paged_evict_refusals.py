@@ -59,7 +59,7 @@ def test_select_arguments():
     for kw in (dict(n=-1), dict(n=33), dict(h=0), dict(h=65537), dict(first=-1), dict(recent=-1),
                dict(tok=None), dict(keep=None), dict(tok=[100, -1]), dict(keep=[11, 500]),
                dict(keep=[101, 500]), dict(keep=[12, -1]), dict(first=1 << 30, recent=1 << 30),
-               dict(ld=19999), dict(ld_kept=499), dict(w=0), dict(idx=0), dict(work=0),
+               dict(tok=[100, (1 << 30) + 1], ld=1 << 31), dict(ld=19999), dict(ld_kept=499), dict(w=0), dict(idx=0), dict(work=0),
                dict(w=4097), dict(idx=(1 << 20) + 2), dict(kept=(1 << 22) + 1), dict(work=(1 << 24) + 2),
                dict(size=16)):
         assert refused(call(**kw)), kw
@@ -69,7 +69,7 @@ def test_select_arguments():
     assert L.eakv_evict_select_work_bytes(2, E.ints([8193, 100])) > 0
     assert L.eakv_evict_select_work_bytes(0, None) == 0
     assert L.eakv_last_error() == E.EAKV_OK
-    for n, tok in ((-1, [1]), (33, [1] * 33), (1, None), (2, [5, -1])):
+    for n, tok in ((-1, [1]), (33, [1] * 33), (1, None), (2, [5, -1]), (1, [(1 << 30) + 1])):
         assert L.eakv_evict_select_work_bytes(n, tok and E.ints(tok)) == 0
         assert refused(INVALID), (n, tok)
 
