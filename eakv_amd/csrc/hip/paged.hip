@@ -849,21 +849,35 @@ __global__ __launch_bounds__(D * 4) void paged_join_kernel(PagedJob J, int grid)
     if (c.n == 0 || j >= c.rows) return;
     const float *po = J.part, *pm = J.part + (int64_t)grid * 2 * J.rbr * D;
     auto row = [&](int k) { return (int64_t)(k ? 2 * (b + k) : 2 * b + 1) * J.rbr + j; };
-    float m = kMInit;
-    for (int k = 0; k < c.n; k++) {
-        const float2 x = *(const float2 *)(pm + row(k) * 2);
-        if (x.y != 0.0f) m = fmaxf(m, x.x);
-    }
-    float l = 0.0f;
+    // (eight parts' loads in flight)
+    float m = kMInit, l = 0.0f;
     v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k = 0; k < c.n; k++) {
-        const float2 x = *(const float2 *)(pm + row(k) * 2);
-        const v4f v = *(const v4f *)(po + row(k) * D + dim);
-        if (x.y == 0.0f) continue;                               // (nothing seen there)
-        const float al = __builtin_amdgcn_exp2f(x.x - m), half = __builtin_amdgcn_exp2f(0.5f * (x.x - m));
-        l = fmaf(half * x.y, half, l);
+    for (int k0 = 0; k0 < c.n; k0 += 8) {
+        float2 x[8];
+        v4f v[8];
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[e] = fmaf(al, v[e], o[e]);
+        for (int k = 0; k < 8; k++) {
+            const int64_t r = row(min(k0 + k, c.n - 1));
+            x[k] = *(const float2 *)(pm + r * 2);
+            v[k] = *(const v4f *)(po + r * D + dim);
+            if (k0 + k >= c.n) x[k].y = 0.0f;
+        }
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < 8; k++) top = x[k].y != 0.0f ? fmaxf(top, x[k].x) : top;      // (0: nothing seen there)
+        const float was = __builtin_amdgcn_exp2f(m - top), was2 = __builtin_amdgcn_exp2f(0.5f * (m - top));
+        l = l * was2 * was2;
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] *= was;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            if (x[k].y == 0.0f) continue;
+            const float al = __builtin_amdgcn_exp2f(x[k].x - top), half = __builtin_amdgcn_exp2f(0.5f * (x[k].x - top));
+            l = fmaf(half * x[k].y, half, l);
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = fmaf(al, v[k][e], o[e]);
+        }
+        m = top;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const float y[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
