@@ -838,52 +838,79 @@ __global__ __launch_bounds__(64 * kWaves, NR > 1 ? 2 : 3) void paged_kernel(eakv
     if (!J.whole && tid == 0) J.cut[bl] = cut;
 }
 
-// The parts of units that were cut, joined: a block for each 16 rows of a cut, 4 dims
-// and a row to a thread.
-template <int D, bool F32>
-__global__ __launch_bounds__(D * 4) void paged_join_kernel(PagedJob J, int grid)
+// Parts k, k + step, .. of `n` joined, eight at a time (their loads in flight together): M, l and 4
+// dims of O.
+struct Joined {
+    float m, l;
+    v4f o;
+};
+template <class ML, class O>
+__device__ __forceinline__ Joined join_parts(int k, int step, int n, const ML &ml, const O &sums)
 {
-    const int b = blockIdx.x, j = 16 * (int)blockIdx.y + (int)threadIdx.x / (D / 4);
-    const int dim = (int)threadIdx.x % (D / 4) * 4;
-    const PagedCut c = J.cut[b];
-    if (c.n == 0 || j >= c.rows) return;
-    const float *po = J.part, *pm = J.part + (int64_t)grid * 2 * J.rbr * D;
-    auto row = [&](int k) { return (int64_t)(k ? 2 * (b + k) : 2 * b + 1) * J.rbr + j; };
-    // (eight parts' loads in flight)
-    float m = kMInit, l = 0.0f;
-    v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k0 = 0; k0 < c.n; k0 += 8) {
+    Joined j = {kMInit, 0.0f, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
+    for (; k < n; k += 8 * step) {
         float2 x[8];
         v4f v[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const int64_t r = row(min(k0 + k, c.n - 1));
-            x[k] = *(const float2 *)(pm + r * 2);
-            v[k] = *(const v4f *)(po + r * D + dim);
-            if (k0 + k >= c.n) x[k].y = 0.0f;
+        for (int i = 0; i < 8; i++) {
+            const int at = k + i * step;
+            x[i] = ml(min(at, n - 1));
+            v[i] = sums(min(at, n - 1));
+            if (at >= n) x[i].y = 0.0f;
         }
-        float top = m;
+        float top = j.m;
 #pragma unroll
-        for (int k = 0; k < 8; k++) top = x[k].y != 0.0f ? fmaxf(top, x[k].x) : top;      // (0: nothing seen there)
-        const float was = __builtin_amdgcn_exp2f(m - top), was2 = __builtin_amdgcn_exp2f(0.5f * (m - top));
-        l = l * was2 * was2;
+        for (int i = 0; i < 8; i++) top = x[i].y != 0.0f ? fmaxf(top, x[i].x) : top;      // (0: nothing seen there)
+        const float was = __builtin_amdgcn_exp2f(j.m - top), half = __builtin_amdgcn_exp2f(0.5f * (j.m - top));
+        j.l = j.l * half * half;
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[e] *= was;
+        for (int e = 0; e < 4; e++) j.o[e] *= was;
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            if (x[k].y == 0.0f) continue;
-            const float al = __builtin_amdgcn_exp2f(x[k].x - top), half = __builtin_amdgcn_exp2f(0.5f * (x[k].x - top));
-            l = fmaf(half * x[k].y, half, l);
+        for (int i = 0; i < 8; i++) {
+            if (x[i].y == 0.0f) continue;
+            const float al = __builtin_amdgcn_exp2f(x[i].x - top), h = __builtin_amdgcn_exp2f(0.5f * (x[i].x - top));
+            j.l = fmaf(h * x[i].y, h, j.l);
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[e] = fmaf(al, v[k][e], o[e]);
+            for (int e = 0; e < 4; e++) j.o[e] = fmaf(al, v[i][e], j.o[e]);
         }
-        m = top;
+        j.m = top;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const float y[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+    return j;
+}
+
+// The parts of units that were cut, joined: a block for each 16 rows of a cut, 4 dims and a row to
+// a thread.  Fewer rows: several threads to these, each with a share of the parts.
+template <int D, bool F32>
+__global__ __launch_bounds__(D * 4) void paged_join_kernel(PagedJob J, int grid)
+{
+    __shared__ float2 sml[D * 4];
+    __shared__ v4f so[D * 4];
+    const int b = blockIdx.x, tid = threadIdx.x, dim = tid % (D / 4) * 4, slot = tid / (D / 4);
+    const PagedCut c = J.cut[b];
+    const int rows = min(16, c.rows - 16 * (int)blockIdx.y);
+    if (c.n == 0 || rows <= 0) return;
+    // (up to 16 parts by one thread: 1 us less than their sharing costs)
+    const int log2r = c.n <= 16 ? 4 : rows <= 1 ? 0 : 32 - __clz(rows - 1), rp = 1 << log2r, groups = 16 >> log2r;
+    const int r = slot & (rp - 1), j = 16 * (int)blockIdx.y + r;
+    if (groups == 1 && r >= rows) return;
+    const float *po = J.part, *pm = J.part + (int64_t)grid * 2 * J.rbr * D;
+    auto row = [&](int k) { return (int64_t)(k ? 2 * (b + k) : 2 * b + 1) * J.rbr + j; };
+    Joined y = join_parts(slot >> log2r, groups, c.n, [&](int k) { return *(const float2 *)(pm + row(k) * 2); },
+                          [&](int k) { return *(const v4f *)(po + row(k) * D + dim); });
+    if (groups > 1) {
+        sml[tid] = float2{y.m, y.l};
+        so[tid] = y.o;
+        __syncthreads();
+        if (slot >= rp) return;
+        y = join_parts(0, 1, groups, [&](int k) { return sml[tid + k * rp * (D / 4)]; },
+                       [&](int k) { return so[tid + k * rp * (D / 4)]; });
+    }
+    if (r >= rows) return;
+    const float inv = y.l == 0.0f ? 0.0f : 1.0f / y.l;
+    const float out[4] = {y.o[0] * inv, y.o[1] * inv, y.o[2] * inv, y.o[3] * inv};
     const int t = J.hb == 1 ? j / J.qpk : 0;
     store4<F32>(J.out, (int64_t)(c.tok + t) * J.ld_out + (int64_t)(c.head + j - t * J.qpk) * D + dim,
-                J.vec & 2, y);
+                J.vec & 2, out);
 }
 
 struct PagedPlan {
