@@ -78,16 +78,34 @@ __device__ __forceinline__ float logit(const void *x, int64_t at)
     else return ((const float *)x)[at];
 }
 
-// ln s of a sum: its exponent and the logarithm of what is left of it, of 1 to 2, each in one
-// instruction (2^-23 off; with the library's in 64 bits a launch took 0.3 us more).
+// e^x, |x| <= 0.35, to 2e-10: the series' terms up to x^8.
+__device__ __forceinline__ double exp_near(double x)
+{
+    double y = 1.0 / 40320;
+    y = fma(y, x, 1.0 / 5040);
+    y = fma(y, x, 1.0 / 720);
+    y = fma(y, x, 1.0 / 120);
+    y = fma(y, x, 1.0 / 24);
+    y = fma(y, x, 1.0 / 6);
+    y = fma(y, x, 0.5);
+    y = fma(y, x, 1.0);
+    return fma(y, x, 1.0);
+}
+
+// ln s of a sum, from its exponent e and the rest f, of 1 to 2: g = log2 f by the f32 instruction,
+// then f 2^-g - 1, which is ln f - g ln 2 but for its square.  (With the library's functions of 64
+// bits, here and in put_right, a launch took 0.3 us more.)
 __device__ __forceinline__ double ln_of(double s)
 {
+    constexpr double ln2 = 0.6931471805599453;
     const uint64_t b = (uint64_t)__double_as_longlong(s);
-    const int e = (int)(b >> 52);               // (0, infinite and NaN sums: 0, 0x7ff, above)
-    const bool plain = e > 0 && e < 0x7ff;
-    const double f = plain ? __longlong_as_double((long long)((b & 0xfffffffffffffull) | 0x3ff0000000000000ull)) : s;
-    return fma(0.6931471805599453, (double)__builtin_amdgcn_logf((float)f),
-               plain ? 0.6931471805599453 * (double)(e - 1023) : 0.0);
+    const int e = (int)(b >> 52);
+    // 0, infinite and NaN sums as f32 has them
+    if (e <= 0 || e >= 0x7ff) return (double)__builtin_amdgcn_logf((float)s);
+    const double f = __longlong_as_double((long long)((b & 0xfffffffffffffull) | 0x3ff0000000000000ull));
+    const double g = (double)__builtin_amdgcn_logf((float)f);
+    const double d = fma(f, 0.7071067811865476 * exp_near(ln2 * (0.5 - g)), -1.0);
+    return fma(ln2, g + (double)(e - 1023), d);
 }
 
 // A row's results from M, S, T (in units of ln 2), the given token's logit and the sorted
@@ -100,7 +118,11 @@ __device__ __forceinline__ void finish(const LpJob &J, int64_t row, float m, dou
         if (J.lp)
             J.lp[row] = token >= 0 && token < J.vocab ? (float)((double)given - (double)m - ln_s)
                                                       : -__builtin_inff();
-        if (J.entropy) J.entropy[row] = (float)(ln_s - 0.6931471805599453 * (double)((float)t * __builtin_amdgcn_rcpf((float)s)));
+        if (J.entropy) {
+            // t / s: the f32 reciprocal and a step of Newton's
+            const double y = (double)__builtin_amdgcn_rcpf((float)s);
+            J.entropy[row] = (float)(ln_s - 0.6931471805599453 * (t * (y * fma(-s, y, 2.0))));
+        }
     }
     if (tid < J.k) {
         const u64 key = best[tid];
@@ -113,7 +135,7 @@ __device__ __forceinline__ void finish(const LpJob &J, int64_t row, float m, dou
 // S and T of terms whose exponents are all off by r
 __device__ __forceinline__ void put_right(double r, double &s, double &t)
 {
-    const double f = (double)__builtin_amdgcn_exp2f(-(float)r);
+    const double f = exp_near(-0.6931471805599453 * r);         // (|r| < 0.1)
     t = f * (t - r * s);
     s = f * s;
 }
