@@ -135,7 +135,8 @@ extern "C" int eakvd_paged_append(const eakvd_geom *g, uint8_t *base, const eakv
     if (parts > all) parts = all;
     J.heads = (int)((all + parts - 1) / parts);
     J.parts = (all + J.heads - 1) / J.heads;
-    if (chunks * J.parts > INT32_MAX) return (int)hipErrorInvalidValue;
+    // (a launch has fewer than 2^32 threads)
+    if (chunks * J.parts >= (1 << 24)) return (int)hipErrorInvalidValue;
     const dim3 grid((unsigned)(chunks * J.parts));
     auto run = [&](auto *kern) {
         hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, (hipStream_t)stream, *g, J);
