@@ -85,10 +85,10 @@ __device__ __forceinline__ void keys_of(const EvictJob &J, int s, int t0, int st
 }
 
 // Tokens t0 + i * step of sequence s stay, as the rank[i]-th (-1: do not): x holds their weights of
-// up to kHeadsOf heads, else they are read again, all tokens' loads of some heads in flight.
+// the first kHeadsOf heads (have), the others' are read, all tokens' loads of some heads in flight.
 template <int E>
 __device__ __forceinline__ void put_all(const EvictJob &J, int s, int t0, int step, int n, const int *rank,
-                                        float (&x)[E][kHeadsOf<E>])
+                                        float (&x)[E][kHeadsOf<E>], bool have)
 {
     constexpr int H = kHeadsOf<E>;
     int32_t *index = J.index + J.e.first[s];
@@ -98,7 +98,7 @@ __device__ __forceinline__ void put_all(const EvictJob &J, int s, int t0, int st
     if (!J.kept) return;
     float *k = J.kept + (int64_t)s * J.e.n_heads * J.ld_kept;
     for (int h0 = 0; h0 < J.e.n_heads; h0 += H) {
-        if (J.e.n_heads > H) load_heads<E>(J, s, t0, step, n, h0, x);
+        if (h0 > 0 || !have) load_heads<E>(J, s, t0, step, n, h0, x);
 #pragma unroll
         for (int h = 0; h < H; h++)
 #pragma unroll
@@ -207,7 +207,7 @@ __global__ __launch_bounds__(kOneThreads) void evict_one_kernel(EvictJob J)
         gt_before += (int)__popcll(g);
         eq_before += (int)__popcll(e);
     }
-    put_all<E>(J, s, t0, 64, n, rank, x);
+    put_all<E>(J, s, t0, 64, n, rank, x, J.e.n_heads <= kHeadsOf<E>);
 }
 
 __global__ __launch_bounds__(256) void evict_clear_kernel(uint32_t *p, int n)
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(kPartThreads) void evict_part_kernel(EvictJob J)
 
 __global__ __launch_bounds__(kPartThreads) void evict_write_kernel(EvictJob J)
 {
-    __shared__ int sh[2], sums[kPartEach][kPartThreads / 64][2];
+    __shared__ int before[kPartThreads / 64][2], sums[kPartEach][kPartThreads / 64][2];
     const int s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, t0 = (int)blockIdx.x * kPart;
     const int n = J.e.n_tokens[s];
     clear_rest(J, s, (int)blockIdx.x * kPartThreads + tid, (int)gridDim.x * kPartThreads);
@@ -336,18 +336,17 @@ __global__ __launch_bounds__(kPartThreads) void evict_write_kernel(EvictJob J)
 #pragma unroll
     for (int i = 0; i < kPartEach; i++) key[i] = keys[min(t0 + i * kPartThreads + tid, n - 1)];
     const Known k = J.known[3 * s + 2];         // (k.keep of the keys at the threshold stay)
-    if (tid < 2) sh[tid] = 0;
-    __syncthreads();
-    {
-        int g = 0, e = 0;
-        for (int p = tid; p < (int)blockIdx.x; p += kPartThreads) {
-            const uint32_t *c = J.count + ((int64_t)s * J.parts + p) * 2;
-            g += (int)c[0];
-            e += (int)c[1];
-        }
-        if (g) atomicAdd(&sh[0], g);
-        if (e) atomicAdd(&sh[1], e);
+    int g0 = 0, e0 = 0;                         // of the parts before
+    for (int p = tid; p < (int)blockIdx.x; p += kPartThreads) {
+        const uint32_t *c = J.count + ((int64_t)s * J.parts + p) * 2;
+        g0 += (int)c[0];
+        e0 += (int)c[1];
     }
+    float w4[kPartEach][kHeadsOf<kPartEach>];
+    if (J.kept) load_heads<kPartEach>(J, s, t0 + tid, kPartThreads, n, 0, w4);
+    g0 = __builtin_amdgcn_readlane(wave_scan_i(g0), 63);
+    e0 = __builtin_amdgcn_readlane(wave_scan_i(e0), 63);
+    if (lane == 0) before[w][0] = g0, before[w][1] = e0;
     const uint64_t below = (1ull << lane) - 1;
     uint64_t gs[kPartEach], es[kPartEach];
 #pragma unroll
@@ -361,7 +360,12 @@ __global__ __launch_bounds__(kPartThreads) void evict_write_kernel(EvictJob J)
         }
     }
     __syncthreads();
-    int gt_before = sh[0], eq_before = sh[1];
+    int gt_before = 0, eq_before = 0;
+#pragma unroll
+    for (int j = 0; j < kPartThreads / 64; j++) {
+        gt_before += before[j][0];
+        eq_before += before[j][1];
+    }
     int rank[kPartEach];
 #pragma unroll
     for (int i = 0; i < kPartEach; i++) {
@@ -376,9 +380,7 @@ __global__ __launch_bounds__(kPartThreads) void evict_write_kernel(EvictJob J)
         }
         rank[i] = (gs[i] >> lane & 1) || ((es[i] >> lane & 1) && e_at < k.keep) ? g_at + min(e_at, k.keep) : -1;
     }
-    float w4[kPartEach][kHeadsOf<kPartEach>];
-    if (J.kept && J.e.n_heads <= kHeadsOf<kPartEach>) load_heads<kPartEach>(J, s, t0 + tid, kPartThreads, n, 0, w4);
-    put_all<kPartEach>(J, s, t0 + tid, kPartThreads, n, rank, w4);
+    put_all<kPartEach>(J, s, t0 + tid, kPartThreads, n, rank, w4, true);
 }
 
 int most_of(int n_seq, const int32_t *n)
