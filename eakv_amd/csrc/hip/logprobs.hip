@@ -17,6 +17,11 @@
 // Exponents are z = x log2(e) - c, one instruction, c = M log2(e) rounded: all are off by the
 // same r = M log2(e) - c, which S, T and H are rid of at the end (S 2^-r).  (From 2^20 on r is
 // not small: differences first.)
+//
+// Bound by vector instructions (14 a bf16 value with entropy and alternatives, 92 % of the cycles)
+// for bf16, by HBM for f32; small calls by two launches' latency.  500 rows of 151665, 20
+// alternatives: bf16 49-51 us (3.0 TB/s; without alternatives 34), f32 66 us (4.6); one row of
+// 32000 f32 9.2-9.9 us.
 #include <math.h>
 #include <string.h>
 

@@ -8,10 +8,17 @@
 // exact for both types).  A first pass over K leaves each row's (M, L) of a chunk of tokens.
 // Few rows (up to kStore to a kv head, a decode step): it also leaves the scores, and the
 // second launch adds their weights up: 8 bytes a row and token more against K's 80, and no
-// products.  More: the second pass makes the scores again.  Rows (window tokens x q heads) are
-// taken kRowTiles row tiles at a time, their operands in LDS; a wave holds 32 tokens'
-// operands of K in registers and goes through the rows.  A token's sum is one thread's or one
-// wave's: no atomics, the same bits on every call.
+// products.  More: the second pass makes the scores again, with tokens across the lanes so that
+// rows add up in a lane's registers.  Rows (window tokens x q heads) are taken several row tiles
+// at a time, their operands in LDS; a wave holds 32 tokens' operands of K in registers and goes
+// through the rows.  The first pass gives groups of row tiles to blocks of their own; the
+// second, which sums over all rows, has them one after the other.  A token's sum is one
+// thread's or one wave's: no atomics, the same bits on every call.
+//
+// Few rows are bound by memory (one f32 token x 8 at 32768, 32 q / 8 kv: 65 us; K and the scores
+// both ways at a copy's 4.66 TB/s 54); many by instructions issued (32 bf16 tokens x 4 to 20011, 64 q /
+// 8 kv: 85-97 us, the passes alike; vector ALUs 72 % and all kinds 93 to 96 % of the cycles,
+// matrix cores 29 to 35 %; 90 and 73 vector instructions for 16 rows x 32 tokens).
 #include <string.h>
 
 #include "rows16.h"
