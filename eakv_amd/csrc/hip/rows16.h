@@ -133,17 +133,25 @@ __device__ __forceinline__ void k_operands(const uint2 &x, float z, const NibCon
 }
 
 // K's operands of the bias product for 32 tokens: lane l holds c of token l % 32, group l /
-// 32 (own: whether it counts), and stands in its own k-block of its half's operand.  e: what is
+// 32, and stands in its own k-block of its half's operand, nothing in the other's.  e: what is
 // added to the token's scores, in units of 1.
-__device__ __forceinline__ void bias_operands(float c, float e, bool first, b8 (&half)[2], int n32)
+__device__ __forceinline__ b8 bias_own(float c, float e, bool first)
 {
     __bf16 p1, p2, p3;
     pieces(c, p1, p2, p3);
     const __bf16 none = (__bf16)0.0f;
-    const b8 own = {p1, p1, p1, p2, p2, p3, first ? (__bf16)e : none, none};
+    return b8{p1, p1, p1, p2, p2, p3, first ? (__bf16)e : none, none};
+}
+__device__ __forceinline__ void bias_halves(const b8 &own, b8 (&half)[2], int n32)
+{
+    const __bf16 none = (__bf16)0.0f;
     const b8 zero = {none, none, none, none, none, none, none, none};
     half[0] = n32 < 16 ? own : zero;
     half[1] = n32 < 16 ? zero : own;
+}
+__device__ __forceinline__ void bias_operands(float c, float e, bool first, b8 (&half)[2], int n32)
+{
+    bias_halves(bias_own(c, e, first), half, n32);
 }
 
 // The dots of one group of 16 tokens with 16 rows.

@@ -107,7 +107,7 @@ static int heads_check(const eakv_cache_t *pool, const eakvd_pages *d, int n_q, 
     int rc = eakvi_attn_check(pool, 0, n_q, n_kv);
     if (rc) return rc;
     const int64_t units = ((int64_t)d->n_new + d->n_seqs) * n_q;
-    const int64_t tiles = (int64_t)d->max_len / 256 + 1;
+    const int64_t tiles = (int64_t)d->max_len / 64 + 1;
     if (units > INT32_MAX || units * tiles > INT32_MAX)
         return eakvi_set_error(EAKV_ERR_INVALID, "attention_paged: %d rows of up to %d tokens in one call",
                                d->n_new, d->max_len);

@@ -303,7 +303,7 @@ int eakv_append_paged_device(eakv_cache_t *pool, const eakv_paged_batch_t *batch
  * Rows that see nothing give zeros.  What a row does not see has no part in its
  * result.  Precision, non-finite values and ranges: as eakv_attention_window_batch_device.
  *   d_work  device scratch of the call's own, 16-byte aligned, over none of the buffers and
- *           of eakv_attention_paged_work_bytes() for the same batch (some MB at most), or
+ *           of eakv_attention_paged_work_bytes() for the same batch (prompts: some 100 MB), or
  *           NULL: the pool's workspace.  Calls that share one and overlap in time race.  A
  *           call on a stream that records a graph needs its own (unless 0 bytes are needed).
  * Streams: as eakv_attention_fused_batch_device. */

@@ -135,3 +135,106 @@ def test_logprobs_of_many_short_rows(E, rng):
     assert (np.abs(lp.download() - want) <= 80 * E32 + E32 * np.abs(want)).all()
     h = -(np.exp(ln) * ln).sum(1)
     assert (np.abs(ent.download() - h) <= (80 + 165 * h) * E32).all()
+
+
+# Large work gives each wave rows of its own; the bound on lengths decides, whatever they are.
+LARGE = 1 << 27
+
+
+def large(p, n_q, **kw):
+    """The batch with a bound on lengths that makes its work large."""
+    return p.make(max_len=LARGE // (p.rows * n_q) + 1, **kw)
+
+
+def large_pool(E, rng, lens, new, page, n_q, n_kv, d, **kw):
+    return P.Pool(E, rng, lens, new, page, n_kv, d, ld_more=LARGE // (sum(new) * n_q) // page + 2, **kw)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("n_q,n_kv,d", [(8, 2, 128), (32, 4, 64), (3, 1, 128), (10, 2, 64), (2, 2, 128),
+                                        (40, 2, 64), (64, 1, 128), (300, 1, 64), (70, 70, 64)])
+@pytest.mark.parametrize("page,lens,new", [
+    (64, [700, 3, 1300, 90], [60, 3, 2, 40]),
+    (128, [600, 31, 0, 300, 7], [170, 31, 0, 1, 2]),
+    (16, [40, 9, 33, 65, 64], [40, 9, 33, 17, 16]),
+])
+def test_rows_of_waves(E, rng, bf16, n_q, n_kv, d, page, lens, new):
+    p = large_pool(E, rng, lens, new, page, n_q, n_kv, d)
+    p.fill(P.contents(rng, p))
+    c = P.Call(p, n_q, n_kv, bf16)
+    q = c.put(rng.standard_normal((p.rows, n_q, d)).astype(np.float32))
+    b = large(p, n_q)
+    c.run(batch=b)
+    got = c.get()
+    W.check(got, *P.attend(p, 0, q, n_q, n_kv), bf16)
+    c.run(batch=b)
+    assert np.array_equal(got.view(np.uint32), c.get().view(np.uint32))
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("d,n_q,n_kv,lens,new", [
+    (64, 8, 1, [20000, 100, 9000], [300, 1, 1]),    # cut units, single tokens beside them
+    (128, 16, 1, [3000, 2500], [513, 20]),
+    (128, 4, 4, [9000], [700]),
+])
+def test_rows_of_waves_long(E, rng, bf16, d, n_q, n_kv, lens, new):
+    p = large_pool(E, rng, lens, new, 16, n_q, n_kv, d)
+    p.fill(P.contents(rng, p))
+    c = P.Call(p, n_q, n_kv, bf16, more=(8, 3), shift=1)
+    q = c.put(rng.standard_normal((p.rows, n_q, d)).astype(np.float32))
+    c.run(batch=large(p, n_q))
+    W.check(c.get(), *P.attend(p, 0, q, n_q, n_kv), bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_rows_of_waves_any_values(E, rng, bf16):
+    """Pages that hold nothing, tokens of very different size, and a non-finite group that some rows
+    see; rows before position 0."""
+    p = large_pool(E, rng, [900, 500, 90, 30], [100, 20, 30, 40], 16, 8, 2, 128,
+                   bad=((0, 0, -1), (0, 2, 1 << 30), (1, 3, -5)) + tuple((2, k, -1) for k in range(6)))
+    x = P.contents(rng, p)
+    x[0][1] *= np.exp2(rng.integers(-30, 30, (1, 900, 1))).astype(np.float32)
+    x[1][1] += 100.0
+    x[1][0] += 20.0
+    p.fill(x)
+    c = P.Call(p, 8, 2, bf16)
+    q = c.put(rng.standard_normal((p.rows, 8, 128)).astype(np.float32))
+    b = large(p, 8)
+    c.run(batch=b)
+    got, (want, tol, half) = c.get(), P.attend(p, 0, q, 8, 2)
+    lim = tol + (half + W.O16 * np.abs(want) if bf16 else 0)
+    assert (np.abs(got.astype(np.float64) - want) <= lim).all()
+    assert (got[120:150] == 0).all() and (got[150:160] == 0).all()
+    x[0][1, 0, 880, 70] = np.inf                # of the first sequence: its last 20 rows see it
+    p.fill(x)
+    c.run(batch=b)
+    new = c.get()
+    hit = np.zeros(new.shape, bool)
+    hit[80:100, :4, 64:] = True
+    assert np.isnan(new[hit]).all()
+    assert np.array_equal(new[~hit].view(np.uint32), got[~hit].view(np.uint32))
+
+
+def test_rows_of_waves_in_place_and_in_a_graph(E, rng):
+    from eakv_amd.hipmem import DeviceArray, synchronize
+    p = large_pool(E, rng, [300, 200], [50, 50], 32, 8, 2, 64)
+    p.fill(P.contents(rng, p))
+    c = P.Call(p, 8, 2, False)
+    q = rng.standard_normal((p.rows, 8, 64)).astype(np.float32)
+    c.put(q)
+    b = large(p, 8, ragged=False)
+    need = b.work_bytes(8, 2)
+    work = DeviceArray((need,), np.uint8)
+    c.run(batch=b)
+    want = c.get()
+    W.check(want, *P.attend(p, 0, q, 8, 2), False)
+    synchronize()
+    g = W.Graph(lambda st: b.attend(0, c.at(0), c.at(0), 8, 2, d_work=work.ptr, work_bytes=need, stream=st))
+    for _ in range(3):
+        c.put(q)
+        synchronize()
+        g.launch()
+        synchronize()
+        got = c._rows(0, c.buf[0].download()).reshape(want.shape)
+        assert np.array_equal(got.view(np.uint32), want.view(np.uint32))
+    g.free()
