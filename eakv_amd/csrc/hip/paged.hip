@@ -968,11 +968,13 @@ __device__ __forceinline__ void unit_rows(const eakvd_geom &geo, const PagedJob 
     };
     const int pos0 = U.q.pos + P.tok0 + 1;                       // positions that token 0's rows see
     const int vis_min = pos0 + token(r0), vis_max = r0 < rows ? pos0 + token(r0 + 16 * n_u - 1) : 0;
+    // (f32 at d = 128: V as its tokens' turn comes; a step ahead it does not fit the registers)
+    constexpr bool late = F32 && D == 128;
     Stage<GPD> st;
     if (src.n_i > 0) {
         src.pages(0);
         src.template load<0>(0, st, Lanes<GPD>(lane));
-        src.template load_v<0>(st);
+        if constexpr (!late) src.template load_v<0>(st);
     }
     // (a lane's places are worked out again where they are wanted, not kept in registers)
     auto again = [&]() __attribute__((always_inline)) {
@@ -984,6 +986,7 @@ __device__ __forceinline__ void unit_rows(const eakvd_geom &geo, const PagedJob 
     auto make = [&](int i) __attribute__((always_inline)) {
         Slot<D, F32> &S = slots[w];
         const Lanes<GPD> ln(again());
+        if constexpr (late) src.template load_v<0>(st);
         const int t0 = lo + 32 * (w + kWaves * i);
         const bool ok_a = st.at_a >= 0, ok_b = st.at_b >= 0;
         const bool live = t0 + ln.n32 < hi && (ln.n32 < 16 ? ok_a : ok_b);
@@ -1037,7 +1040,7 @@ __device__ __forceinline__ void unit_rows(const eakvd_geom &geo, const PagedJob 
         // ---- the next ones
         if (((i + 1) & 63) == 0 && i + 1 < src.n_i) src.pages(i + 1);
         src.template load<0>(i + 1, st, ln);
-        src.template load_v<0>(st);
+        if constexpr (!late) src.template load_v<0>(st);
     };
 
     // N: row tiles of a wave (1, or NR)
