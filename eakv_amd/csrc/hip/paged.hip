@@ -1316,7 +1316,7 @@ __global__ __launch_bounds__(D * 4) void paged_join_kernel(PagedJob J, int grid)
 {
     __shared__ float2 sml[D * 4];
     __shared__ v4f so[D * 4];
-    const int b = blockIdx.x, tid = threadIdx.x, dim = tid % (D / 4) * 4, slot = tid / (D / 4);
+    const int b = line_block((int)blockIdx.x, grid), tid = threadIdx.x, dim = tid % (D / 4) * 4, slot = tid / (D / 4);
     const PagedCut c = J.cut[b];
     const int rows = min(16, c.rows - 16 * (int)blockIdx.y);
     if (c.n == 0 || rows <= 0) return;
