@@ -106,7 +106,9 @@ static int heads_check(const eakv_cache_t *pool, const eakvd_pages *d, int n_q, 
                                dtype);
     int rc = eakvi_attn_check(pool, 0, n_q, n_kv);
     if (rc) return rc;
-    const int64_t units = ((int64_t)d->n_new + d->n_seqs) * n_q;
+    /* row blocks have 16 rows or more, but for a sequence's last; tiles 64 tokens */
+    const int64_t seqs = d->n_seqs < d->n_new ? d->n_seqs : d->n_new;
+    const int64_t units = (int64_t)d->n_new * n_q / 16 + seqs * n_q;
     const int64_t tiles = (int64_t)d->max_len / 64 + 1;
     if (units > INT32_MAX || units * tiles > INT32_MAX)
         return eakvi_set_error(EAKV_ERR_INVALID, "attention_paged: %d rows of up to %d tokens in one call",

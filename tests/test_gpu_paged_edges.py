@@ -238,3 +238,15 @@ def test_rows_of_waves_in_place_and_in_a_graph(E, rng):
         got = c._rows(0, c.buf[0].download()).reshape(want.shape)
         assert np.array_equal(got.view(np.uint32), want.view(np.uint32))
     g.free()
+
+
+def test_long_prompts_of_many_heads_are_accepted(E):
+    """8 million rows of a bound of 3200 tokens; 16 times as many pass what the line counts."""
+    import ctypes as C
+    pool = E.Cache(1, 2, 128, 4096)
+    for n, ok in ((1 << 23, True), (1 << 27, False)):
+        s = E.PagedBatchStruct(1 << 40, 200, 1 << 41, 1 << 42, 3, 16, n, n, 3200)
+        E.lib().eakv_clear_error()
+        assert (E.lib().eakv_attention_paged_work_bytes(pool.h, C.addressof(s), 1, 8, 2) > 0) == ok
+        assert (E.last_error()[0] == 0) == ok
+    E.lib().eakv_clear_error()
