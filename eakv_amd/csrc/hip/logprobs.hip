@@ -371,9 +371,9 @@ __global__ __launch_bounds__(kThreads, 4) void logprob_kernel(LpJob J)
     if (tid < J.k) J.list[p * J.k + tid] = best[tid];
 }
 
-// A row's segments joined, a wave to a row.  Alternatives: every segment's list is sorted, so the
-// least of the lists' n-th entries, n = k / segments, is reached by k keys; those that do are
-// ranked by counting (or, where the lists are more than LDS holds, taken one after the other).
+// A row's segments joined, a wave to a row.  Alternatives: a bound that k of the lists' keys reach,
+// bit by bit; those that do are ranked by counting (or, where the lists are more than LDS
+// holds, taken one after the other).
 template <bool BF16>
 __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LpJob J, int n_rows)
 {
@@ -417,23 +417,24 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(LpJob J, int n_r
         t += __shfl_xor(t, o, 64);
     }
     if (k) {
-        const int n = (k + n_seg - 1) / n_seg;
         int found = kHeld + 1;
         if (all <= kHeld) {
+            // a bound that k keys reach, in 16 bits of the value's order (0: there are fewer); up to 64 keys
+            // are ranked without
+            uint32_t t = 0;
+#pragma unroll 1
+            for (int bit = all > 64 ? 31 : 15; bit >= 16; bit--) {
+                const uint32_t c = t | 1u << bit;
+                int n = 0;
 #pragma unroll
-            for (int i = 0; i < kHeld / 64; i++) cand[lane + 64 * i] = key[i];
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            u64 least = ~0ull;
-            for (int i = lane; i < n_seg; i += 64) {
-                const u64 x = cand[i * k + n - 1];
-                least = x < least ? x : least;
+                for (int i = 0; i < kHeld / 64; i++)
+                    if (64 * i < all) n += (int)__popcll(ballot((uint32_t)(key[i] >> 32) >= c));
+                t = n >= k ? c : t;
             }
-            least = ~wave_max64(~least);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             found = 0;
 #pragma unroll
             for (int i = 0; i < kHeld / 64; i++) {
-                const bool in = key[i] != 0 && key[i] >= least;
+                const bool in = key[i] != 0 && (uint32_t)(key[i] >> 32) >= t;
                 const uint64_t b = ballot(in);
                 const int p = found + (int)__popcll(b & ((1ull << lane) - 1));
                 if (in) cand[p] = key[i];
