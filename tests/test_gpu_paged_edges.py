@@ -250,3 +250,15 @@ def test_long_prompts_of_many_heads_are_accepted(E):
         assert (E.lib().eakv_attention_paged_work_bytes(pool.h, C.addressof(s), 1, 8, 2) > 0) == ok
         assert (E.last_error()[0] == 0) == ok
     E.lib().eakv_clear_error()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_rows_of_waves_of_many_sequences(E, rng, bf16):
+    lens = [int(x) for x in rng.integers(0, 700, 90)]
+    new = [min(int(x), m) for x, m in zip(rng.integers(0, 70, 90), lens)]
+    p = large_pool(E, rng, lens, new, 128, 8, 2, 64)
+    p.fill(P.contents(rng, p))
+    c = P.Call(p, 8, 2, bf16)
+    q = c.put(rng.standard_normal((p.rows, 8, 64)).astype(np.float32))
+    c.run(batch=large(p, 8))
+    W.check(c.get(), *P.attend(p, 0, q, 8, 2), bf16)
