@@ -118,7 +118,10 @@ __device__ __forceinline__ double ln_of(double s)
 __device__ __forceinline__ void finish(const LpJob &J, int64_t row, float m, double s, double t, int token,
                                        float given, const u64 *best, int tid)
 {
-    const double ln_s = ln_of(s);
+    // The largest logit's own term is 1, but rounded here (its z is r), so that a sum of little else may
+    // come out below: ln S >= 0 and H >= 0 are kept.  (A sum of 0, nothing but -inf, stays -inf.)
+    double ln_s = ln_of(s);
+    if (s > 0.0 && ln_s < 0.0) ln_s = 0.0;
     if (tid == 0) {
         if (J.lp)
             J.lp[row] = token >= 0 && token < J.vocab ? (float)((double)given - (double)m - ln_s)
@@ -126,7 +129,8 @@ __device__ __forceinline__ void finish(const LpJob &J, int64_t row, float m, dou
         if (J.entropy) {
             // t / s: the f32 reciprocal and a step of Newton's
             const double y = (double)__builtin_amdgcn_rcpf((float)s);
-            J.entropy[row] = (float)(ln_s - 0.6931471805599453 * (t * (y * fma(-s, y, 2.0))));
+            const double h = ln_s - 0.6931471805599453 * (t * (y * fma(-s, y, 2.0)));
+            J.entropy[row] = h < 0.0 ? 0.0f : (float)h;
         }
     }
     if (tid < J.k) {
