@@ -18,6 +18,11 @@
 // same r = M log2(e) - c, which S, T and H are rid of at the end (S 2^-r).  (From 2^20 on r is
 // not small: differences first.)
 //
+// Errors, e = 2^-24, u = M - x: a term by 2 e (exponential) and 1.3 e u (z's rounding and log2(e)'s;
+// differences 2.3, a segment's factor 1 more), its sum by 18 roundings (8 terms, 3 steps, 6 over a wave,
+// 2 over waves).  The mean of u is at most H, so ln S is off by (22 + 3.3 H) e; T by 24 e of itself and 3.3 e
+// of the mean of u^2, at most 30 H: H by (24 + 128 H) e.
+//
 // Bound by vector instructions (14 a bf16 value with entropy and alternatives, 92 % of the cycles)
 // for bf16, by HBM for f32; small calls by two launches' latency.  500 rows of 151665, 20
 // alternatives: bf16 46-47 us (3.3 TB/s; without alternatives 34), f32 61-62 us (4.9); one row of
@@ -35,6 +40,10 @@ constexpr int kThreads = 256;
 constexpr int kEach = 64;
 constexpr int kSeg = kThreads * kEach;
 static_assert(kThreads == 256, "four waves");
+// S and T of a lane, each so many sums side by side: in one chain of 64 equal terms the roundings are
+// alike and add up (ln p 2.7e-6 off, entropies 1e-5; so 4e-7 and 3e-6, at 44.7 against 44.2 us for 500
+// rows of 151665 bf16).
+constexpr int kSums = 8;
 constexpr int kCand = 512;              // candidates that LDS holds for a block
 constexpr int kGroups = 128;            // and groups of 8 values with one
 constexpr int kHeld = 512;              // keys of a row's segments that its joining wave holds
@@ -272,21 +281,32 @@ __global__ __launch_bounds__(kThreads, 4) void logprob_kernel(LpJob J)
     // (nothing but -inf: every term is 0)
     const float from = m == none ? 0.0f : m;
     const float c = from * EAKV_LOG2E;
-    float r = fmaf(from, EAKV_LOG2E, -c), s = 0.0f, t = 0.0f;
+    float r = fmaf(from, EAKV_LOG2E, -c), s8[kSums] = {}, t8[kSums] = {};
 #pragma unroll
     for (int e = 0; e < kEach; e++) {
         const float z = fmaf(x(e), EAKV_LOG2E, -c), p = __builtin_amdgcn_exp2f(z);
-        s += p;
-        if constexpr (ENT) t = fmaf(p, fmaxf(z, -1000.0f), t);      // (a term of 0, not NaN, for -inf)
+        s8[e % kSums] += p;
+        if constexpr (ENT) t8[e % kSums] = fmaf(p, fmaxf(z, -1000.0f), t8[e % kSums]);  // (a term of 0, not NaN, for -inf)
     }
+#pragma unroll
+    for (int n = kSums / 2; n >= 1; n /= 2)
+#pragma unroll
+        for (int k = 0; k < n; k++) {
+            s8[k] += s8[k + n];
+            t8[k] += t8[k + n];
+        }
+    float s = s8[0], t = t8[0];
     if (!(fabsf(from) < 0x1p20f)) {
         // r is not small: from differences, read again
-        s = t = r = 0.0f;
+        double sd = 0.0, td = 0.0;
         for (int i = max(seg * kSeg - shift, 0) + tid; i < min((seg + 1) * kSeg - shift, J.vocab); i += kThreads) {
             const float z = (logit<BF16>(J.x, at + i) - from) * EAKV_LOG2E, p = __builtin_amdgcn_exp2f(z);
-            s += p;
-            t = fmaf(p, fmaxf(z, -1000.0f), t);
+            sd += (double)p;
+            td = fma((double)p, (double)fmaxf(z, -1000.0f), td);
         }
+        s = (float)sd;
+        t = (float)td;
+        r = 0.0f;
     }
     hold();
     s = wave_sum(s);

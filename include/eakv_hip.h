@@ -368,7 +368,9 @@ size_t eakv_evict_select_work_bytes(int n_seqs, const int32_t *n_tokens);
  *                   most likely tokens, ties to the lower one, and their ln p; -1 and -inf
  *                   where fewer have a logit above -inf
  * Logits of -inf have p = 0.  Rows with NaN or +inf, or nothing but -inf, give NaN where a ln p is
- * taken; NaN is no alternative.  Sums in f32, results 1e-6 or less off.
+ * taken; NaN is no alternative.  No ln p is above 0, no entropy below.  Sums in f32: with H the row's
+ * entropy, ln p is off by at most (24 + 4 H) 2^-24 and half a step of itself, the entropy by
+ * (24 + 128 H) 2^-24 and half a step (rows of many equal logits: 4e-7 and 3e-6 measured).
  *   d_work  eakv_token_logprobs_work_bytes() of device scratch, 16-byte aligned, the call's
  *           own (0 bytes up to 16377 tokens)
  * The results and d_work overlap nothing else (refused).  Asynchronous; may be recorded in a

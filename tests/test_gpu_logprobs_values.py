@@ -1,8 +1,17 @@
-"""Log probabilities where their sums are hardest.  Bounds: test_gpu_logprobs.py."""
+"""Log probabilities where their sums are hardest.
+
+Bounds, e = 2^-24, H the row's entropy: (24 + 4 H) e and half a step for ln p, (24 + 128 H) e and half
+a step for H.  A term is off by 2 e (its exponential), e u 1.3 (its exponent's rounding and that of
+log2(e); u = M - x) or, by differences, e u 2.3, and e u 1 by its segment's factor, itself 2 e off.  A
+lane adds 8 terms 8 times, then 3, 6 and 2 steps: 18 roundings.  sum p u <= H, so ln S is off by
+(18 + 2 + 2 + 3.3 H) e.  T, the sum of p u, by (18 + 1 + 2 + 2 + 1) e H and 3.3 e sum p u^2, and as 2^30
+terms beyond u = 30 hold less than 1e-3, sum p u^2 <= 30 H and little: together
+(22 + (3.3 + 24 + 99) H) e."""
 import numpy as np
 import pytest
 
 from test_gpu_logprobs import Job
+from windows import E32
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +44,28 @@ def test_no_probability_above_one(E, rng, bf16, vocab, rest):
     assert (lp <= 0.0).all(), float(lp.max())
     assert (tlp <= 0.0).all(), float(tlp.max())
     assert (ent >= 0.0).all(), float(ent.min())
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("vocab", [16001, 130001])
+@pytest.mark.parametrize("away", [0.0, 3e6])
+def test_many_equal_logits_below_the_largest(E, rng, bf16, vocab, away):
+    """Terms whose roundings are all alike, within what the header says; also of rows far from 0."""
+    n = 64
+    x = np.empty((n, vocab), np.float32)
+    top = rng.uniform(-30.0, 30.0, n) + away
+    x[:] = (top - rng.uniform(7.0, 14.0, n))[:, None]
+    at = rng.integers(0, vocab, n)
+    x[np.arange(n), at] = top
+    tokens = np.where(np.arange(n) % 2, at, (at + 1) % vocab)
+    j = Job(E, x, vocab, tokens, 2, bf16)
+    j.run()
+    j.check()
+    lp, ent = [o.download()[:-1].astype(np.float64) for o in j.out[:2]]
+    y = j.x.astype(np.float64)
+    z = y - y.max(1, keepdims=True)
+    p = np.exp(z)
+    s = p.sum(1)
+    want, h = z[np.arange(n), tokens] - np.log(s), np.log(s) - (p * z).sum(1) / s
+    assert (np.abs(lp - want) <= ((24 + 4 * h) + np.abs(want)) * E32).all()
+    assert (np.abs(ent - h) <= ((24 + 128 * h) + h) * E32).all()
