@@ -69,3 +69,22 @@ def test_many_equal_logits_below_the_largest(E, rng, bf16, vocab, away):
     want, h = z[np.arange(n), tokens] - np.log(s), np.log(s) - (p * z).sum(1) / s
     assert (np.abs(lp - want) <= ((24 + 4 * h) + np.abs(want)) * E32).all()
     assert (np.abs(ent - h) <= ((24 + 128 * h) + h) * E32).all()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("vocab", [65 * 16384 - 7, 2150001])
+@pytest.mark.parametrize("top", [0, 1, 20])
+def test_rows_of_many_segments(E, rng, bf16, vocab, top):
+    """More segments than a wave has lanes (65 and 132): the largest and the given token behind the
+    64th, segments of nothing but -inf before and behind it."""
+    seg = 16384
+    x = (rng.standard_normal((3, vocab)) * 3).astype(np.float32)
+    tokens = np.array([64 * seg + 77, 5, vocab - 1])
+    x[0, tokens[0]] = 30.0                              # the largest and the given one: behind the 64th
+    x[1, 64 * seg + 1000] = 40.0
+    x[1, 2 * seg - 50:9 * seg + 50] = -np.inf
+    x[2, :64 * seg + 100] = -np.inf                     # all there is is behind the 64th
+    x[2, 40 * seg] = 1.0
+    j = Job(E, x, vocab, tokens, top, bf16)
+    j.run()
+    j.check()
