@@ -27,10 +27,15 @@ int eakv_attention_weights_batch_device(eakv_cache_t *const *caches, int n_cache
     int64_t total;
     int rc = eakvi_window_check(caches, n_caches, layer, starts, n_tokens, dtype, n_q, n_kv, 0, &b, &total);
     if (rc) return rc;
-    for (int i = 0; i < n_caches; i++)
-        if (b.ntok[i] && ld < (int64_t)b.start[i] + b.ntok[i])
-            return eakvi_set_error(EAKV_ERR_INVALID, "weights: rows of %lld for %d tokens", (long long)ld,
-                                   b.start[i] + b.ntok[i]);
+    int64_t most = 0;
+    for (int i = 0; i < n_caches; i++) {
+        const int64_t t = (int64_t)b.start[i] + b.ntok[i];
+        if (!b.ntok[i]) continue;
+        if (ld < t)
+            return eakvi_set_error(EAKV_ERR_INVALID, "weights: rows of %lld for %lld tokens", (long long)ld,
+                                   (long long)t);
+        most = t > most ? t : most;
+    }
     if (total == 0) return EAKV_OK;
     const uintptr_t odd = dtype == EAKV_F32 ? 3 : 1;
     if (!d_q || !d_weights || (uintptr_t)d_q & odd || (uintptr_t)d_weights & 3 || (uintptr_t)d_work & 15)
@@ -42,7 +47,7 @@ int eakv_attention_weights_batch_device(eakv_cache_t *const *caches, int n_cache
     const size_t need = eakvd_weights_work_bytes(&b, n_q, n_kv, dtype == EAKV_BF16);
     const int own = !d_work;
     const eakvi_span q = {d_q, (size_t)total * n_q * c0->head_dim * (dtype == EAKV_F32 ? 4 : 2)},
-                     out = {d_weights, (size_t)n_caches * n_kv * (size_t)ld * 4}, work = {d_work, need};
+                     out = {d_weights, eakvi_rows_bytes((int64_t)n_caches * n_kv, ld, most, 4)}, work = {d_work, need};
     int capturing = 0;
     if (d_work && work_bytes < need) {
         rc = eakvi_set_error(EAKV_ERR_INVALID, "weights: %zu bytes of workspace, %zu needed", work_bytes, need);
@@ -102,7 +107,7 @@ int eakv_evict_select_device(int n_seqs, int n_heads, const float *d_weights, in
     j.n_heads = n_heads;
     j.n_first = n_first;
     j.n_recent = n_recent;
-    int64_t total = 0;
+    int64_t total = 0, most = 0;
     for (int i = 0; i < n_seqs; i++) {
         const int64_t n = n_tokens[i], stay = (int64_t)n_first + n_recent;
         if (n < 0 || n > MOST_TOKENS || n_keep[i] < (stay < n ? stay : n) || n_keep[i] > n || ld < n ||
@@ -114,6 +119,7 @@ int eakv_evict_select_device(int n_seqs, int n_heads, const float *d_weights, in
         j.n_keep[i] = n_keep[i];
         j.first[i] = total;
         total += n_keep[i];
+        most = n > most ? n : most;
     }
     if (n_seqs == 0 || (total == 0 && !d_kept)) return EAKV_OK;
     const size_t need = eakvd_evict_work_bytes(n_seqs, n_tokens);
@@ -122,10 +128,10 @@ int eakv_evict_select_device(int n_seqs, int n_heads, const float *d_weights, in
         return eakvi_set_error(EAKV_ERR_INVALID, "evict: NULL or misaligned buffer");
     if (work_bytes < need)
         return eakvi_set_error(EAKV_ERR_INVALID, "evict: %zu bytes of workspace, %zu needed", work_bytes, need);
-    const size_t rows = (size_t)n_seqs * (size_t)n_heads;
-    const eakvi_span in = {d_weights, rows * (size_t)ld * 4},
+    const int64_t rows = (int64_t)n_seqs * n_heads;
+    const eakvi_span in = {d_weights, eakvi_rows_bytes(rows, ld, most, 4)},
                      out[3] = {{d_index, (size_t)total * 4},
-                               {d_kept, d_kept ? rows * (size_t)ld_kept * 4 : 0},
+                               {d_kept, d_kept ? (size_t)rows * (size_t)ld_kept * 4 : 0},
                                {d_work, need}};
     for (int i = 0; i < 3; i++)
         if (eakvi_overlap(out[i], out[(i + 1) % 3]) || eakvi_overlap(out[i], in))

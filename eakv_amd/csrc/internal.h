@@ -61,6 +61,12 @@ typedef struct {
     const void *p;
     size_t n;
 } eakvi_span;
+/* Bytes of rows of `width` values of `size` bytes, ld values apart (the last one's end, not the next
+ * row's begin: what is between rows may be another buffer's). */
+static inline size_t eakvi_rows_bytes(int64_t rows, int64_t ld, int64_t width, size_t size)
+{
+    return rows > 0 ? ((size_t)(rows - 1) * (size_t)ld + (size_t)width) * size : 0;
+}
 static inline int eakvi_overlap(eakvi_span a, eakvi_span b)
 {
     const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;

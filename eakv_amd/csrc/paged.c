@@ -46,11 +46,6 @@ static int batch_check(const eakv_cache_t *pool, const eakv_paged_batch_t *b, co
 
 static int nothing(const eakvd_pages *d) { return !d->n_seqs || !d->n_new || !d->max_new; }
 
-static size_t rows_bytes(int64_t rows, int64_t ld, int64_t width, size_t size)
-{
-    return rows > 0 ? ((size_t)(rows - 1) * (size_t)ld + (size_t)width) * size : 0;
-}
-
 /* The spans of a batch's own buffers. */
 static void batch_spans(const eakvd_pages *d, eakvi_span *s)
 {
@@ -154,8 +149,8 @@ int eakv_attention_paged_device(const eakv_cache_t *cpool, const eakv_paged_batc
     const size_t need = eakvd_paged_work_bytes(&pool->geom, &d, n_q, n_kv, dtype == EAKV_BF16);
     const size_t size = dtype == EAKV_F32 ? 4 : 2;
     const int own = !d_work && need;
-    const eakvi_span q = {d_q, rows_bytes(d.n_new, ld_q, width, size)},
-                     out = {d_out, rows_bytes(d.n_new, ld_out, width, size)}, work = {d_work, need};
+    const eakvi_span q = {d_q, eakvi_rows_bytes(d.n_new, ld_q, width, size)},
+                     out = {d_out, eakvi_rows_bytes(d.n_new, ld_out, width, size)}, work = {d_work, need};
     eakvi_span in[3];
     batch_spans(&d, in);
     /* a row is written when its own query has been read, others may not have been */
