@@ -130,7 +130,7 @@ extern "C" int eakvd_paged_append(const eakvd_geom *g, uint8_t *base, const eakv
     const bool vec = (((uintptr_t)k | (uintptr_t)v) & odd) == 0 && ld % 4 == 0;
     const int t = kThreads / 8 / (int)g->gpd;
     // about kBlocks blocks, heads of the same tokens side by side
-    const int64_t chunks = (b->n_new + t - 1) / t;
+    const int64_t chunks = ((int64_t)b->n_new + t - 1) / t;
     const int all = 2 * g->n_kv_heads;
     int64_t parts = (kBlocks + chunks - 1) / chunks;
     if (parts > all) parts = all;
