@@ -220,7 +220,9 @@ size_t eakvd_paged_work_bytes(const eakvd_geom *g, const eakvd_pages *b, int n_q
 int eakvd_paged_attend(const eakvd_geom *g, const uint8_t *base, const eakvd_pages *b, int layer,
                        const void *q, int64_t ld_q, int bf16, int n_q, int n_kv, void *out,
                        int64_t ld_out, void *work, void *stream);
-/* K and V rows [n_new][n_kv][head_dim] (f32 or bf16), ld values from one token to the next */
+/* K and V rows [n_new][n_kv][head_dim] (f32 or bf16), ld values from one token to the next; n_new at
+ * most eakvd_paged_append_most() */
+int64_t eakvd_paged_append_most(const eakvd_geom *g);
 int eakvd_paged_append(const eakvd_geom *g, uint8_t *base, const eakvd_pages *b, int layer,
                        const void *k, const void *v, int64_t ld, int bf16, void *stream);
 

@@ -110,7 +110,15 @@ __global__ __launch_bounds__(kThreads) void append_kernel(eakvd_geom g, AppendJo
     }
 }
 
+int block_tokens(const eakvd_geom *g) { return kThreads / 8 / (int)g->gpd; }
+
 }  // namespace
+
+// (A launch has fewer than 2^32 threads; one of that many chunks gives a block all heads.)
+extern "C" int64_t eakvd_paged_append_most(const eakvd_geom *g)
+{
+    return ((1ll << 32) / kThreads - 1) * block_tokens(g);
+}
 
 extern "C" int eakvd_paged_append(const eakvd_geom *g, uint8_t *base, const eakvd_pages *b, int layer,
                                   const void *k, const void *v, int64_t ld, int bf16, void *stream)
@@ -128,7 +136,7 @@ extern "C" int eakvd_paged_append(const eakvd_geom *g, uint8_t *base, const eakv
     // 16-byte loads (bf16: 8)
     const uintptr_t odd = bf16 ? 7 : 15;
     const bool vec = (((uintptr_t)k | (uintptr_t)v) & odd) == 0 && ld % 4 == 0;
-    const int t = kThreads / 8 / (int)g->gpd;
+    const int t = block_tokens(g);
     // about kBlocks blocks, heads of the same tokens side by side
     const int64_t chunks = ((int64_t)b->n_new + t - 1) / t;
     const int all = 2 * g->n_kv_heads;
@@ -136,8 +144,6 @@ extern "C" int eakvd_paged_append(const eakvd_geom *g, uint8_t *base, const eakv
     if (parts > all) parts = all;
     J.heads = (int)((all + parts - 1) / parts);
     J.parts = (all + J.heads - 1) / J.heads;
-    // (a launch has fewer than 2^32 threads)
-    if (chunks * J.parts >= (1 << 24)) return (int)hipErrorInvalidValue;
     const dim3 grid((unsigned)(chunks * J.parts));
     auto run = [&](auto *kern) {
         hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, (hipStream_t)stream, *g, J);

@@ -69,6 +69,9 @@ int eakv_append_paged_device(eakv_cache_t *pool, const eakv_paged_batch_t *b, in
         return eakvi_set_error(EAKV_ERR_INVALID, "append_paged: layer %d, %lld values from token to token",
                                layer, (long long)ld);
     if (nothing(&d)) return EAKV_OK;
+    if (d.n_new > eakvd_paged_append_most(&pool->geom))
+        return eakvi_set_error(EAKV_ERR_INVALID, "append_paged: %d rows, %lld at most", d.n_new,
+                               (long long)eakvd_paged_append_most(&pool->geom));
     const uintptr_t odd = dtype == EAKV_F32 ? 3 : 1;
     if (!d_k || !d_v || ((uintptr_t)d_k | (uintptr_t)d_v) & odd)
         return eakvi_set_error(EAKV_ERR_INVALID, "append_paged: NULL or misaligned buffer");

@@ -290,9 +290,9 @@ typedef struct eakv_paged_batch {
  * bits of eakv_cache_append.  d_k, d_v: [n_new][n_kv_heads][head_dim] of type dtype
  * (EAKV_F32 or EAKV_BF16), ld values from one token to the next (n_kv_heads * head_dim or
  * more).  Where one place is written twice in a call (a page in two tables), what is left
- * there is unspecified.  Streams: as eakv_append_batch_device; on a stream that records a
- * graph nothing outside the graph is waited for, and what later reads the pages must wait
- * for the replay. */
+ * there is unspecified.  At most 2^28 - 16 rows (head_dim 64: 2^29 - 32).  Streams: as
+ * eakv_append_batch_device; on a stream that records a graph nothing outside the graph is
+ * waited for, and what later reads the pages must wait for the replay. */
 int eakv_append_paged_device(eakv_cache_t *pool, const eakv_paged_batch_t *batch, int layer,
                              const void *d_k, const void *d_v, int dtype, int64_t ld, void *stream);
 
