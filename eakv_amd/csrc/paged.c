@@ -5,6 +5,10 @@
 
 #include "internal.h"
 
+/* Positions and rows are 32 bits in the kernels, which look up to 64 sub-tiles behind a sequence's end
+ * (and hold what they find there to it). */
+#define MOST (INT32_MAX - 65535)
+
 /* The batch against the pool: sizes, tables that hold the bound on lengths. */
 static int batch_check(const eakv_cache_t *pool, const eakv_paged_batch_t *b, const char *what,
                        eakvd_pages *d)
@@ -21,6 +25,9 @@ static int batch_check(const eakv_cache_t *pool, const eakv_paged_batch_t *b, co
     if (b->n_seqs < 0 || b->n_seqs > EAKV_PAGED_SEQS || b->n_new < 0 || b->max_new < 0 || b->max_len < 0)
         return eakvi_set_error(EAKV_ERR_INVALID, "%s: %d sequences, %d rows, at most %d new of %d tokens",
                                what, b->n_seqs, b->n_new, b->max_new, b->max_len);
+    if (b->max_len > MOST || b->n_new > MOST)
+        return eakvi_set_error(EAKV_ERR_INVALID, "%s: %d rows of up to %d tokens, %d at most", what, b->n_new,
+                               b->max_len, MOST);
     /* the kernels' offsets from a kv head's first group are 32 bits */
     if ((int64_t)pool->geom.gph > INT32_MAX / 2)
         return eakvi_set_error(EAKV_ERR_INVALID, "%s: a pool of %d tokens", what, pool->max_seq_len);

@@ -272,8 +272,8 @@ int eakv_cache_compact(eakv_cache_t *cache, int start, const int32_t *keep, int 
  *                (rows before position 0, of sequences shorter than n, see nothing and
  *                are not appended).  Rows of no sequence are left alone.
  *   n_new        rows of those buffers
- *   max_new, max_len  the most rows and tokens that a sequence has.  Values on the device that
- *                pass these bounds are held to them.
+ *   max_new, max_len  the most rows and tokens (at most 2^31 - 2^16) that a sequence has.  Values on
+ *                the device that pass these bounds are held to them.
  * d_tables, d_lens and d_first are device memory, read when the call runs: a recorded graph
  * follows what they hold at each replay.  At most EAKV_PAGED_SEQS sequences. */
 #define EAKV_PAGE_MIN 16

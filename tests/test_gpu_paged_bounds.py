@@ -4,7 +4,7 @@ import ctypes as C
 
 import pytest
 
-from test_gpu_paged_evict_refusals import BASE, N_KV, batch, refused
+from test_gpu_paged_evict_refusals import BASE, D, N_KV, N_Q, ROOM, batch, refused
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +43,24 @@ def test_append_of_too_many_rows_is_refused(E, d, most):
     s = batch(E, n_new=most, max_new=most)
     rc = E.lib().eakv_append_paged_device(pool.h, C.addressof(s), 0, None, BASE + (2 << 24), 1, N_KV * d, None)
     assert "NULL" in E.last_error()[1] and refused(E, rc)
+
+
+@pytest.mark.parametrize("max_len,n_new", [(INT_MAX, 1), (2 ** 31 - 65535, 1), (16, INT_MAX)])
+def test_positions_that_pass_32_bits_are_refused(E, max_len, n_new):
+    """A bound so near 2^31 that the places looked up behind a sequence's end are not 32 bits."""
+    pool = E.Cache(1, N_KV, D, ROOM)
+    L = E.lib()
+    s = batch(E, n_seqs=1, n_new=n_new, max_new=1, max_len=max_len, ld=1 << 30)
+    assert L.eakv_attention_paged_work_bytes(pool.h, C.addressof(s), 1, N_KV, N_KV) == 0
+    assert refused(E, E.EAKV_ERR_INVALID)
+    a = BASE + (1 << 40)
+    assert refused(E, L.eakv_attention_paged_device(pool.h, C.addressof(s), 0, a, N_Q * D, 1, N_KV, N_KV, a, N_Q * D, None,
+                                                    0, None))
+    assert refused(E, L.eakv_append_paged_device(pool.h, C.addressof(s), 0, a, a, 1, N_KV * D, None))
+
+
+def test_the_longest_bound_is_accepted(E):
+    pool = E.Cache(1, N_KV, D, ROOM)
+    s = batch(E, n_seqs=1, n_new=1, max_new=1, max_len=2 ** 31 - 65536, ld=1 << 30)
+    assert E.lib().eakv_attention_paged_work_bytes(pool.h, C.addressof(s), 1, N_KV, N_KV) > 0
+    assert E.lib().eakv_last_error() == E.EAKV_OK
