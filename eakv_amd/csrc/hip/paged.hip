@@ -167,29 +167,42 @@ __device__ __forceinline__ int head_length(const PagedJob &J, const Seq &q, int 
 // The line, in LDS; its length is the result.  Up to 64 sequences: one to a lane, every wave for
 // itself (all write the same), [5][64]: its length of one kv head, that before it, and itself, so
 // that no barrier and, at a unit, no memory is waited for (0.9 us less of the 11.8 of a token of
-// 512).  More: pre[s], the length of one kv head before sequence s, s <= n_seqs.
+// 512).  More: pre[s], the length of one kv head before sequence s, s <= n_seqs.  A list of rows that
+// falls gives no line: its length might pass 32 bits, and blocks lose their places in it.
 constexpr int kFew = 64;
 __device__ __forceinline__ int line_of(const PagedJob &J, int *pre, int *sums, int tid)
 {
     const int lane = tid & 63, w = tid >> 6, n = J.b.n_seqs;
     if (n <= kFew) {
         Seq q = {0, 0, 0};
-        if (lane < n) q = seq_at(J.b, lane);
+        bool fell = false;
+        if (lane < n) {
+            q = seq_at(J.b, lane);
+            fell = falls_at(J.b, lane);
+        }
         const int len = head_length(J, q, lane), upto = wave_scan_i(len);
         const int x[5] = {len, upto - len, q.row, q.n, q.pos};
 #pragma unroll
         for (int k = 0; k < 5; k++) pre[k * kFew + lane] = x[k];
-        return __builtin_amdgcn_readlane(upto, 63) * J.n_kv;
+        return __ballot(fell) ? 0 : __builtin_amdgcn_readlane(upto, 63) * J.n_kv;
     }
-    int carry = 0;
+    int carry = 0, fallen = 0;
     for (int s0 = 0; s0 < n; s0 += 64 * kWaves) {
         const int s = s0 + tid;
         Seq q = {0, 0, 0};
-        if (s < n) q = seq_at(J.b, s);
+        bool fell = false;
+        if (s < n) {
+            q = seq_at(J.b, s);
+            fell = falls_at(J.b, s);
+        }
         const int v = head_length(J, q, lane);
         const int upto = wave_scan_i(v);
+        const uint64_t any = __ballot(fell);
         __syncthreads();
-        if (lane == 63) sums[w] = upto;
+        if (lane == 63) {
+            sums[w] = upto;
+            sums[kWaves + w] = any != 0;
+        }
         __syncthreads();
         int before = carry;
 #pragma unroll
@@ -197,12 +210,13 @@ __device__ __forceinline__ int line_of(const PagedJob &J, int *pre, int *sums, i
             const int x = sums[i];
             before += i < w ? x : 0;
             carry += x;
+            fallen |= sums[kWaves + i];
         }
         if (s < n) pre[s] = before + upto - v;
     }
     if (tid == 0) pre[n] = carry;
     __syncthreads();
-    return uni(carry) * J.n_kv;
+    return uni(fallen) ? 0 : uni(carry) * J.n_kv;
 }
 
 // Where place x of the line is.

@@ -22,6 +22,10 @@ __device__ __forceinline__ Seq seq_at(const eakvd_pages &b, int s)
     return q;
 }
 
+// A list of rows that falls after sequence s: rows would be several sequences', and all of these
+// together more than the host counted on.
+__device__ __forceinline__ bool falls_at(const eakvd_pages &b, int s) { return b.first && b.first[s + 1] < b.first[s]; }
+
 // Where position t (0 <= t < max_len) of a sequence is in the pool, or -1.
 __device__ __forceinline__ int place_of(const int32_t *table, int t, int log2p, int n_pages)
 {

@@ -270,7 +270,9 @@ int eakv_cache_compact(eakv_cache_t *cache, int start, const int32_t *keep, int 
  *                new tokens are d_first[s] to d_first[s + 1]; NULL: max_new rows each.
  *                The last of n rows is position d_lens[s] - 1, the first d_lens[s] - n
  *                (rows before position 0, of sequences shorter than n, see nothing and
- *                are not appended).  Rows of no sequence are left alone.
+ *                are not appended).  Rows of no sequence are left alone.  (A list that falls:
+ *                attention leaves all rows alone, what is appended to the tables' pages is
+ *                unspecified.)
  *   n_new        rows of those buffers
  *   max_new, max_len  the most rows and tokens (at most 2^31 - 2^16) that a sequence has.  Values on
  *                the device that pass these bounds are held to them.

@@ -2,8 +2,11 @@
 addresses stand for buffers and nothing is launched."""
 import ctypes as C
 
+import numpy as np
 import pytest
 
+import paging as P
+import windows as W
 from test_gpu_paged_evict_refusals import BASE, D, N_KV, N_Q, ROOM, batch, refused
 
 pytestmark = pytest.mark.gpu
@@ -64,3 +67,27 @@ def test_the_longest_bound_is_accepted(E):
     s = batch(E, n_seqs=1, n_new=1, max_new=1, max_len=2 ** 31 - 65536, ld=1 << 30)
     assert E.lib().eakv_attention_paged_work_bytes(pool.h, C.addressof(s), 1, N_KV, N_KV) > 0
     assert E.lib().eakv_last_error() == E.EAKV_OK
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("n", [2, 64, 70, 300])
+@pytest.mark.parametrize("large", [False, True])
+def test_rows_of_a_list_that_falls_are_left_alone(E, rng, bf16, n, large):
+    """Its sequences would share rows, and their work together might be more than the call counts
+    (2048 sequences of 4096 new tokens each: a line of 2.8e9 tiles)."""
+    from eakv_amd.hipmem import DeviceArray
+    p = P.Pool(E, rng, [40] * n, [4] * n, 16, 2, 64, ld_more=(1 << 22) // (4 * n) if large else 0)
+    p.fill(P.contents(rng, p))
+    c = P.Call(p, 8, 2, bf16)
+    c.put(rng.standard_normal((p.rows, 8, 64)).astype(np.float32))
+    kw = dict(max_len=(1 << 24) // p.rows + 1, max_new=p.rows) if large else {}
+    lists = [np.arange(n + 1) % 2 * p.rows, np.arange(n, -1, -1), p.first + (np.arange(n + 1) == n - 1) * p.rows]
+    for x in lists:
+        first = DeviceArray.from_host(x.astype(np.int32))
+        c.run(batch=p.make(d_first=first.ptr, **kw))
+        got = c.get()
+        guard = np.frombuffer(bytes([c.GUARD]) * 4, np.float32)[0] if not bf16 else W.from_bf16(
+            np.array([c.GUARD * 257], np.uint16))[0]
+        assert (got == guard).all()
+    c.run()                                             # (the pool's own list)
+    assert np.isfinite(c.get()).all()
