@@ -428,6 +428,7 @@ class PagedBatch:
             if d_first is not None:
                 raise ValueError("n_new: the rows that d_first divides")
             n_new = n_seqs * max_new
+        ints([n_seqs, page_tokens, n_new, max_new, max_len])    # (a field would keep the low 32 bits)
         self.pool = pool
         self.args = PagedBatchStruct(d_tables, ld_table, d_lens, d_first, n_seqs, page_tokens, n_new,
                                      max_new, max_len)
