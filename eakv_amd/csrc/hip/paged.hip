@@ -30,8 +30,9 @@
 //                  tokens of the step are numbered so that the scores' registers are P's
 //                  operand as they stand.
 //
-// K's operands: bf16 queries, the nibbles' own bits as subnormal f16 (2^-24 of them, which
-// the matrix cores take exactly); f32 queries, n - z with z the nibble nearest the value 0.
+// K's operands: bf16 queries, the nibbles' own bits as subnormal f16 (2^-24 of them; a group's sum is
+// good to 2^-11 of a step times the largest of q, against 2^-9 of q itself: nib_sub, window.h); f32
+// queries, n - z with z the nibble nearest the value 0.
 // Scales are applied to the f32 dots; the biases c = b + z*s enter by one product of three
 // bf16 pieces each (24 bits).
 // V: the weights carry the scales, x = p s.
@@ -39,8 +40,8 @@
 //                 O[g] = sum_t x n + (p c - x z), nibbles as subnormals and the same rounded x
 //                 in both places, so that n - z cancels what it should; the second term is
 //                 one product with -z and one with c in every operand row.  x, p and c are
-//                 rounded to f16, 2^-12 each, against the output's 2^-9.  (A product with a
-//                 subnormal comes out to 2^-17 only, which f32 results would show.)
+//                 rounded to f16, 2^-12 each, against the output's 2^-9.  The first sum is good
+//                 to 2^-11 of the largest x for each 32 tokens (nib_sub; f32 results would show it).
 //   f32 queries   O[g] = sum_t x (n - z) + p c, x a pair of f16 (24 bits), p c by f32 sums.
 // Softmax, V's exponents and the reference point M: as in window.hip.
 //

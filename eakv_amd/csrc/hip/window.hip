@@ -13,7 +13,8 @@
 //                  the tokens of a K = 16 step are numbered so that the scores'
 //                  registers are P's operand as they stand.
 // K's operands are n - z, exact in f16 (z: the nibble nearest the value 0; bf16
-// queries: 0, the nibbles' own bits as subnormal f16): score = sum over groups of
+// queries of few rows: 0, the nibbles' own bits as subnormal f16, whose sums over a group are good
+// to 2^-11 of a step times the largest of q, see nib_sub): score = sum over groups of
 // s*(q.(n - z)) + c*sum(q), c = b + z*s, with s applied to the f32 dots and the c terms
 // computed by one bf16 product of three pieces each (24 bits).
 // Few rows: each wave makes the operands it needs in registers (window_draft.hip).

@@ -169,8 +169,9 @@ int eakv_attention_fused_plan(eakv_cache_t *const *caches, int n_caches, int n_q
  * f32, results 0.5e-6 to 2e-6 off the exact ones (norms; up to 1e-5 where V is near the
  * ends of f32's range); one token per sequence without
  * a tree takes the launch of eakv_attention_fused_batch_device.  bf16 queries: V and the
- * weights are rounded to f16 (2^-12 relative), sums in f32, the result to bf16.  Scores
- * (q.k/sqrt(d)) are taken to be below 2^22 in size.
+ * weights are rounded to f16 (2^-12 relative), sums in f32, the result to bf16; q.k of a group
+ * of 64 dims may be off by 2^-11 of its scale times the largest |q| (q's own rounding to bf16:
+ * 2^-9 of each q times k).  Scores (q.k/sqrt(d)) are taken to be below 2^22 in size.
  * A non-finite scale or bias gives NaN in the scores of its token or in its 64 dims.
  *   d_work     device scratch of the call's own, 16-byte aligned, over none of the
  *              buffers (refused) and of at least
@@ -303,7 +304,8 @@ int eakv_append_paged_device(eakv_cache_t *pool, const eakv_paged_batch_t *batch
  * [n_new][n_q_heads][head_dim] of type dtype, ld_q and ld_out values from one token to
  * the next (n_q_heads * head_dim or more); one buffer with one ld, or two that do not overlap.
  * Rows that see nothing give zeros.  What a row does not see has no part in its
- * result.  Precision, non-finite values and ranges: as eakv_attention_window_batch_device.
+ * result.  Precision, non-finite values and ranges: as eakv_attention_window_batch_device (bf16: the
+ * sum over 32 tokens may also be off by 2^-11 of the largest weight times V's scale).
  *   d_work  device scratch of the call's own, 16-byte aligned, over none of the buffers and
  *           of eakv_attention_paged_work_bytes() for the same batch (prompts: some 100 MB), or
  *           NULL: the pool's workspace.  Calls that share one and overlap in time race.  A
