@@ -25,7 +25,7 @@
 //
 // Bound by vector instructions (14 a bf16 value with entropy and alternatives, 92 % of the cycles)
 // for bf16, by HBM for f32; small calls by two launches' latency.  500 rows of 151665, 20
-// alternatives: bf16 46-47 us (3.3 TB/s; without alternatives 34), f32 61-62 us (4.9); one row of
+// alternatives: bf16 45-47 us (3.3 TB/s; without alternatives 34), f32 61-62 us (4.9); one row of
 // 32000 f32 9.1 us.
 #include <math.h>
 #include <string.h>

@@ -46,11 +46,11 @@
 // Softmax, V's exponents and the reference point M: as in window.hip.
 //
 // Bound by instructions issued: single tokens' vector ALUs 68 % and all kinds together 94 % of the
-// cycles, at HBM's rate at the same time; prompts' 59 to 64 and 76 to 82 %, matrix cores 31 to
+// cycles, at nine tenths of HBM's rate at the same time; prompts' 59 to 64 and 76 to 82 %, matrix cores 31 to
 // 36 %, with waits for operands and barriers of two waves to a SIMD, then 16 to 20 us of joining
-// parts.  Measured (with the join; a copy of the same bytes at 4.66 TB/s, a library product 1145
-// Tflop/s): a bf16 token of 32 q / 8 kv heads, d = 128, 64 sequences of 1000 to 16384 93-102 us (copy
-// 97), 8 of 32768 77 us (72), one of 32768 27 us (9), one of 2048 11.3-11.6 us, two launches' latency;
+// parts.  Measured (with the join; a copy of the same bytes at 5.17 TB/s, a library product 1257
+// Tflop/s): a bf16 token of 32 q / 8 kv heads, d = 128, 64 sequences of 1000 to 16384 92-102 us (copy
+// 87), 8 of 32768 77 us (65), one of 32768 27 us (8), one of 2048 11.2-11.6 us, two launches' latency;
 // f32 tokens of the 64 sequences 133-147 us; prompts of 1500 of 4 sequences to 6001, 32 q / 4 kv, d =
 // 64, 268-290 us (480 Tflop/s); 512 and 15 tokens f32 to 8200, 64 q / 8 kv, 360-411 us (370).
 #include <string.h>

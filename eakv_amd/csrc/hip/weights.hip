@@ -16,7 +16,7 @@
 // thread's or one wave's: no atomics, the same bits on every call.
 //
 // Few rows are bound by memory (one f32 token x 8 at 32768, 32 q / 8 kv: 65 us; K and the scores
-// both ways at a copy's 4.66 TB/s 54); many by instructions issued (32 bf16 tokens x 4 to 20011, 64 q /
+// both ways at a copy's 5.17 TB/s 49); many by instructions issued (32 bf16 tokens x 4 to 20011, 64 q /
 // 8 kv: 85-97 us, the passes alike; vector ALUs 72 % and all kinds 93 to 96 % of the cycles,
 // matrix cores 29 to 35 %; 90 and 73 vector instructions for 16 rows x 32 tokens).
 #include <string.h>
