@@ -327,7 +327,10 @@ size_t eakv_attention_paged_work_bytes(const eakv_cache_t *pool, const eakv_page
  * a tree; only K is read).  keep 0: what was there is not read.  Entries from starts[c] +
  * n_tokens[c] on, and those of a cache without queries, are left alone.
  *   ld       at least the most starts[c] + n_tokens[c]
- *   d_work   as there: eakv_attention_weights_work_bytes() of scratch, or NULL
+ *   d_work   as there: eakv_attention_weights_work_bytes() of scratch, or NULL.  Windows of up to 8
+ *            rows (tokens x q heads per kv head), single tokens among them, keep their scores there, 4
+ *            bytes a token and row of q (n_tokens x n_q_heads rows): 34 MB for one token of 64 q heads
+ *            at 131072, 1.1 GB for 32 such caches
  * A token that a query does not see has no part in its softmax, whatever its size.
  * Streams and graphs: as eakv_attention_window_batch_device. */
 int eakv_attention_weights_batch_device(eakv_cache_t *const *caches, int n_caches, int layer,
