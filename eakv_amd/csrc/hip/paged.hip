@@ -47,8 +47,8 @@
 //
 // Bound by instructions issued: single tokens' vector ALUs 68 % and all kinds together 94 % of the
 // cycles, at nine tenths of HBM's rate at the same time; prompts' 59 to 64 and 76 to 82 %, matrix cores 31 to
-// 36 %, with waits for operands and barriers of two waves to a SIMD, then 16 to 20 us of joining
-// parts.  Measured (with the join; a copy of the same bytes at 5.17 TB/s, a library product 1257
+// 36 %, with waits for operands, barriers and (d = 128) spilled registers of two waves to a SIMD, then
+// 16 to 20 us of joining parts.  Measured (with the join; a copy of the same bytes at 5.17 TB/s, a library product 1257
 // Tflop/s): a bf16 token of 32 q / 8 kv heads, d = 128, 64 sequences of 1000 to 16384 92-102 us (copy
 // 87), 8 of 32768 77 us (65), one of 32768 27 us (8), one of 2048 11.2-11.6 us, two launches' latency;
 // f32 tokens of the 64 sequences 133-147 us; prompts of 1500 of 4 sequences to 6001, 32 q / 4 kv, d =
@@ -292,7 +292,9 @@ __device__ __forceinline__ int line_block(int b, int grid)
 
 // Row tiles of a wave whose rows are its own: what 256 registers hold beside their queries.
 // (bf16, 1500 x 4 to 6001 of 32Q/4KV, d = 64: 3 293 us, 4 289, 5 310; 8 kv heads, d = 128: 2 506, 3 485.  f32,
-// the first of these: 3 427, 4 452; 512 and 15 tokens to 8200 of 64Q/8KV, d = 128: 1 609, 2 442.)
+// the first of these: 3 427, 4 452; 512 and 15 tokens to 8200 of 64Q/8KV, d = 128: 1 609, 2 442.)  At d = 128
+// they hold too much: 43 registers of bf16's and 35 of f32's are in scratch memory (168 and 136 bytes a
+// lane), and what make() reads of it waits for all loads in flight.
 template <int D, bool F32>
 constexpr int kMany = D == 64 ? (F32 ? 3 : 4) : (F32 ? 2 : 3);
 
@@ -639,7 +641,8 @@ __device__ __forceinline__ void unit_tokens(const eakvd_geom &geo, const PagedJo
         const int t0 = lo + 32 * (w + kWaves * i);
         const bool ok_a = st.at_a >= 0, ok_b = st.at_b >= 0;
         // (d = 128: worked out again rather than kept, f32's in scratch memory, whose reads wait for the
-        // loads in flight: 152 against 162 us for f32 tokens of 64 sequences, bf16 8 at 32768 78 against 83)
+        // loads in flight: 152 against 162 us for f32 tokens of 64 sequences, bf16 8 at 32768 78 against 83.
+        // 17 of f32's registers still are there, read once a unit)
         int l = lane;
         if constexpr (D == 128) asm("" : "+v"(l));
         const Lanes<GPD> ln = D == 128 ? Lanes<GPD>(l) : places;
