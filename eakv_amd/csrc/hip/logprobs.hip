@@ -23,7 +23,7 @@
 // 2 over waves).  The mean of u is at most H, so ln S is off by (22 + 3.3 H) e; T by 24 e of itself and 3.3 e
 // of the mean of u^2, at most 30 H: H by (24 + 128 H) e.
 //
-// Bound by vector instructions (14 a bf16 value with entropy and alternatives, 92 % of the cycles)
+// Bound by vector instructions (14 a bf16 value with entropy and alternatives, 90 % of the cycles)
 // for bf16, by HBM for f32; small calls by two launches' latency.  500 rows of 151665, 20
 // alternatives: bf16 45-47 us (3.3 TB/s; without alternatives 34), f32 61-62 us (4.9); one row of
 // 32000 f32 9.1 us.
